@@ -530,6 +530,42 @@ int escat_recover_factored(const int32_t *rowptr, const int32_t *col, const floa
                            const int32_t *part_ptr, int n_parts, int max_part_rows, int max_part_nnz /* most entries of a part */,
                            float *frames_out, float *val3_out, float *max_err, void *stream);
 
+/* ------------------------------------------------------------------------------------------------------------------
+ * What trains the head that reads the coefficients (esc_gnn_amd.train_dp): element types of its operators. */
+#define ESCAT_F32  0
+#define ESCAT_BF16 1
+#define ESCAT_F16  2
+
+/* One AdamW step over many tensors, states in 32 or in 8 bits, with the clip by the global norm of the gradients
+ * (training/prep_optimizer.py:9, training/train.py:411-415).  `tensors` is a HOST array (it travels as kernel arguments;
+ * nothing is kept of it).
+ *   n        elements of param, grad, m and v, each contiguous, with no more alignment than an element's own
+ *   m, v     fp32 (state_bits 32) or uint8 codes (state_bits 8) with one fp32 scale per 256 consecutive elements in
+ *            m_scale / v_scale (ceil(n / 256) each); the code format is described in csrc/escat_adamw.hip
+ *   ordinal  number of the tensor among all that share `seed` (the rounding bits of 8-bit states depend on it)
+ * A step is escat_adamw_begin (sums of squares when max_norm > 0, the step count, the scalars), then one
+ * escat_adamw_update per group and pair of types, on one stream, with one workspace:
+ *   escat_adamw_begin  returns the number of partial-sum slots filled so far (>= 0) or an error (< 0).  Gradients of several
+ *      types: one call per type with finish = 0, each given the previous call's return as partial_slot, the last with finish = 1.
+ *      finish = 1 joins the sums, adds 1 to *step (device) and, if max_norm > 0, leaves the norm in *norm_out (device).
+ *   escat_adamw_update reads the scalars of groups[group_index] as escat_adamw_begin left them.
+ * No atomics: the same inputs give the same bits. */
+#define ESCAT_ADAMW_MAX_GROUPS 16
+typedef struct {
+    void *param; const void *grad; void *m; void *v; float *m_scale; float *v_scale;
+    int64_t n; uint32_t ordinal, reserved;
+} escat_adamw_tensor;
+typedef struct { double lr, beta1, beta2, eps, weight_decay; } escat_adamw_group;
+size_t escat_adamw_workspace_bytes(int n_tensors);
+int escat_adamw_begin(const escat_adamw_tensor *tensors, int n_tensors, int grad_type, double max_norm, int partial_slot, int finish,
+                      const escat_adamw_group *groups, int n_groups, int32_t *step, float *norm_out,
+                      void *workspace, size_t workspace_bytes, void *stream);
+int escat_adamw_update(const escat_adamw_tensor *tensors, int n_tensors, int param_type, int grad_type, int state_bits,
+                       const escat_adamw_group *group, int group_index, uint32_t seed, const int32_t *step,
+                       const void *workspace, void *stream);
+/* the fp32 values of an 8-bit state (is_signed: a first moment's codes, else a second moment's) */
+int escat_state8_values(const uint8_t *codes, const float *scales, int64_t n, int is_signed, float *out, void *stream);
+
 /* host utility (no GPU): Jenkins lookup3 "hashlittle", the checksum of HDF5 version-2 object headers
  * (esc_gnn_amd/hdf5_min.py, the writer of the reference's operator layout). */
 uint32_t escat_lookup3(const uint8_t *data, size_t n, uint32_t initval);
