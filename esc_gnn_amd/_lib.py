@@ -85,6 +85,8 @@ SIGNATURES = {
     "escat_adamw_begin": (ci, [vp, ci, ci, ctypes.c_double, ci, ci, vp, ci, vp, vp, vp, sz, vp]),
     "escat_adamw_update": (ci, [vp, ci, ci, ci, ci, vp, ci, ctypes.c_uint32, vp, vp, vp]),
     "escat_state8_values": (ci, [vp, vp, i64, ci, vp, vp]),
+    "escat_route": (ci, [vp, ci, i64, ci, ci, ci, vp, ci, ci, ci, ci, ctypes.c_float, vp, vp, vp]),
+    "escat_route_bwd": (ci, [vp, ci, i64, ci, ci, ci, ci, ctypes.c_float, vp, vp, vp, vp, vp]),
     "escat_lookup3": (ctypes.c_uint32, [ctypes.c_char_p, sz, ctypes.c_uint32]),
     "escat_build_workspace_bytes": (sz, [i64, ci, ci]),
     "escat_build_knn_P": (ci, [vp, vp, ci, i64, ci, ci, vp, vp, vp, i64, vp, vp, sz, vp]),

@@ -1,0 +1,394 @@
+// escat_route.hip -- routing of rows (nodes) to experts, forward and backward: scores of E logits a row, k experts and weights.
+//
+//   s = softmax(l) or sigmoid(l)        key = s + bias  (no bias: the order of l, which is that of s)
+//   group score = sum of the group's group_top largest keys; the keep best groups stay; top-k of key; ties to the lowest index
+//   w_j = scale s_j / sum_chosen s  (softmax over the chosen logits; sigmoid: + 1e-20),  or scale s_j without renormalising
+//   a logit or bias of -inf is never chosen; expert -1 with weight 0 where fewer than k can be; NaN counts as the largest
+//
+// A row belongs to LPR lanes of a wave with EPL consecutive experts each, all in registers: one read of the logits, no pass
+// over memory for the selection.  k rounds of "largest key left": the lanes' maxima meet by DPP, the first lane that holds the
+// maximum holds the lowest index.
+//
+// Which experts win is a matter of whole numbers, and s + bias in 32 bits would decide near-equal keys by the rounding of an
+// exponential.  64-bit exponentials for every logit cost more than the memory traffic (E = 256: ~26 us of issue against 14 us), so
+// keys are computed in 32 bits with a bound on their error, and a wave in which two keys that decide something lie within that
+// bound repeats the selection with 64-bit keys (about one wave in 500 at E = 256, k = 8).
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+#include "escat_dev.h"
+#include "escat_half.h"
+
+#define RT 256
+#define R_INF __builtin_inff()
+// two 32-bit keys further apart than this (times max(1, size)) are in the order of their exact values: exp and the sum of up to
+// 1024 of them err by at most 1e-6 of s <= 1, a pair of them (group score) by 2e-6, the sum with the bias by 2^-24 of its size
+#define R_GAP 7.62939453125e-6f
+
+struct RouteArgs {
+    const void *logits; const float *bias; float *weights; int *experts;
+    int64_t rows; int E, k, groups, keep, group_top, score, renorm; float scale;
+};
+
+// ------------------------------------------------------------------ reductions over the LPR lanes of a row
+template <int CTRL> __device__ __forceinline__ float dpp(float v) { return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, true)); }
+template <int CTRL> __device__ __forceinline__ double dpp(double v)
+{
+    const int lo = __builtin_amdgcn_mov_dpp(__double2loint(v), CTRL, 0xf, 0xf, true), hi = __builtin_amdgcn_mov_dpp(__double2hiint(v), CTRL, 0xf, 0xf, true);
+    return __hiloint2double(hi, lo);
+}
+struct OpMax { template <typename K> __device__ static K f(K a, K b) { return a > b ? a : b; } };
+struct OpSum { template <typename K> __device__ static K f(K a, K b) { return a + b; } };
+template <int LPR, typename OP, typename K> __device__ __forceinline__ K row_reduce(K v)
+{
+    if (LPR > 1) v = OP::f(v, dpp<0xB1>(v));                // quad_perm 1,0,3,2
+    if (LPR > 2) v = OP::f(v, dpp<0x4E>(v));                // quad_perm 2,3,0,1
+    if (LPR > 4) v = OP::f(v, dpp<0x141>(v));               // row_half_mirror: the other four of eight
+    if (LPR > 8) v = OP::f(v, dpp<0x140>(v));               // row_mirror: the other eight of sixteen
+    if (LPR > 16) v = OP::f(v, (K)__shfl_xor(v, 16, 64));
+    if (LPR > 32) v = OP::f(v, (K)__shfl_xor(v, 32, 64));
+    return v;
+}
+// first of the row's lanes for which `has` holds (one does); l0 = the row's first lane
+template <int LPR> __device__ __forceinline__ int first_lane(bool has, int l0)
+{
+    if (LPR == 1) return l0;
+    const uint64_t b = __ballot(has) >> l0;
+    return l0 + __builtin_ctzll(b);                          // lanes of later rows lie above the one that is found
+}
+
+// lanes of one wave hand values over through LDS: order the accesses, no barrier between waves
+__device__ __forceinline__ void wave_lds_sync() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup"); __builtin_amdgcn_wave_barrier(); }
+
+// ------------------------------------------------------------------ the selection
+// key / gkey: the lane's EPL keys for experts and for group scores (-inf: cannot be chosen).  sel (LDS, of the row): k results.
+// Returns whether two keys that decided something were closer than their error (CHECK only).
+template <int LPR, int EPL, typename K, bool CHECK>
+__device__ bool pick(const RouteArgs &a, K (&key)[EPL], const K (&gkey)[EPL], bool key_exact, int lane_in_row, int l0, K *buf, int *sel)
+{
+    const K inf = (K)R_INF;
+    const int e0 = lane_in_row * EPL;
+    bool close = false;
+    if (a.groups > 1) {
+        const int gs = a.E / a.groups;
+#pragma unroll
+        for (int i = 0; i < EPL; ++i) if (e0 + i < a.E) buf[e0 + i] = gkey[i];
+        wave_lds_sync();
+        K score = -inf;
+        if (lane_in_row < a.groups) {                        // one group a lane (LPR >= groups)
+            K b1 = -inf, b2 = -inf;
+            int at = lane_in_row % gs;                       // start at another place in each lane: other LDS banks
+            for (int i = 0; i < gs; ++i) {
+                const K v = buf[lane_in_row * gs + at];
+                at = at + 1 == gs ? 0 : at + 1;
+                if (v > b1) { b2 = b1; b1 = v; } else if (v > b2) b2 = v;
+            }
+            score = b1 == -inf ? -inf : b1 + (a.group_top == 2 && b2 > -inf ? b2 : (K)0);
+        }
+        wave_lds_sync();
+        uint64_t kept = 0;
+        K last = inf;
+        for (int r = 0; r <= a.keep; ++r) {
+            const K m = row_reduce<LPR, OpMax>(score);
+            if (CHECK && r > 0 && m > -inf) close |= !(last - m > (K)R_GAP * fmaxf(1.f, fabsf((float)last)));
+            if (r == a.keep || m == -inf) break;
+            const int at = first_lane<LPR>(score == m, l0);
+            kept |= 1ull << (at - l0);
+            if ((int)(threadIdx.x & 63) == at) score = -inf;
+            last = m;
+        }
+#pragma unroll
+        for (int i = 0; i < EPL; ++i) {
+            const int e = e0 + i;
+            if (e >= a.E || !((kept >> (e / gs)) & 1)) key[i] = -inf;
+        }
+    }
+    K last = inf;
+    for (int j = 0; j <= a.k; ++j) {
+        K best = key[0];
+#pragma unroll
+        for (int i = 1; i < EPL; ++i) best = key[i] > best ? key[i] : best;
+        const K m = row_reduce<LPR, OpMax>(best);
+        if (CHECK && !key_exact && j > 0 && m > -inf) close |= !(last - m > (K)R_GAP * fmaxf(1.f, fabsf((float)last)));
+        if (j == a.k) break;
+        if (m == -inf) {
+            if (lane_in_row == 0) for (int q = j; q < a.k; ++q) sel[q] = -1;
+            break;
+        }
+        const int at = first_lane<LPR>(best == m, l0);
+        if ((int)(threadIdx.x & 63) == at) {
+            int w = EPL - 1;
+#pragma unroll
+            for (int i = EPL - 2; i >= 0; --i) if (key[i] == m) w = i;
+#pragma unroll
+            for (int i = 0; i < EPL; ++i) if (i == w) key[i] = -inf;
+            sel[j] = e0 + w;
+        }
+        last = m;
+    }
+    return close;
+}
+
+__device__ __forceinline__ float sigmoid_f(float x) { return 1.f / (1.f + expf(-x)); }
+
+// key of a score that is NaN: largest where the logit itself is the cause (NaN, or +inf under a softmax), next to it in the
+// rest of such a row
+__device__ __forceinline__ float spoiled(float x, float next) { return x == x && x < R_INF ? next : R_INF; }
+
+template <typename T, int LPR, int EPL>
+__global__ void __launch_bounds__(RT) k_route(const RouteArgs a)
+{
+    extern __shared__ __align__(8) unsigned char lds[];
+    constexpr int RPB = RT / LPR;
+    const int lane = threadIdx.x & 63, lane_in_row = threadIdx.x % LPR, l0 = lane - lane % LPR, r_in_b = threadIdx.x / LPR;
+    const int e0 = lane_in_row * EPL;
+    int *sel = (int *)lds + r_in_b * a.k;
+    double *buf = (double *)(lds + ((size_t)RPB * a.k * 4 + 7) / 8 * 8) + (size_t)r_in_b * a.E;      // groups only
+    const bool fp64_keys = a.bias != nullptr || a.groups > 1;
+    // all lanes of a wave go through the same number of rows: rows behind the last are worked on as rows without an expert
+    for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.rows; r0 += (int64_t)gridDim.x * RPB) {
+        const int64_t row = r0 + r_in_b;
+        const bool in = row < a.rows;
+        const T *lg = (const T *)a.logits + (in ? row : 0) * a.E;
+        float x[EPL], key[EPL];
+        if (in && e0 + EPL <= a.E) {
+            const Pack<T, EPL> q = *(const Pack<T, EPL> *)(lg + e0);
+#pragma unroll
+            for (int i = 0; i < EPL; ++i) x[i] = to_f32(q.v[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < EPL; ++i) x[i] = in && e0 + i < a.E ? to_f32(lg[e0 + i]) : -R_INF;
+        }
+        float top = -R_INF, sum = 0.f;                        // softmax's statistics over the whole row
+        if (a.score == 0 && (fp64_keys || !a.renorm)) {
+#pragma unroll
+            for (int i = 0; i < EPL; ++i) top = fmaxf(top, x[i]);           // (a NaN shows in the sum)
+            top = row_reduce<LPR, OpMax>(top);
+            const float base = top == -R_INF ? 0.f : top;
+#pragma unroll
+            for (int i = 0; i < EPL; ++i) sum += a.renorm ? __expf(x[i] - base) : expf(x[i] - base);
+            sum = row_reduce<LPR, OpSum>(sum);
+            top = base;
+        }
+        bool again = false;
+        if (!fp64_keys) {
+#pragma unroll
+            for (int i = 0; i < EPL; ++i) key[i] = x[i] == x[i] ? x[i] : R_INF;
+            pick<LPR, EPL, float, false>(a, key, key, true, lane_in_row, l0, (float *)buf, sel);
+        } else {
+            float gkey[EPL];
+            const float inv = 1.f / sum;
+#pragma unroll
+            for (int i = 0; i < EPL; ++i) {
+                const float s = a.score == 0 ? __expf(x[i] - top) * inv : 1.f / (1.f + __expf(-x[i]));
+                const float b = a.bias && e0 + i < a.E ? a.bias[e0 + i] : 0.f;
+                const float v = s + b;
+                gkey[i] = x[i] == -R_INF ? -R_INF : v == v ? v : spoiled(x[i], 3.4e38f);
+                key[i] = a.bias ? gkey[i] : x[i] == x[i] ? x[i] : R_INF;
+            }
+            again = pick<LPR, EPL, float, true>(a, key, gkey, !a.bias, lane_in_row, l0, (float *)buf, sel);
+        }
+        if (__any(again)) {
+            double key2[EPL], gkey2[EPL];
+            double top2 = -(double)R_INF, sum2 = 0.0;
+            if (a.score == 0) {
+#pragma unroll
+                for (int i = 0; i < EPL; ++i) top2 = fmax(top2, (double)x[i]);
+                top2 = row_reduce<LPR, OpMax>(top2);
+                top2 = top2 == -(double)R_INF ? 0.0 : top2;
+                for (int i = 0; i < EPL; ++i) sum2 += exp((double)x[i] - top2);
+                sum2 = row_reduce<LPR, OpSum>(sum2);
+            }
+#pragma unroll
+            for (int i = 0; i < EPL; ++i) {
+                const double s = a.score == 0 ? exp((double)x[i] - top2) / sum2 : 1.0 / (1.0 + exp(-(double)x[i]));
+                const double v = s + (a.bias && e0 + i < a.E ? (double)a.bias[e0 + i] : 0.0);
+                gkey2[i] = x[i] == -R_INF ? -(double)R_INF : v == v ? v : (double)spoiled(x[i], 3.4e38f);
+                key2[i] = a.bias ? gkey2[i] : x[i] == x[i] ? (double)x[i] : (double)R_INF;
+            }
+            pick<LPR, EPL, double, false>(a, key2, gkey2, true, lane_in_row, l0, buf, sel);
+        }
+        wave_lds_sync();
+        // weights: the chosen logits once more (they are in the cache), k of them over the row's lanes
+        const float base = top;
+        float m = -R_INF, z = 0.f;
+        if (a.score == 0 && a.renorm) {
+            for (int j = lane_in_row; j < a.k; j += LPR) { const int e = sel[j]; if (in && e >= 0) { const float v = to_f32(lg[e]); m = v > m ? v : m; } }
+            m = row_reduce<LPR, OpMax>(m);
+        }
+        if (a.renorm) {
+            for (int j = lane_in_row; j < a.k; j += LPR) {
+                const int e = sel[j];
+                if (in && e >= 0) { const float v = to_f32(lg[e]); z += a.score == 0 ? expf(v - m) : sigmoid_f(v); }
+            }
+            z = row_reduce<LPR, OpSum>(z);
+            z = a.score == 0 ? z : z + 1e-20f;
+        } else z = a.score == 0 ? sum : 1.f;
+        for (int j = lane_in_row; j < a.k; j += LPR) {
+            const int e = sel[j];
+            if (!in) continue;
+            float w = 0.f;
+            if (e >= 0) {
+                const float v = to_f32(lg[e]);
+                w = a.scale * ((a.score == 0 ? expf(v - (a.renorm ? m : base)) : sigmoid_f(v)) / z);
+            }
+            a.weights[row * a.k + j] = w;
+            a.experts[row * a.k + j] = e;
+        }
+        wave_lds_sync();
+    }
+}
+
+// ------------------------------------------------------------------ backward
+// dl from dw: renormalised softmax  dl_j = w_j (dw_j - sum_i w_i dw_i / scale);  softmax  dl_e = scale s_e ([e chosen] dw_e - sum_j s_j dw_j);
+// sigmoid  dl_j = ds_j s_j (1 - s_j) with ds = scale dw, or scale (dw_j / Z - sum_i dw_i s_i / Z^2).  The whole row of dl is written once.
+struct RouteBwdArgs {
+    const void *logits; const float *weights; const int *experts; const float *dw; void *dl;
+    int64_t rows; int E, k, score, renorm; float scale;
+};
+
+template <typename T, int LPR, int EPL>
+__global__ void __launch_bounds__(RT) k_route_bwd(const RouteBwdArgs a)
+{
+    constexpr int RPB = RT / LPR;
+    const int lane_in_row = threadIdx.x % LPR, r_in_b = threadIdx.x / LPR, e0 = lane_in_row * EPL;
+    for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.rows; r0 += (int64_t)gridDim.x * RPB) {
+        const int64_t row = r0 + r_in_b;
+        const bool in = row < a.rows;
+        const int64_t rr = in ? row : 0;
+        const T *lg = (const T *)a.logits + rr * a.E;
+        const float *dw = a.dw + rr * a.k, *w = a.weights + rr * a.k;
+        const int *ex = a.experts + rr * a.k;
+        float d[EPL], s[EPL];
+        float z = 1.f, dot = 0.f;
+        if (a.score == 0 && !a.renorm) {
+            float top = -R_INF, sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < EPL; ++i) { s[i] = in && e0 + i < a.E ? to_f32(lg[e0 + i]) : -R_INF; top = fmaxf(top, s[i]); }
+            top = row_reduce<LPR, OpMax>(top);
+            top = top == -R_INF ? 0.f : top;
+#pragma unroll
+            for (int i = 0; i < EPL; ++i) { s[i] = expf(s[i] - top); sum += s[i]; }
+            sum = row_reduce<LPR, OpSum>(sum);
+            sum = sum == 0.f ? 1.f : sum;                        // no logit above -inf: nothing was chosen
+#pragma unroll
+            for (int i = 0; i < EPL; ++i) s[i] /= sum;
+            for (int j = lane_in_row; j < a.k; j += LPR) if (in && ex[j] >= 0) dot += w[j] * dw[j];
+            dot = row_reduce<LPR, OpSum>(dot);                   // = scale sum_j s_j dw_j
+#pragma unroll
+            for (int i = 0; i < EPL; ++i) d[i] = -s[i] * dot;
+        } else {
+#pragma unroll
+            for (int i = 0; i < EPL; ++i) d[i] = 0.f;
+            if (a.renorm) {
+                float zz = 0.f;
+                for (int j = lane_in_row; j < a.k; j += LPR)
+                    if (in && ex[j] >= 0) {
+                        const float p = a.score == 0 ? w[j] : sigmoid_f(to_f32(lg[ex[j]]));
+                        dot += p * dw[j];
+                        zz += p;
+                    }
+                dot = row_reduce<LPR, OpSum>(dot);
+                if (a.score == 1) { z = row_reduce<LPR, OpSum>(zz) + 1e-20f; dot /= z; } else dot /= a.scale;
+            }
+        }
+        for (int j = 0; j < a.k; ++j) {                           // every lane looks at all k: k is small and they sit in the cache
+            const int e = in ? ex[j] : -1;
+            if (e < e0 || e >= e0 + EPL) continue;                // (another lane's, or -1)
+            float v;
+            if (a.score == 0) v = a.renorm ? w[j] * (dw[j] - dot) : w[j] * dw[j];
+            else {
+                const float q = sigmoid_f(to_f32(lg[e]));
+                v = a.scale * q * (1.f - q) * (a.renorm ? (dw[j] - dot) / z : dw[j]);
+            }
+#pragma unroll
+            for (int i = 0; i < EPL; ++i) if (i == e - e0) d[i] += v;
+        }
+        T *out = (T *)a.dl + rr * a.E;
+        if (in && e0 + EPL <= a.E) {
+            Pack<T, EPL> q;
+#pragma unroll
+            for (int i = 0; i < EPL; ++i) q.v[i] = from_f32<T>(d[i]);
+            *(Pack<T, EPL> *)(out + e0) = q;
+        } else if (in) {
+#pragma unroll
+            for (int i = 0; i < EPL; ++i) if (e0 + i < a.E) out[e0 + i] = from_f32<T>(d[i]);
+        }
+    }
+}
+
+// ------------------------------------------------------------------ entry points
+// lanes of a row: enough for E experts at EPL each, and one a group
+static int lanes_per_row(int E, int epl, int groups)
+{
+    int l = 1;
+    while (l * epl < E || l < groups) l *= 2;
+    return l;
+}
+
+template <template <typename, int, int> class L, typename A> static int route_dispatch(int type, int lpr, int epl, const A &a, unsigned blocks, size_t lds, hipStream_t st)
+{
+#define ROUTE_CASE(LPR, EPL)                                                                 \
+    if (lpr == LPR && epl == EPL) {                                                          \
+        if (type == ESCAT_F32) return L<float, LPR, EPL>::go(a, blocks, lds, st);            \
+        if (type == ESCAT_BF16) return L<bf16_t, LPR, EPL>::go(a, blocks, lds, st);          \
+        return L<f16_t, LPR, EPL>::go(a, blocks, lds, st);                                   \
+    }
+    ROUTE_CASE(1, 8) ROUTE_CASE(2, 8) ROUTE_CASE(4, 8) ROUTE_CASE(8, 8) ROUTE_CASE(16, 8) ROUTE_CASE(32, 8) ROUTE_CASE(64, 8) ROUTE_CASE(64, 16)
+#undef ROUTE_CASE
+    return fail(ESCAT_ERANGE, "route: %d lanes of %d experts", lpr, epl);
+}
+template <typename T, int LPR, int EPL> struct LaunchFwd {
+    static int go(const RouteArgs &a, unsigned blocks, size_t lds, hipStream_t st)
+    {
+        int rc = set_lds(k_route<T, LPR, EPL>, lds); if (rc) return rc;
+        k_route<T, LPR, EPL><<<blocks, RT, lds, st>>>(a);
+        CHECK_LAUNCH("escat_route");
+        return ESCAT_OK;
+    }
+};
+template <typename T, int LPR, int EPL> struct LaunchBwd {
+    static int go(const RouteBwdArgs &a, unsigned blocks, size_t, hipStream_t st)
+    {
+        k_route_bwd<T, LPR, EPL><<<blocks, RT, 0, st>>>(a);
+        CHECK_LAUNCH("escat_route_bwd");
+        return ESCAT_OK;
+    }
+};
+
+static int check_route(const char *who, int type, int64_t rows, int E, int k, int score, float scale)
+{
+    if (!escat_type_bytes(type)) return fail(ESCAT_EINVAL, "%s: type = %d", who, type);
+    if (rows < 0 || E < 1 || k < 1 || k > E) return fail(ESCAT_EINVAL, "%s: rows = %lld, E = %d, k = %d", who, (long long)rows, E, k);
+    if (E > ESCAT_ROUTE_MAX_EXPERTS || k > ESCAT_ROUTE_MAX_K) return fail(ESCAT_ERANGE, "%s: E = %d (at most %d), k = %d (at most %d)", who, E, ESCAT_ROUTE_MAX_EXPERTS, k, ESCAT_ROUTE_MAX_K);
+    if (score != 0 && score != 1) return fail(ESCAT_EINVAL, "%s: score = %d (0 softmax, 1 sigmoid)", who, score);
+    if (!(scale > 0.f)) return fail(ESCAT_EINVAL, "%s: scale = %g", who, (double)scale);
+    return ESCAT_OK;
+}
+
+extern "C" int escat_route(const void *logits, int type, int64_t rows, int E, int k, int score, const float *bias, int groups, int keep_groups,
+                           int group_top, int renorm, float scale, float *weights, int32_t *experts, void *stream)
+{
+    int rc = check_route("escat_route", type, rows, E, k, score, scale); if (rc) return rc;
+    if (groups < 1 || groups > 64 || E % groups || keep_groups < 1 || keep_groups > groups || (group_top != 1 && group_top != 2))
+        return fail(ESCAT_EINVAL, "escat_route: groups = %d (1..64, dividing E = %d), keep_groups = %d, group_top = %d (1 or 2)", groups, E, keep_groups, group_top);
+    if (rows == 0) return ESCAT_OK;
+    if (!logits || !weights || !experts) return fail(ESCAT_EINVAL, "escat_route: null pointer");
+    if (keep_groups == groups) groups = keep_groups = 1;             // every group stays: no groups
+    const int epl = E > 512 ? 16 : 8, lpr = lanes_per_row(E, epl, groups), rpb = RT / lpr;
+    const size_t lds = ((size_t)rpb * k * 4 + 7) / 8 * 8 + (groups > 1 ? (size_t)rpb * E * 8 : 0);
+    const int64_t want = (rows + rpb - 1) / rpb;
+    const RouteArgs a = {logits, bias, weights, experts, rows, E, k, groups, keep_groups, group_top, score, renorm ? 1 : 0, scale};
+    return route_dispatch<LaunchFwd>(type, lpr, epl, a, (unsigned)(want < 65536 ? want : 65536), lds, (hipStream_t)stream);
+}
+
+extern "C" int escat_route_bwd(const void *logits, int type, int64_t rows, int E, int k, int score, int renorm, float scale, const float *weights,
+                               const int32_t *experts, const float *dweights, void *dlogits, void *stream)
+{
+    int rc = check_route("escat_route_bwd", type, rows, E, k, score, scale); if (rc) return rc;
+    if (rows == 0) return ESCAT_OK;
+    if (!logits || !weights || !experts || !dweights || !dlogits) return fail(ESCAT_EINVAL, "escat_route_bwd: null pointer");
+    const int epl = E > 512 ? 16 : 8, lpr = lanes_per_row(E, epl, 1), rpb = RT / lpr;
+    const int64_t want = (rows + rpb - 1) / rpb;
+    const RouteBwdArgs a = {logits, weights, experts, dweights, dlogits, rows, E, k, score, renorm ? 1 : 0, scale};
+    return route_dispatch<LaunchBwd>(type, lpr, epl, a, (unsigned)(want < 65536 ? want : 65536), 0, (hipStream_t)stream);
+}

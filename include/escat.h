@@ -566,6 +566,17 @@ int escat_adamw_update(const escat_adamw_tensor *tensors, int n_tensors, int par
 /* the fp32 values of an 8-bit state (is_signed: a first moment's codes, else a second moment's) */
 int escat_state8_values(const uint8_t *codes, const float *scales, int64_t n, int is_signed, float *out, void *stream);
 
+/* Routing of rows to experts (csrc/escat_route.hip has the formulas).  logits (rows, E) of `type`, bias (E) fp32 or NULL,
+ * weights and experts (rows, k): fp32 and int32, expert -1 with weight 0 where fewer than k experts can be chosen.
+ * score 0 = softmax, 1 = sigmoid; E divides into `groups` (at most 64) of which keep_groups stay, by the sum of their group_top
+ * (1 or 2) largest keys; scale > 0.  escat_route_bwd writes the whole of dlogits (rows, E) in the logits' type. */
+#define ESCAT_ROUTE_MAX_EXPERTS 1024
+#define ESCAT_ROUTE_MAX_K 16
+int escat_route(const void *logits, int type, int64_t rows, int E, int k, int score, const float *bias, int groups, int keep_groups,
+                int group_top, int renorm, float scale, float *weights, int32_t *experts, void *stream);
+int escat_route_bwd(const void *logits, int type, int64_t rows, int E, int k, int score, int renorm, float scale, const float *weights,
+                    const int32_t *experts, const float *dweights, void *dlogits, void *stream);
+
 /* host utility (no GPU): Jenkins lookup3 "hashlittle", the checksum of HDF5 version-2 object headers
  * (esc_gnn_amd/hdf5_min.py, the writer of the reference's operator layout). */
 uint32_t escat_lookup3(const uint8_t *data, size_t n, uint32_t initval);
