@@ -23,4 +23,4 @@ from .store import load_operator_store, ScatteringStore       # noqa: F401
 from .invariants import get_vector_invariants                 # noqa: F401
 from .infogain import calc_infogain_wavelet_scales            # noqa: F401
 from .optim import AdamW, adamw_step, dequantize_state, new_state8     # noqa: F401
-from .experts import route_experts                            # noqa: F401
+from .experts import route_experts, expert_mlp, expert_counts        # noqa: F401

@@ -41,6 +41,11 @@ class EscatSellDims(ctypes.Structure):
                 ("val_floats", ctypes.c_int64), ("lc_words", ctypes.c_int64), ("row_len_hist", ctypes.c_int32 * 34)]
 
 
+class EscatExpertsDims(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_int64), ("type", ctypes.c_int32), ("d", ctypes.c_int32), ("h", ctypes.c_int32), ("o", ctypes.c_int32),
+                ("experts", ctypes.c_int32), ("k", ctypes.c_int32)]
+
+
 # name -> (restype, argtypes); every symbol include/escat.h declares
 SIGNATURES = {
     "escat_last_error": (ctypes.c_char_p, []),
@@ -87,6 +92,11 @@ SIGNATURES = {
     "escat_state8_values": (ci, [vp, vp, i64, ci, vp, vp]),
     "escat_route": (ci, [vp, ci, i64, ci, ci, ci, vp, ci, ci, ci, ci, ctypes.c_float, vp, vp, vp]),
     "escat_route_bwd": (ci, [vp, ci, i64, ci, ci, ci, ci, ctypes.c_float, vp, vp, vp, vp, vp]),
+    "escat_experts_plan_bytes": (sz, [i64, ci]),
+    "escat_experts_plan": (ci, [vp, i64, ci, vp, sz, vp, vp]),
+    "escat_experts_workspace_bytes": (sz, [vp, ci]),
+    "escat_experts_fwd": (ci, [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]),
+    "escat_experts_bwd": (ci, [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]),
     "escat_lookup3": (ctypes.c_uint32, [ctypes.c_char_p, sz, ctypes.c_uint32]),
     "escat_build_workspace_bytes": (sz, [i64, ci, ci]),
     "escat_build_knn_P": (ci, [vp, vp, ci, i64, ci, ci, vp, vp, vp, i64, vp, vp, sz, vp]),

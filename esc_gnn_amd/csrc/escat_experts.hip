@@ -1,0 +1,84 @@
+// escat_experts.hip -- entry points of the experts' products (include/escat.h): argument checks and workspaces
+#include "escat_experts.h"
+
+__attribute__((visibility("hidden"))) int escat_experts_rows_fwd(int type, const EDims &n, const EPlan &p, const void *x, const float *weights, const void *w1, const void *b1,
+                           const void *w2, const void *b2, void *h, float *part, void *y, hipStream_t st);
+__attribute__((visibility("hidden"))) int escat_experts_rows_bwd(int type, const EDims &n, const EPlan &p, const void *x, const float *weights, const void *w1, const void *b1,
+                           const void *w2, const void *b2, const void *dy, void *h, void *du, float *part, float *dwp, void *dx, float *dw, hipStream_t st);
+__attribute__((visibility("hidden"))) int escat_experts_grad_chunk(int64_t P, int E, int M, int N);
+__attribute__((visibility("hidden"))) int64_t escat_experts_grad_chunks(int64_t P, int E, int chunk);
+__attribute__((visibility("hidden"))) int escat_experts_grad(int type, const EDims &n, const EPlan &p, bool w2, const void *a, const void *b, const float *weights, int M, int N,
+                       int chunk, float *part, void *out, void *db, hipStream_t st);
+
+static int check_dims(const char *who, const escat_experts_dims *n)
+{
+    if (!n) return fail(ESCAT_EINVAL, "%s: dims is null", who);
+    if (!escat_type_bytes(n->type)) return fail(ESCAT_EINVAL, "%s: type = %d", who, n->type);
+    if (n->rows < 0 || n->d < 1 || n->h < 1 || n->o < 1 || n->experts < 1 || n->k < 1)
+        return fail(ESCAT_EINVAL, "%s: rows = %lld, d = %d, h = %d, o = %d, experts = %d, k = %d", who, (long long)n->rows, n->d, n->h, n->o, n->experts, n->k);
+    if (n->experts > ESCAT_ROUTE_MAX_EXPERTS || n->k > 64 || n->rows > 0x3fffffff / n->k || n->d > 65536 || n->h > 65536 || n->o > 65536)
+        return fail(ESCAT_ERANGE, "%s: rows * k = %lld * %d (below 2^30), experts = %d (at most %d), k at most 64, d = %d, h = %d, o = %d (at most 65536)", who,
+                    (long long)n->rows, n->k, n->experts, ESCAT_ROUTE_MAX_EXPERTS, n->d, n->h, n->o);
+    return ESCAT_OK;
+}
+static EDims dims_of(const escat_experts_dims *n) { return {n->rows, n->d, n->h, n->o, n->experts, n->k}; }
+static size_t up(size_t b) { return (b + 255) & ~(size_t)255; }
+
+// workspace of the forward: h | results of the pairs;  of the backward: h | du | results of the pairs | parts of dw | chunks of the
+// weight gradients (one after the other in the same place)
+static size_t part_bytes(const escat_experts_dims *n, int M) { return up((size_t)n->rows * n->k * M * 4); }
+static size_t hidden_bytes(const escat_experts_dims *n) { return up((size_t)n->rows * n->k * n->h * escat_type_bytes(n->type)); }
+static size_t chunk_bytes(const escat_experts_dims *n, int M, int N)
+{
+    const int64_t P = n->rows * n->k;
+    const int c = escat_experts_grad_chunk(P, n->experts, M, N);
+    return c ? up((size_t)escat_experts_grad_chunks(P, n->experts, c) * ((size_t)M * N + N) * 4) : 0;
+}
+
+extern "C" size_t escat_experts_workspace_bytes(const escat_experts_dims *n, int backward)
+{
+    if (check_dims("escat_experts_workspace_bytes", n)) return 0;
+    if (!backward) return hidden_bytes(n) + part_bytes(n, n->o) + 256;
+    const size_t c1 = chunk_bytes(n, n->d, n->h), c2 = chunk_bytes(n, n->h, n->o);
+    return 2 * hidden_bytes(n) + part_bytes(n, n->d) + up((size_t)((n->h + XN - 1) / XN) * n->rows * n->k * 4) + (c1 > c2 ? c1 : c2) + 256;
+}
+
+extern "C" int escat_experts_fwd(const escat_experts_dims *n, const void *x, const float *weights, const void *w1, const void *b1, const void *w2,
+                                 const void *b2, const void *plan, void *y, void *workspace, size_t workspace_bytes, void *stream)
+{
+    int rc = check_dims("escat_experts_fwd", n); if (rc) return rc;
+    if (n->rows == 0) return ESCAT_OK;
+    if (!x || !weights || !w1 || !w2 || !plan || !y) return fail(ESCAT_EINVAL, "escat_experts_fwd: null pointer");
+    if (!workspace || workspace_bytes < escat_experts_workspace_bytes(n, 0) || ((uintptr_t)workspace & 15))
+        return fail(ESCAT_EWORKSPACE, "escat_experts_fwd: workspace of %zu bytes (16-byte aligned), needs %zu", workspace_bytes, escat_experts_workspace_bytes(n, 0));
+    char *ws = (char *)workspace;
+    const EPlan p = plan_view(const_cast<void *>(plan), n->rows * n->k, n->experts);
+    return escat_experts_rows_fwd(n->type, dims_of(n), p, x, weights, w1, b1, w2, b2, ws, (float *)(ws + hidden_bytes(n)), y, (hipStream_t)stream);
+}
+
+extern "C" int escat_experts_bwd(const escat_experts_dims *n, const void *x, const float *weights, const void *w1, const void *b1, const void *w2,
+                                 const void *b2, const void *plan, const void *dy, void *dx, float *dweights, void *dw1, void *db1, void *dw2, void *db2,
+                                 void *workspace, size_t workspace_bytes, void *stream)
+{
+    int rc = check_dims("escat_experts_bwd", n); if (rc) return rc;
+    hipStream_t st = (hipStream_t)stream;
+    if (!w1 || !w2 || !plan) return fail(ESCAT_EINVAL, "escat_experts_bwd: null pointer");
+    if (n->rows > 0 && (!x || !weights || !dy)) return fail(ESCAT_EINVAL, "escat_experts_bwd: null pointer");
+    if ((db1 && !dw1) || (db2 && !dw2)) return fail(ESCAT_EINVAL, "escat_experts_bwd: a bias's gradient comes with its weight's");
+    if (!workspace || workspace_bytes < escat_experts_workspace_bytes(n, 1) || ((uintptr_t)workspace & 15))
+        return fail(ESCAT_EWORKSPACE, "escat_experts_bwd: workspace of %zu bytes (16-byte aligned), needs %zu", workspace_bytes, escat_experts_workspace_bytes(n, 1));
+    const int64_t P = n->rows * n->k;
+    char *ws = (char *)workspace;
+    void *h = ws; ws += hidden_bytes(n);
+    void *du = ws; ws += hidden_bytes(n);
+    float *part = (float *)ws; ws += part_bytes(n, n->d);
+    float *dwp = (float *)ws; ws += up((size_t)((n->h + XN - 1) / XN) * P * 4);
+    float *chunks = (float *)ws;
+    const EDims d = dims_of(n);
+    const EPlan p = plan_view(const_cast<void *>(plan), P, n->experts);
+    if (n->rows > 0) { rc = escat_experts_rows_bwd(n->type, d, p, x, weights, w1, b1, w2, b2, dy, h, du, part, dwp, dx, dweights, st); if (rc) return rc; }
+    // (without rows: zeros)
+    if (dw2) { rc = escat_experts_grad(n->type, d, p, true, h, dy, weights, n->h, n->o, escat_experts_grad_chunk(P, n->experts, n->h, n->o), chunks, dw2, db2, st); if (rc) return rc; }
+    if (dw1) { rc = escat_experts_grad(n->type, d, p, false, x, du, weights, n->d, n->h, escat_experts_grad_chunk(P, n->experts, n->d, n->h), chunks, dw1, db1, st); if (rc) return rc; }
+    return ESCAT_OK;
+}

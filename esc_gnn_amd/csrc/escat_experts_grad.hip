@@ -1,0 +1,237 @@
+// escat_experts_grad.hip -- gradients of the experts' weights: sums over an expert's rows of outer products,
+//
+//   dW2_e[o][h] = sum_r dy_r[o] (w h)_r[h]    db2_e[o] = sum_r w_r dy_r[o]    dW1_e[h][d] = sum_r du_r[h] x_r[d]    db1_e[h] = sum_r du_r[h]
+//
+// as matrix tiles with the rows as the summed index: both operands lie in memory with their features contiguous, so they are staged
+// as they are and transposed on the way out of LDS.  A tile of 128 x 128 results sums all of an expert's rows where there are
+// tiles enough to fill the chip; otherwise the rows are cut into chunks, whose fp32 results a second kernel adds in order.  The bias
+// gradients ride along: a tile's B pieces pass through registers anyway.
+#include "escat_experts_tile.h"
+
+struct GradArgs {
+    EDims n;
+    EPlan p;
+    const void *a, *b;         // A: (w h) sorted, or x by row; B: dy by row, or du sorted
+    const float *weights;      // of the pairs: db2's
+    void *out, *db;            // (E, N, M), (E, N) of the operands' type
+    float *part;               // chunked: [chunk][N * M + N]
+    int M, N;                  // A's and B's features
+    int chunk;                 // rows of a chunk; 0 = all of an expert's
+};
+
+__device__ __forceinline__ int wave_incl(int v)
+{
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) { const int o = __shfl_up(v, m, 64); if (lane >= m) v += o; }
+    return v;
+}
+
+// chunk q -> its expert (-1: none) and the number of its chunk; every wave does it for itself
+__device__ __forceinline__ int find_chunk(const int *count, int E, int chunk, int q, int &of)
+{
+    const int lane = threadIdx.x & 63;
+    int run = 0;
+    for (int e0 = 0; e0 < E; e0 += 64) {
+        const int v = e0 + lane < E ? (count[e0 + lane] + chunk - 1) / chunk : 0;
+        const int inc = run + wave_incl(v);
+        const uint64_t hit = __ballot(q < inc);
+        if (hit) {
+            const int l = __builtin_ctzll(hit);
+            of = q - (__shfl(inc, l, 64) - __shfl(v, l, 64));
+            return __builtin_amdgcn_readfirstlane(e0 + l);
+        }
+        run = __shfl(inc, 63, 64);
+    }
+    return -1;
+}
+
+// W2: A by sorted position, B gathered by row and weighted for db; else A gathered by row, B by sorted position
+template <typename T, bool W2>
+__global__ void __launch_bounds__(XT, 2) k_expert_grad(const GradArgs g)
+{
+    constexpr int PER = Elem<T>::PER, KB = Elem<T>::KB;
+    extern __shared__ __align__(16) char lds[];
+    typedef Stage<T, true> SM;
+    const int M = g.M, N = g.N, k = g.n.k, mt = (M + XN - 1) / XN, nt = (N + XN - 1) / XN;
+    const int work = xcd_swizzle(blockIdx.x, gridDim.x), q = work / (mt * nt), tile = work - q * mt * nt;
+    const int m0 = (tile % mt) * XN, n0 = (tile / mt) * XN;
+    int e = q, of = 0;
+    if (g.chunk) { e = find_chunk(g.p.count, g.n.E, g.chunk, q, of); if (e < 0) return; }
+    const int end = g.p.first[e + 1], ra = g.p.first[e] + of * g.chunk;
+    const int rb = g.chunk && ra + g.chunk < end ? ra + g.chunk : end;
+
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, am = (wave & 1) * 64, bn = (wave >> 1) * 64;
+    const int ma = m0 + SM::chunk() * PER, nb = n0 + SM::chunk() * PER;
+    const bool sums = m0 == 0 && g.db != nullptr;
+    int row[4], row_next[4];
+    float w[4], w_next[4], db[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) db[i] = 0.f;
+    auto fetch = [&](int k0) {                               // rows (and weights) of step k0, one step ahead of the data
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int s = ra + k0 + SM::row(i);
+            const int pr = s < rb ? g.p.pair[s] : -1;
+            row_next[i] = pr < 0 ? -1 : pr / k;
+            w_next[i] = W2 && sums && pr >= 0 ? g.weights[pr] : 0.f;
+        }
+    };
+    acc_t acc[2][2];
+    clear(acc);
+    fetch(0);
+    tile_loop<T, true, true>(rb - ra, lds, am, bn, acc,
+        [&](int k0, u4 (&r)[4]) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) row[i] = row_next[i];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int64_t at = W2 ? (int64_t)(ra + k0 + SM::row(i)) : (int64_t)row[i];
+                r[i] = load16((const T *)g.a + at * M + ma, row[i] >= 0 ? M - ma : 0);
+            } },
+        [&](int k0, u4 (&r)[4]) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int64_t at = W2 ? (int64_t)row[i] : (int64_t)(ra + k0 + SM::row(i));
+                r[i] = load16((const T *)g.b + at * N + nb, row[i] >= 0 ? N - nb : 0);
+                w[i] = w_next[i];
+            }
+            fetch(k0 + KB); },
+        [&](int, const u4 (&r)[4]) {
+            if (sums) {
+                float f[PER];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    to_floats<T>(r[i], f);
+#pragma unroll
+                    for (int z = 0; z < PER; ++z) db[z] = W2 ? fmaf(w[i], f[z], db[z]) : db[z] + f[z];
+                }
+            } });
+
+    float *part = g.chunk ? g.part + (int64_t)q * ((int64_t)N * M + N) : nullptr;
+    if (sums) {                                               // the threads that hold the same features join in a fixed order
+        float *red = (float *)lds;
+#pragma unroll
+        for (int z = 0; z < PER; ++z) red[threadIdx.x * PER + z] = db[z];
+        __syncthreads();
+        if (threadIdx.x < 128 && n0 + (int)threadIdx.x < N) {
+            float v = 0.f;
+            for (int i = 0; i < SM::RPP; ++i) v += red[i * 128 + threadIdx.x];
+            const int n = n0 + threadIdx.x;
+            if (part) part[(int64_t)N * M + n] = v;
+            else ((T *)g.db)[(int64_t)e * N + n] = from_f32<T>(v);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int n = n0 + bn + 32 * j + (lane & 31);
+        if (n >= N) continue;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int z4 = 0; z4 < 4; ++z4) {
+                const int m = m0 + am + 32 * i + 8 * z4 + 4 * (lane >> 5);
+                const int left = M - m;
+                if (left <= 0) continue;
+                if (part) {
+                    float *o = part + (int64_t)n * M + m;
+                    Pack<float, 4> v;
+#pragma unroll
+                    for (int z = 0; z < 4; ++z) v.v[z] = acc[i][j][4 * z4 + z];
+                    if (left >= 4) *(Pack<float, 4> *)o = v;
+                    else {
+#pragma unroll
+                        for (int z = 0; z < 4; ++z) if (z < left) o[z] = v.v[z];
+                    }
+                } else {
+                    T *o = (T *)g.out + ((int64_t)e * N + n) * M + m;
+                    Pack<T, 4> v;
+#pragma unroll
+                    for (int z = 0; z < 4; ++z) v.v[z] = from_f32<T>(acc[i][j][4 * z4 + z]);
+                    if (left >= 4) *(Pack<T, 4> *)o = v;
+                    else {
+#pragma unroll
+                        for (int z = 0; z < 4; ++z) if (z < left) o[z] = v.v[z];
+                    }
+                }
+            }
+    }
+}
+
+// adds an expert's chunks in order: out[e][i] = sum_c part[first chunk + c][i]; the last N of a chunk's values are db's
+template <typename T>
+__global__ void __launch_bounds__(XT) k_grad_join(const GradArgs g)
+{
+    const int e = blockIdx.y;
+    const int64_t NM = (int64_t)g.N * g.M, len = NM + g.N;
+    int first = 0, chunks = 0;
+    for (int i0 = 0; i0 <= e; i0 += 64) {
+        const int lane = threadIdx.x & 63;
+        int v = i0 + lane <= e ? (g.p.count[i0 + lane] + g.chunk - 1) / g.chunk : 0;
+        chunks = __shfl(v, (e - i0) & 63, 64);               // (of the last round: e itself)
+#pragma unroll
+        for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
+        first += v;
+    }
+    first -= chunks;
+    const float *p = g.part + (int64_t)first * len;
+    for (int64_t i = ((int64_t)blockIdx.x * XT + threadIdx.x) * 4; i < len; i += (int64_t)gridDim.x * XT * 4) {
+        if (i + 4 <= NM) {
+            float s[4] = {0.f, 0.f, 0.f, 0.f};
+            for (int c = 0; c < chunks; ++c) {
+                const Pack<float, 4> v = *(const Pack<float, 4> *)(p + c * len + i);
+#pragma unroll
+                for (int z = 0; z < 4; ++z) s[z] += v.v[z];
+            }
+            Pack<T, 4> o;
+#pragma unroll
+            for (int z = 0; z < 4; ++z) o.v[z] = from_f32<T>(s[z]);
+            *(Pack<T, 4> *)((T *)g.out + e * NM + i) = o;
+        } else {
+            for (int64_t j = i; j < i + 4 && j < len; ++j) {
+                if (j >= NM && !g.db) continue;              // (no bias: its places were never written)
+                float s = 0.f;
+                for (int c = 0; c < chunks; ++c) s += p[c * len + j];
+                if (j < NM) ((T *)g.out)[e * NM + j] = from_f32<T>(s);
+                else ((T *)g.db)[(int64_t)e * g.N + (j - NM)] = from_f32<T>(s);
+            }
+        }
+    }
+}
+
+// rows of a chunk: none cut where an expert's tiles alone fill the chip four times over, else about 1024 workgroups in all, none of
+// fewer than 512 rows
+int escat_experts_grad_chunk(int64_t P, int E, int M, int N)
+{
+    const int64_t tiles = (int64_t)((M + XN - 1) / XN) * ((N + XN - 1) / XN);
+    if (tiles * E >= 1024 || P <= 512) return 0;
+    const int64_t want = (1024 + tiles - 1) / tiles;
+    int64_t r = (P + want - 1) / want;
+    r = (r + 63) / 64 * 64;
+    return (int)(r < 512 ? 512 : r);
+}
+int64_t escat_experts_grad_chunks(int64_t P, int E, int chunk) { return chunk ? P / chunk + (E < P ? E : P) : E; }
+
+template <typename T, bool W2> static int launch(const GradArgs &g, hipStream_t st)
+{
+    const int64_t tiles = (int64_t)((g.M + XN - 1) / XN) * ((g.N + XN - 1) / XN);
+    const int64_t wgs = tiles * escat_experts_grad_chunks(g.n.rows * g.n.k, g.n.E, g.chunk);
+    if (wgs > 0xffffff) return fail(ESCAT_ERANGE, "experts: %lld tiles", (long long)wgs);
+    int rc = set_lds(k_expert_grad<T, W2>, 4 * TILE_BYTES); if (rc) return rc;
+    k_expert_grad<T, W2><<<(unsigned)wgs, XT, 4 * TILE_BYTES, st>>>(g);
+    CHECK_LAUNCH("experts: weight gradient");
+    if (g.chunk) {
+        const int64_t len = (int64_t)g.N * g.M + g.N, b = (len / 4 + XT) / XT;
+        k_grad_join<T><<<dim3((unsigned)(b < 4096 ? b : 4096), (unsigned)g.n.E), XT, 0, st>>>(g);
+        CHECK_LAUNCH("experts: weight gradient, joined");
+    }
+    return ESCAT_OK;
+}
+
+int escat_experts_grad(int type, const EDims &n, const EPlan &p, bool w2, const void *a, const void *b, const float *weights, int M, int N,
+                       int chunk, float *part, void *out, void *db, hipStream_t st)
+{
+    const GradArgs g = {n, p, a, b, weights, out, db, part, M, N, chunk};
+    if (w2) return type == ESCAT_F32 ? launch<float, true>(g, st) : type == ESCAT_BF16 ? launch<bf16_t, true>(g, st) : launch<f16_t, true>(g, st);
+    return type == ESCAT_F32 ? launch<float, false>(g, st) : type == ESCAT_BF16 ? launch<bf16_t, false>(g, st) : launch<f16_t, false>(g, st);
+}

@@ -1,0 +1,181 @@
+// escat_experts_tile.h -- the 128 x 128 matrix tile that all products of the experts share (device code)
+//
+// C[m][n] += sum_k A[m][k] B[n][k], m = features (A side), n = rows of activations or features (B side).  256 threads, four
+// waves of 64 x 64 each (2 x 2 MFMA blocks of 32 x 32, fp32 accumulators).  One step covers KB values of k: 64 of 16 bits or 32 of
+// 32 bits, 128 bytes of a row.  Operands come from memory through registers into one of two LDS buffers while the other is
+// multiplied: one barrier a step.
+//
+// An operand lies in memory with k contiguous ("KC": rows of activations, W1 / W2 in the forward) or with m contiguous ("KM": the
+// weights in the backward, both operands of a weight gradient).  In LDS:
+//   KC  row r: 128 bytes = 8 chunks of 16, chunk c at c ^ (r & 7): a wave's 16-byte reads of 32 rows and its writes both hit every bank once
+//   KM  row k: 16 bits: 256 bytes = 4 granules of 64, granule q at q ^ (k & 3), read by ds_read_tr16_b64, which hands each lane
+//       four k of one column (4 rows x 64 bytes of a half wave on distinct banks);  32 bits: 512 bytes, read one value a lane
+// MFMA operands: 16 bits 32x32x16, lane l holds k = 8 (l / 32) + 0..7 of row l % 32.  32 bits 32x32x2 (full fp32 products), lane l holds k = l / 32
+// of its pair; which two k make a pair is free as long as A and B agree: KC pairs k with k + 4 so that one 16-byte read serves four.
+// Result: lane l, register i: m = 8 (i / 4) + 4 (l / 32) + i % 4, n = l % 32.
+#ifndef ESCAT_EXPERTS_TILE_H
+#define ESCAT_EXPERTS_TILE_H
+#include "escat_experts.h"
+
+#define XT 256
+#define TILE_BYTES 16384                          // one operand, one buffer
+
+typedef float acc_t __attribute__((ext_vector_type(16)));
+typedef short s4 __attribute__((ext_vector_type(4)));
+typedef short s8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+
+template <typename T> struct Elem;                // PER: elements of 16 bytes; KB: k of a step; SUB: MFMA groups of a step
+template <> struct Elem<float> { static constexpr int PER = 4, KB = 32; };
+template <> struct Elem<bf16_t> { static constexpr int PER = 8, KB = 64; };
+template <> struct Elem<f16_t> { static constexpr int PER = 8, KB = 64; };
+
+typedef unsigned u4 __attribute__((ext_vector_type(4)));
+template <typename T> struct Vec { T v[Elem<T>::PER]; };
+
+// 16 bytes at p of which the first `left` elements exist; zero behind them
+template <typename T> __device__ __forceinline__ u4 load16(const T *p, int left)
+{
+    constexpr int PER = Elem<T>::PER;
+    u4 r = {0, 0, 0, 0};
+    if (left >= PER) { const Pack<T, PER> q = *(const Pack<T, PER> *)p; __builtin_memcpy(&r, &q, 16); }
+    else if (left > 0) {
+        Vec<T> q;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) q.v[i] = i < left ? p[i] : (T)0.f;
+        __builtin_memcpy(&r, &q, 16);
+    }
+    return r;
+}
+template <typename T> __device__ __forceinline__ void to_floats(u4 r, float (&f)[Elem<T>::PER])
+{
+    Vec<T> q; __builtin_memcpy(&q, &r, 16);
+#pragma unroll
+    for (int i = 0; i < Elem<T>::PER; ++i) f[i] = (float)q.v[i];
+}
+
+// ---- staging: thread t's four 16-byte pieces of an operand's tile
+template <typename T, bool KM> struct Stage {
+    static constexpr int PER = Elem<T>::PER;
+    static constexpr int CPR = KM ? 128 / PER : 8;          // chunks of an LDS row
+    static constexpr int RPP = XT / CPR;                    // rows of a pass: KC 32; KM 16 (16 bits), 8 (32 bits)
+    static __device__ __forceinline__ int chunk() { return threadIdx.x % CPR; }
+    static __device__ __forceinline__ int row(int i) { return threadIdx.x / CPR + i * RPP; }
+    static __device__ __forceinline__ void store(char *lds, const u4 (&v)[4])
+    {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = row(i), c = chunk();
+            const int at = !KM ? r * 128 + ((c ^ (r & 7)) << 4) : sizeof(T) == 4 ? r * 512 + c * 16 : r * 256 + (((c >> 2) ^ (r & 3)) << 6) + (c & 3) * 16;
+            *(u4 *)(lds + at) = v[i];
+        }
+    }
+};
+
+// ---- one step's products of a wave: acc[i][j] += A block i x B block j
+template <typename T, bool KM> struct Frag;
+template <typename T> struct Frag16 { s8 v; };
+
+template <typename T> __device__ __forceinline__ s8 frag_kc(const char *lds, int row, int sub)
+{
+    const int l = threadIdx.x & 63, r = row + (l & 31), c = sub * 2 + (l >> 5);
+    return *(const s8 *)(lds + r * 128 + ((c ^ (r & 7)) << 4));
+}
+__device__ __forceinline__ s8 frag_km16(const char *lds, int col, int sub)
+{
+    const int l = threadIdx.x & 63, g = l >> 4, i = l & 15;
+    const int k = sub * 16 + (g >> 1) * 8 + (i >> 2);
+    const char *p = lds + k * 256 + (((col >> 5) ^ (k & 3)) << 6) + ((g & 1) * 16 + (i & 3) * 4) * 2;
+    typedef __attribute__((address_space(3))) s4 ls4;
+    const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ls4 *)p), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ls4 *)(p + 4 * 256));
+    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+__device__ __forceinline__ acc_t mma16(bf16_t, s8 a, s8 b, acc_t c)
+{
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ acc_t mma16(f16_t, s8 a, s8 b, acc_t c)
+{
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+}
+
+template <typename T, bool AKM, bool BKM>
+__device__ __forceinline__ void tile_step(const char *la, const char *lb, int am, int bn, acc_t (&acc)[2][2])
+{
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            s8 a[2], b[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if constexpr (AKM) a[i] = frag_km16(la, am + 32 * i, s); else a[i] = frag_kc<T>(la, am + 32 * i, s);
+                if constexpr (BKM) b[i] = frag_km16(lb, bn + 32 * i, s); else b[i] = frag_kc<T>(lb, bn + 32 * i, s);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) acc[i][j] = mma16(T{}, a[i], b[j], acc[i][j]);
+        }
+    } else {
+        const int l = threadIdx.x & 63;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {                        // eight k: four pairs (k, k + 4)
+            f4 a[2], b[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if constexpr (AKM) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) a[i][q] = *(const float *)(la + (s * 8 + (l >> 5) * 4 + q) * 512 + (am + 32 * i + (l & 31)) * 4);
+                } else a[i] = __builtin_bit_cast(f4, frag_kc<T>(la, am + 32 * i, s));
+                if constexpr (BKM) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) b[i][q] = *(const float *)(lb + (s * 8 + (l >> 5) * 4 + q) * 512 + (bn + 32 * i + (l & 31)) * 4);
+                } else b[i] = __builtin_bit_cast(f4, frag_kc<T>(lb, bn + 32 * i, s));
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i][q], b[j][q], acc[i][j], 0, 0, 0);
+        }
+    }
+}
+
+// ---- the loop over k.  loadA / loadB(k0, regs): the thread's pieces of step k0; seenB(k0, regs): the B pieces of step k0 once
+// they have arrived (a use inside loadB would wait for them there).  lds: 4 tiles (A0 B0 A1 B1), free to be written on return.
+struct Unseen { __device__ void operator()(int, const u4 (&)[4]) const {} };
+template <typename T, bool AKM, bool BKM, typename FA, typename FB, typename FS = Unseen>
+__device__ __forceinline__ void tile_loop(int K, char *lds, int am, int bn, acc_t (&acc)[2][2], FA loadA, FB loadB, FS seenB = FS())
+{
+    constexpr int KB = Elem<T>::KB;
+    const int steps = (K + KB - 1) / KB;
+    if (steps == 0) return;
+    u4 ra[4], rb[4];
+    loadA(0, ra); loadB(0, rb);
+    seenB(0, rb);
+    Stage<T, AKM>::store(lds, ra); Stage<T, BKM>::store(lds + TILE_BYTES, rb);
+    __syncthreads();
+    for (int s = 0; s < steps; ++s) {
+        char *cur = lds + (s & 1) * 2 * TILE_BYTES, *nxt = lds + ((s + 1) & 1) * 2 * TILE_BYTES;
+        const bool more = s + 1 < steps;
+        if (more) { loadA((s + 1) * KB, ra); loadB((s + 1) * KB, rb); }
+        tile_step<T, AKM, BKM>(cur, cur + TILE_BYTES, am, bn, acc);
+        if (more) { seenB((s + 1) * KB, rb); Stage<T, AKM>::store(nxt, ra); Stage<T, BKM>::store(nxt + TILE_BYTES, rb); }
+        __syncthreads();
+    }
+}
+
+__device__ __forceinline__ void clear(acc_t (&acc)[2][2])
+{
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.f;
+}
+#endif

@@ -9,6 +9,7 @@ router picks for it.
 All three run on the current stream, read nothing back to the host, and give the same bits for the same inputs (no
 floating-point atomics); they can be captured into a graph.  There is no CPU path.
 """
+import ctypes
 import math
 from typing import Optional, Tuple
 import torch
@@ -95,3 +96,109 @@ def route_experts(logits: torch.Tensor, k: int, *, score: str = "softmax", bias:
     _need_gpu(logits, "logits")
     return _Route.apply(logits, None if bias is None else bias.detach().contiguous(), k, _SCORES[score], groups, keep, group_top,
                         int(bool(renormalize)), float(scale))
+
+
+def _plan(experts: torch.Tensor, E: int, counts: Optional[torch.Tensor], stream) -> torch.Tensor:
+    lib = _lib.load()
+    P = experts.numel()
+    size = lib.escat_experts_plan_bytes(P, E)
+    plan = torch.empty(size, dtype=torch.uint8, device=experts.device)
+    _lib.check(lib.escat_experts_plan(experts.data_ptr(), P, E, plan.data_ptr(), size, _ptr(counts), stream), "escat_experts_plan")
+    return plan
+
+
+def _check_experts(experts: torch.Tensor, E: int):
+    if experts.dtype is not torch.int32:
+        raise ValueError(f"escat: experts must be int32: {experts.dtype}")
+    if not 1 <= E <= MAX_EXPERTS:
+        raise ValueError(f"escat: E = {E} (1..{MAX_EXPERTS})")
+    if experts.numel() >= 1 << 30:
+        raise ValueError(f"escat: {experts.numel()} (row, slot) pairs: fewer than 2^30 are supported")
+
+
+def expert_counts(experts: torch.Tensor, n_experts: int) -> torch.Tensor:
+    """(n_experts,) int32: how many (row, slot) pairs go to each expert; entries outside [0, n_experts) are left out"""
+    _check_experts(experts, n_experts)
+    _need_gpu(experts, "experts")
+    counts = torch.empty(n_experts, dtype=torch.int32, device=experts.device)
+    with _on(experts.device) as stream:
+        _plan(experts.contiguous(), n_experts, counts, stream)
+    return counts
+
+
+class _ExpertMLP(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weights, experts, w1, b1, w2, b2):
+        lib = _lib.load()
+        (rows, d), k, (E, h, _), o = x.shape, experts.shape[1], w1.shape, w2.shape[1]
+        dims = _lib.EscatExpertsDims(rows, DTYPE_CODES[x.dtype], d, h, o, E, k)
+        at = ctypes.addressof(dims)
+        y = torch.empty(rows, o, dtype=x.dtype, device=x.device)
+        size = lib.escat_experts_workspace_bytes(at, 0)
+        with _on(x.device) as stream:
+            plan = _plan(experts, E, None, stream)
+            ws = torch.empty(size, dtype=torch.uint8, device=x.device)
+            rc = lib.escat_experts_fwd(at, x.data_ptr(), weights.data_ptr(), w1.data_ptr(), _ptr(b1), w2.data_ptr(), _ptr(b2), plan.data_ptr(),
+                                       y.data_ptr(), ws.data_ptr(), size, stream)
+        _lib.check(rc, "escat_experts_fwd")
+        ctx.save_for_backward(x, weights, w1, b1, w2, b2)
+        ctx.plan, ctx.dims = plan, dims
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        lib = _lib.load()
+        x, weights, w1, b1, w2, b2 = ctx.saved_tensors
+        dims = ctx.dims
+        at = ctypes.addressof(dims)
+        dy = dy.contiguous()
+        need = ctx.needs_input_grad
+        new = lambda t, n: torch.empty_like(t) if t is not None and n else None                  # noqa: E731
+        dx, dweights = new(x, need[0]), new(weights, need[1])
+        db1, db2 = new(b1, need[4]), new(b2, need[6])
+        dw1, dw2 = new(w1, need[3] or need[4]), new(w2, need[5] or need[6])
+        size = lib.escat_experts_workspace_bytes(at, 1)
+        with _on(x.device) as stream:
+            ws = torch.empty(size, dtype=torch.uint8, device=x.device)
+            rc = lib.escat_experts_bwd(at, x.data_ptr(), weights.data_ptr(), w1.data_ptr(), _ptr(b1), w2.data_ptr(), _ptr(b2), ctx.plan.data_ptr(),
+                                       dy.data_ptr(), _ptr(dx), _ptr(dweights), _ptr(dw1), _ptr(db1), _ptr(dw2), _ptr(db2), ws.data_ptr(), size,
+                                       stream)
+        _lib.check(rc, "escat_experts_bwd")
+        return dx, dweights, None, dw1 if need[3] else None, db1, dw2 if need[5] else None, db2
+
+
+def expert_mlp(x: torch.Tensor, weights: torch.Tensor, experts: torch.Tensor, w1: torch.Tensor, b1: Optional[torch.Tensor],
+               w2: torch.Tensor, b2: Optional[torch.Tensor]) -> torch.Tensor:
+    """
+    y_t = sum_j weights[t, j] (W2_e silu(W1_e x_t + b1_e) + b2_e) with e = experts[t, j]; gradients for all but `experts`.
+
+    x (rows, d), w1 (E, h, d), b1 (E, h) or None, w2 (E, o, h), b2 (E, o) or None: one type, fp32, bf16 or fp16 (under autocast
+    they are cast to its type); weights (rows, k) fp32, experts (rows, k) int32 as route_experts gives them.  A pair whose
+    expert lies outside [0, E) counts for nothing and gets no gradient; the same expert may come twice in a row.  Sums are
+    fp32; with 16-bit types the weighted hidden rows and their gradients are rounded to the type in between.  The backward
+    computes the hidden rows again: the forward keeps nothing but its arguments and the sorted pairs.  Weights must be
+    contiguous; d, h, o are free (any alignment), k <= 64, E <= 1024, rows * k < 2^30.
+    """
+    if torch.is_autocast_enabled("cuda") and x.is_cuda:
+        t = torch.get_autocast_dtype("cuda")
+        x, w1, w2 = x.to(t), w1.to(t), w2.to(t)
+        b1, b2 = None if b1 is None else b1.to(t), None if b2 is None else b2.to(t)
+    if x.dim() != 2 or w1.dim() != 3 or w2.dim() != 3 or x.dtype not in DTYPE_CODES:
+        raise ValueError(f"escat: x (rows, d), w1 (E, h, d), w2 (E, o, h) in fp32, bf16 or fp16: {tuple(x.shape)} {x.dtype}, {tuple(w1.shape)}, {tuple(w2.shape)}")
+    (rows, d), (E, h, d1), (E2, o, h2) = x.shape, w1.shape, w2.shape
+    if d != d1 or h != h2 or E != E2 or min(d, h, o) < 1 or max(d, h, o) > 65536:
+        raise ValueError(f"escat: x {tuple(x.shape)}, w1 {tuple(w1.shape)}, w2 {tuple(w2.shape)} do not fit each other")
+    if weights.dim() != 2 or weights.shape[0] != rows or experts.shape != weights.shape or not 1 <= weights.shape[1] <= 64 or weights.dtype is not torch.float32:
+        raise ValueError(f"escat: weights and experts must be ({rows}, k), k <= 64, weights fp32: {tuple(weights.shape)} {weights.dtype}, {tuple(experts.shape)}")
+    _check_experts(experts, E)
+    for name, t, shape in (("w1", w1, w1.shape), ("w2", w2, w2.shape), ("b1", b1, (E, h)), ("b2", b2, (E, o))):
+        if t is not None and (t.shape != shape or t.dtype is not x.dtype):
+            raise ValueError(f"escat: {name} must be {tuple(shape)} {x.dtype}: {tuple(t.shape)} {t.dtype}")
+        if t is not None and not t.is_contiguous():
+            raise ValueError(f"escat: {name} must be contiguous (strides {t.stride()})")
+    for name, t in (("weights", weights), ("experts", experts), ("w1", w1), ("w2", w2), ("b1", b1), ("b2", b2)):
+        if t is not None and t.device != x.device:
+            raise RuntimeError(f"escat: {name} lives on {t.device}, x on {x.device}")
+    _need_gpu(x, "x")
+    return _ExpertMLP.apply(x.contiguous(), weights.contiguous(), experts.contiguous(), w1, b1, w2, b2)

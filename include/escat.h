@@ -577,6 +577,26 @@ int escat_route(const void *logits, int type, int64_t rows, int E, int k, int sc
 int escat_route_bwd(const void *logits, int type, int64_t rows, int E, int k, int score, int renorm, float scale, const float *weights,
                     const int32_t *experts, const float *dweights, void *dlogits, void *stream);
 
+/* The experts' products: y_t = sum_j w_tj (W2_e silu(W1_e x_t + b1_e) + b2_e), e = experts[t, j]; pairs whose expert lies
+ * outside [0, experts) count for nothing.
+ *   x (rows, d), w1 (experts, h, d), b1 (experts, h) or NULL, w2 (experts, o, h), b2 (experts, o) or NULL, y (rows, o), all of `type`;
+ *   weights (rows, k) fp32.
+ * escat_experts_plan sorts the rows * k pairs by expert into `plan` (escat_experts_plan_bytes), on the GPU, nothing read back;
+ * counts (experts) int32, optional: pairs of each expert.  escat_experts_fwd / _bwd read a plan of the same experts array.
+ * escat_experts_bwd: gradients for dy (rows, o); dx, dweights, dw1 + db1, dw2 + db2 may each be NULL (a bias's gradient only
+ * together with its weight's); the others are written whole (experts without a row: zeros).  Workspaces: 16-byte aligned, contents
+ * only used within the call.  No atomics: the same inputs give the same bits. */
+typedef struct { int64_t rows; int32_t type, d, h, o, experts, k; } escat_experts_dims;
+size_t escat_experts_plan_bytes(int64_t pairs, int experts);
+int escat_experts_plan(const int32_t *experts_of_pairs, int64_t pairs, int experts, void *plan, size_t plan_bytes, int32_t *counts,
+                       void *stream);
+size_t escat_experts_workspace_bytes(const escat_experts_dims *dims, int backward);
+int escat_experts_fwd(const escat_experts_dims *dims, const void *x, const float *weights, const void *w1, const void *b1,
+                      const void *w2, const void *b2, const void *plan, void *y, void *workspace, size_t workspace_bytes, void *stream);
+int escat_experts_bwd(const escat_experts_dims *dims, const void *x, const float *weights, const void *w1, const void *b1,
+                      const void *w2, const void *b2, const void *plan, const void *dy, void *dx, float *dweights, void *dw1, void *db1,
+                      void *dw2, void *db2, void *workspace, size_t workspace_bytes, void *stream);
+
 /* host utility (no GPU): Jenkins lookup3 "hashlittle", the checksum of HDF5 version-2 object headers
  * (esc_gnn_amd/hdf5_min.py, the writer of the reference's operator layout). */
 uint32_t escat_lookup3(const uint8_t *data, size_t n, uint32_t initval);
