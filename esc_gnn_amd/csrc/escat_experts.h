@@ -12,6 +12,7 @@ struct EPlan {
     int *tile;        // 2 x max_tiles: expert, first position
     int *pair;        // P      sorted position -> pair
     int *pos;         // P      pair -> sorted position, -1 = not routed
+    int *row;         // P      sorted position -> row of the activations (pair / k)
     int *hist;        // E x blocks: scratch of the sort
 };
 #define XM 128                                    // sorted positions of a tile (rows of activations)
@@ -24,13 +25,13 @@ static inline int64_t plan_blocks(int64_t P) { return (P + PLAN_CHUNK - 1) / PLA
 static inline int64_t plan_max_tiles(int64_t P, int E) { return P / XM + (E < P ? E : P) + 1; }
 static inline int64_t plan_ints(int64_t P, int E)
 {
-    return (int64_t)E + (E + 1) + 1 + 2 * plan_max_tiles(P, E) + 2 * P + E * plan_blocks(P) + 64;
+    return (int64_t)E + (E + 1) + 1 + 2 * plan_max_tiles(P, E) + 3 * P + E * plan_blocks(P) + 64;
 }
 static inline EPlan plan_view(void *mem, int64_t P, int E)
 {
     EPlan p; int *q = (int *)mem;
     p.count = q; q += E; p.first = q; q += E + 1; p.n_tiles = q; q += 1; p.tile = q; q += 2 * plan_max_tiles(P, E);
-    p.pair = q; q += P; p.pos = q; q += P; p.hist = q;
+    p.pair = q; q += P; p.pos = q; q += P; p.row = q; q += P; p.hist = q;
     return p;
 }
 

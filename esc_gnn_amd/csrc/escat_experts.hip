@@ -4,7 +4,7 @@
 __attribute__((visibility("hidden"))) int escat_experts_rows_fwd(int type, const EDims &n, const EPlan &p, const void *x, const float *weights, const void *w1, const void *b1,
                            const void *w2, const void *b2, void *h, float *part, void *y, hipStream_t st);
 __attribute__((visibility("hidden"))) int escat_experts_rows_bwd(int type, const EDims &n, const EPlan &p, const void *x, const float *weights, const void *w1, const void *b1,
-                           const void *w2, const void *b2, const void *dy, void *h, void *du, float *part, float *dwp, void *dx, float *dw, hipStream_t st);
+                           const void *w2, const void *b2, const void *dy, void *h, void *du, float *part, float *dwp, float *ws, void *dx, float *dw, hipStream_t st);
 __attribute__((visibility("hidden"))) int escat_experts_grad_chunk(int64_t P, int E, int M, int N);
 __attribute__((visibility("hidden"))) int64_t escat_experts_grad_chunks(int64_t P, int E, int chunk);
 __attribute__((visibility("hidden"))) int escat_experts_grad(int type, const EDims &n, const EPlan &p, bool w2, const void *a, const void *b, const float *weights, int M, int N,
@@ -24,7 +24,7 @@ static int check_dims(const char *who, const escat_experts_dims *n)
 static EDims dims_of(const escat_experts_dims *n) { return {n->rows, n->d, n->h, n->o, n->experts, n->k}; }
 static size_t up(size_t b) { return (b + 255) & ~(size_t)255; }
 
-// workspace of the forward: h | results of the pairs;  of the backward: h | du | results of the pairs | parts of dw | chunks of the
+// workspace of the forward: h | results of the pairs;  of the backward: h | du | results of the pairs | parts of dw | weights, sorted | chunks of the
 // weight gradients (one after the other in the same place)
 static size_t part_bytes(const escat_experts_dims *n, int M) { return up((size_t)n->rows * n->k * M * 4); }
 static size_t hidden_bytes(const escat_experts_dims *n) { return up((size_t)n->rows * n->k * n->h * escat_type_bytes(n->type)); }
@@ -40,7 +40,7 @@ extern "C" size_t escat_experts_workspace_bytes(const escat_experts_dims *n, int
     if (check_dims("escat_experts_workspace_bytes", n)) return 0;
     if (!backward) return hidden_bytes(n) + part_bytes(n, n->o) + 256;
     const size_t c1 = chunk_bytes(n, n->d, n->h), c2 = chunk_bytes(n, n->h, n->o);
-    return 2 * hidden_bytes(n) + part_bytes(n, n->d) + up((size_t)((n->h + XN - 1) / XN) * n->rows * n->k * 4) + (c1 > c2 ? c1 : c2) + 256;
+    return 2 * hidden_bytes(n) + part_bytes(n, n->d) + up((size_t)((n->h + XN - 1) / XN) * n->rows * n->k * 4) + up((size_t)n->rows * n->k * 4) + (c1 > c2 ? c1 : c2) + 256;
 }
 
 extern "C" int escat_experts_fwd(const escat_experts_dims *n, const void *x, const float *weights, const void *w1, const void *b1, const void *w2,
@@ -73,12 +73,13 @@ extern "C" int escat_experts_bwd(const escat_experts_dims *n, const void *x, con
     void *du = ws; ws += hidden_bytes(n);
     float *part = (float *)ws; ws += part_bytes(n, n->d);
     float *dwp = (float *)ws; ws += up((size_t)((n->h + XN - 1) / XN) * P * 4);
+    float *sw = (float *)ws; ws += up((size_t)P * 4);
     float *chunks = (float *)ws;
     const EDims d = dims_of(n);
     const EPlan p = plan_view(const_cast<void *>(plan), P, n->experts);
-    if (n->rows > 0) { rc = escat_experts_rows_bwd(n->type, d, p, x, weights, w1, b1, w2, b2, dy, h, du, part, dwp, dx, dweights, st); if (rc) return rc; }
+    if (n->rows > 0) { rc = escat_experts_rows_bwd(n->type, d, p, x, weights, w1, b1, w2, b2, dy, h, du, part, dwp, sw, dx, dweights, st); if (rc) return rc; }
     // (without rows: zeros)
-    if (dw2) { rc = escat_experts_grad(n->type, d, p, true, h, dy, weights, n->h, n->o, escat_experts_grad_chunk(P, n->experts, n->h, n->o), chunks, dw2, db2, st); if (rc) return rc; }
-    if (dw1) { rc = escat_experts_grad(n->type, d, p, false, x, du, weights, n->d, n->h, escat_experts_grad_chunk(P, n->experts, n->d, n->h), chunks, dw1, db1, st); if (rc) return rc; }
+    if (dw2) { rc = escat_experts_grad(n->type, d, p, true, h, dy, sw, n->h, n->o, escat_experts_grad_chunk(P, n->experts, n->h, n->o), chunks, dw2, db2, st); if (rc) return rc; }
+    if (dw1) { rc = escat_experts_grad(n->type, d, p, false, x, du, sw, n->d, n->h, escat_experts_grad_chunk(P, n->experts, n->d, n->h), chunks, dw1, db1, st); if (rc) return rc; }
     return ESCAT_OK;
 }

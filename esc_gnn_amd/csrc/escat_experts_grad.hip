@@ -12,7 +12,7 @@ struct GradArgs {
     EDims n;
     EPlan p;
     const void *a, *b;         // A: (w h) sorted, or x by row; B: dy by row, or du sorted
-    const float *weights;      // of the pairs: db2's
+    const float *weights;      // sorted: db2's
     void *out, *db;            // (E, N, M), (E, N) of the operands' type
     float *part;               // chunked: [chunk][N * M + N]
     int M, N;                  // A's and B's features
@@ -46,6 +46,23 @@ __device__ __forceinline__ int find_chunk(const int *count, int E, int chunk, in
     return -1;
 }
 
+template <typename OUT> __device__ __forceinline__ void spill(char *lds, const acc_t (&acc)[2][2], int am, int bn)
+{
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                float v[4];
+#pragma unroll
+                for (int z = 0; z < 4; ++z) v[z] = acc[i][j][4 * q + z];
+                Spill<OUT>::put(lds, bn + 32 * j + (lane & 31), am + 32 * i + 8 * q + 4 * (lane >> 5), v);
+            }
+    __syncthreads();
+}
+
 // W2: A by sorted position, B gathered by row and weighted for db; else A gathered by row, B by sorted position
 template <typename T, bool W2>
 __global__ void __launch_bounds__(XT, 2) k_expert_grad(const GradArgs g)
@@ -53,7 +70,7 @@ __global__ void __launch_bounds__(XT, 2) k_expert_grad(const GradArgs g)
     constexpr int PER = Elem<T>::PER, KB = Elem<T>::KB;
     extern __shared__ __align__(16) char lds[];
     typedef Stage<T, true> SM;
-    const int M = g.M, N = g.N, k = g.n.k, mt = (M + XN - 1) / XN, nt = (N + XN - 1) / XN;
+    const int M = g.M, N = g.N, mt = (M + XN - 1) / XN, nt = (N + XN - 1) / XN;
     const int work = xcd_swizzle(blockIdx.x, gridDim.x), q = work / (mt * nt), tile = work - q * mt * nt;
     const int m0 = (tile % mt) * XN, n0 = (tile / mt) * XN;
     int e = q, of = 0;
@@ -61,27 +78,26 @@ __global__ void __launch_bounds__(XT, 2) k_expert_grad(const GradArgs g)
     const int end = g.p.first[e + 1], ra = g.p.first[e] + of * g.chunk;
     const int rb = g.chunk && ra + g.chunk < end ? ra + g.chunk : end;
 
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, am = (wave & 1) * 64, bn = (wave >> 1) * 64;
+    const int wave = threadIdx.x >> 6, am = (wave & 1) * 64, bn = (wave >> 1) * 64;
     const int ma = m0 + SM::chunk() * PER, nb = n0 + SM::chunk() * PER;
     const bool sums = m0 == 0 && g.db != nullptr;
     int row[4], row_next[4];
-    float w[4], w_next[4], db[PER];
+    float w[2][4], w_next[4], db[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) db[i] = 0.f;
     auto fetch = [&](int k0) {                               // rows (and weights) of step k0, one step ahead of the data
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int s = ra + k0 + SM::row(i);
-            const int pr = s < rb ? g.p.pair[s] : -1;
-            row_next[i] = pr < 0 ? -1 : pr / k;
-            w_next[i] = W2 && sums && pr >= 0 ? g.weights[pr] : 0.f;
+            row_next[i] = s < rb ? g.p.row[s] : -1;
+            w_next[i] = W2 && sums && s < rb ? g.weights[s] : 0.f;
         }
     };
     acc_t acc[2][2];
     clear(acc);
     fetch(0);
     tile_loop<T, true, true>(rb - ra, lds, am, bn, acc,
-        [&](int k0, u4 (&r)[4]) {
+        [&](int k0, u4 (&r)[4], int) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) row[i] = row_next[i];
 #pragma unroll
@@ -89,22 +105,22 @@ __global__ void __launch_bounds__(XT, 2) k_expert_grad(const GradArgs g)
                 const int64_t at = W2 ? (int64_t)(ra + k0 + SM::row(i)) : (int64_t)row[i];
                 r[i] = load16((const T *)g.a + at * M + ma, row[i] >= 0 ? M - ma : 0);
             } },
-        [&](int k0, u4 (&r)[4]) {
+        [&](int k0, u4 (&r)[4], int set) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int64_t at = W2 ? (int64_t)row[i] : (int64_t)(ra + k0 + SM::row(i));
                 r[i] = load16((const T *)g.b + at * N + nb, row[i] >= 0 ? N - nb : 0);
-                w[i] = w_next[i];
+                w[set][i] = w_next[i];
             }
             fetch(k0 + KB); },
-        [&](int, const u4 (&r)[4]) {
+        [&](const u4 (&r)[4], int set) {
             if (sums) {
                 float f[PER];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     to_floats<T>(r[i], f);
 #pragma unroll
-                    for (int z = 0; z < PER; ++z) db[z] = W2 ? fmaf(w[i], f[z], db[z]) : db[z] + f[z];
+                    for (int z = 0; z < PER; ++z) db[z] = W2 ? fmaf(w[set][i], f[z], db[z]) : db[z] + f[z];
                 }
             } });
 
@@ -122,39 +138,14 @@ __global__ void __launch_bounds__(XT, 2) k_expert_grad(const GradArgs g)
             else ((T *)g.db)[(int64_t)e * N + n] = from_f32<T>(v);
         }
     }
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const int n = n0 + bn + 32 * j + (lane & 31);
-        if (n >= N) continue;
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int z4 = 0; z4 < 4; ++z4) {
-                const int m = m0 + am + 32 * i + 8 * z4 + 4 * (lane >> 5);
-                const int left = M - m;
-                if (left <= 0) continue;
-                if (part) {
-                    float *o = part + (int64_t)n * M + m;
-                    Pack<float, 4> v;
-#pragma unroll
-                    for (int z = 0; z < 4; ++z) v.v[z] = acc[i][j][4 * z4 + z];
-                    if (left >= 4) *(Pack<float, 4> *)o = v;
-                    else {
-#pragma unroll
-                        for (int z = 0; z < 4; ++z) if (z < left) o[z] = v.v[z];
-                    }
-                } else {
-                    T *o = (T *)g.out + ((int64_t)e * N + n) * M + m;
-                    Pack<T, 4> v;
-#pragma unroll
-                    for (int z = 0; z < 4; ++z) v.v[z] = from_f32<T>(acc[i][j][4 * z4 + z]);
-                    if (left >= 4) *(Pack<T, 4> *)o = v;
-                    else {
-#pragma unroll
-                        for (int z = 0; z < 4; ++z) if (z < left) o[z] = v.v[z];
-                    }
-                }
-            }
+    if (sums) __syncthreads();
+    const int cols = M - m0 < XN ? M - m0 : XN, rows = N - n0 < XN ? N - n0 : XN;
+    if (part) {
+        spill<float>(lds, acc, am, bn);
+        Spill<float>::write(lds, part + (int64_t)n0 * M + m0, M, rows, cols);
+    } else {
+        spill<T>(lds, acc, am, bn);
+        Spill<T>::write(lds, (T *)g.out + ((int64_t)e * N + n0) * M + m0, M, rows, cols);
     }
 }
 
@@ -217,8 +208,9 @@ template <typename T, bool W2> static int launch(const GradArgs &g, hipStream_t 
     const int64_t tiles = (int64_t)((g.M + XN - 1) / XN) * ((g.N + XN - 1) / XN);
     const int64_t wgs = tiles * escat_experts_grad_chunks(g.n.rows * g.n.k, g.n.E, g.chunk);
     if (wgs > 0xffffff) return fail(ESCAT_ERANGE, "experts: %lld tiles", (long long)wgs);
-    int rc = set_lds(k_expert_grad<T, W2>, 4 * TILE_BYTES); if (rc) return rc;
-    k_expert_grad<T, W2><<<(unsigned)wgs, XT, 4 * TILE_BYTES, st>>>(g);
+    const size_t lds = g.chunk || sizeof(T) == 4 ? LDS_ROWS : LDS_TILES;
+    int rc = set_lds(k_expert_grad<T, W2>, lds); if (rc) return rc;
+    k_expert_grad<T, W2><<<(unsigned)wgs, XT, lds, st>>>(g);
     CHECK_LAUNCH("experts: weight gradient");
     if (g.chunk) {
         const int64_t len = (int64_t)g.N * g.M + g.N, b = (len / 4 + XT) / XT;

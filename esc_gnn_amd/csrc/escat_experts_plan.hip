@@ -95,7 +95,7 @@ __global__ void __launch_bounds__(1024) k_plan_scan(int E, int blocks, EPlan p)
         for (int t = tfirst[e] + lane; t < tfirst[e + 1]; t += 64) { p.tile[2 * t] = e; p.tile[2 * t + 1] = first[e] + (t - tfirst[e]) * XM; }
 }
 
-__global__ void __launch_bounds__(PT) k_plan_place(const int *__restrict__ experts, int64_t P, int E, int bits, EPlan p)
+__global__ void __launch_bounds__(PT) k_plan_place(const int *__restrict__ experts, int64_t P, int k, int E, int bits, EPlan p)
 {
     extern __shared__ int cnt[];
     const int64_t c0 = (int64_t)blockIdx.x * PLAN_CHUNK;
@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(PT) k_plan_place(const int *__restrict__ exper
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup"); __builtin_amdgcn_wave_barrier();      // all lanes have read before one writes
         if (e >= 0 && below == 0) cnt[wave * E + e] += __popcll(m);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup"); __builtin_amdgcn_wave_barrier();
-        if (i < P) { p.pos[i] = e >= 0 ? at : -1; if (e >= 0) p.pair[at] = (int)i; }
+        if (i < P) { p.pos[i] = e >= 0 ? at : -1; if (e >= 0) { p.pair[at] = (int)i; p.row[at] = (int)i / k; } }
     }
 }
 
@@ -137,9 +137,10 @@ extern "C" size_t escat_experts_plan_bytes(int64_t pairs, int E)
     return pairs < 0 || E < 1 || E > ESCAT_ROUTE_MAX_EXPERTS ? 0 : (size_t)plan_ints(pairs, E) * 4;
 }
 
-extern "C" int escat_experts_plan(const int32_t *experts, int64_t pairs, int E, void *plan, size_t plan_bytes, int32_t *counts, void *stream)
+extern "C" int escat_experts_plan(const int32_t *experts, int64_t pairs, int k, int E, void *plan, size_t plan_bytes, int32_t *counts, void *stream)
 {
     int rc = plan_check("escat_experts_plan", pairs, E); if (rc) return rc;
+    if (k < 1) return fail(ESCAT_EINVAL, "escat_experts_plan: k = %d", k);
     if (pairs > 0 && !experts) return fail(ESCAT_EINVAL, "escat_experts_plan: experts is null");
     if (!plan || plan_bytes < escat_experts_plan_bytes(pairs, E)) return fail(ESCAT_EWORKSPACE, "escat_experts_plan: plan of %zu bytes, needs %zu", plan_bytes, escat_experts_plan_bytes(pairs, E));
     hipStream_t st = (hipStream_t)stream;
@@ -150,7 +151,7 @@ extern "C" int escat_experts_plan(const int32_t *experts, int64_t pairs, int E, 
     if (blocks) { k_plan_hist<<<blocks, PT, lds, st>>>(experts, pairs, E, bits, p.hist); CHECK_LAUNCH("escat_experts_plan: histogram"); }
     k_plan_scan<<<1, 1024, 0, st>>>(E, blocks, p);
     CHECK_LAUNCH("escat_experts_plan: scan");
-    if (blocks) { k_plan_place<<<blocks, PT, lds, st>>>(experts, pairs, E, bits, p); CHECK_LAUNCH("escat_experts_plan: place"); }
+    if (blocks) { k_plan_place<<<blocks, PT, lds, st>>>(experts, pairs, k, E, bits, p); CHECK_LAUNCH("escat_experts_plan: place"); }
     if (counts) { k_copy_counts<<<1, PT, 0, st>>>(p.count, E, counts); CHECK_LAUNCH("escat_experts_plan: counts"); }
     return ESCAT_OK;
 }

@@ -7,6 +7,7 @@
 // rounded to the operands' type (w h): it then serves W2's product and W2's gradient without another pass.  Nothing of the
 // forward is kept for the backward: u is computed again next to G, in fp32, so that dw and silu' see no rounding of u, and the
 // forward writes no u.  Results of the pairs are joined in fp32 by a pass of their own, in the order of the slots: no atomics.
+#include <type_traits>
 #include "escat_experts_tile.h"
 
 struct RowArgs {
@@ -18,6 +19,7 @@ struct RowArgs {
     void *du;                  // (P, H) sorted
     float *part;               // (P, O) or (P, D) fp32, sorted: what the joining pass reads
     float *dwp;                // (feature tiles of H, P) sorted: parts of dw
+    float *ws;                 // (P) sorted: w (BWD1 leaves them for the weights' gradients)
 };
 
 enum { FWD1, FWD2, BWD1, BWD2 };
@@ -30,7 +32,7 @@ __global__ void __launch_bounds__(XT, 2) k_expert_rows(const RowArgs a)
 {
     constexpr int PER = Elem<T>::PER;
     extern __shared__ __align__(16) char lds[];
-    const int D = a.n.d, H = a.n.h, O = a.n.o, k = a.n.k;
+    const int D = a.n.d, H = a.n.h, O = a.n.o;
     const int M = MODE == FWD2 ? O : MODE == BWD2 ? D : H;          // features of the result
     const int mt = (M + XN - 1) / XN;
     const int work = xcd_swizzle(blockIdx.x, gridDim.x), t = work / mt, m0 = (work - t * mt) * XN;
@@ -46,8 +48,11 @@ __global__ void __launch_bounds__(XT, 2) k_expert_rows(const RowArgs a)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int r = SC::row(i) < rows ? SC::row(i) : rows - 1;
-        br[i] = MODE == FWD2 || MODE == BWD2 ? (int64_t)(r0 + r) : (int64_t)(a.p.pair[r0 + r] / k);
+        br[i] = MODE == FWD2 || MODE == BWD2 ? (int64_t)(r0 + r) : (int64_t)a.p.row[r0 + r];
     }
+    float wr[2];                                                    // weights of the two rows whose results the lane holds
+#pragma unroll
+    for (int j = 0; j < 2; ++j) { const int r = bn + 32 * j + (lane & 31); wr[j] = MODE == BWD2 ? 1.f : a.weights[a.p.pair[r0 + (r < rows ? r : 0)]]; }
     acc_t acc[2][2];
     clear(acc);
 
@@ -63,10 +68,10 @@ __global__ void __launch_bounds__(XT, 2) k_expert_rows(const RowArgs a)
             bp[i] = B + br[i] * K + c;
         }
         tile_loop<T, false, false>(K, lds, am, bn, acc,
-            [&](int k0, u4 (&r)[4]) {
+            [&](int k0, u4 (&r)[4], int) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) r[i] = load16(ap[i] + k0, K - k0 - c); },
-            [&](int k0, u4 (&r)[4]) {
+            [&](int k0, u4 (&r)[4], int) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) r[i] = load16(bp[i] + k0, K - k0 - c); });
     }
@@ -81,20 +86,22 @@ __global__ void __launch_bounds__(XT, 2) k_expert_rows(const RowArgs a)
         const T *bp[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) bp[i] = B + br[i] * K + c;
+        int kd = 0;
         const bool with_dot = MODE == BWD1 && m0 == 0 && a.b2 != nullptr;
         const T *b2 = MODE == BWD1 ? (const T *)a.b2 + (int64_t)e * O + c : nullptr;
         if (MODE == BWD1) clear(acc2);
         tile_loop<T, true, false>(K, lds, am, bn, MODE == BWD1 ? acc2 : acc,
-            [&](int k0, u4 (&r)[4]) {
+            [&](int k0, u4 (&r)[4], int) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) { const int kk = k0 + SM::row(i); r[i] = load16(A + (int64_t)kk * M + mc, kk < K ? M - mc : 0); } },
-            [&](int k0, u4 (&r)[4]) {
+            [&](int k0, u4 (&r)[4], int) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) r[i] = load16(bp[i] + k0, K - k0 - c); },
-            [&](int k0, const u4 (&r)[4]) {
+            [&](const u4 (&r)[4], int) {
                 if (with_dot) {
                     float f[PER], g[PER];
-                    to_floats<T>(load16(b2 + k0, K - k0 - c), f);
+                    to_floats<T>(load16(b2 + kd, K - kd - c), f);
+                    kd += Elem<T>::KB;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         to_floats<T>(r[i], g);
@@ -104,9 +111,11 @@ __global__ void __launch_bounds__(XT, 2) k_expert_rows(const RowArgs a)
                 } });
     }
 
-    // ---- epilogue.  The lane holds, for each of two rows, runs of four features
+    // ---- epilogue.  The lane holds, for each of two rows, runs of four features; they leave through LDS
+    typedef typename std::conditional<MODE == FWD1 || MODE == BWD1, T, float>::type OUT;
     const T *bias = MODE == FWD2 ? (const T *)a.b2 : (const T *)a.b1;
-    float *red = (float *)lds;                                      // BWD1: [2][128] sums over the features of a half, [128] b2 . dy
+    const int cols = M - m0 < XN ? M - m0 : XN;
+    __shared__ float red[3 * 128];                                  // BWD1: sums over the features of a half, b2 . dy
     if (MODE == BWD1) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -118,15 +127,13 @@ __global__ void __launch_bounds__(XT, 2) k_expert_rows(const RowArgs a)
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         const int r = bn + 32 * j + (lane & 31);
-        const bool in = r < rows;
-        const int64_t s = r0 + (in ? r : 0);
-        const float w = MODE == BWD2 ? 1.f : a.weights[a.p.pair[s]];
+        const float w = wr[j];
         float sum = 0.f;
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                const int m = m0 + am + 32 * i + 8 * q + 4 * (lane >> 5);
+                const int mt_ = am + 32 * i + 8 * q + 4 * (lane >> 5), m = m0 + mt_;
                 float u[4], g[4];
 #pragma unroll
                 for (int z = 0; z < 4; ++z) {
@@ -143,46 +150,38 @@ __global__ void __launch_bounds__(XT, 2) k_expert_rows(const RowArgs a)
                     for (int z = 0; z < 4; ++z) {
                         const float sg = sigmoid_of<T>(u[z]), hh = u[z] * sg;
                         if (m + z < M) sum = fmaf(hh, g[z], sum);
-                        g[z] = w * g[z] * (sg * (1.f + u[z] * (1.f - sg)));
+                        acc2[i][j][4 * q + z] = w * g[z] * (sg * (1.f + u[z] * (1.f - sg)));
                         u[z] = w * hh;
                     }
                 }
-                if (!in) continue;
-                if (MODE == FWD1 || MODE == BWD1) {
-                    T *o = (T *)a.h + s * H + m, *o2 = (T *)a.du + s * H + m;
-                    if (m + 4 <= M) {
-                        Pack<T, 4> v, v2;
-#pragma unroll
-                        for (int z = 0; z < 4; ++z) { v.v[z] = from_f32<T>(u[z]); if (MODE == BWD1) v2.v[z] = from_f32<T>(g[z]); }
-                        *(Pack<T, 4> *)o = v;
-                        if (MODE == BWD1) *(Pack<T, 4> *)o2 = v2;
-                    } else {
-#pragma unroll
-                        for (int z = 0; z < 4; ++z) if (m + z < M) { o[z] = from_f32<T>(u[z]); if (MODE == BWD1) o2[z] = from_f32<T>(g[z]); }
-                    }
-                } else {
-                    float *o = a.part + s * M + m;
-                    if (m + 4 <= M) {
-                        Pack<float, 4> v;
-#pragma unroll
-                        for (int z = 0; z < 4; ++z) v.v[z] = u[z];
-                        *(Pack<float, 4> *)o = v;
-                    } else {
-#pragma unroll
-                        for (int z = 0; z < 4; ++z) if (m + z < M) o[z] = u[z];
-                    }
-                }
+                Spill<OUT>::put(lds, r, mt_, u);
             }
+        if (MODE == BWD1 && m0 == 0 && am == 0 && lane < 32 && r < rows) a.ws[r0 + r] = w;
         if (MODE == BWD1) {
             sum += __shfl_xor(sum, 32, 64);
             if (lane < 32) red[(wave & 1) * 128 + r] = sum;
         }
     }
+    __syncthreads();
+    Spill<OUT>::write(lds, (MODE == FWD1 || MODE == BWD1 ? (OUT *)a.h : (OUT *)a.part) + (int64_t)r0 * M + m0, M, rows, cols);
     if (MODE == BWD1) {
-        __syncthreads();
         const int r = threadIdx.x;
-        const int64_t P = a.n.rows * k;
+        const int64_t P = a.n.rows * a.n.k;
         if (r < rows) a.dwp[(int64_t)(m0 / XN) * P + r0 + r] = red[r] + red[128 + r] + (m0 == 0 && a.b2 ? red[256 + r] : 0.f);
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    float g[4];
+#pragma unroll
+                    for (int z = 0; z < 4; ++z) g[z] = acc2[i][j][4 * q + z];
+                    Spill<OUT>::put(lds, bn + 32 * j + (lane & 31), am + 32 * i + 8 * q + 4 * (lane >> 5), g);
+                }
+        __syncthreads();
+        Spill<OUT>::write(lds, (OUT *)a.du + (int64_t)r0 * M + m0, M, rows, cols);
     }
 }
 
@@ -237,8 +236,9 @@ template <typename T, int MODE> static int rows_launch(const RowArgs &a, int M, 
 {
     const int64_t P = a.n.rows * a.n.k, wgs = plan_max_tiles(P, a.n.E) * ((M + XN - 1) / XN);
     if (wgs > 0xffffff) return fail(ESCAT_ERANGE, "experts: %lld tiles", (long long)wgs);
-    int rc = set_lds(k_expert_rows<T, MODE>, 4 * TILE_BYTES); if (rc) return rc;
-    k_expert_rows<T, MODE><<<(unsigned)wgs, XT, 4 * TILE_BYTES, st>>>(a);
+    const size_t lds = MODE == FWD2 || MODE == BWD2 || sizeof(T) == 4 ? LDS_ROWS : LDS_TILES;
+    int rc = set_lds(k_expert_rows<T, MODE>, lds); if (rc) return rc;
+    k_expert_rows<T, MODE><<<(unsigned)wgs, XT, lds, st>>>(a);
     CHECK_LAUNCH("experts: rows");
     return ESCAT_OK;
 }
@@ -271,13 +271,13 @@ template <typename T> static int bwd(const RowArgs &a, void *dx, float *dw, hipS
 int escat_experts_rows_fwd(int type, const EDims &n, const EPlan &p, const void *x, const float *weights, const void *w1, const void *b1, const void *w2,
                            const void *b2, void *h, float *part, void *y, hipStream_t st)
 {
-    RowArgs a = {n, p, x, w1, b1, w2, b2, nullptr, weights, h, nullptr, part, nullptr};
+    RowArgs a = {n, p, x, w1, b1, w2, b2, nullptr, weights, h, nullptr, part, nullptr, nullptr};
     return type == ESCAT_F32 ? fwd<float>(a, y, st) : type == ESCAT_BF16 ? fwd<bf16_t>(a, y, st) : fwd<f16_t>(a, y, st);
 }
 int escat_experts_rows_bwd(int type, const EDims &n, const EPlan &p, const void *x, const float *weights, const void *w1, const void *b1, const void *w2,
-                           const void *b2, const void *dy, void *h, void *du, float *part, float *dwp, void *dx, float *dw, hipStream_t st)
+                           const void *b2, const void *dy, void *h, void *du, float *part, float *dwp, float *ws, void *dx, float *dw, hipStream_t st)
 {
-    RowArgs a = {n, p, x, w1, b1, w2, b2, dy, weights, h, du, part, dwp};
+    RowArgs a = {n, p, x, w1, b1, w2, b2, dy, weights, h, du, part, dwp, ws};
     return type == ESCAT_F32 ? bwd<float>(a, dx, dw, st) : type == ESCAT_BF16 ? bwd<bf16_t>(a, dx, dw, st) : bwd<f16_t>(a, dx, dw, st);
 }
 

@@ -7,7 +7,8 @@
 //
 // An operand lies in memory with k contiguous ("KC": rows of activations, W1 / W2 in the forward) or with m contiguous ("KM": the
 // weights in the backward, both operands of a weight gradient).  In LDS:
-//   KC  row r: 128 bytes = 8 chunks of 16, chunk c at c ^ (r & 7): a wave's 16-byte reads of 32 rows and its writes both hit every bank once
+//   KC  row r: 128 bytes = 8 chunks of 16, chunk c at c ^ ((r >> 1) & 7): the 16 lanes that a 16-byte read serves at once (rows 0-3, 12-15, 20-27
+//       or the other half of 32) fall on the 16 slots of two rows once each, the 8 lanes of a write on 8
 //   KM  row k: 16 bits: 256 bytes = 4 granules of 64, granule q at q ^ (k & 3), read by ds_read_tr16_b64, which hands each lane
 //       four k of one column (4 rows x 64 bytes of a half wave on distinct banks);  32 bits: 512 bytes, read one value a lane
 // MFMA operands: 16 bits 32x32x16, lane l holds k = 8 (l / 32) + 0..7 of row l % 32.  32 bits 32x32x2 (full fp32 products), lane l holds k = l / 32
@@ -68,7 +69,7 @@ template <typename T, bool KM> struct Stage {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int r = row(i), c = chunk();
-            const int at = !KM ? r * 128 + ((c ^ (r & 7)) << 4) : sizeof(T) == 4 ? r * 512 + c * 16 : r * 256 + (((c >> 2) ^ (r & 3)) << 6) + (c & 3) * 16;
+            const int at = !KM ? r * 128 + ((c ^ ((r >> 1) & 7)) << 4) : sizeof(T) == 4 ? r * 512 + c * 16 : r * 256 + (((c >> 2) ^ (r & 3)) << 6) + (c & 3) * 16;
             *(u4 *)(lds + at) = v[i];
         }
     }
@@ -81,7 +82,7 @@ template <typename T> struct Frag16 { s8 v; };
 template <typename T> __device__ __forceinline__ s8 frag_kc(const char *lds, int row, int sub)
 {
     const int l = threadIdx.x & 63, r = row + (l & 31), c = sub * 2 + (l >> 5);
-    return *(const s8 *)(lds + r * 128 + ((c ^ (r & 7)) << 4));
+    return *(const s8 *)(lds + r * 128 + ((c ^ ((r >> 1) & 7)) << 4));
 }
 __device__ __forceinline__ s8 frag_km16(const char *lds, int col, int sub)
 {
@@ -145,29 +146,69 @@ __device__ __forceinline__ void tile_step(const char *la, const char *lb, int am
     }
 }
 
-// ---- the loop over k.  loadA / loadB(k0, regs): the thread's pieces of step k0; seenB(k0, regs): the B pieces of step k0 once
-// they have arrived (a use inside loadB would wait for them there).  lds: 4 tiles (A0 B0 A1 B1), free to be written on return.
-struct Unseen { __device__ void operator()(int, const u4 (&)[4]) const {} };
+// ---- the loop over k.  loadA / loadB(k0, regs, set): the thread's pieces of step k0, two steps ahead of their use (a step's products
+// take less time than memory does); set = step & 1; seenB(regs, set): the B pieces once they have arrived (a use inside loadB would wait for
+// them there).  lds: 4 tiles (A0 B0 A1 B1), free to be written on return.
+struct Unseen { __device__ void operator()(const u4 (&)[4], int) const {} };
 template <typename T, bool AKM, bool BKM, typename FA, typename FB, typename FS = Unseen>
 __device__ __forceinline__ void tile_loop(int K, char *lds, int am, int bn, acc_t (&acc)[2][2], FA loadA, FB loadB, FS seenB = FS())
 {
     constexpr int KB = Elem<T>::KB;
     const int steps = (K + KB - 1) / KB;
     if (steps == 0) return;
-    u4 ra[4], rb[4];
-    loadA(0, ra); loadB(0, rb);
-    seenB(0, rb);
-    Stage<T, AKM>::store(lds, ra); Stage<T, BKM>::store(lds + TILE_BYTES, rb);
+    u4 ra[2][4], rb[2][4];
+    loadA(0, ra[0], 0); loadB(0, rb[0], 0);
+    if (steps > 1) { loadA(KB, ra[1], 1); loadB(KB, rb[1], 1); }
+    seenB(rb[0], 0);
+    Stage<T, AKM>::store(lds, ra[0]); Stage<T, BKM>::store(lds + TILE_BYTES, rb[0]);
     __syncthreads();
-    for (int s = 0; s < steps; ++s) {
-        char *cur = lds + (s & 1) * 2 * TILE_BYTES, *nxt = lds + ((s + 1) & 1) * 2 * TILE_BYTES;
-        const bool more = s + 1 < steps;
-        if (more) { loadA((s + 1) * KB, ra); loadB((s + 1) * KB, rb); }
-        tile_step<T, AKM, BKM>(cur, cur + TILE_BYTES, am, bn, acc);
-        if (more) { seenB((s + 1) * KB, rb); Stage<T, AKM>::store(nxt, ra); Stage<T, BKM>::store(nxt + TILE_BYTES, rb); }
-        __syncthreads();
+    for (int s0 = 0; s0 < steps; s0 += 2) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int s = s0 + h;
+            if (s >= steps) break;
+            char *cur = lds + h * 2 * TILE_BYTES, *nxt = lds + (1 - h) * 2 * TILE_BYTES;
+            if (s + 2 < steps) { loadA((s + 2) * KB, ra[h], h); loadB((s + 2) * KB, rb[h], h); }
+            tile_step<T, AKM, BKM>(cur, cur + TILE_BYTES, am, bn, acc);
+            if (s + 1 < steps) { seenB(rb[1 - h], 1 - h); Stage<T, AKM>::store(nxt, ra[1 - h]); Stage<T, BKM>::store(nxt + TILE_BYTES, rb[1 - h]); }
+            __syncthreads();
+        }
     }
 }
+
+// ---- results through LDS, so that memory is written in whole rows of the tile.  put: the lane's run of four features m.. of row n
+// (tile coordinates); write: rows [0, rows), features [0, cols) to out + n * ld.  OUT: element type.  A row of 128 OUT is OSTRIDE bytes apart
+// from the next: 16 more than its size, so that the runs of 32 rows fall on different banks.
+template <typename OUT> struct Spill {
+    static constexpr int STRIDE = 128 * (int)sizeof(OUT) + 16;
+    static constexpr int BYTES = 128 * STRIDE;
+    static __device__ __forceinline__ void put(char *lds, int n, int m, const float (&v)[4])
+    {
+        struct alignas(4 * sizeof(OUT)) { OUT v[4]; } q;
+#pragma unroll
+        for (int z = 0; z < 4; ++z) q.v[z] = from_f32<OUT>(v[z]);
+        __builtin_memcpy(__builtin_assume_aligned(lds + n * STRIDE + m * (int)sizeof(OUT), 4 * sizeof(OUT)), &q, sizeof(q));
+    }
+    // the caller has a barrier before and, if lds is used again, after
+    static __device__ __forceinline__ void write(const char *lds, OUT *out, int64_t ld, int rows, int cols)
+    {
+        constexpr int PER = 16 / (int)sizeof(OUT), CPR = 128 / PER;
+        const int c = threadIdx.x % CPR * PER;
+        if (c >= cols) return;
+        for (int r = threadIdx.x / CPR; r < rows; r += XT / CPR) {
+            struct alignas(16) { OUT v[PER]; } q;
+            __builtin_memcpy(&q, __builtin_assume_aligned(lds + r * STRIDE + c * (int)sizeof(OUT), 16), 16);
+            OUT *o = out + r * ld + c;
+            if (c + PER <= cols) { Pack<OUT, PER> p; __builtin_memcpy(&p, &q, 16); *(Pack<OUT, PER> *)o = p; }
+            else {
+#pragma unroll
+                for (int z = 0; z < PER; ++z) if (c + z < cols) o[z] = q.v[z];
+            }
+        }
+    }
+};
+#define LDS_TILES (4 * TILE_BYTES)
+#define LDS_ROWS (Spill<float>::BYTES > LDS_TILES ? Spill<float>::BYTES : LDS_TILES)
 
 __device__ __forceinline__ void clear(acc_t (&acc)[2][2])
 {

@@ -588,7 +588,7 @@ int escat_route_bwd(const void *logits, int type, int64_t rows, int E, int k, in
  * only used within the call.  No atomics: the same inputs give the same bits. */
 typedef struct { int64_t rows; int32_t type, d, h, o, experts, k; } escat_experts_dims;
 size_t escat_experts_plan_bytes(int64_t pairs, int experts);
-int escat_experts_plan(const int32_t *experts_of_pairs, int64_t pairs, int experts, void *plan, size_t plan_bytes, int32_t *counts,
+int escat_experts_plan(const int32_t *experts_of_pairs, int64_t pairs, int k, int experts, void *plan, size_t plan_bytes, int32_t *counts,
                        void *stream);
 size_t escat_experts_workspace_bytes(const escat_experts_dims *dims, int backward);
 int escat_experts_fwd(const escat_experts_dims *dims, const void *x, const float *weights, const void *w1, const void *b1,

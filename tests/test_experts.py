@@ -104,6 +104,6 @@ def test_experts_library_checks_its_arguments():
     assert lib.escat_experts_fwd(dims(*good), *[16] * 8, 16, 64, 0) == -3                        # small workspace
     assert lib.escat_experts_fwd(dims(0, 0, 8, 8, 8, 2, 1), *[0] * 9, 0, 0) == 0                 # no rows
     assert lib.escat_experts_bwd(dims(*good), *[16] * 8, 0, 0, 0, 16, 0, 0, 16, 1 << 20, 0) == -1          # db1 without dw1
-    assert lib.escat_experts_plan(0, 5, 4, 16, 1 << 20, 0, 0) == -1
-    assert lib.escat_experts_plan(16, 5, 4, 16, 8, 0, 0) == -3
-    assert lib.escat_experts_plan(16, 1 << 31, 4, 16, 8, 0, 0) == -2
+    assert lib.escat_experts_plan(0, 5, 1, 4, 16, 1 << 20, 0, 0) == -1
+    assert lib.escat_experts_plan(16, 5, 1, 4, 16, 8, 0, 0) == -3
+    assert lib.escat_experts_plan(16, 1 << 31, 1, 4, 16, 8, 0, 0) == -2
