@@ -16,6 +16,8 @@ static int check_dims(const char *who, const escat_experts_dims *n)
     if (!escat_type_bytes(n->type)) return fail(ESCAT_EINVAL, "%s: type = %d", who, n->type);
     if (n->rows < 0 || n->d < 1 || n->h < 1 || n->o < 1 || n->experts < 1 || n->k < 1)
         return fail(ESCAT_EINVAL, "%s: rows = %lld, d = %d, h = %d, o = %d, experts = %d, k = %d", who, (long long)n->rows, n->d, n->h, n->o, n->experts, n->k);
+    const int least = 16 / escat_type_bytes(n->type);
+    if (n->d < least || n->h < least || n->o < least) return fail(ESCAT_ERANGE, "%s: d = %d, h = %d, o = %d: rows of at least 16 bytes (%d elements)", who, n->d, n->h, n->o, least);
     if (n->experts > ESCAT_ROUTE_MAX_EXPERTS || n->k > 64 || n->rows > 0x3fffffff / n->k || n->d > 65536 || n->h > 65536 || n->o > 65536)
         return fail(ESCAT_ERANGE, "%s: rows * k = %lld * %d (below 2^30), experts = %d (at most %d), k at most 64, d = %d, h = %d, o = %d (at most 65536)", who,
                     (long long)n->rows, n->k, n->experts, ESCAT_ROUTE_MAX_EXPERTS, n->d, n->h, n->o);

@@ -79,7 +79,7 @@ __global__ void __launch_bounds__(XT, 2) k_expert_grad(const GradArgs g)
     const int rb = g.chunk && ra + g.chunk < end ? ra + g.chunk : end;
 
     const int wave = threadIdx.x >> 6, am = (wave & 1) * 64, bn = (wave >> 1) * 64;
-    const int ma = m0 + SM::chunk() * PER, nb = n0 + SM::chunk() * PER;
+    const ColsKM<T> ca(m0, M), cb(n0, N);
     const bool sums = m0 == 0 && g.db != nullptr;
     int row[4], row_next[4];
     float w[2][4], w_next[4], db[PER];
@@ -88,32 +88,32 @@ __global__ void __launch_bounds__(XT, 2) k_expert_grad(const GradArgs g)
     auto fetch = [&](int k0) {                               // rows (and weights) of step k0, one step ahead of the data
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int s = ra + k0 + SM::row(i);
-            row_next[i] = s < rb ? g.p.row[s] : -1;
-            w_next[i] = W2 && sums && s < rb ? g.weights[s] : 0.f;
+            const int s = ra + k0 + SM::row(i) < rb ? ra + k0 + SM::row(i) : rb - 1;
+            row_next[i] = g.p.row[s];
+            if (W2 && sums) w_next[i] = g.weights[s];
         }
     };
     acc_t acc[2][2];
     clear(acc);
-    fetch(0);
-    tile_loop<T, true, true>(rb - ra, lds, am, bn, acc,
+    if (rb > ra) fetch(0);
+    auto sorted = [&](int k0, int i) { const int s = ra + k0 + SM::row(i); return (int64_t)(s < rb ? s : rb - 1); };
+    const int K = rb - ra;
+    tile_loop<2, T, true, true>(K, lds, am, bn, acc,
         [&](int k0, u4 (&r)[4], int) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) row[i] = row_next[i];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int64_t at = W2 ? (int64_t)(ra + k0 + SM::row(i)) : (int64_t)row[i];
-                r[i] = load16((const T *)g.a + at * M + ma, row[i] >= 0 ? M - ma : 0);
-            } },
+            for (int i = 0; i < 4; ++i) r[i] = ca.load((const T *)g.a + (W2 ? sorted(k0, i) : (int64_t)row[i]) * M); },
         [&](int k0, u4 (&r)[4], int set) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int64_t at = W2 ? (int64_t)row[i] : (int64_t)(ra + k0 + SM::row(i));
-                r[i] = load16((const T *)g.b + at * N + nb, row[i] >= 0 ? N - nb : 0);
-                w[set][i] = w_next[i];
+                r[i] = cb.load((const T *)g.b + (W2 ? (int64_t)row[i] : sorted(k0, i)) * N);
+                if (W2) w[set][i] = w_next[i];
             }
-            fetch(k0 + KB); },
-        [&](const u4 (&r)[4], int set) {
+            if (k0 + KB < K) fetch(k0 + KB); },
+        [&](int k0, u4 (&r)[4], int) { ca.fix(r, K - k0, k0 + KB <= K); },
+        [&](int k0, u4 (&r)[4], int set) {
+            cb.fix(r, K - k0, k0 + KB <= K);
             if (sums) {
                 float f[PER];
 #pragma unroll

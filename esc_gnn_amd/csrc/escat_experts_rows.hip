@@ -30,13 +30,14 @@ template <typename T> __device__ __forceinline__ float sigmoid_of(float u) { ret
 template <typename T, int MODE>
 __global__ void __launch_bounds__(XT, 2) k_expert_rows(const RowArgs a)
 {
-    constexpr int PER = Elem<T>::PER;
+    constexpr int PER = Elem<T>::PER, KB = Elem<T>::KB;
     extern __shared__ __align__(16) char lds[];
     const int D = a.n.d, H = a.n.h, O = a.n.o;
     const int M = MODE == FWD2 ? O : MODE == BWD2 ? D : H;          // features of the result
     const int mt = (M + XN - 1) / XN;
-    const int work = xcd_swizzle(blockIdx.x, gridDim.x), t = work / mt, m0 = (work - t * mt) * XN;
-    if (t >= *a.p.n_tiles) return;
+    const int live = *a.p.n_tiles * mt;                              // (the grid covers the most tiles there can be)
+    if ((int)blockIdx.x >= live) return;
+    const int work = xcd_swizzle(blockIdx.x, live), t = work / mt, m0 = (work - t * mt) * XN;
     const int e = a.p.tile[2 * t], r0 = a.p.tile[2 * t + 1];
     const int rows = a.p.first[e + 1] - r0 < XM ? a.p.first[e + 1] - r0 : XM;
 
@@ -53,6 +54,11 @@ __global__ void __launch_bounds__(XT, 2) k_expert_rows(const RowArgs a)
     float wr[2];                                                    // weights of the two rows whose results the lane holds
 #pragma unroll
     for (int j = 0; j < 2; ++j) { const int r = bn + 32 * j + (lane & 31); wr[j] = MODE == BWD2 ? 1.f : a.weights[a.p.pair[r0 + (r < rows ? r : 0)]]; }
+    __shared__ __align__(16) float bias[XN];
+    if (MODE != BWD2 && threadIdx.x < XN) {
+        const T *b = MODE == FWD2 ? (const T *)a.b2 : (const T *)a.b1;
+        bias[threadIdx.x] = b && m0 + (int)threadIdx.x < M ? to_f32(b[(int64_t)e * M + m0 + threadIdx.x]) : 0.f;
+    }
     acc_t acc[2][2];
     clear(acc);
 
@@ -60,20 +66,16 @@ __global__ void __launch_bounds__(XT, 2) k_expert_rows(const RowArgs a)
     if (MODE != BWD2) {
         const int K = MODE == FWD2 ? H : D;
         const T *A = (const T *)(MODE == FWD2 ? a.w2 : a.w1) + (int64_t)e * M * K, *B = (const T *)(MODE == FWD2 ? a.h : a.x);
-        const T *ap[4], *bp[4];
+        RowsKC<T> la, lb;
+        la.K = lb.K = K; la.c = lb.c = c;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int m = m0 + SC::row(i) < M ? m0 + SC::row(i) : M - 1;
-            ap[i] = A + (int64_t)m * K + c;
-            bp[i] = B + br[i] * K + c;
+            la.p[i] = A + (int64_t)m * K;
+            lb.p[i] = B + br[i] * K;
         }
-        tile_loop<T, false, false>(K, lds, am, bn, acc,
-            [&](int k0, u4 (&r)[4], int) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) r[i] = load16(ap[i] + k0, K - k0 - c); },
-            [&](int k0, u4 (&r)[4], int) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) r[i] = load16(bp[i] + k0, K - k0 - c); });
+        tile_loop<MODE == BWD1 ? 1 : 2, T, false, false>(K, lds, am, bn, acc, [&](int k0, u4 (&r)[4], int) { la.load(k0, r); }, [&](int k0, u4 (&r)[4], int) { lb.load(k0, r); },
+                                   [&](int k0, u4 (&r)[4], int) { la.fix(k0, r); }, [&](int k0, u4 (&r)[4], int) { lb.fix(k0, r); });
     }
     // ---- W2^T dy (BWD1, into a second set), W1^T du (BWD2): weights with the result's features contiguous
     acc_t acc2[2][2];
@@ -82,26 +84,26 @@ __global__ void __launch_bounds__(XT, 2) k_expert_rows(const RowArgs a)
         const int K = MODE == BWD1 ? O : H;
         const T *A = (const T *)(MODE == BWD1 ? a.w2 : a.w1) + (int64_t)e * K * M, *B = (const T *)(MODE == BWD1 ? a.dy : a.du);
         typedef Stage<T, true> SM;
-        const int mc = m0 + SM::chunk() * PER;
-        const T *bp[4];
+        const ColsKM<T> cols_a(m0, M);
+        RowsKC<T> lb;
+        lb.K = K; lb.c = c;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) bp[i] = B + br[i] * K + c;
-        int kd = 0;
+        for (int i = 0; i < 4; ++i) lb.p[i] = B + br[i] * K;
         const bool with_dot = MODE == BWD1 && m0 == 0 && a.b2 != nullptr;
-        const T *b2 = MODE == BWD1 ? (const T *)a.b2 + (int64_t)e * O + c : nullptr;
+        const T *b2 = MODE == BWD1 ? (const T *)a.b2 + (int64_t)e * O : nullptr;
         if (MODE == BWD1) clear(acc2);
-        tile_loop<T, true, false>(K, lds, am, bn, MODE == BWD1 ? acc2 : acc,
+        tile_loop<MODE == BWD1 ? 1 : 2, T, true, false>(K, lds, am, bn, MODE == BWD1 ? acc2 : acc,
             [&](int k0, u4 (&r)[4], int) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) { const int kk = k0 + SM::row(i); r[i] = load16(A + (int64_t)kk * M + mc, kk < K ? M - mc : 0); } },
+                for (int i = 0; i < 4; ++i) { const int kk = k0 + SM::row(i); r[i] = cols_a.load(A + (int64_t)(kk < K ? kk : K - 1) * M); } },
+            [&](int k0, u4 (&r)[4], int) { lb.load(k0, r); },
+            [&](int k0, u4 (&r)[4], int) { cols_a.fix(r, K - k0, k0 + KB <= K); },
             [&](int k0, u4 (&r)[4], int) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) r[i] = load16(bp[i] + k0, K - k0 - c); },
-            [&](const u4 (&r)[4], int) {
+                lb.fix(k0, r);
                 if (with_dot) {
                     float f[PER], g[PER];
-                    to_floats<T>(load16(b2 + kd, K - kd - c), f);
-                    kd += Elem<T>::KB;
+#pragma unroll
+                    for (int q = 0; q < PER; ++q) f[q] = to_f32(b2[k0 + c + q < K ? k0 + c + q : K - 1]);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         to_floats<T>(r[i], g);
@@ -113,7 +115,6 @@ __global__ void __launch_bounds__(XT, 2) k_expert_rows(const RowArgs a)
 
     // ---- epilogue.  The lane holds, for each of two rows, runs of four features; they leave through LDS
     typedef typename std::conditional<MODE == FWD1 || MODE == BWD1, T, float>::type OUT;
-    const T *bias = MODE == FWD2 ? (const T *)a.b2 : (const T *)a.b1;
     const int cols = M - m0 < XN ? M - m0 : XN;
     __shared__ float red[3 * 128];                                  // BWD1: sums over the features of a half, b2 . dy
     if (MODE == BWD1) {
@@ -135,11 +136,13 @@ __global__ void __launch_bounds__(XT, 2) k_expert_rows(const RowArgs a)
             for (int q = 0; q < 4; ++q) {
                 const int mt_ = am + 32 * i + 8 * q + 4 * (lane >> 5), m = m0 + mt_;
                 float u[4], g[4];
+                f4 bv = {0.f, 0.f, 0.f, 0.f};
+                if (MODE != BWD2) bv = *(const f4 *)(bias + mt_);
 #pragma unroll
                 for (int z = 0; z < 4; ++z) {
                     u[z] = acc[i][j][4 * q + z];
                     if (MODE == BWD1) g[z] = acc2[i][j][4 * q + z];
-                    if (MODE != BWD2 && bias && m + z < M) u[z] += (MODE == FWD2 ? w : 1.f) * to_f32(bias[(int64_t)e * M + m + z]);
+                    if (MODE != BWD2) u[z] += MODE == FWD2 ? w * bv[z] : bv[z];
                 }
                 if (MODE == FWD1) {
 #pragma unroll

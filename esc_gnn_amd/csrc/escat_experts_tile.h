@@ -36,19 +36,20 @@ template <> struct Elem<f16_t> { static constexpr int PER = 8, KB = 64; };
 typedef unsigned u4 __attribute__((ext_vector_type(4)));
 template <typename T> struct Vec { T v[Elem<T>::PER]; };
 
-// 16 bytes at p of which the first `left` elements exist; zero behind them
-template <typename T> __device__ __forceinline__ u4 load16(const T *p, int left)
+// Pieces at the ragged end of a row: 16 bytes are loaded so that they end with the row (one unguarded load whatever the row's length; the entry points see to it that
+// it has 16 bytes) and, once they have arrived, moved down by the s elements that the piece begins behind where it was loaded, zeros behind.
+template <typename T> __device__ __forceinline__ u4 load16(const T *p)
 {
-    constexpr int PER = Elem<T>::PER;
-    u4 r = {0, 0, 0, 0};
-    if (left >= PER) { const Pack<T, PER> q = *(const Pack<T, PER> *)p; __builtin_memcpy(&r, &q, 16); }
-    else if (left > 0) {
-        Vec<T> q;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) q.v[i] = i < left ? p[i] : (T)0.f;
-        __builtin_memcpy(&r, &q, 16);
-    }
+    const Pack<T, Elem<T>::PER> q = *(const Pack<T, Elem<T>::PER> *)p;
+    u4 r; __builtin_memcpy(&r, &q, 16);
     return r;
+}
+template <typename T> __device__ __forceinline__ u4 moved(u4 v, int s)
+{
+    unsigned __int128 x; __builtin_memcpy(&x, &v, 16);
+    x = s >= Elem<T>::PER ? 0 : x >> (s * 8 * (int)sizeof(T));
+    __builtin_memcpy(&v, &x, 16);
+    return v;
 }
 template <typename T> __device__ __forceinline__ void to_floats(u4 r, float (&f)[Elem<T>::PER])
 {
@@ -146,35 +147,120 @@ __device__ __forceinline__ void tile_step(const char *la, const char *lb, int am
     }
 }
 
-// ---- the loop over k.  loadA / loadB(k0, regs, set): the thread's pieces of step k0, two steps ahead of their use (a step's products
-// take less time than memory does); set = step & 1; seenB(regs, set): the B pieces once they have arrived (a use inside loadB would wait for
-// them there).  lds: 4 tiles (A0 B0 A1 B1), free to be written on return.
-struct Unseen { __device__ void operator()(const u4 (&)[4], int) const {} };
-template <typename T, bool AKM, bool BKM, typename FA, typename FB, typename FS = Unseen>
-__device__ __forceinline__ void tile_loop(int K, char *lds, int am, int bn, acc_t (&acc)[2][2], FA loadA, FB loadB, FS seenB = FS())
+// ---- the loop over k.  loadA / loadB(k0, regs, set): the thread's pieces of step k0, AHEAD = 1 or 2 steps ahead of their use (a step's
+// products take less time than memory does; 1 where two sets of accumulators leave no registers for 2); set = step & 1, or 0; fixA / fixB(k0, regs, set): the same pieces once they have arrived (a use inside load
+// would wait for them there).  lds: 4 tiles (A0 B0 A1 B1), free to be written on return.
+template <int AHEAD, typename T, bool AKM, bool BKM, typename FA, typename FB, typename XA, typename XB>
+__device__ __forceinline__ void tile_loop(int K, char *lds, int am, int bn, acc_t (&acc)[2][2], FA loadA, FB loadB, XA fixA, XB fixB)
 {
     constexpr int KB = Elem<T>::KB;
     const int steps = (K + KB - 1) / KB;
     if (steps == 0) return;
-    u4 ra[2][4], rb[2][4];
-    loadA(0, ra[0], 0); loadB(0, rb[0], 0);
-    if (steps > 1) { loadA(KB, ra[1], 1); loadB(KB, rb[1], 1); }
-    seenB(rb[0], 0);
-    Stage<T, AKM>::store(lds, ra[0]); Stage<T, BKM>::store(lds + TILE_BYTES, rb[0]);
-    __syncthreads();
-    for (int s0 = 0; s0 < steps; s0 += 2) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int s = s0 + h;
-            if (s >= steps) break;
-            char *cur = lds + h * 2 * TILE_BYTES, *nxt = lds + (1 - h) * 2 * TILE_BYTES;
-            if (s + 2 < steps) { loadA((s + 2) * KB, ra[h], h); loadB((s + 2) * KB, rb[h], h); }
-            tile_step<T, AKM, BKM>(cur, cur + TILE_BYTES, am, bn, acc);
-            if (s + 1 < steps) { seenB(rb[1 - h], 1 - h); Stage<T, AKM>::store(nxt, ra[1 - h]); Stage<T, BKM>::store(nxt + TILE_BYTES, rb[1 - h]); }
-            __syncthreads();
+    char *buf0 = lds, *buf1 = lds + 2 * TILE_BYTES;
+    u4 a0[4], b0[4], a1[4], b1[4];
+    // no load under a condition inside the loop: it would make the compiler wait for all of them at every turn
+#define LOAD(s, S) { loadA((s) * KB, a##S, S); loadB((s) * KB, b##S, S); }
+#define STORE(s, S) { fixA((s) * KB, a##S, S); fixB((s) * KB, b##S, S); Stage<T, AKM>::store(buf##S, a##S); Stage<T, BKM>::store(buf##S + TILE_BYTES, b##S); __syncthreads(); }
+#define MULTIPLY(S) tile_step<T, AKM, BKM>(buf##S, buf##S + TILE_BYTES, am, bn, acc);
+    LOAD(0, 0)
+    if constexpr (AHEAD == 1) {
+#define STORE1(s, B) { fixA((s) * KB, a0, 0); fixB((s) * KB, b0, 0); Stage<T, AKM>::store(buf##B, a0); Stage<T, BKM>::store(buf##B + TILE_BYTES, b0); __syncthreads(); }
+        STORE1(0, 0)
+        int s = 0;
+        for (; s + 2 < steps; s += 2) {
+            LOAD(s + 1, 0)
+            MULTIPLY(0)
+            STORE1(s + 1, 1)
+            LOAD(s + 2, 0)
+            MULTIPLY(1)
+            STORE1(s + 2, 0)
+        }
+        if (s + 2 == steps) {
+            LOAD(s + 1, 0)
+            MULTIPLY(0)
+            STORE1(s + 1, 1)
+            MULTIPLY(1)
+        } else MULTIPLY(0)
+#undef STORE1
+    } else if (steps == 1) {
+        STORE(0, 0)
+        MULTIPLY(0)
+    } else {
+        LOAD(1, 1)
+        STORE(0, 0)
+        int s = 0;
+        for (; s + 3 < steps; s += 2) {
+            LOAD(s + 2, 0)
+            MULTIPLY(0)
+            STORE(s + 1, 1)
+            LOAD(s + 3, 1)
+            MULTIPLY(1)
+            STORE(s + 2, 0)
+        }
+        if (s + 3 == steps) {
+            LOAD(s + 2, 0)
+            MULTIPLY(0)
+            STORE(s + 1, 1)
+            MULTIPLY(1)
+            STORE(s + 2, 0)
+            MULTIPLY(0)
+        } else {
+            MULTIPLY(0)
+            STORE(s + 1, 1)
+            MULTIPLY(1)
         }
     }
+    __syncthreads();
+#undef LOAD
+#undef STORE
+#undef MULTIPLY
 }
+
+// loads of an operand with k contiguous: four rows, p[i] their first elements
+template <typename T> struct RowsKC {
+    const T *p[4];
+    int K, c;
+    __device__ __forceinline__ void load(int k0, u4 (&r)[4]) const
+    {
+        constexpr int PER = Elem<T>::PER;
+        const int at = k0 + c < K - PER ? k0 + c : K - PER;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = load16(p[i] + at);
+    }
+    __device__ __forceinline__ void fix(int k0, u4 (&r)[4]) const
+    {
+        constexpr int PER = Elem<T>::PER;
+        if (k0 + Elem<T>::KB <= K) return;
+        const int s = k0 + c > K - PER ? k0 + c - (K - PER) : 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = moved<T>(r[i], s);
+    }
+};
+// where the thread's pieces of a row of M features begin (KM), and how far they are to be moved
+template <typename T> struct ColsKM {
+    int at, s;
+    bool ragged;                                        // the tile has a piece that ends behind the row
+    __device__ __forceinline__ ColsKM(int m0, int M)
+    {
+        constexpr int PER = Elem<T>::PER;
+        const int m = m0 + Stage<T, true>::chunk() * PER;
+        at = m < M - PER ? m : M - PER;
+        s = m - at;
+        ragged = m0 + 128 > M;
+    }
+    __device__ __forceinline__ u4 load(const T *row) const { return load16(row + at); }
+    __device__ __forceinline__ void fix(u4 (&r)[4], int live, bool whole) const          // live: rows of the step that exist
+    {
+        if (ragged) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) r[i] = moved<T>(r[i], s);
+        }
+        if (!whole) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) if (Stage<T, true>::row(i) >= live) r[i] = u4{0, 0, 0, 0};
+        }
+    }
+};
 
 // ---- results through LDS, so that memory is written in whole rows of the tile.  put: the lane's run of four features m.. of row n
 // (tile coordinates); write: rows [0, rows), features [0, cols) to out + n * ld.  OUT: element type.  A row of 128 OUT is OSTRIDE bytes apart

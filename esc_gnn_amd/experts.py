@@ -14,6 +14,7 @@ import math
 from typing import Optional, Tuple
 import torch
 from torch.autograd.function import once_differentiable
+from torch.nn.functional import pad
 
 from . import _lib
 from .optim import DTYPE_CODES, _on
@@ -201,4 +202,11 @@ def expert_mlp(x: torch.Tensor, weights: torch.Tensor, experts: torch.Tensor, w1
         if t is not None and t.device != x.device:
             raise RuntimeError(f"escat: {name} lives on {t.device}, x on {x.device}")
     _need_gpu(x, "x")
-    return _ExpertMLP.apply(x.contiguous(), weights.contiguous(), experts.contiguous(), w1, b1, w2, b2)
+    least = 4 if x.dtype is torch.float32 else 8            # the kernels move 16 bytes of a row at once: narrower ones get zeros
+    if min(d, h, o) < least:
+        more = lambda n: max(0, least - n)                                                       # noqa: E731
+        x = pad(x, (0, more(d)))
+        w1, w2 = pad(w1, (0, more(d), 0, more(h))), pad(w2, (0, more(h), 0, more(o)))
+        b1, b2 = None if b1 is None else pad(b1, (0, more(h))), None if b2 is None else pad(b2, (0, more(o)))
+    y = _ExpertMLP.apply(x.contiguous(), weights.contiguous(), experts.contiguous(), w1, b1, w2, b2)
+    return y if o >= least else y[:, :o].contiguous()

@@ -581,6 +581,7 @@ int escat_route_bwd(const void *logits, int type, int64_t rows, int E, int k, in
  * outside [0, experts) count for nothing.
  *   x (rows, d), w1 (experts, h, d), b1 (experts, h) or NULL, w2 (experts, o, h), b2 (experts, o) or NULL, y (rows, o), all of `type`;
  *   weights (rows, k) fp32.
+ * Rows have at least 16 bytes: d, h and o >= 4 (fp32) or 8 (pad narrower ones with zeros).
  * escat_experts_plan sorts the rows * k pairs by expert into `plan` (escat_experts_plan_bytes), on the GPU, nothing read back;
  * counts (experts) int32, optional: pairs of each expert.  escat_experts_fwd / _bwd read a plan of the same experts array.
  * escat_experts_bwd: gradients for dy (rows, o); dx, dweights, dw1 + db1, dw2 + db2 may each be NULL (a bias's gradient only

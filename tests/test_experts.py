@@ -100,6 +100,7 @@ def test_experts_library_checks_its_arguments():
         assert lib.escat_experts_fwd(dims(*bad), *[0] * 9, 0, 0) == -1
     assert lib.escat_experts_fwd(dims(1 << 30, 0, 8, 8, 8, 2, 1), *[0] * 9, 0, 0) == -2
     assert lib.escat_experts_fwd(dims(4, 0, 8, 8, 8, 2000, 1), *[0] * 9, 0, 0) == -2
+    assert lib.escat_experts_fwd(dims(4, 1, 8, 4, 8, 2, 1), *[0] * 9, 0, 0) == -2                # bf16 rows of 8 bytes
     assert lib.escat_experts_fwd(dims(*good), *[0] * 9, 0, 0) == -1                              # null pointers
     assert lib.escat_experts_fwd(dims(*good), *[16] * 8, 16, 64, 0) == -3                        # small workspace
     assert lib.escat_experts_fwd(dims(0, 0, 8, 8, 8, 2, 1), *[0] * 9, 0, 0) == 0                 # no rows
