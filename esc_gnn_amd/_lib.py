@@ -92,7 +92,7 @@ SIGNATURES = {
     "escat_state8_values": (ci, [vp, vp, i64, ci, vp, vp]),
     "escat_route": (ci, [vp, ci, i64, ci, ci, ci, vp, ci, ci, ci, ci, ctypes.c_float, vp, vp, vp]),
     "escat_route_bwd": (ci, [vp, ci, i64, ci, ci, ci, ci, ctypes.c_float, vp, vp, vp, vp, vp]),
-    "escat_experts_plan_bytes": (sz, [i64, ci]),
+    "escat_experts_plan_bytes": (sz, [i64, ci, ci]),
     "escat_experts_plan": (ci, [vp, i64, ci, ci, vp, sz, vp, vp]),
     "escat_experts_workspace_bytes": (sz, [vp, ci]),
     "escat_experts_fwd": (ci, [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]),

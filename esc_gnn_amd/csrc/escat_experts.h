@@ -4,35 +4,70 @@
 #include "escat_dev.h"
 #include "escat_half.h"
 
-// Pairs = (row, slot) with a routed expert, sorted by expert, stable.  Of the plan (device memory, int32):
-struct EPlan {
-    int *count;       // E      pairs of each expert
-    int *first;       // E + 1  its first sorted position; first[E] = routed pairs
-    int *n_tiles;     // 1      tiles of XM sorted positions, none across two experts
-    int *tile;        // 2 x max_tiles: expert, first position
-    int *pair;        // P      sorted position -> pair
-    int *pos;         // P      pair -> sorted position, -1 = not routed
-    int *row;         // P      sorted position -> row of the activations (pair / k)
-    int *hist;        // E x blocks: scratch of the sort
-};
-#define XM 128                                    // sorted positions of a tile (rows of activations)
-#define XN 128                                    // features of a tile
-#define PLAN_CHUNK 2048                           // pairs of a workgroup of the sort
-
+// How rows meet experts.  A tile is 128 items that share a key, and the products of a tile go to `per` experts, the digits of its key:
+//
+//   by pair         items = (row, slot) pairs, key = the pair's expert, per = 1: each pair's result is kept in fp32 and the k of a row are
+//                   added by a pass of their own.
+//   by combination  items = rows, key = the sorted k experts of a row as digits to the base E + 1 (E: routed nowhere), per = k: the k products
+//                   of a tile's rows end in the same accumulators, and results are written once, in their own type.
+//
+// By combination moves less memory (524288 rows x 256, k = 2: no 2.1 GB of fp32 results written and read again, 0.5 ms of 3.5) but
+// cuts the rows into E^k / k! groups and pads each to whole tiles: taken with 512 rows or more to a group (4 tiles: 12 % padding; at 128
+// the padding costs what it saves) and at most 1024 keys; k = 1 is always its case, the two are the same there.
 struct EDims { int64_t rows; int d, h, o, E, k; };
-
-static inline int64_t plan_blocks(int64_t P) { return (P + PLAN_CHUNK - 1) / PLAN_CHUNK; }
-static inline int64_t plan_max_tiles(int64_t P, int E) { return P / XM + (E < P ? E : P) + 1; }
-static inline int64_t plan_ints(int64_t P, int E)
+static inline int combo_keys(int64_t rows, int E, int k)        // number of keys by combination, 0 = by pair
 {
-    return (int64_t)E + (E + 1) + 1 + 2 * plan_max_tiles(P, E) + 3 * P + E * plan_blocks(P) + 64;
+    int64_t keys = 1, groups = 1;
+    for (int j = 0; j < k; ++j) { keys *= E + 1; if (keys > 1025) return 0; }
+    if (k == 1) return (int)keys;
+    if (keys > 1024) return 0;
+    for (int j = 0; j < k; ++j) groups = groups * (E + j) / (j + 1);         // multisets of k experts
+    return rows >= 512 * groups ? (int)keys : 0;
 }
-static inline EPlan plan_view(void *mem, int64_t P, int E)
+
+// A position is item * per + digit; of the plan (device memory, int32):
+struct EPlan {
+    int per, base;    // base: E + 1 by combination, 0 by pair (the key is the expert)
+    int keys;
+    int *count;       // keys      items of each key
+    int *first;       // keys + 1  its first item in sorted order; first[keys] = all items
+    int *n_tiles;     // 1         tiles of XM items, none across two keys
+    int *tile;        // 2 x max_tiles: key, first item
+    int *pair;        // P         position -> pair
+    int *row;         // P         position -> row of the activations
+    int *expert;      // P         position -> expert, -1 = none
+    int *pos;         // P         pair -> position, -1 = not routed
+    int *hist;        // keys x blocks: scratch of the sort
+};
+#define XM 128                                    // items of a tile (rows of activations)
+#define XN 128                                    // features of a tile
+#define PLAN_CHUNK 2048                           // items of a workgroup of the sort
+
+static inline int64_t plan_items(int64_t rows, int k, int combo) { return combo ? rows : rows * k; }
+static inline int64_t plan_blocks(int64_t items) { return (items + PLAN_CHUNK - 1) / PLAN_CHUNK; }
+static inline int64_t plan_max_tiles(int64_t items, int keys) { return items / XM + (keys < items ? keys : items) + 1; }
+static inline int plan_keys(int64_t rows, int k, int E) { const int c = combo_keys(rows, E, k); return c ? c : E; }
+static inline EPlan plan_view(void *mem, int64_t rows, int k, int E, int combo, int64_t *ints)
 {
     EPlan p; int *q = (int *)mem;
-    p.count = q; q += E; p.first = q; q += E + 1; p.n_tiles = q; q += 1; p.tile = q; q += 2 * plan_max_tiles(P, E);
-    p.pair = q; q += P; p.pos = q; q += P; p.row = q; q += P; p.hist = q;
+    const int64_t items = plan_items(rows, k, combo), P = rows * k;
+    p.per = combo ? k : 1; p.base = combo ? E + 1 : 0; p.keys = combo ? combo : E;
+    p.count = q; q += p.keys; p.first = q; q += p.keys + 1; p.n_tiles = q; q += 1; p.tile = q; q += 2 * plan_max_tiles(items, p.keys);
+    p.pair = q; q += P; p.row = q; q += P; p.expert = q; q += P; p.pos = q; q += P;
+    p.hist = q; q += p.keys * plan_blocks(items);
+    if (ints) *ints = q - (int *)mem;
     return p;
+}
+// the plan of a routing, as escat_experts_plan lays it out
+static inline EPlan plan_of(void *mem, int64_t rows, int k, int E) { return plan_view(mem, rows, k, E, combo_keys(rows, E, k), nullptr); }
+static inline int64_t plan_ints(int64_t rows, int k, int E) { int64_t n; plan_view(nullptr, rows, k, E, combo_keys(rows, E, k), &n); return n; }
+
+// expert of digit j of a key; E (base - 1): none
+__device__ __forceinline__ int key_digit(const EPlan &p, int key, int j)
+{
+    if (p.base == 0) return key;
+    for (int i = p.per - 1; i > j; --i) key /= p.base;
+    return key % p.base;
 }
 
 // workgroups of a launch go round the eight XCDs one by one, each with its own L2: give each XCD a run of neighbouring work items

@@ -10,9 +10,10 @@
 
 struct GradArgs {
     EDims n;
-    EPlan p;
-    const void *a, *b;         // A: (w h) sorted, or x by row; B: dy by row, or du sorted
-    const float *weights;      // sorted: db2's
+    EPlan p;                   // by pair: items in the order of the sums
+    const int *at;             // position of an item's hidden row; NULL: the item itself
+    const void *a, *b;         // A: (w h) by position, or x by row; B: dy by row, or du by position
+    const float *weights;      // by position: db2's
     void *out, *db;            // (E, N, M), (E, N) of the operands' type
     float *part;               // chunked: [chunk][N * M + N]
     int M, N;                  // A's and B's features
@@ -79,56 +80,73 @@ __global__ void __launch_bounds__(XT, 2) k_expert_grad(const GradArgs g)
     const int rb = g.chunk && ra + g.chunk < end ? ra + g.chunk : end;
 
     const int wave = threadIdx.x >> 6, am = (wave & 1) * 64, bn = (wave >> 1) * 64;
-    const ColsKM<T> ca(m0, M), cb(n0, N);
     const bool sums = m0 == 0 && g.db != nullptr;
-    int row[4], row_next[4];
-    float w[2][4], w_next[4], db[PER];
-#pragma unroll
-    for (int i = 0; i < PER; ++i) db[i] = 0.f;
-    auto fetch = [&](int k0) {                               // rows (and weights) of step k0, one step ahead of the data
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int s = ra + k0 + SM::row(i) < rb ? ra + k0 + SM::row(i) : rb - 1;
-            row_next[i] = g.p.row[s];
-            if (W2 && sums) w_next[i] = g.weights[s];
-        }
-    };
-    acc_t acc[2][2];
-    clear(acc);
-    if (rb > ra) fetch(0);
-    auto sorted = [&](int k0, int i) { const int s = ra + k0 + SM::row(i); return (int64_t)(s < rb ? s : rb - 1); };
     const int K = rb - ra;
-    tile_loop<2, T, true, true>(K, lds, am, bn, acc,
-        [&](int k0, u4 (&r)[4], int) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) row[i] = row_next[i];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) r[i] = ca.load((const T *)g.a + (W2 ? sorted(k0, i) : (int64_t)row[i]) * M); },
-        [&](int k0, u4 (&r)[4], int set) {
+    // the two operands and the items' rows and positions, which are fetched a step ahead of the data
+    struct Items {
+        const GradArgs &g;
+        int ra, rb, k0;
+        int row[4], pos[4], row_next[4], pos_next[4];
+        __device__ __forceinline__ void fetch()
+        {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                r[i] = cb.load((const T *)g.b + (W2 ? (int64_t)row[i] : sorted(k0, i)) * N);
-                if (W2) w[set][i] = w_next[i];
+                const int s = ra + k0 + SM::row(i) < rb ? ra + k0 + SM::row(i) : rb - 1;
+                row_next[i] = g.p.row[s];
+                pos_next[i] = g.at ? g.at[s] : s;
             }
-            if (k0 + KB < K) fetch(k0 + KB); },
-        [&](int k0, u4 (&r)[4], int) { ca.fix(r, K - k0, k0 + KB <= K); },
-        [&](int k0, u4 (&r)[4], int set) {
-            cb.fix(r, K - k0, k0 + KB <= K);
-            if (sums) {
-                float f[PER];
+            k0 += KB;
+        }
+    } it{g, ra, rb, 0};
+    struct OpA {
+        Items &it; const GradArgs &g; ColsKM<T> cols; int K, fk0;
+        __device__ __forceinline__ void load(u4 (&r)[4], int)
+        {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    to_floats<T>(r[i], f);
+            for (int i = 0; i < 4; ++i) { it.row[i] = it.row_next[i]; it.pos[i] = it.pos_next[i]; }
 #pragma unroll
-                    for (int z = 0; z < PER; ++z) db[z] = W2 ? fmaf(w[set][i], f[z], db[z]) : db[z] + f[z];
-                }
-            } });
+            for (int i = 0; i < 4; ++i) r[i] = load16((const T *)g.a + (int64_t)(W2 ? it.pos[i] : it.row[i]) * g.M + cols.at);
+        }
+        __device__ __forceinline__ void fix(u4 (&r)[4], int) { cols.fix(r, K - fk0, fk0 + KB <= K); fk0 += KB; }
+    } A{it, g, ColsKM<T>(m0, M), K, 0};
+    struct OpB {
+        Items &it; const GradArgs &g; ColsKM<T> cols; int K, fk0; bool sums;
+        float w[2][4], db[PER];
+        __device__ __forceinline__ void load(u4 (&r)[4], int set)
+        {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                r[i] = load16((const T *)g.b + (int64_t)(W2 ? it.row[i] : it.pos[i]) * g.N + cols.at);
+                if (W2) w[set][i] = g.weights[it.pos[i]];
+            }
+            it.fetch();
+        }
+        __device__ __forceinline__ void fix(u4 (&r)[4], int set)
+        {
+            cols.fix(r, K - fk0, fk0 + KB <= K);
+            fk0 += KB;
+            if (!sums) return;
+            float f[PER];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                to_floats<T>(r[i], f);
+#pragma unroll
+                for (int z = 0; z < PER; ++z) db[z] = W2 ? fmaf(w[set][i], f[z], db[z]) : db[z] + f[z];
+            }
+        }
+    } B{it, g, ColsKM<T>(n0, N), K, 0, sums};
+#pragma unroll
+    for (int i = 0; i < PER; ++i) B.db[i] = 0.f;
+    acc_t acc[2][2];
+    clear(acc);
+    if (K > 0) it.fetch();
+    tile_loop<2, T, true, true>((K + KB - 1) / KB, lds, am, bn, acc, A, B);
 
     float *part = g.chunk ? g.part + (int64_t)q * ((int64_t)N * M + N) : nullptr;
     if (sums) {                                               // the threads that hold the same features join in a fixed order
         float *red = (float *)lds;
 #pragma unroll
-        for (int z = 0; z < PER; ++z) red[threadIdx.x * PER + z] = db[z];
+        for (int z = 0; z < PER; ++z) red[threadIdx.x * PER + z] = B.db[z];
         __syncthreads();
         if (threadIdx.x < 128 && n0 + (int)threadIdx.x < N) {
             float v = 0.f;
@@ -142,10 +160,10 @@ __global__ void __launch_bounds__(XT, 2) k_expert_grad(const GradArgs g)
     const int cols = M - m0 < XN ? M - m0 : XN, rows = N - n0 < XN ? N - n0 : XN;
     if (part) {
         spill<float>(lds, acc, am, bn);
-        Spill<float>::write(lds, part + (int64_t)n0 * M + m0, M, rows, cols);
+        Spill<float>::write(lds, part + (int64_t)n0 * M + m0, M, rows, cols, [](int r) { return r; });
     } else {
         spill<T>(lds, acc, am, bn);
-        Spill<T>::write(lds, (T *)g.out + ((int64_t)e * N + n0) * M + m0, M, rows, cols);
+        Spill<T>::write(lds, (T *)g.out + ((int64_t)e * N + n0) * M + m0, M, rows, cols, [](int r) { return r; });
     }
 }
 
@@ -220,10 +238,10 @@ template <typename T, bool W2> static int launch(const GradArgs &g, hipStream_t 
     return ESCAT_OK;
 }
 
-int escat_experts_grad(int type, const EDims &n, const EPlan &p, bool w2, const void *a, const void *b, const float *weights, int M, int N,
+int escat_experts_grad(int type, const EDims &n, const EPlan &p, const int *at, bool w2, const void *a, const void *b, const float *weights, int M, int N,
                        int chunk, float *part, void *out, void *db, hipStream_t st)
 {
-    const GradArgs g = {n, p, a, b, weights, out, db, part, M, N, chunk};
+    const GradArgs g = {n, p, at, a, b, weights, out, db, part, M, N, chunk};
     if (w2) return type == ESCAT_F32 ? launch<float, true>(g, st) : type == ESCAT_BF16 ? launch<bf16_t, true>(g, st) : launch<f16_t, true>(g, st);
     return type == ESCAT_F32 ? launch<float, false>(g, st) : type == ESCAT_BF16 ? launch<bf16_t, false>(g, st) : launch<f16_t, false>(g, st);
 }

@@ -1,17 +1,42 @@
-// escat_experts_plan.hip -- sorts the (row, slot) pairs of a routing by expert: what every product of the experts goes by.
+// escat_experts_plan.hip -- sorts the rows or (row, slot) pairs of a routing by expert (escat_experts.h): what every product of the experts
+// goes by.
 //
 // A stable counting sort without atomics on memory, so that the order of the sums over an expert's rows is the same every
-// time: a histogram per chunk of 2048 pairs, one workgroup that scans experts x chunks, a second pass over the pairs that ranks them (a wave
-// ranks 64 pairs at once: lanes with the same expert find each other by one ballot per bit of the expert's number).
+// time: a histogram per chunk of 2048 items, one workgroup that scans keys x chunks, a second pass over the items that ranks them (a wave
+// ranks 64 items at once: lanes with the same key find each other by one ballot per bit of the key).
 #include "escat_experts.h"
 
 #define PT 256
 #define PW (PT / 64)
 
-__device__ __forceinline__ int expert_of(const int *experts, int64_t i, int64_t P, int E)
+// what is sorted: `n` items.  base = 0: item i has key experts[i] (one in [0, keys), else left out).  Else item i is a row of k experts.
+struct Items { const int *experts; const int *rows; int64_t n; int k, base, keys; };
+
+__device__ __forceinline__ int valid(int e, int E) { return e >= 0 && e < E ? e : E; }
+
+// digit that entry i of a row's experts becomes: its rank among them
+__device__ __forceinline__ int rank_of(const int *ex, int i, int k, int E)
 {
-    const int e = i < P ? experts[i] : -1;
-    return e >= 0 && e < E ? e : -1;
+    const int e = valid(ex[i], E);
+    int r = 0;
+    for (int j = 0; j < k; ++j) { const int o = valid(ex[j], E); r += o < e || (o == e && j < i); }
+    return r;
+}
+
+__device__ __forceinline__ int key_of(const Items &it, int64_t i)
+{
+    if (i >= it.n) return -1;
+    if (it.base == 0) { const int e = it.experts[i]; return e >= 0 && e < it.keys ? e : -1; }
+    const int E = it.base - 1;
+    const int *ex = it.experts + i * it.k;
+    if (it.k == 1) return valid(ex[0], E);
+    int key = 0;
+    for (int j = 0; j < it.k; ++j) {
+        int v = valid(ex[j], E);
+        for (int q = it.k - 1 - rank_of(ex, j, it.k, E); q > 0; --q) v *= it.base;
+        key += v;
+    }
+    return key;
 }
 
 // lanes of the wave that hold the same e (e >= 0); `bits` = bits of E - 1
@@ -26,25 +51,27 @@ __device__ __forceinline__ uint64_t same_lanes(int e, int bits)
     return m & __ballot(e >= 0);
 }
 
-// counts of the chunk's waves in LDS: cnt[wave][E]
-__device__ __forceinline__ void wave_counts(const int *experts, int64_t c0, int64_t P, int E, int bits, int *cnt)
+// counts of the chunk's waves in LDS: cnt[wave][key]
+__device__ __forceinline__ void wave_counts(const Items &it, int64_t c0, int bits, int *cnt)
 {
+    const int E = it.keys;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     for (int i = threadIdx.x; i < PW * E; i += PT) cnt[i] = 0;
     __syncthreads();
     for (int s = 0; s < PLAN_CHUNK / PT; ++s) {
         const int64_t i = c0 + wave * (PLAN_CHUNK / PW) + s * 64 + lane;
-        const int e = expert_of(experts, i, P, E);
+        const int e = key_of(it, i);
         const uint64_t m = same_lanes(e, bits);
         if (e >= 0 && (m & ((1ull << lane) - 1)) == 0) cnt[wave * E + e] += __popcll(m);
     }
     __syncthreads();
 }
 
-__global__ void __launch_bounds__(PT) k_plan_hist(const int *__restrict__ experts, int64_t P, int E, int bits, int *__restrict__ hist)
+__global__ void __launch_bounds__(PT) k_plan_hist(const Items it, int bits, int *__restrict__ hist)
 {
+    const int E = it.keys;
     extern __shared__ int cnt[];
-    wave_counts(experts, (int64_t)blockIdx.x * PLAN_CHUNK, P, E, bits, cnt);
+    wave_counts(it, (int64_t)blockIdx.x * PLAN_CHUNK, bits, cnt);
     for (int e = threadIdx.x; e < E; e += PT) {
         int s = 0;
 #pragma unroll
@@ -64,7 +91,7 @@ __device__ __forceinline__ int wave_scan_incl(int v)
 // one workgroup of 1024: hist becomes each chunk's first position within its expert; counts, first positions, tiles
 __global__ void __launch_bounds__(1024) k_plan_scan(int E, int blocks, EPlan p)
 {
-    __shared__ int cnt[1024], first[1025], tfirst[1025];
+    __shared__ int cnt[1025], first[1026], tfirst[1026];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     for (int e = wave; e < E; e += 16) {
         int *h = p.hist + (int64_t)e * blocks;
@@ -95,12 +122,13 @@ __global__ void __launch_bounds__(1024) k_plan_scan(int E, int blocks, EPlan p)
         for (int t = tfirst[e] + lane; t < tfirst[e + 1]; t += 64) { p.tile[2 * t] = e; p.tile[2 * t + 1] = first[e] + (t - tfirst[e]) * XM; }
 }
 
-__global__ void __launch_bounds__(PT) k_plan_place(const int *__restrict__ experts, int64_t P, int k, int E, int bits, EPlan p)
+__global__ void __launch_bounds__(PT) k_plan_place(const Items it, int bits, EPlan p)
 {
+    const int E = it.keys;
     extern __shared__ int cnt[];
     const int64_t c0 = (int64_t)blockIdx.x * PLAN_CHUNK;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    wave_counts(experts, c0, P, E, bits, cnt);
+    wave_counts(it, c0, bits, cnt);
     for (int e = threadIdx.x; e < E; e += PT) {               // counts -> the next position of each wave
         int s = p.first[e] + p.hist[(int64_t)e * gridDim.x + blockIdx.x];
 #pragma unroll
@@ -109,14 +137,26 @@ __global__ void __launch_bounds__(PT) k_plan_place(const int *__restrict__ exper
     __syncthreads();
     for (int s = 0; s < PLAN_CHUNK / PT; ++s) {
         const int64_t i = c0 + wave * (PLAN_CHUNK / PW) + s * 64 + lane;
-        const int e = expert_of(experts, i, P, E);
+        const int e = key_of(it, i);
         const uint64_t m = same_lanes(e, bits), below = m & ((1ull << lane) - 1);
         int at = 0;
         if (e >= 0) at = cnt[wave * E + e] + __popcll(below);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup"); __builtin_amdgcn_wave_barrier();      // all lanes have read before one writes
         if (e >= 0 && below == 0) cnt[wave * E + e] += __popcll(m);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup"); __builtin_amdgcn_wave_barrier();
-        if (i < P) { p.pos[i] = e >= 0 ? at : -1; if (e >= 0) { p.pair[at] = (int)i; p.row[at] = (int)i / k; } }
+        if (i >= it.n) continue;
+        if (it.base == 0) {                                  // `rows`: the items' rows where they are not i / k
+            if (p.pos) p.pos[i] = e >= 0 ? at : -1;
+            if (e >= 0) { p.pair[at] = (int)i; p.row[at] = it.rows ? it.rows[i] : (int)i / it.k; if (p.expert) p.expert[at] = e; }
+        } else {
+            const int *ex = it.experts + i * it.k;
+            for (int j = 0; j < it.k; ++j) {
+                const int v = valid(ex[j], it.base - 1), s2 = at * it.k + (it.k == 1 ? 0 : rank_of(ex, j, it.k, it.base - 1));
+                const bool to = v < it.base - 1;
+                p.pair[s2] = (int)i * it.k + j; p.row[s2] = (int)i; p.expert[s2] = to ? v : -1;
+                p.pos[i * it.k + j] = to ? s2 : -1;
+            }
+        }
     }
 }
 
@@ -125,33 +165,46 @@ __global__ void __launch_bounds__(PT) k_copy_counts(const int *__restrict__ coun
     for (int e = threadIdx.x; e < E; e += PT) out[e] = count[e];
 }
 
-static int plan_check(const char *who, int64_t P, int E)
+// sorts `it` into p (hist in place)
+static int run_plan(const Items &it, const EPlan &p, hipStream_t st)
 {
-    if (P < 0 || E < 1) return fail(ESCAT_EINVAL, "%s: pairs = %lld, E = %d", who, (long long)P, E);
-    if (P > 0x3fffffff || E > ESCAT_ROUTE_MAX_EXPERTS) return fail(ESCAT_ERANGE, "%s: pairs = %lld (below 2^30), E = %d (at most %d)", who, (long long)P, E, ESCAT_ROUTE_MAX_EXPERTS);
+    const int blocks = (int)plan_blocks(it.n);
+    int bits = 0; while ((1 << bits) < it.keys) ++bits;
+    const size_t lds = (size_t)PW * it.keys * 4;
+    if (blocks) { k_plan_hist<<<blocks, PT, lds, st>>>(it, bits, p.hist); CHECK_LAUNCH("escat_experts_plan: histogram"); }
+    k_plan_scan<<<1, 1024, 0, st>>>(it.keys, blocks, p);
+    CHECK_LAUNCH("escat_experts_plan: scan");
+    if (blocks) { k_plan_place<<<blocks, PT, lds, st>>>(it, bits, p); CHECK_LAUNCH("escat_experts_plan: place"); }
     return ESCAT_OK;
 }
 
-extern "C" size_t escat_experts_plan_bytes(int64_t pairs, int E)
+// positions of a plan by combination, sorted by expert (for the weights' gradients): by.pair = positions, by.row = their rows
+int escat_experts_plan_by_expert(const EPlan &p, int64_t P, int E, const EPlan &by, hipStream_t st)
 {
-    return pairs < 0 || E < 1 || E > ESCAT_ROUTE_MAX_EXPERTS ? 0 : (size_t)plan_ints(pairs, E) * 4;
+    return run_plan({p.expert, p.row, P, 1, 0, E}, by, st);
 }
 
-extern "C" int escat_experts_plan(const int32_t *experts, int64_t pairs, int k, int E, void *plan, size_t plan_bytes, int32_t *counts, void *stream)
+static int plan_check(const char *who, int64_t rows, int k, int E)
 {
-    int rc = plan_check("escat_experts_plan", pairs, E); if (rc) return rc;
-    if (k < 1) return fail(ESCAT_EINVAL, "escat_experts_plan: k = %d", k);
-    if (pairs > 0 && !experts) return fail(ESCAT_EINVAL, "escat_experts_plan: experts is null");
-    if (!plan || plan_bytes < escat_experts_plan_bytes(pairs, E)) return fail(ESCAT_EWORKSPACE, "escat_experts_plan: plan of %zu bytes, needs %zu", plan_bytes, escat_experts_plan_bytes(pairs, E));
+    if (rows < 0 || k < 1 || E < 1) return fail(ESCAT_EINVAL, "%s: rows = %lld, k = %d, experts = %d", who, (long long)rows, k, E);
+    if (rows > 0x3fffffff / k || E > ESCAT_ROUTE_MAX_EXPERTS) return fail(ESCAT_ERANGE, "%s: rows * k = %lld * %d (below 2^30), experts = %d (at most %d)", who, (long long)rows, k, E, ESCAT_ROUTE_MAX_EXPERTS);
+    return ESCAT_OK;
+}
+
+extern "C" size_t escat_experts_plan_bytes(int64_t rows, int k, int E)
+{
+    return plan_check("escat_experts_plan_bytes", rows, k, E) ? 0 : (size_t)plan_ints(rows, k, E) * 4;
+}
+
+extern "C" int escat_experts_plan(const int32_t *experts, int64_t rows, int k, int E, void *plan, size_t plan_bytes, int32_t *counts, void *stream)
+{
+    int rc = plan_check("escat_experts_plan", rows, k, E); if (rc) return rc;
+    if (rows > 0 && !experts) return fail(ESCAT_EINVAL, "escat_experts_plan: experts is null");
+    if (counts && k != 1) return fail(ESCAT_EINVAL, "escat_experts_plan: counts are given for k = 1 (k = %d)", k);
+    if (!plan || plan_bytes < escat_experts_plan_bytes(rows, k, E)) return fail(ESCAT_EWORKSPACE, "escat_experts_plan: plan of %zu bytes, needs %zu", plan_bytes, escat_experts_plan_bytes(rows, k, E));
     hipStream_t st = (hipStream_t)stream;
-    const EPlan p = plan_view(plan, pairs, E);
-    const int blocks = (int)plan_blocks(pairs);
-    int bits = 0; while ((1 << bits) < E) ++bits;
-    const size_t lds = (size_t)PW * E * 4;
-    if (blocks) { k_plan_hist<<<blocks, PT, lds, st>>>(experts, pairs, E, bits, p.hist); CHECK_LAUNCH("escat_experts_plan: histogram"); }
-    k_plan_scan<<<1, 1024, 0, st>>>(E, blocks, p);
-    CHECK_LAUNCH("escat_experts_plan: scan");
-    if (blocks) { k_plan_place<<<blocks, PT, lds, st>>>(experts, pairs, k, E, bits, p); CHECK_LAUNCH("escat_experts_plan: place"); }
+    const EPlan p = plan_of(plan, rows, k, E);
+    rc = run_plan({experts, nullptr, p.base ? rows : rows * k, k, p.base, p.keys}, p, st); if (rc) return rc;
     if (counts) { k_copy_counts<<<1, PT, 0, st>>>(p.count, E, counts); CHECK_LAUNCH("escat_experts_plan: counts"); }
     return ESCAT_OK;
 }

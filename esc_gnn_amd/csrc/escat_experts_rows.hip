@@ -15,11 +15,12 @@ struct RowArgs {
     EPlan p;
     const void *x, *w1, *b1, *w2, *b2, *dy;
     const float *weights;
-    void *h;                   // (P, H) sorted: w silu(u)
-    void *du;                  // (P, H) sorted
-    float *part;               // (P, O) or (P, D) fp32, sorted: what the joining pass reads
-    float *dwp;                // (feature tiles of H, P) sorted: parts of dw
-    float *ws;                 // (P) sorted: w (BWD1 leaves them for the weights' gradients)
+    void *h;                   // (P, H) by position: w silu(u)
+    void *du;                  // (P, H) by position
+    float *part;               // by pair: (P, O) or (P, D) fp32, what the joining pass reads
+    void *out;                 // by combination: y or dx
+    float *dwp;                // (feature tiles of H, P) by position: parts of dw
+    float *ws;                 // (P) by position: w (BWD1 leaves them for the weights' gradients)
 };
 
 enum { FWD1, FWD2, BWD1, BWD2 };
@@ -27,94 +28,130 @@ enum { FWD1, FWD2, BWD1, BWD2 };
 // the hardware's exponential errs by |u| 2^-24: below what 16-bit operands leave, not below what fp32 ones do
 template <typename T> __device__ __forceinline__ float sigmoid_of(float u) { return 1.f / (1.f + (sizeof(T) == 4 ? expf(-u) : __expf(-u))); }
 
-template <typename T, int MODE>
+template <typename T, int MODE, bool DIRECT>
 __global__ void __launch_bounds__(XT, 2) k_expert_rows(const RowArgs a)
 {
     constexpr int PER = Elem<T>::PER, KB = Elem<T>::KB;
     extern __shared__ __align__(16) char lds[];
     const int D = a.n.d, H = a.n.h, O = a.n.o;
     const int M = MODE == FWD2 ? O : MODE == BWD2 ? D : H;          // features of the result
-    const int mt = (M + XN - 1) / XN;
-    const int live = *a.p.n_tiles * mt;                              // (the grid covers the most tiles there can be)
+    constexpr bool ONE = MODE == FWD1 || MODE == BWD1;             // a tile's product with one of its experts, or with all
+    const int mt = (M + XN - 1) / XN, per = a.p.per, of = ONE ? per * mt : mt;
+    const int live = *a.p.n_tiles * of;                              // (the grid covers the most tiles there can be)
     if ((int)blockIdx.x >= live) return;
-    const int work = xcd_swizzle(blockIdx.x, live), t = work / mt, m0 = (work - t * mt) * XN;
-    const int e = a.p.tile[2 * t], r0 = a.p.tile[2 * t + 1];
-    const int rows = a.p.first[e + 1] - r0 < XM ? a.p.first[e + 1] - r0 : XM;
+    const int work = xcd_swizzle(blockIdx.x, live), t = work / of, rest = work - t * of, dig = ONE ? rest / mt : 0, m0 = (rest - dig * mt) * XN;
+    const int key = a.p.tile[2 * t], r0 = a.p.tile[2 * t + 1];
+    const int e = key_digit(a.p, key, dig);
+    if (ONE && e >= a.n.E) return;
+    const int rows = a.p.first[key + 1] - r0 < XM ? a.p.first[key + 1] - r0 : XM;
 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, am = (wave & 1) * 64, bn = (wave >> 1) * 64;
     typedef Stage<T, false> SC;
-    const int c = SC::chunk() * PER;
-    // the thread's four rows of activations (rows behind the last of the tile repeat it: their results are not written)
-    int64_t br[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int r = SC::row(i) < rows ? SC::row(i) : rows - 1;
-        br[i] = MODE == FWD2 || MODE == BWD2 ? (int64_t)(r0 + r) : (int64_t)a.p.row[r0 + r];
-    }
+    // rows behind the last of the tile repeat it: their results are not written
+    const int rl[2] = {bn + (lane & 31) < rows ? bn + (lane & 31) : 0, bn + 32 + (lane & 31) < rows ? bn + 32 + (lane & 31) : 0};
     float wr[2];                                                    // weights of the two rows whose results the lane holds
 #pragma unroll
-    for (int j = 0; j < 2; ++j) { const int r = bn + 32 * j + (lane & 31); wr[j] = MODE == BWD2 ? 1.f : a.weights[a.p.pair[r0 + (r < rows ? r : 0)]]; }
+    for (int j = 0; j < 2; ++j) wr[j] = ONE ? a.weights[a.p.pair[(int64_t)(r0 + rl[j]) * per + dig]] : 0.f;
     __shared__ __align__(16) float bias[XN];
-    if (MODE != BWD2 && threadIdx.x < XN) {
-        const T *b = MODE == FWD2 ? (const T *)a.b2 : (const T *)a.b1;
-        bias[threadIdx.x] = b && m0 + (int)threadIdx.x < M ? to_f32(b[(int64_t)e * M + m0 + threadIdx.x]) : 0.f;
-    }
-    acc_t acc[2][2];
+    if (ONE && threadIdx.x < XN) bias[threadIdx.x] = a.b1 && m0 + (int)threadIdx.x < M ? to_f32(((const T *)a.b1)[(int64_t)e * M + m0 + threadIdx.x]) : 0.f;
+    acc_t acc[2][2], acc2[2][2];
     clear(acc);
+    float dot[4] = {0.f, 0.f, 0.f, 0.f};                            // BWD1: the thread's share of b2 . dy of its rows
 
-    // ---- first product: W1 x (FWD1, BWD1), W2 (w h) (FWD2), W1^T du (BWD2)
-    if (MODE != BWD2) {
-        const int K = MODE == FWD2 ? H : D;
-        const T *A = (const T *)(MODE == FWD2 ? a.w2 : a.w1) + (int64_t)e * M * K, *B = (const T *)(MODE == FWD2 ? a.h : a.x);
-        RowsKC<T> la, lb;
-        la.K = lb.K = K; la.c = lb.c = c;
+    if constexpr (ONE) {
+        // ---- W1 x
+        auto w1 = [&](int) { return (const char *)a.w1 + (int64_t)e * H * D * (int64_t)sizeof(T); };
+        OperandKC<T, decltype(w1)> A(D, w1);
+        OperandKCRows<T> B(D);
+        const T *dy[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int m = m0 + SC::row(i) < M ? m0 + SC::row(i) : M - 1;
-            la.p[i] = A + (int64_t)m * K;
-            lb.p[i] = B + br[i] * K;
+            const int m = m0 + SC::row(i) < M ? m0 + SC::row(i) : M - 1, r = SC::row(i) < rows ? SC::row(i) : rows - 1;
+            const int64_t row = a.p.row[(int64_t)(r0 + r) * per + dig];
+            A.off[i] = (uint32_t)m * (uint32_t)D * (uint32_t)sizeof(T);
+            B.p[i] = (const T *)a.x + row * D;
+            if (MODE == BWD1) dy[i] = (const T *)a.dy + row * O;
         }
-        tile_loop<MODE == BWD1 ? 1 : 2, T, false, false>(K, lds, am, bn, acc, [&](int k0, u4 (&r)[4], int) { la.load(k0, r); }, [&](int k0, u4 (&r)[4], int) { lb.load(k0, r); },
-                                   [&](int k0, u4 (&r)[4], int) { la.fix(k0, r); }, [&](int k0, u4 (&r)[4], int) { lb.fix(k0, r); });
-    }
-    // ---- W2^T dy (BWD1, into a second set), W1^T du (BWD2): weights with the result's features contiguous
-    acc_t acc2[2][2];
-    float dot[4] = {0.f, 0.f, 0.f, 0.f};                            // BWD1: the thread's share of b2 . dy of its rows
-    if (MODE == BWD1 || MODE == BWD2) {
-        const int K = MODE == BWD1 ? O : H;
-        const T *A = (const T *)(MODE == BWD1 ? a.w2 : a.w1) + (int64_t)e * K * M, *B = (const T *)(MODE == BWD1 ? a.dy : a.du);
-        typedef Stage<T, true> SM;
-        const ColsKM<T> cols_a(m0, M);
-        RowsKC<T> lb;
-        lb.K = K; lb.c = c;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) lb.p[i] = B + br[i] * K;
-        const bool with_dot = MODE == BWD1 && m0 == 0 && a.b2 != nullptr;
-        const T *b2 = MODE == BWD1 ? (const T *)a.b2 + (int64_t)e * O : nullptr;
-        if (MODE == BWD1) clear(acc2);
-        tile_loop<MODE == BWD1 ? 1 : 2, T, true, false>(K, lds, am, bn, MODE == BWD1 ? acc2 : acc,
-            [&](int k0, u4 (&r)[4], int) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) { const int kk = k0 + SM::row(i); r[i] = cols_a.load(A + (int64_t)(kk < K ? kk : K - 1) * M); } },
-            [&](int k0, u4 (&r)[4], int) { lb.load(k0, r); },
-            [&](int k0, u4 (&r)[4], int) { cols_a.fix(r, K - k0, k0 + KB <= K); },
-            [&](int k0, u4 (&r)[4], int) {
-                lb.fix(k0, r);
-                if (with_dot) {
+        tile_loop<MODE == BWD1 ? 1 : 2, T, false, false>((D + KB - 1) / KB, lds, am, bn, acc, A, B);
+        if constexpr (MODE == BWD1) {
+            // ---- W2^T dy into the second set, and b2 . dy on the way
+            auto w2 = [&](int) { return (const char *)a.w2 + (int64_t)e * O * H * (int64_t)sizeof(T); };
+            OperandKM<T, decltype(w2)> A2(O, m0, M, w2);
+            struct WithDot : OperandKCRows<T> {
+                const T *b2;
+                float (&dot)[4];
+                __device__ __forceinline__ WithDot(int K, const T *b2, float (&dot)[4]) : OperandKCRows<T>(K), b2(b2), dot(dot) {}
+                __device__ __forceinline__ void fix(u4 (&r)[4], int set)
+                {
+                    const int k0 = this->fk0 + this->c, K = this->K;
+                    OperandKCRows<T>::fix(r, set);
+                    if (!b2) return;
                     float f[PER], g[PER];
 #pragma unroll
-                    for (int q = 0; q < PER; ++q) f[q] = to_f32(b2[k0 + c + q < K ? k0 + c + q : K - 1]);
+                    for (int q = 0; q < PER; ++q) f[q] = to_f32(b2[k0 + q < K ? k0 + q : K - 1]);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         to_floats<T>(r[i], g);
 #pragma unroll
                         for (int q = 0; q < PER; ++q) dot[i] = fmaf(f[q], g[q], dot[i]);
                     }
-                } });
+                }
+            } B2(O, m0 == 0 && a.b2 ? (const T *)a.b2 + (int64_t)e * O : nullptr, dot);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) B2.p[i] = dy[i];
+            clear(acc2);
+            tile_loop<1, T, true, false>((O + KB - 1) / KB, lds, am, bn, acc2, A2, B2);
+        }
+    } else {
+        // ---- W2 (w h) or W1^T du of the tile's experts, one after the other into the same accumulators
+        uint64_t live_at = 0; int n_live = 0;                             // the digits that name an expert, four bits each
+        for (int j = per - 1; j >= 0; --j) if (key_digit(a.p, key, j) < a.n.E) { live_at = live_at << 4 | (unsigned)j; ++n_live; }
+        auto weights = [&](int j) {
+            const int dj = (int)(live_at >> 4 * j) & 15, q = j < n_live ? key_digit(a.p, key, dj) : 0;
+            return (const char *)(MODE == FWD2 ? a.w2 : a.w1) + (int64_t)q * M * H * (int64_t)sizeof(T);
+        };
+        auto hidden = [&](int j) {
+            const int dj = (int)(live_at >> 4 * j) & 15;
+            return (const char *)(MODE == FWD2 ? a.h : a.du) + ((int64_t)r0 * per + dj) * H * (int64_t)sizeof(T);
+        };
+        OperandKC<T, decltype(hidden)> B(H, hidden);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) B.off[i] = (uint32_t)((SC::row(i) < rows ? SC::row(i) : rows - 1) * per) * (uint32_t)H * (uint32_t)sizeof(T);
+        const int steps = n_live * ((H + KB - 1) / KB);
+        if constexpr (MODE == FWD2) {
+            OperandKC<T, decltype(weights)> A(H, weights);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) A.off[i] = (uint32_t)(m0 + SC::row(i) < M ? m0 + SC::row(i) : M - 1) * (uint32_t)H * (uint32_t)sizeof(T);
+            tile_loop<2, T, false, false>(steps, lds, am, bn, acc, A, B);
+        } else {
+            OperandKM<T, decltype(weights)> A(H, m0, M, weights);
+            tile_loop<2, T, true, false>(steps, lds, am, bn, acc, A, B);
+        }
     }
 
+    if (MODE == FWD2 && a.b2)                                       // + w b2 of each expert
+        for (int j = 0; j < per; ++j) {
+            const int ej = key_digit(a.p, key, j);
+            if (ej >= a.n.E) continue;
+            __syncthreads();
+            if (threadIdx.x < XN) bias[threadIdx.x] = m0 + (int)threadIdx.x < M ? to_f32(((const T *)a.b2)[(int64_t)ej * M + m0 + threadIdx.x]) : 0.f;
+            __syncthreads();
+#pragma unroll
+            for (int jj = 0; jj < 2; ++jj) {
+                const float w = a.weights[a.p.pair[(int64_t)(r0 + rl[jj]) * per + j]];
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const f4 bv = *(const f4 *)(bias + am + 32 * i + 8 * q + 4 * (lane >> 5));
+#pragma unroll
+                        for (int z = 0; z < 4; ++z) acc[i][jj][4 * q + z] = fmaf(w, bv[z], acc[i][jj][4 * q + z]);
+                    }
+            }
+        }
+
     // ---- epilogue.  The lane holds, for each of two rows, runs of four features; they leave through LDS
-    typedef typename std::conditional<MODE == FWD1 || MODE == BWD1, T, float>::type OUT;
+    typedef typename std::conditional<ONE || DIRECT, T, float>::type OUT;
     const int cols = M - m0 < XN ? M - m0 : XN;
     __shared__ float red[3 * 128];                                  // BWD1: sums over the features of a half, b2 . dy
     if (MODE == BWD1) {
@@ -137,12 +174,12 @@ __global__ void __launch_bounds__(XT, 2) k_expert_rows(const RowArgs a)
                 const int mt_ = am + 32 * i + 8 * q + 4 * (lane >> 5), m = m0 + mt_;
                 float u[4], g[4];
                 f4 bv = {0.f, 0.f, 0.f, 0.f};
-                if (MODE != BWD2) bv = *(const f4 *)(bias + mt_);
+                if (ONE) bv = *(const f4 *)(bias + mt_);
 #pragma unroll
                 for (int z = 0; z < 4; ++z) {
                     u[z] = acc[i][j][4 * q + z];
                     if (MODE == BWD1) g[z] = acc2[i][j][4 * q + z];
-                    if (MODE != BWD2) u[z] += MODE == FWD2 ? w * bv[z] : bv[z];
+                    if (ONE) u[z] += bv[z];
                 }
                 if (MODE == FWD1) {
 #pragma unroll
@@ -159,18 +196,21 @@ __global__ void __launch_bounds__(XT, 2) k_expert_rows(const RowArgs a)
                 }
                 Spill<OUT>::put(lds, r, mt_, u);
             }
-        if (MODE == BWD1 && m0 == 0 && am == 0 && lane < 32 && r < rows) a.ws[r0 + r] = w;
+        if (MODE == BWD1 && m0 == 0 && am == 0 && lane < 32 && r < rows) a.ws[(int64_t)(r0 + r) * per + dig] = w;
         if (MODE == BWD1) {
             sum += __shfl_xor(sum, 32, 64);
             if (lane < 32) red[(wave & 1) * 128 + r] = sum;
         }
     }
     __syncthreads();
-    Spill<OUT>::write(lds, (MODE == FWD1 || MODE == BWD1 ? (OUT *)a.h : (OUT *)a.part) + (int64_t)r0 * M + m0, M, rows, cols);
+    const int *row = a.p.row;
+    if (ONE) Spill<OUT>::write(lds, (OUT *)a.h + m0, M, rows, cols, [&](int r) { return (int64_t)(r0 + r) * per + dig; });
+    else if (DIRECT) Spill<OUT>::write(lds, (OUT *)a.out + m0, M, rows, cols, [&](int r) { return row[(int64_t)(r0 + r) * per]; });
+    else Spill<OUT>::write(lds, (OUT *)a.part + m0, M, rows, cols, [&](int r) { return r0 + r; });
     if (MODE == BWD1) {
         const int r = threadIdx.x;
         const int64_t P = a.n.rows * a.n.k;
-        if (r < rows) a.dwp[(int64_t)(m0 / XN) * P + r0 + r] = red[r] + red[128 + r] + (m0 == 0 && a.b2 ? red[256 + r] : 0.f);
+        if (r < rows) a.dwp[(int64_t)(m0 / XN) * P + (int64_t)(r0 + r) * per + dig] = red[r] + red[128 + r] + (m0 == 0 && a.b2 ? red[256 + r] : 0.f);
         __syncthreads();
 #pragma unroll
         for (int j = 0; j < 2; ++j)
@@ -184,7 +224,7 @@ __global__ void __launch_bounds__(XT, 2) k_expert_rows(const RowArgs a)
                     Spill<OUT>::put(lds, bn + 32 * j + (lane & 31), am + 32 * i + 8 * q + 4 * (lane >> 5), g);
                 }
         __syncthreads();
-        Spill<OUT>::write(lds, (OUT *)a.du + (int64_t)r0 * M + m0, M, rows, cols);
+        Spill<OUT>::write(lds, (OUT *)a.du + m0, M, rows, cols, [&](int r) { return (int64_t)(r0 + r) * per + dig; });
     }
 }
 
@@ -235,52 +275,54 @@ __global__ void __launch_bounds__(XT) k_join_dw(const float *__restrict__ dwp, c
 }
 
 // ------------------------------------------------------------------ launches (called by escat_experts.hip)
-template <typename T, int MODE> static int rows_launch(const RowArgs &a, int M, hipStream_t st)
+template <typename T, int MODE, bool DIRECT> static int rows_launch(const RowArgs &a, int M, hipStream_t st)
 {
-    const int64_t P = a.n.rows * a.n.k, wgs = plan_max_tiles(P, a.n.E) * ((M + XN - 1) / XN);
+    constexpr bool ONE = MODE == FWD1 || MODE == BWD1;
+    const int64_t items = a.p.base ? a.n.rows : a.n.rows * a.n.k;
+    const int64_t wgs = plan_max_tiles(items, a.p.keys) * ((M + XN - 1) / XN) * (ONE ? a.p.per : 1);
     if (wgs > 0xffffff) return fail(ESCAT_ERANGE, "experts: %lld tiles", (long long)wgs);
-    const size_t lds = MODE == FWD2 || MODE == BWD2 || sizeof(T) == 4 ? LDS_ROWS : LDS_TILES;
-    int rc = set_lds(k_expert_rows<T, MODE>, lds); if (rc) return rc;
-    k_expert_rows<T, MODE><<<(unsigned)wgs, XT, lds, st>>>(a);
+    const size_t lds = !(ONE || DIRECT) || sizeof(T) == 4 ? LDS_ROWS : LDS_TILES;
+    int rc = set_lds(k_expert_rows<T, MODE, DIRECT>, lds); if (rc) return rc;
+    k_expert_rows<T, MODE, DIRECT><<<(unsigned)wgs, XT, lds, st>>>(a);
     CHECK_LAUNCH("experts: rows");
     return ESCAT_OK;
 }
 
 static unsigned grid_for(int64_t n) { const int64_t b = (n + XT - 1) / XT; return (unsigned)(b < 65536 ? b : 65536); }
 
-template <typename T> static int join_launch(const float *part, const int *pos, int64_t rows, int k, int M, void *out, hipStream_t st)
+// second product of a pass: results of M features to `out` by row
+template <typename T, int MODE> static int second(RowArgs &a, int M, void *out, hipStream_t st)
 {
-    k_join<T><<<grid_for(rows * ((M + 3) / 4)), XT, 0, st>>>(part, pos, rows, k, M, (T *)out);
+    a.out = out;
+    if (a.p.base) return rows_launch<T, MODE, true>(a, M, st);
+    int rc = rows_launch<T, MODE, false>(a, M, st); if (rc) return rc;
+    k_join<T><<<grid_for(a.n.rows * ((M + 3) / 4)), XT, 0, st>>>(a.part, a.p.pos, a.n.rows, a.n.k, M, (T *)out);
     CHECK_LAUNCH("experts: join");
     return ESCAT_OK;
 }
 
-template <typename T> static int fwd(const RowArgs &a, void *y, hipStream_t st)
+template <typename T> static int fwd(RowArgs &a, void *y, hipStream_t st)
 {
-    int rc = rows_launch<T, FWD1>(a, a.n.h, st); if (rc) return rc;
-    rc = rows_launch<T, FWD2>(a, a.n.o, st); if (rc) return rc;
-    return join_launch<T>(a.part, a.p.pos, a.n.rows, a.n.k, a.n.o, y, st);
+    int rc = rows_launch<T, FWD1, false>(a, a.n.h, st); if (rc) return rc;
+    return second<T, FWD2>(a, a.n.o, y, st);
 }
-template <typename T> static int bwd(const RowArgs &a, void *dx, float *dw, hipStream_t st)
+template <typename T> static int bwd(RowArgs &a, void *dx, float *dw, hipStream_t st)
 {
-    int rc = rows_launch<T, BWD1>(a, a.n.h, st); if (rc) return rc;
+    int rc = rows_launch<T, BWD1, false>(a, a.n.h, st); if (rc) return rc;
     const int64_t P = a.n.rows * a.n.k;
     if (dw) { k_join_dw<<<grid_for(P), XT, 0, st>>>(a.dwp, a.p.pos, P, (a.n.h + XN - 1) / XN, dw); CHECK_LAUNCH("experts: dw"); }
-    if (!dx) return ESCAT_OK;
-    rc = rows_launch<T, BWD2>(a, a.n.d, st); if (rc) return rc;
-    return join_launch<T>(a.part, a.p.pos, a.n.rows, a.n.k, a.n.d, dx, st);
+    return dx ? second<T, BWD2>(a, a.n.d, dx, st) : ESCAT_OK;
 }
 
 int escat_experts_rows_fwd(int type, const EDims &n, const EPlan &p, const void *x, const float *weights, const void *w1, const void *b1, const void *w2,
                            const void *b2, void *h, float *part, void *y, hipStream_t st)
 {
-    RowArgs a = {n, p, x, w1, b1, w2, b2, nullptr, weights, h, nullptr, part, nullptr, nullptr};
+    RowArgs a = {n, p, x, w1, b1, w2, b2, nullptr, weights, h, nullptr, part, nullptr, nullptr, nullptr};
     return type == ESCAT_F32 ? fwd<float>(a, y, st) : type == ESCAT_BF16 ? fwd<bf16_t>(a, y, st) : fwd<f16_t>(a, y, st);
 }
 int escat_experts_rows_bwd(int type, const EDims &n, const EPlan &p, const void *x, const float *weights, const void *w1, const void *b1, const void *w2,
                            const void *b2, const void *dy, void *h, void *du, float *part, float *dwp, float *ws, void *dx, float *dw, hipStream_t st)
 {
-    RowArgs a = {n, p, x, w1, b1, w2, b2, dy, weights, h, du, part, dwp, ws};
+    RowArgs a = {n, p, x, w1, b1, w2, b2, dy, weights, h, du, part, nullptr, dwp, ws};
     return type == ESCAT_F32 ? bwd<float>(a, dx, dw, st) : type == ESCAT_BF16 ? bwd<bf16_t>(a, dx, dw, st) : bwd<f16_t>(a, dx, dw, st);
 }
-

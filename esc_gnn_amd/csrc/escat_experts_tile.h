@@ -147,94 +147,120 @@ __device__ __forceinline__ void tile_step(const char *la, const char *lb, int am
     }
 }
 
-// ---- the loop over k.  loadA / loadB(k0, regs, set): the thread's pieces of step k0, AHEAD = 1 or 2 steps ahead of their use (a step's
-// products take less time than memory does; 1 where two sets of accumulators leave no registers for 2); set = step & 1, or 0; fixA / fixB(k0, regs, set): the same pieces once they have arrived (a use inside load
-// would wait for them there).  lds: 4 tiles (A0 B0 A1 B1), free to be written on return.
-template <int AHEAD, typename T, bool AKM, bool BKM, typename FA, typename FB, typename XA, typename XB>
-__device__ __forceinline__ void tile_loop(int K, char *lds, int am, int bn, acc_t (&acc)[2][2], FA loadA, FB loadB, XA fixA, XB fixB)
+// ---- the loop over the steps.  a / b: operands with load(regs, set) -- the thread's pieces of the next step, AHEAD = 1 or 2 steps ahead of
+// their use (a step's products take less time than memory does; 1 where two sets of accumulators leave no registers for 2) -- and
+// fix(regs, set) -- the same pieces once they have arrived (a use inside load would wait for them there); both are called once a step, in
+// order; set = step & 1, or 0.  lds: 4 tiles (A0 B0 A1 B1), free to be written on return.
+template <int AHEAD, typename T, bool AKM, bool BKM, typename A, typename B>
+__device__ __forceinline__ void tile_loop(int steps, char *lds, int am, int bn, acc_t (&acc)[2][2], A &a, B &b)
 {
-    constexpr int KB = Elem<T>::KB;
-    const int steps = (K + KB - 1) / KB;
     if (steps == 0) return;
     char *buf0 = lds, *buf1 = lds + 2 * TILE_BYTES;
     u4 a0[4], b0[4], a1[4], b1[4];
     // no load under a condition inside the loop: it would make the compiler wait for all of them at every turn
-#define LOAD(s, S) { loadA((s) * KB, a##S, S); loadB((s) * KB, b##S, S); }
-#define STORE(s, S) { fixA((s) * KB, a##S, S); fixB((s) * KB, b##S, S); Stage<T, AKM>::store(buf##S, a##S); Stage<T, BKM>::store(buf##S + TILE_BYTES, b##S); __syncthreads(); }
+#define LOAD(S) { a.load(a##S, S); b.load(b##S, S); }
+#define STORE_TO(S, D) { a.fix(a##S, S); b.fix(b##S, S); Stage<T, AKM>::store(buf##D, a##S); Stage<T, BKM>::store(buf##D + TILE_BYTES, b##S); __syncthreads(); }
+#define STORE(S) STORE_TO(S, S)
 #define MULTIPLY(S) tile_step<T, AKM, BKM>(buf##S, buf##S + TILE_BYTES, am, bn, acc);
-    LOAD(0, 0)
+    LOAD(0)
     if constexpr (AHEAD == 1) {
-#define STORE1(s, B) { fixA((s) * KB, a0, 0); fixB((s) * KB, b0, 0); Stage<T, AKM>::store(buf##B, a0); Stage<T, BKM>::store(buf##B + TILE_BYTES, b0); __syncthreads(); }
-        STORE1(0, 0)
+        STORE(0)
         int s = 0;
         for (; s + 2 < steps; s += 2) {
-            LOAD(s + 1, 0)
+            LOAD(0)
             MULTIPLY(0)
-            STORE1(s + 1, 1)
-            LOAD(s + 2, 0)
+            STORE_TO(0, 1)
+            LOAD(0)
             MULTIPLY(1)
-            STORE1(s + 2, 0)
+            STORE(0)
         }
         if (s + 2 == steps) {
-            LOAD(s + 1, 0)
+            LOAD(0)
             MULTIPLY(0)
-            STORE1(s + 1, 1)
+            STORE_TO(0, 1)
             MULTIPLY(1)
         } else MULTIPLY(0)
-#undef STORE1
     } else if (steps == 1) {
-        STORE(0, 0)
+        STORE(0)
         MULTIPLY(0)
     } else {
-        LOAD(1, 1)
-        STORE(0, 0)
+        LOAD(1)
+        STORE(0)
         int s = 0;
         for (; s + 3 < steps; s += 2) {
-            LOAD(s + 2, 0)
+            LOAD(0)
             MULTIPLY(0)
-            STORE(s + 1, 1)
-            LOAD(s + 3, 1)
+            STORE(1)
+            LOAD(1)
             MULTIPLY(1)
-            STORE(s + 2, 0)
+            STORE(0)
         }
         if (s + 3 == steps) {
-            LOAD(s + 2, 0)
+            LOAD(0)
             MULTIPLY(0)
-            STORE(s + 1, 1)
+            STORE(1)
             MULTIPLY(1)
-            STORE(s + 2, 0)
+            STORE(0)
             MULTIPLY(0)
         } else {
             MULTIPLY(0)
-            STORE(s + 1, 1)
+            STORE(1)
             MULTIPLY(1)
         }
     }
     __syncthreads();
 #undef LOAD
 #undef STORE
+#undef STORE_TO
 #undef MULTIPLY
 }
 
-// loads of an operand with k contiguous: four rows, p[i] their first elements
-template <typename T> struct RowsKC {
+template <typename T> __device__ __forceinline__ void fix_kc(u4 (&r)[4], int K, int c, int &k0);
+// ---- operands.  An operand walks through one or more segments of K values of k (by combination: one for each expert of the tile), each
+// padded to whole steps; `seg(j)` says where segment j begins.
+// k contiguous, rows at 32-bit offsets from a base that a segment moves
+template <typename T, typename SEG> struct OperandKC {
+    SEG seg;
+    int K, c, k0, j, fk0;
+    const char *base;
+    uint32_t off[4];
+    __device__ __forceinline__ OperandKC(int K, SEG seg) : seg(seg), K(K), c(Stage<T, false>::chunk() * Elem<T>::PER), k0(0), j(0), fk0(0), base(seg(0)) {}
+    __device__ __forceinline__ void load(u4 (&r)[4], int)
+    {
+        constexpr int PER = Elem<T>::PER;
+        const uint32_t at = (uint32_t)(k0 + c < K - PER ? k0 + c : K - PER) * (uint32_t)sizeof(T);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = load16((const T *)(base + (size_t)(off[i] + at)));
+        k0 += Elem<T>::KB;
+        if (k0 >= K) { k0 = 0; base = seg(++j); }
+    }
+    __device__ __forceinline__ void fix(u4 (&r)[4], int) { fix_kc<T>(r, K, c, fk0); }
+};
+template <typename T> __device__ __forceinline__ void fix_kc(u4 (&r)[4], int K, int c, int &k0)
+{
+    constexpr int PER = Elem<T>::PER;
+    if (k0 + Elem<T>::KB > K) {
+        const int s = k0 + c > K - PER ? k0 + c - (K - PER) : 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = moved<T>(r[i], s);
+    }
+    k0 += Elem<T>::KB;
+    if (k0 >= K) k0 = 0;
+}
+// k contiguous, rows anywhere (activations by row); one segment
+template <typename T> struct OperandKCRows {
     const T *p[4];
-    int K, c;
-    __device__ __forceinline__ void load(int k0, u4 (&r)[4]) const
+    int K, c, k0, fk0;
+    __device__ __forceinline__ explicit OperandKCRows(int K) : K(K), c(Stage<T, false>::chunk() * Elem<T>::PER), k0(0), fk0(0) {}
+    __device__ __forceinline__ void load(u4 (&r)[4], int)
     {
         constexpr int PER = Elem<T>::PER;
         const int at = k0 + c < K - PER ? k0 + c : K - PER;
 #pragma unroll
         for (int i = 0; i < 4; ++i) r[i] = load16(p[i] + at);
+        k0 += Elem<T>::KB;
     }
-    __device__ __forceinline__ void fix(int k0, u4 (&r)[4]) const
-    {
-        constexpr int PER = Elem<T>::PER;
-        if (k0 + Elem<T>::KB <= K) return;
-        const int s = k0 + c > K - PER ? k0 + c - (K - PER) : 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) r[i] = moved<T>(r[i], s);
-    }
+    __device__ __forceinline__ void fix(u4 (&r)[4], int) { fix_kc<T>(r, K, c, fk0); }
 };
 // where the thread's pieces of a row of M features begin (KM), and how far they are to be moved
 template <typename T> struct ColsKM {
@@ -248,7 +274,6 @@ template <typename T> struct ColsKM {
         s = m - at;
         ragged = m0 + 128 > M;
     }
-    __device__ __forceinline__ u4 load(const T *row) const { return load16(row + at); }
     __device__ __forceinline__ void fix(u4 (&r)[4], int live, bool whole) const          // live: rows of the step that exist
     {
         if (ragged) {
@@ -261,9 +286,40 @@ template <typename T> struct ColsKM {
         }
     }
 };
+// features contiguous, rows of k one after the other from a base that a segment moves (weights in the backward)
+template <typename T, typename SEG> struct OperandKM {
+    SEG seg;
+    ColsKM<T> cols;
+    int K, k0, j, fk0;
+    uint32_t row, off, last;                            // bytes: of a row, of the thread's piece in row k0 + row(0), in row K - 1
+    const char *base;
+    __device__ __forceinline__ OperandKM(int K, int m0, int M, SEG seg)
+        : seg(seg), cols(m0, M), K(K), k0(0), j(0), fk0(0), row((uint32_t)M * (uint32_t)sizeof(T)), base(seg(0))
+    {
+        off = (uint32_t)Stage<T, true>::row(0) * row + (uint32_t)cols.at * (uint32_t)sizeof(T);
+        last = (uint32_t)(K - 1) * row + (uint32_t)cols.at * (uint32_t)sizeof(T);
+    }
+    __device__ __forceinline__ void load(u4 (&r)[4], int)
+    {
+        const uint32_t o = off + (uint32_t)k0 * row;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t q = o + (uint32_t)(i * Stage<T, true>::RPP) * row;
+            r[i] = load16((const T *)(base + (size_t)(q < last ? q : last)));
+        }
+        k0 += Elem<T>::KB;
+        if (k0 >= K) { k0 = 0; base = seg(++j); }
+    }
+    __device__ __forceinline__ void fix(u4 (&r)[4], int)
+    {
+        cols.fix(r, K - fk0, fk0 + Elem<T>::KB <= K);
+        fk0 += Elem<T>::KB;
+        if (fk0 >= K) fk0 = 0;
+    }
+};
 
 // ---- results through LDS, so that memory is written in whole rows of the tile.  put: the lane's run of four features m.. of row n
-// (tile coordinates); write: rows [0, rows), features [0, cols) to out + n * ld.  OUT: element type.  A row of 128 OUT is OSTRIDE bytes apart
+// (tile coordinates); write: rows [0, rows), features [0, cols) to out + at(n) * ld.  OUT: element type.  A row of 128 OUT is OSTRIDE bytes apart
 // from the next: 16 more than its size, so that the runs of 32 rows fall on different banks.
 template <typename OUT> struct Spill {
     static constexpr int STRIDE = 128 * (int)sizeof(OUT) + 16;
@@ -276,7 +332,7 @@ template <typename OUT> struct Spill {
         __builtin_memcpy(__builtin_assume_aligned(lds + n * STRIDE + m * (int)sizeof(OUT), 4 * sizeof(OUT)), &q, sizeof(q));
     }
     // the caller has a barrier before and, if lds is used again, after
-    static __device__ __forceinline__ void write(const char *lds, OUT *out, int64_t ld, int rows, int cols)
+    template <typename AT> static __device__ __forceinline__ void write(const char *lds, OUT *out, int64_t ld, int rows, int cols, AT at)
     {
         constexpr int PER = 16 / (int)sizeof(OUT), CPR = 128 / PER;
         const int c = threadIdx.x % CPR * PER;
@@ -284,7 +340,7 @@ template <typename OUT> struct Spill {
         for (int r = threadIdx.x / CPR; r < rows; r += XT / CPR) {
             struct alignas(16) { OUT v[PER]; } q;
             __builtin_memcpy(&q, __builtin_assume_aligned(lds + r * STRIDE + c * (int)sizeof(OUT), 16), 16);
-            OUT *o = out + r * ld + c;
+            OUT *o = out + (int64_t)at(r) * ld + c;
             if (c + PER <= cols) { Pack<OUT, PER> p; __builtin_memcpy(&p, &q, 16); *(Pack<OUT, PER> *)o = p; }
             else {
 #pragma unroll

@@ -99,12 +99,11 @@ def route_experts(logits: torch.Tensor, k: int, *, score: str = "softmax", bias:
                         int(bool(renormalize)), float(scale))
 
 
-def _plan(experts: torch.Tensor, k: int, E: int, counts: Optional[torch.Tensor], stream) -> torch.Tensor:
+def _plan(experts: torch.Tensor, rows: int, k: int, E: int, counts: Optional[torch.Tensor], stream) -> torch.Tensor:
     lib = _lib.load()
-    P = experts.numel()
-    size = lib.escat_experts_plan_bytes(P, E)
+    size = lib.escat_experts_plan_bytes(rows, k, E)
     plan = torch.empty(size, dtype=torch.uint8, device=experts.device)
-    _lib.check(lib.escat_experts_plan(experts.data_ptr(), P, k, E, plan.data_ptr(), size, _ptr(counts), stream), "escat_experts_plan")
+    _lib.check(lib.escat_experts_plan(experts.data_ptr(), rows, k, E, plan.data_ptr(), size, _ptr(counts), stream), "escat_experts_plan")
     return plan
 
 
@@ -123,7 +122,7 @@ def expert_counts(experts: torch.Tensor, n_experts: int) -> torch.Tensor:
     _need_gpu(experts, "experts")
     counts = torch.empty(n_experts, dtype=torch.int32, device=experts.device)
     with _on(experts.device) as stream:
-        _plan(experts.contiguous(), 1, n_experts, counts, stream)
+        _plan(experts.contiguous(), experts.numel(), 1, n_experts, counts, stream)
     return counts
 
 
@@ -137,7 +136,7 @@ class _ExpertMLP(torch.autograd.Function):
         y = torch.empty(rows, o, dtype=x.dtype, device=x.device)
         size = lib.escat_experts_workspace_bytes(at, 0)
         with _on(x.device) as stream:
-            plan = _plan(experts, k, E, None, stream)
+            plan = _plan(experts, rows, k, E, None, stream)
             ws = torch.empty(size, dtype=torch.uint8, device=x.device)
             rc = lib.escat_experts_fwd(at, x.data_ptr(), weights.data_ptr(), w1.data_ptr(), _ptr(b1), w2.data_ptr(), _ptr(b2), plan.data_ptr(),
                                        y.data_ptr(), ws.data_ptr(), size, stream)

@@ -108,3 +108,4 @@ def test_experts_library_checks_its_arguments():
     assert lib.escat_experts_plan(0, 5, 1, 4, 16, 1 << 20, 0, 0) == -1
     assert lib.escat_experts_plan(16, 5, 1, 4, 16, 8, 0, 0) == -3
     assert lib.escat_experts_plan(16, 1 << 31, 1, 4, 16, 8, 0, 0) == -2
+    assert lib.escat_experts_plan(16, 5, 2, 4, 16, 1 << 20, 16, 0) == -1                          # counts of k = 2
