@@ -32,7 +32,7 @@ struct EPlan {
     int *count;       // keys      items of each key
     int *first;       // keys + 1  its first item in sorted order; first[keys] = all items
     int *n_tiles;     // 1         tiles of XM items, none across two keys
-    int *tile;        // 2 x max_tiles: key, first item
+    int *tile;        // 4 x max_tiles: key, first item, items, 0
     int *pair;        // P         position -> pair
     int *row;         // P         position -> row of the activations
     int *expert;      // P         position -> expert, -1 = none
@@ -52,7 +52,9 @@ static inline EPlan plan_view(void *mem, int64_t rows, int k, int E, int combo, 
     EPlan p; int *q = (int *)mem;
     const int64_t items = plan_items(rows, k, combo), P = rows * k;
     p.per = combo ? k : 1; p.base = combo ? E + 1 : 0; p.keys = combo ? combo : E;
-    p.count = q; q += p.keys; p.first = q; q += p.keys + 1; p.n_tiles = q; q += 1; p.tile = q; q += 2 * plan_max_tiles(items, p.keys);
+    p.count = q; q += p.keys; p.first = q; q += p.keys + 1; p.n_tiles = q; q += 1;
+    q += (4 - (q - (int *)mem) % 4) % 4;
+    p.tile = q; q += 4 * plan_max_tiles(items, p.keys);
     p.pair = q; q += P; p.row = q; q += P; p.expert = q; q += P; p.pos = q; q += P;
     p.hist = q; q += p.keys * plan_blocks(items);
     if (ints) *ints = q - (int *)mem;

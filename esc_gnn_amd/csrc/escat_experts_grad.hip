@@ -104,6 +104,7 @@ __global__ void __launch_bounds__(XT, 2) k_expert_grad(const GradArgs g)
         {
 #pragma unroll
             for (int i = 0; i < 4; ++i) { it.row[i] = it.row_next[i]; it.pos[i] = it.pos_next[i]; }
+            it.fetch();                                       // before the data: memory answers in order, and the next step waits for these
 #pragma unroll
             for (int i = 0; i < 4; ++i) r[i] = load16((const T *)g.a + (int64_t)(W2 ? it.pos[i] : it.row[i]) * g.M + cols.at);
         }
@@ -119,7 +120,6 @@ __global__ void __launch_bounds__(XT, 2) k_expert_grad(const GradArgs g)
                 r[i] = load16((const T *)g.b + (int64_t)(W2 ? it.row[i] : it.pos[i]) * g.N + cols.at);
                 if (W2) w[set][i] = g.weights[it.pos[i]];
             }
-            it.fetch();
         }
         __device__ __forceinline__ void fix(u4 (&r)[4], int set)
         {
@@ -140,7 +140,10 @@ __global__ void __launch_bounds__(XT, 2) k_expert_grad(const GradArgs g)
     acc_t acc[2][2];
     clear(acc);
     if (K > 0) it.fetch();
-    tile_loop<2, T, true, true>((K + KB - 1) / KB, lds, am, bn, acc, A, B);
+    const int steps = (K + KB - 1) / KB;
+    Pipe<2, T, true, true> pipe;
+    pipe.start(steps, A, B);
+    pipe.run(steps, lds, am, bn, acc, A, B);
 
     float *part = g.chunk ? g.part + (int64_t)q * ((int64_t)N * M + N) : nullptr;
     if (sums) {                                               // the threads that hold the same features join in a fixed order

@@ -119,7 +119,10 @@ __global__ void __launch_bounds__(1024) k_plan_scan(int E, int blocks, EPlan p)
     for (int e = threadIdx.x; e < E; e += 1024) { p.count[e] = cnt[e]; p.first[e] = first[e]; }
     if (threadIdx.x == 0) p.first[E] = first[E];
     for (int e = wave; e < E; e += 16)
-        for (int t = tfirst[e] + lane; t < tfirst[e + 1]; t += 64) { p.tile[2 * t] = e; p.tile[2 * t + 1] = first[e] + (t - tfirst[e]) * XM; }
+        for (int t = tfirst[e] + lane; t < tfirst[e + 1]; t += 64) {
+            const int at = (t - tfirst[e]) * XM;
+            *(int4 *)(p.tile + 4 * t) = make_int4(e, first[e] + at, cnt[e] - at < XM ? cnt[e] - at : XM, 0);
+        }
 }
 
 __global__ void __launch_bounds__(PT) k_plan_place(const Items it, int bits, EPlan p)
@@ -201,6 +204,7 @@ extern "C" int escat_experts_plan(const int32_t *experts, int64_t rows, int k, i
     int rc = plan_check("escat_experts_plan", rows, k, E); if (rc) return rc;
     if (rows > 0 && !experts) return fail(ESCAT_EINVAL, "escat_experts_plan: experts is null");
     if (counts && k != 1) return fail(ESCAT_EINVAL, "escat_experts_plan: counts are given for k = 1 (k = %d)", k);
+    if (((uintptr_t)plan & 15) != 0) return fail(ESCAT_EINVAL, "escat_experts_plan: plan is not aligned to 16 bytes");
     if (!plan || plan_bytes < escat_experts_plan_bytes(rows, k, E)) return fail(ESCAT_EWORKSPACE, "escat_experts_plan: plan of %zu bytes, needs %zu", plan_bytes, escat_experts_plan_bytes(rows, k, E));
     hipStream_t st = (hipStream_t)stream;
     const EPlan p = plan_of(plan, rows, k, E);

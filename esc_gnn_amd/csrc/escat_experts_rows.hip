@@ -26,7 +26,7 @@ struct RowArgs {
 enum { FWD1, FWD2, BWD1, BWD2 };
 
 // the hardware's exponential errs by |u| 2^-24: below what 16-bit operands leave, not below what fp32 ones do
-template <typename T> __device__ __forceinline__ float sigmoid_of(float u) { return 1.f / (1.f + (sizeof(T) == 4 ? expf(-u) : __expf(-u))); }
+template <typename T> __device__ __forceinline__ float sigmoid_of(float u) { return __builtin_amdgcn_rcpf(1.f + (sizeof(T) == 4 ? expf(-u) : __expf(-u))); }
 
 template <typename T, int MODE, bool DIRECT>
 __global__ void __launch_bounds__(XT, 2) k_expert_rows(const RowArgs a)
@@ -40,20 +40,25 @@ __global__ void __launch_bounds__(XT, 2) k_expert_rows(const RowArgs a)
     const int live = *a.p.n_tiles * of;                              // (the grid covers the most tiles there can be)
     if ((int)blockIdx.x >= live) return;
     const int work = xcd_swizzle(blockIdx.x, live), t = work / of, rest = work - t * of, dig = ONE ? rest / mt : 0, m0 = (rest - dig * mt) * XN;
-    const int key = a.p.tile[2 * t], r0 = a.p.tile[2 * t + 1];
+    const int4 tile = *(const int4 *)(a.p.tile + 4 * t);
+    const int key = tile.x, r0 = tile.y, rows = tile.z;
     const int e = key_digit(a.p, key, dig);
     if (ONE && e >= a.n.E) return;
-    const int rows = a.p.first[key + 1] - r0 < XM ? a.p.first[key + 1] - r0 : XM;
 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, am = (wave & 1) * 64, bn = (wave >> 1) * 64;
     typedef Stage<T, false> SC;
     // rows behind the last of the tile repeat it: their results are not written
     const int rl[2] = {bn + (lane & 31) < rows ? bn + (lane & 31) : 0, bn + 32 + (lane & 31) < rows ? bn + 32 + (lane & 31) : 0};
     float wr[2];                                                    // weights of the two rows whose results the lane holds
-#pragma unroll
-    for (int j = 0; j < 2; ++j) wr[j] = ONE ? a.weights[a.p.pair[(int64_t)(r0 + rl[j]) * per + dig]] : 0.f;
     __shared__ __align__(16) float bias[XN];
-    if (ONE && threadIdx.x < XN) bias[threadIdx.x] = a.b1 && m0 + (int)threadIdx.x < M ? to_f32(((const T *)a.b1)[(int64_t)e * M + m0 + threadIdx.x]) : 0.f;
+    float bias_m = 0.f;
+    // what the epilogue needs, asked for once the first pieces of the operands are on their way
+    auto fetch_rest = [&]() {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) wr[j] = ONE ? a.weights[a.p.pair[(int64_t)(r0 + rl[j]) * per + dig]] : 0.f;
+        const int m = m0 + (int)(threadIdx.x % XN);
+        if (ONE && a.b1) bias_m = to_f32(((const T *)a.b1)[(int64_t)e * M + (m < M ? m : M - 1)]);
+    };
     acc_t acc[2][2], acc2[2][2];
     clear(acc);
     float dot[4] = {0.f, 0.f, 0.f, 0.f};                            // BWD1: the thread's share of b2 . dy of its rows
@@ -72,23 +77,34 @@ __global__ void __launch_bounds__(XT, 2) k_expert_rows(const RowArgs a)
             B.p[i] = (const T *)a.x + row * D;
             if (MODE == BWD1) dy[i] = (const T *)a.dy + row * O;
         }
-        tile_loop<MODE == BWD1 ? 1 : 2, T, false, false>((D + KB - 1) / KB, lds, am, bn, acc, A, B);
-        if constexpr (MODE == BWD1) {
+        Pipe<MODE == BWD1 ? 1 : 2, T, false, false> pipe;
+        const int steps_d = (D + KB - 1) / KB;
+        pipe.start(steps_d, A, B);
+        fetch_rest();
+        if constexpr (MODE == FWD1) pipe.run(steps_d, lds, am, bn, acc, A, B);
+        else {
             // ---- W2^T dy into the second set, and b2 . dy on the way
             auto w2 = [&](int) { return (const char *)a.w2 + (int64_t)e * O * H * (int64_t)sizeof(T); };
             OperandKM<T, decltype(w2)> A2(O, m0, M, w2);
             struct WithDot : OperandKCRows<T> {
                 const T *b2;
                 float (&dot)[4];
+                u4 piece;
                 __device__ __forceinline__ WithDot(int K, const T *b2, float (&dot)[4]) : OperandKCRows<T>(K), b2(b2), dot(dot) {}
+                __device__ __forceinline__ void load(u4 (&r)[4], int set)
+                {
+                    const int k0 = this->k0 + this->c, K = this->K;
+                    piece = load16(b2 + (k0 < K - PER ? k0 : K - PER));
+                    OperandKCRows<T>::load(r, set);
+                }
                 __device__ __forceinline__ void fix(u4 (&r)[4], int set)
                 {
-                    const int k0 = this->fk0 + this->c, K = this->K;
+                    u4 b[4] = {piece, piece, piece, piece};
+                    int k0 = this->fk0;
+                    fix_kc<T>(b, this->K, this->c, k0);
                     OperandKCRows<T>::fix(r, set);
-                    if (!b2) return;
                     float f[PER], g[PER];
-#pragma unroll
-                    for (int q = 0; q < PER; ++q) f[q] = to_f32(b2[k0 + q < K ? k0 + q : K - 1]);
+                    to_floats<T>(b[0], f);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         to_floats<T>(r[i], g);
@@ -96,11 +112,23 @@ __global__ void __launch_bounds__(XT, 2) k_expert_rows(const RowArgs a)
                         for (int q = 0; q < PER; ++q) dot[i] = fmaf(f[q], g[q], dot[i]);
                     }
                 }
-            } B2(O, m0 == 0 && a.b2 ? (const T *)a.b2 + (int64_t)e * O : nullptr, dot);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) B2.p[i] = dy[i];
+            };
             clear(acc2);
-            tile_loop<1, T, true, false>((O + KB - 1) / KB, lds, am, bn, acc2, A2, B2);
+            const int steps = (O + KB - 1) / KB;
+            Pipe<1, T, true, false> pipe2;
+            if (m0 == 0 && a.b2) {
+                WithDot B2(O, (const T *)a.b2 + (int64_t)e * O, dot);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) B2.p[i] = dy[i];
+                pipe.run(steps_d, lds, am, bn, acc, A, B, [&]() { pipe2.start(steps, A2, B2); });
+                pipe2.run(steps, lds, am, bn, acc2, A2, B2);
+            } else {
+                OperandKCRows<T> B2(O);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) B2.p[i] = dy[i];
+                pipe.run(steps_d, lds, am, bn, acc, A, B, [&]() { pipe2.start(steps, A2, B2); });
+                pipe2.run(steps, lds, am, bn, acc2, A2, B2);
+            }
         }
     } else {
         // ---- W2 (w h) or W1^T du of the tile's experts, one after the other into the same accumulators
@@ -122,10 +150,14 @@ __global__ void __launch_bounds__(XT, 2) k_expert_rows(const RowArgs a)
             OperandKC<T, decltype(weights)> A(H, weights);
 #pragma unroll
             for (int i = 0; i < 4; ++i) A.off[i] = (uint32_t)(m0 + SC::row(i) < M ? m0 + SC::row(i) : M - 1) * (uint32_t)H * (uint32_t)sizeof(T);
-            tile_loop<2, T, false, false>(steps, lds, am, bn, acc, A, B);
+            Pipe<2, T, false, false> pipe;
+            pipe.start(steps, A, B);
+            pipe.run(steps, lds, am, bn, acc, A, B);
         } else {
             OperandKM<T, decltype(weights)> A(H, m0, M, weights);
-            tile_loop<2, T, true, false>(steps, lds, am, bn, acc, A, B);
+            Pipe<2, T, true, false> pipe;
+            pipe.start(steps, A, B);
+            pipe.run(steps, lds, am, bn, acc, A, B);
         }
     }
 
@@ -153,6 +185,10 @@ __global__ void __launch_bounds__(XT, 2) k_expert_rows(const RowArgs a)
     // ---- epilogue.  The lane holds, for each of two rows, runs of four features; they leave through LDS
     typedef typename std::conditional<ONE || DIRECT, T, float>::type OUT;
     const int cols = M - m0 < XN ? M - m0 : XN;
+    if (ONE) {
+        if (threadIdx.x < XN) bias[threadIdx.x] = bias_m;
+        __syncthreads();
+    }
     __shared__ float red[3 * 128];                                  // BWD1: sums over the features of a half, b2 . dy
     if (MODE == BWD1) {
 #pragma unroll
@@ -171,7 +207,7 @@ __global__ void __launch_bounds__(XT, 2) k_expert_rows(const RowArgs a)
         for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                const int mt_ = am + 32 * i + 8 * q + 4 * (lane >> 5), m = m0 + mt_;
+                const int mt_ = am + 32 * i + 8 * q + 4 * (lane >> 5);
                 float u[4], g[4];
                 f4 bv = {0.f, 0.f, 0.f, 0.f};
                 if (ONE) bv = *(const f4 *)(bias + mt_);
@@ -189,7 +225,7 @@ __global__ void __launch_bounds__(XT, 2) k_expert_rows(const RowArgs a)
 #pragma unroll
                     for (int z = 0; z < 4; ++z) {
                         const float sg = sigmoid_of<T>(u[z]), hh = u[z] * sg;
-                        if (m + z < M) sum = fmaf(hh, g[z], sum);
+                        sum = fmaf(hh, g[z], sum);                  // (features behind the last: g = 0)
                         acc2[i][j][4 * q + z] = w * g[z] * (sg * (1.f + u[z] * (1.f - sg)));
                         u[z] = w * hh;
                     }

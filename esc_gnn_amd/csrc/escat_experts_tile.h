@@ -150,70 +150,84 @@ __device__ __forceinline__ void tile_step(const char *la, const char *lb, int am
 // ---- the loop over the steps.  a / b: operands with load(regs, set) -- the thread's pieces of the next step, AHEAD = 1 or 2 steps ahead of
 // their use (a step's products take less time than memory does; 1 where two sets of accumulators leave no registers for 2) -- and
 // fix(regs, set) -- the same pieces once they have arrived (a use inside load would wait for them there); both are called once a step, in
-// order; set = step & 1, or 0.  lds: 4 tiles (A0 B0 A1 B1), free to be written on return.
-template <int AHEAD, typename T, bool AKM, bool BKM, typename A, typename B>
-__device__ __forceinline__ void tile_loop(int steps, char *lds, int am, int bn, acc_t (&acc)[2][2], A &a, B &b)
-{
-    if (steps == 0) return;
-    char *buf0 = lds, *buf1 = lds + 2 * TILE_BYTES;
+// order; set = step & 1, or 0.  start() issues the first loads, so that a kernel can do other things until run(); run calls `next` before
+// the last products, when no load is left to issue.  lds: 4 tiles (A0 B0 A1 B1), free to be written on return.
+struct Nothing { __device__ void operator()() const {} };
+template <int AHEAD, typename T, bool AKM, bool BKM> struct Pipe {
     u4 a0[4], b0[4], a1[4], b1[4];
-    // no load under a condition inside the loop: it would make the compiler wait for all of them at every turn
 #define LOAD(S) { a.load(a##S, S); b.load(b##S, S); }
 #define STORE_TO(S, D) { a.fix(a##S, S); b.fix(b##S, S); Stage<T, AKM>::store(buf##D, a##S); Stage<T, BKM>::store(buf##D + TILE_BYTES, b##S); __syncthreads(); }
 #define STORE(S) STORE_TO(S, S)
 #define MULTIPLY(S) tile_step<T, AKM, BKM>(buf##S, buf##S + TILE_BYTES, am, bn, acc);
-    LOAD(0)
-    if constexpr (AHEAD == 1) {
-        STORE(0)
-        int s = 0;
-        for (; s + 2 < steps; s += 2) {
-            LOAD(0)
-            MULTIPLY(0)
-            STORE_TO(0, 1)
-            LOAD(0)
-            MULTIPLY(1)
+    template <typename A, typename B> __device__ __forceinline__ void start(int steps, A &a, B &b)
+    {
+        if (steps > 0) LOAD(0)
+        if (AHEAD == 2 && steps > 1) LOAD(1)
+    }
+    // no load under a condition inside the loop: it would make the compiler wait for all of them at every turn
+    template <typename A, typename B, typename N = Nothing>
+    __device__ __forceinline__ void run(int steps, char *lds, int am, int bn, acc_t (&acc)[2][2], A &a, B &b, N next = N())
+    {
+        if (steps == 0) { next(); return; }
+        char *buf0 = lds, *buf1 = lds + 2 * TILE_BYTES;
+        if constexpr (AHEAD == 1) {
             STORE(0)
-        }
-        if (s + 2 == steps) {
-            LOAD(0)
-            MULTIPLY(0)
-            STORE_TO(0, 1)
-            MULTIPLY(1)
-        } else MULTIPLY(0)
-    } else if (steps == 1) {
-        STORE(0)
-        MULTIPLY(0)
-    } else {
-        LOAD(1)
-        STORE(0)
-        int s = 0;
-        for (; s + 3 < steps; s += 2) {
-            LOAD(0)
-            MULTIPLY(0)
-            STORE(1)
-            LOAD(1)
-            MULTIPLY(1)
+            int s = 0;
+            for (; s + 2 < steps; s += 2) {
+                LOAD(0)
+                MULTIPLY(0)
+                STORE_TO(0, 1)
+                LOAD(0)
+                MULTIPLY(1)
+                STORE(0)
+            }
+            if (s + 2 == steps) {
+                LOAD(0)
+                MULTIPLY(0)
+                STORE_TO(0, 1)
+                next();
+                MULTIPLY(1)
+            } else {
+                next();
+                MULTIPLY(0)
+            }
+        } else if (steps == 1) {
             STORE(0)
-        }
-        if (s + 3 == steps) {
-            LOAD(0)
-            MULTIPLY(0)
-            STORE(1)
-            MULTIPLY(1)
-            STORE(0)
+            next();
             MULTIPLY(0)
         } else {
-            MULTIPLY(0)
-            STORE(1)
-            MULTIPLY(1)
+            STORE(0)
+            int s = 0;
+            for (; s + 3 < steps; s += 2) {
+                LOAD(0)
+                MULTIPLY(0)
+                STORE(1)
+                LOAD(1)
+                MULTIPLY(1)
+                STORE(0)
+            }
+            if (s + 3 == steps) {
+                LOAD(0)
+                MULTIPLY(0)
+                STORE(1)
+                MULTIPLY(1)
+                STORE(0)
+                next();
+                MULTIPLY(0)
+            } else {
+                MULTIPLY(0)
+                STORE(1)
+                next();
+                MULTIPLY(1)
+            }
         }
+        __syncthreads();
     }
-    __syncthreads();
 #undef LOAD
 #undef STORE
 #undef STORE_TO
 #undef MULTIPLY
-}
+};
 
 template <typename T> __device__ __forceinline__ void fix_kc(u4 (&r)[4], int K, int c, int &k0);
 // ---- operands.  An operand walks through one or more segments of K values of k (by combination: one for each expert of the tile), each
