@@ -29,7 +29,7 @@ enum { FWD1, FWD2, BWD1, BWD2 };
 template <typename T> __device__ __forceinline__ float sigmoid_of(float u) { return __builtin_amdgcn_rcpf(1.f + (sizeof(T) == 4 ? expf(-u) : __expf(-u))); }
 
 template <typename T, int MODE, bool DIRECT>
-__global__ void __launch_bounds__(XT, 2) k_expert_rows(const RowArgs a)
+__global__ void __launch_bounds__(XT, sizeof(T) == 2 && MODE != BWD1 ? 3 : 2) k_expert_rows(const RowArgs a)
 {
     constexpr int PER = Elem<T>::PER, KB = Elem<T>::KB;
     extern __shared__ __align__(16) char lds[];
@@ -59,6 +59,7 @@ __global__ void __launch_bounds__(XT, 2) k_expert_rows(const RowArgs a)
         const int m = m0 + (int)(threadIdx.x % XN);
         if (ONE && a.b1) bias_m = to_f32(((const T *)a.b1)[(int64_t)e * M + (m < M ? m : M - 1)]);
     };
+    constexpr int AHEAD = sizeof(T) == 4 ? 2 : 0;
     acc_t acc[2][2], acc2[2][2];
     clear(acc);
     float dot[4] = {0.f, 0.f, 0.f, 0.f};                            // BWD1: the thread's share of b2 . dy of its rows
@@ -77,7 +78,7 @@ __global__ void __launch_bounds__(XT, 2) k_expert_rows(const RowArgs a)
             B.p[i] = (const T *)a.x + row * D;
             if (MODE == BWD1) dy[i] = (const T *)a.dy + row * O;
         }
-        Pipe<MODE == BWD1 ? 1 : 2, T, false, false> pipe;
+        Pipe<MODE == BWD1 ? 1 : AHEAD, T, false, false> pipe;
         const int steps_d = (D + KB - 1) / KB;
         pipe.start(steps_d, A, B);
         fetch_rest();
@@ -150,12 +151,12 @@ __global__ void __launch_bounds__(XT, 2) k_expert_rows(const RowArgs a)
             OperandKC<T, decltype(weights)> A(H, weights);
 #pragma unroll
             for (int i = 0; i < 4; ++i) A.off[i] = (uint32_t)(m0 + SC::row(i) < M ? m0 + SC::row(i) : M - 1) * (uint32_t)H * (uint32_t)sizeof(T);
-            Pipe<2, T, false, false> pipe;
+            Pipe<AHEAD, T, false, false> pipe;
             pipe.start(steps, A, B);
             pipe.run(steps, lds, am, bn, acc, A, B);
         } else {
             OperandKM<T, decltype(weights)> A(H, m0, M, weights);
-            Pipe<2, T, true, false> pipe;
+            Pipe<AHEAD, T, true, false> pipe;
             pipe.start(steps, A, B);
             pipe.run(steps, lds, am, bn, acc, A, B);
         }
@@ -317,7 +318,7 @@ template <typename T, int MODE, bool DIRECT> static int rows_launch(const RowArg
     const int64_t items = a.p.base ? a.n.rows : a.n.rows * a.n.k;
     const int64_t wgs = plan_max_tiles(items, a.p.keys) * ((M + XN - 1) / XN) * (ONE ? a.p.per : 1);
     if (wgs > 0xffffff) return fail(ESCAT_ERANGE, "experts: %lld tiles", (long long)wgs);
-    const size_t lds = !(ONE || DIRECT) || sizeof(T) == 4 ? LDS_ROWS : LDS_TILES;
+    const size_t lds = !(ONE || DIRECT) || sizeof(T) == 4 ? LDS_ROWS : MODE == BWD1 ? LDS_TILES : Spill<T>::BYTES;
     int rc = set_lds(k_expert_rows<T, MODE, DIRECT>, lds); if (rc) return rc;
     k_expert_rows<T, MODE, DIRECT><<<(unsigned)wgs, XT, lds, st>>>(a);
     CHECK_LAUNCH("experts: rows");

@@ -153,6 +153,7 @@ __device__ __forceinline__ void tile_step(const char *la, const char *lb, int am
 // order; set = step & 1, or 0.  start() issues the first loads, so that a kernel can do other things until run(); run calls `next` before
 // the last products, when no load is left to issue.  lds: 4 tiles (A0 B0 A1 B1), free to be written on return.
 struct Nothing { __device__ void operator()() const {} };
+// AHEAD = 0: one buffer (A0 B0) and one set of registers, two barriers a step; three workgroups share a CU and hide each other's waits
 template <int AHEAD, typename T, bool AKM, bool BKM> struct Pipe {
     u4 a0[4], b0[4], a1[4], b1[4];
 #define LOAD(S) { a.load(a##S, S); b.load(b##S, S); }
@@ -170,7 +171,17 @@ template <int AHEAD, typename T, bool AKM, bool BKM> struct Pipe {
     {
         if (steps == 0) { next(); return; }
         char *buf0 = lds, *buf1 = lds + 2 * TILE_BYTES;
-        if constexpr (AHEAD == 1) {
+        if constexpr (AHEAD == 0) {
+            for (int s = 1; s < steps; ++s) {
+                STORE(0)
+                LOAD(0)
+                MULTIPLY(0)
+                __syncthreads();
+            }
+            STORE(0)
+            next();
+            MULTIPLY(0)
+        } else if constexpr (AHEAD == 1) {
             STORE(0)
             int s = 0;
             for (; s + 2 < steps; s += 2) {
