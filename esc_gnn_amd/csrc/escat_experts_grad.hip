@@ -8,6 +8,8 @@
 // gradients ride along: a tile's B pieces pass through registers anyway.
 #include "escat_experts_tile.h"
 
+#define GRAD_AHEAD(T) (sizeof(T) == 4 ? 2 : 0)
+
 struct GradArgs {
     EDims n;
     EPlan p;                   // by pair: items in the order of the sums
@@ -47,26 +49,9 @@ __device__ __forceinline__ int find_chunk(const int *count, int E, int chunk, in
     return -1;
 }
 
-template <typename OUT> __device__ __forceinline__ void spill(char *lds, const acc_t (&acc)[2][2], int am, int bn)
-{
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                float v[4];
-#pragma unroll
-                for (int z = 0; z < 4; ++z) v[z] = acc[i][j][4 * q + z];
-                Spill<OUT>::put(lds, bn + 32 * j + (lane & 31), am + 32 * i + 8 * q + 4 * (lane >> 5), v);
-            }
-    __syncthreads();
-}
-
 // W2: A by sorted position, B gathered by row and weighted for db; else A gathered by row, B by sorted position
 template <typename T, bool W2>
-__global__ void __launch_bounds__(XT, 2) k_expert_grad(const GradArgs g)
+__global__ void __launch_bounds__(XT, GRAD_AHEAD(T) == 0 ? 3 : 2) k_expert_grad(const GradArgs g)
 {
     constexpr int PER = Elem<T>::PER, KB = Elem<T>::KB;
     extern __shared__ __align__(16) char lds[];
@@ -141,7 +126,7 @@ __global__ void __launch_bounds__(XT, 2) k_expert_grad(const GradArgs g)
     clear(acc);
     if (K > 0) it.fetch();
     const int steps = (K + KB - 1) / KB;
-    Pipe<2, T, true, true> pipe;
+    Pipe<GRAD_AHEAD(T), T, true, true> pipe;
     pipe.start(steps, A, B);
     pipe.run(steps, lds, am, bn, acc, A, B);
 
@@ -162,11 +147,9 @@ __global__ void __launch_bounds__(XT, 2) k_expert_grad(const GradArgs g)
     if (sums) __syncthreads();
     const int cols = M - m0 < XN ? M - m0 : XN, rows = N - n0 < XN ? N - n0 : XN;
     if (part) {
-        spill<float>(lds, acc, am, bn);
-        Spill<float>::write(lds, part + (int64_t)n0 * M + m0, M, rows, cols, [](int r) { return r; });
+        Spill<float>::all(lds, acc, am, bn, part + (int64_t)n0 * M + m0, M, rows, cols, [](int r) { return r; });
     } else {
-        spill<T>(lds, acc, am, bn);
-        Spill<T>::write(lds, (T *)g.out + ((int64_t)e * N + n0) * M + m0, M, rows, cols, [](int r) { return r; });
+        Spill<T>::all(lds, acc, am, bn, (T *)g.out + ((int64_t)e * N + n0) * M + m0, M, rows, cols, [](int r) { return r; });
     }
 }
 
@@ -229,7 +212,7 @@ template <typename T, bool W2> static int launch(const GradArgs &g, hipStream_t 
     const int64_t tiles = (int64_t)((g.M + XN - 1) / XN) * ((g.N + XN - 1) / XN);
     const int64_t wgs = tiles * escat_experts_grad_chunks(g.n.rows * g.n.k, g.n.E, g.chunk);
     if (wgs > 0xffffff) return fail(ESCAT_ERANGE, "experts: %lld tiles", (long long)wgs);
-    const size_t lds = g.chunk || sizeof(T) == 4 ? LDS_ROWS : LDS_TILES;
+    constexpr size_t lds = LDS_BYTES(GRAD_AHEAD(T));
     int rc = set_lds(k_expert_grad<T, W2>, lds); if (rc) return rc;
     k_expert_grad<T, W2><<<(unsigned)wgs, XT, lds, st>>>(g);
     CHECK_LAUNCH("experts: weight gradient");

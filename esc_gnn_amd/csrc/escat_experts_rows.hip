@@ -24,14 +24,19 @@ struct RowArgs {
 };
 
 enum { FWD1, FWD2, BWD1, BWD2 };
+// 16-bit products: one LDS buffer and three workgroups a CU, which hide each other's waits (measured against two steps ahead in two workgroups:
+// 349 instead of 391 us for 137 GFLOP at K = 256, the same at K = 1024).  fp32 products are matrix-bound: two steps ahead.  BWD1 holds two
+// sets of accumulators: one step ahead, two workgroups.
+template <typename T, int MODE> constexpr int ahead_of() { return MODE == BWD1 ? 1 : sizeof(T) == 4 ? 2 : 0; }
 
 // the hardware's exponential errs by |u| 2^-24: below what 16-bit operands leave, not below what fp32 ones do
 template <typename T> __device__ __forceinline__ float sigmoid_of(float u) { return __builtin_amdgcn_rcpf(1.f + (sizeof(T) == 4 ? expf(-u) : __expf(-u))); }
 
 template <typename T, int MODE, bool DIRECT>
-__global__ void __launch_bounds__(XT, sizeof(T) == 2 && MODE != BWD1 ? 3 : 2) k_expert_rows(const RowArgs a)
+__global__ void __launch_bounds__(XT, ((ahead_of<T, MODE>()) == 0 ? 3 : 2)) k_expert_rows(const RowArgs a)
 {
     constexpr int PER = Elem<T>::PER, KB = Elem<T>::KB;
+    constexpr int AHEAD = ahead_of<T, MODE>();
     extern __shared__ __align__(16) char lds[];
     const int D = a.n.d, H = a.n.h, O = a.n.o;
     const int M = MODE == FWD2 ? O : MODE == BWD2 ? D : H;          // features of the result
@@ -59,7 +64,6 @@ __global__ void __launch_bounds__(XT, sizeof(T) == 2 && MODE != BWD1 ? 3 : 2) k_
         const int m = m0 + (int)(threadIdx.x % XN);
         if (ONE && a.b1) bias_m = to_f32(((const T *)a.b1)[(int64_t)e * M + (m < M ? m : M - 1)]);
     };
-    constexpr int AHEAD = sizeof(T) == 4 ? 2 : 0;
     acc_t acc[2][2], acc2[2][2];
     clear(acc);
     float dot[4] = {0.f, 0.f, 0.f, 0.f};                            // BWD1: the thread's share of b2 . dy of its rows
@@ -78,12 +82,12 @@ __global__ void __launch_bounds__(XT, sizeof(T) == 2 && MODE != BWD1 ? 3 : 2) k_
             B.p[i] = (const T *)a.x + row * D;
             if (MODE == BWD1) dy[i] = (const T *)a.dy + row * O;
         }
-        Pipe<MODE == BWD1 ? 1 : AHEAD, T, false, false> pipe;
+        Pipe<AHEAD, T, false, false> pipe;
         const int steps_d = (D + KB - 1) / KB;
         pipe.start(steps_d, A, B);
         fetch_rest();
-        if constexpr (MODE == FWD1) pipe.run(steps_d, lds, am, bn, acc, A, B);
-        else {
+        pipe.run(steps_d, lds, am, bn, acc, A, B);
+        if constexpr (MODE == BWD1) {
             // ---- W2^T dy into the second set, and b2 . dy on the way
             auto w2 = [&](int) { return (const char *)a.w2 + (int64_t)e * O * H * (int64_t)sizeof(T); };
             OperandKM<T, decltype(w2)> A2(O, m0, M, w2);
@@ -116,18 +120,18 @@ __global__ void __launch_bounds__(XT, sizeof(T) == 2 && MODE != BWD1 ? 3 : 2) k_
             };
             clear(acc2);
             const int steps = (O + KB - 1) / KB;
-            Pipe<1, T, true, false> pipe2;
+            Pipe<AHEAD, T, true, false> pipe2;
             if (m0 == 0 && a.b2) {
                 WithDot B2(O, (const T *)a.b2 + (int64_t)e * O, dot);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) B2.p[i] = dy[i];
-                pipe.run(steps_d, lds, am, bn, acc, A, B, [&]() { pipe2.start(steps, A2, B2); });
+                pipe2.start(steps, A2, B2);
                 pipe2.run(steps, lds, am, bn, acc2, A2, B2);
             } else {
                 OperandKCRows<T> B2(O);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) B2.p[i] = dy[i];
-                pipe.run(steps_d, lds, am, bn, acc, A, B, [&]() { pipe2.start(steps, A2, B2); });
+                pipe2.start(steps, A2, B2);
                 pipe2.run(steps, lds, am, bn, acc2, A2, B2);
             }
         }
@@ -209,29 +213,22 @@ __global__ void __launch_bounds__(XT, sizeof(T) == 2 && MODE != BWD1 ? 3 : 2) k_
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const int mt_ = am + 32 * i + 8 * q + 4 * (lane >> 5);
-                float u[4], g[4];
                 f4 bv = {0.f, 0.f, 0.f, 0.f};
                 if (ONE) bv = *(const f4 *)(bias + mt_);
 #pragma unroll
                 for (int z = 0; z < 4; ++z) {
-                    u[z] = acc[i][j][4 * q + z];
-                    if (MODE == BWD1) g[z] = acc2[i][j][4 * q + z];
-                    if (ONE) u[z] += bv[z];
-                }
-                if (MODE == FWD1) {
-#pragma unroll
-                    for (int z = 0; z < 4; ++z) u[z] = w * (u[z] * sigmoid_of<T>(u[z]));
-                }
-                if (MODE == BWD1) {
-#pragma unroll
-                    for (int z = 0; z < 4; ++z) {
-                        const float sg = sigmoid_of<T>(u[z]), hh = u[z] * sg;
-                        sum = fmaf(hh, g[z], sum);                  // (features behind the last: g = 0)
-                        acc2[i][j][4 * q + z] = w * g[z] * (sg * (1.f + u[z] * (1.f - sg)));
-                        u[z] = w * hh;
+                    float v = acc[i][j][4 * q + z];
+                    if (ONE) v += bv[z];
+                    if (MODE == FWD1) v = w * (v * sigmoid_of<T>(v));
+                    if (MODE == BWD1) {
+                        const float g = acc2[i][j][4 * q + z];
+                        const float sg = sigmoid_of<T>(v), hh = v * sg;
+                        sum = fmaf(hh, g, sum);                     // (features behind the last: g = 0)
+                        acc2[i][j][4 * q + z] = w * g * (sg * (1.f + v * (1.f - sg)));
+                        v = w * hh;
                     }
+                    acc[i][j][4 * q + z] = v;
                 }
-                Spill<OUT>::put(lds, r, mt_, u);
             }
         if (MODE == BWD1 && m0 == 0 && am == 0 && lane < 32 && r < rows) a.ws[(int64_t)(r0 + r) * per + dig] = w;
         if (MODE == BWD1) {
@@ -239,29 +236,17 @@ __global__ void __launch_bounds__(XT, sizeof(T) == 2 && MODE != BWD1 ? 3 : 2) k_
             if (lane < 32) red[(wave & 1) * 128 + r] = sum;
         }
     }
-    __syncthreads();
     const int *row = a.p.row;
-    if (ONE) Spill<OUT>::write(lds, (OUT *)a.h + m0, M, rows, cols, [&](int r) { return (int64_t)(r0 + r) * per + dig; });
-    else if (DIRECT) Spill<OUT>::write(lds, (OUT *)a.out + m0, M, rows, cols, [&](int r) { return row[(int64_t)(r0 + r) * per]; });
-    else Spill<OUT>::write(lds, (OUT *)a.part + m0, M, rows, cols, [&](int r) { return r0 + r; });
+    auto by_pos = [&](int r) { return (int64_t)(r0 + r) * per + dig; };
+    if (ONE) Spill<OUT>::all(lds, acc, am, bn, (OUT *)a.h + m0, M, rows, cols, by_pos);
+    else if (DIRECT) Spill<OUT>::all(lds, acc, am, bn, (OUT *)a.out + m0, M, rows, cols, [&](int r) { return row[(int64_t)(r0 + r) * per]; });
+    else Spill<OUT>::all(lds, acc, am, bn, (OUT *)a.part + m0, M, rows, cols, [&](int r) { return r0 + r; });
     if (MODE == BWD1) {
         const int r = threadIdx.x;
         const int64_t P = a.n.rows * a.n.k;
-        if (r < rows) a.dwp[(int64_t)(m0 / XN) * P + (int64_t)(r0 + r) * per + dig] = red[r] + red[128 + r] + (m0 == 0 && a.b2 ? red[256 + r] : 0.f);
+        if (r < rows) a.dwp[(int64_t)(m0 / XN) * P + by_pos(r)] = red[r] + red[128 + r] + (m0 == 0 && a.b2 ? red[256 + r] : 0.f);
         __syncthreads();
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    float g[4];
-#pragma unroll
-                    for (int z = 0; z < 4; ++z) g[z] = acc2[i][j][4 * q + z];
-                    Spill<OUT>::put(lds, bn + 32 * j + (lane & 31), am + 32 * i + 8 * q + 4 * (lane >> 5), g);
-                }
-        __syncthreads();
-        Spill<OUT>::write(lds, (OUT *)a.du + m0, M, rows, cols, [&](int r) { return (int64_t)(r0 + r) * per + dig; });
+        Spill<OUT>::all(lds, acc2, am, bn, (OUT *)a.du + m0, M, rows, cols, by_pos);
     }
 }
 
@@ -318,7 +303,7 @@ template <typename T, int MODE, bool DIRECT> static int rows_launch(const RowArg
     const int64_t items = a.p.base ? a.n.rows : a.n.rows * a.n.k;
     const int64_t wgs = plan_max_tiles(items, a.p.keys) * ((M + XN - 1) / XN) * (ONE ? a.p.per : 1);
     if (wgs > 0xffffff) return fail(ESCAT_ERANGE, "experts: %lld tiles", (long long)wgs);
-    const size_t lds = !(ONE || DIRECT) || sizeof(T) == 4 ? LDS_ROWS : MODE == BWD1 ? LDS_TILES : Spill<T>::BYTES;
+    constexpr size_t lds = LDS_BYTES((ahead_of<T, MODE>()));
     int rc = set_lds(k_expert_rows<T, MODE, DIRECT>, lds); if (rc) return rc;
     k_expert_rows<T, MODE, DIRECT><<<(unsigned)wgs, XT, lds, st>>>(a);
     CHECK_LAUNCH("experts: rows");

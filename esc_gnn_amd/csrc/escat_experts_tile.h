@@ -343,39 +343,50 @@ template <typename T, typename SEG> struct OperandKM {
     }
 };
 
-// ---- results through LDS, so that memory is written in whole rows of the tile.  put: the lane's run of four features m.. of row n
-// (tile coordinates); write: rows [0, rows), features [0, cols) to out + at(n) * ld.  OUT: element type.  A row of 128 OUT is OSTRIDE bytes apart
-// from the next: 16 more than its size, so that the runs of 32 rows fall on different banks.
+// ---- results through LDS, so that memory is written in whole rows of the tile: rows [0, rows), features [0, cols) to out + at(row) * ld.
+// A row of 128 OUT is STRIDE bytes from the next: 16 more than its size, so that the runs of 32 rows fall on different banks.  32-bit
+// results go in two halves of 64 rows: 34 KB hold either.  lds is free before (the caller's barrier) and in use on return.
 template <typename OUT> struct Spill {
-    static constexpr int STRIDE = 128 * (int)sizeof(OUT) + 16;
-    static constexpr int BYTES = 128 * STRIDE;
-    static __device__ __forceinline__ void put(char *lds, int n, int m, const float (&v)[4])
-    {
-        struct alignas(4 * sizeof(OUT)) { OUT v[4]; } q;
-#pragma unroll
-        for (int z = 0; z < 4; ++z) q.v[z] = from_f32<OUT>(v[z]);
-        __builtin_memcpy(__builtin_assume_aligned(lds + n * STRIDE + m * (int)sizeof(OUT), 4 * sizeof(OUT)), &q, sizeof(q));
-    }
-    // the caller has a barrier before and, if lds is used again, after
-    template <typename AT> static __device__ __forceinline__ void write(const char *lds, OUT *out, int64_t ld, int rows, int cols, AT at)
+    static constexpr int STRIDE = 128 * (int)sizeof(OUT) + 16, ROWS = sizeof(OUT) == 4 ? 64 : 128, BYTES = ROWS * STRIDE;
+    template <typename AT>
+    static __device__ __forceinline__ void all(char *lds, const acc_t (&acc)[2][2], int am, int bn, OUT *out, int64_t ld, int rows, int cols, AT at)
     {
         constexpr int PER = 16 / (int)sizeof(OUT), CPR = 128 / PER;
-        const int c = threadIdx.x % CPR * PER;
-        if (c >= cols) return;
-        for (int r = threadIdx.x / CPR; r < rows; r += XT / CPR) {
-            struct alignas(16) { OUT v[PER]; } q;
-            __builtin_memcpy(&q, __builtin_assume_aligned(lds + r * STRIDE + c * (int)sizeof(OUT), 16), 16);
-            OUT *o = out + (int64_t)at(r) * ld + c;
-            if (c + PER <= cols) { Pack<OUT, PER> p; __builtin_memcpy(&p, &q, 16); *(Pack<OUT, PER> *)o = p; }
-            else {
+        const int lane = threadIdx.x & 63, c = threadIdx.x % CPR * PER;
 #pragma unroll
-                for (int z = 0; z < PER; ++z) if (c + z < cols) o[z] = q.v[z];
+        for (int half = 0; half < 128 / ROWS; ++half) {
+            if (half) __syncthreads();
+            if (ROWS == 128 || bn == half * 64)
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            const int n = bn - half * 64 + 32 * j + (lane & 31), m = am + 32 * i + 8 * q + 4 * (lane >> 5);
+                            struct alignas(4 * sizeof(OUT)) { OUT v[4]; } p;
+#pragma unroll
+                            for (int z = 0; z < 4; ++z) p.v[z] = from_f32<OUT>(acc[i][j][4 * q + z]);
+                            __builtin_memcpy(__builtin_assume_aligned(lds + n * STRIDE + m * (int)sizeof(OUT), 4 * sizeof(OUT)), &p, sizeof(p));
+                        }
+            __syncthreads();
+            if (c >= cols) continue;
+            for (int r = threadIdx.x / CPR; r < ROWS && r + half * 64 < rows; r += XT / CPR) {
+                struct alignas(16) { OUT v[PER]; } q;
+                __builtin_memcpy(&q, __builtin_assume_aligned(lds + r * STRIDE + c * (int)sizeof(OUT), 16), 16);
+                OUT *o = out + (int64_t)at(r + half * 64) * ld + c;
+                if (c + PER <= cols) { Pack<OUT, PER> p; __builtin_memcpy(&p, &q, 16); *(Pack<OUT, PER> *)o = p; }
+                else {
+#pragma unroll
+                    for (int z = 0; z < PER; ++z) if (c + z < cols) o[z] = q.v[z];
+                }
             }
         }
     }
 };
-#define LDS_TILES (4 * TILE_BYTES)
-#define LDS_ROWS (Spill<float>::BYTES > LDS_TILES ? Spill<float>::BYTES : LDS_TILES)
+// LDS of a kernel whose Pipe is AHEAD steps ahead
+#define LDS_BYTES(AHEAD) ((AHEAD) == 0 ? 34816 : 4 * TILE_BYTES)
+static_assert(Spill<float>::BYTES <= 34816 && Spill<bf16_t>::BYTES <= 34816 && 2 * TILE_BYTES <= 34816, "LDS_BYTES");
 
 __device__ __forceinline__ void clear(acc_t (&acc)[2][2])
 {
