@@ -95,7 +95,8 @@ SIGNATURES = {
     "escat_experts_plan_bytes": (sz, [i64, ci, ci]),
     "escat_experts_plan": (ci, [vp, i64, ci, ci, vp, sz, vp, vp]),
     "escat_experts_workspace_bytes": (sz, [vp, ci]),
-    "escat_experts_fwd": (ci, [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]),
+    "escat_experts_fwd_needs_plan": (ci, [vp]),
+    "escat_experts_fwd": (ci, [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]),
     "escat_experts_bwd": (ci, [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]),
     "escat_lookup3": (ctypes.c_uint32, [ctypes.c_char_p, sz, ctypes.c_uint32]),
     "escat_build_workspace_bytes": (sz, [i64, ci, ci]),

@@ -72,6 +72,11 @@ __device__ __forceinline__ int key_digit(const EPlan &p, int key, int j)
     return key % p.base;
 }
 
+// bytes of weights that the pairs of a call may read, each for itself, in the form for few rows (escat_experts_few.hip)
+#ifndef ESCAT_FEW_BYTES
+#define ESCAT_FEW_BYTES (512ll << 20)
+#endif
+
 // workgroups of a launch go round the eight XCDs one by one, each with its own L2: give each XCD a run of neighbouring work items
 // (neighbours share the expert's weights and the rows).  A permutation of [0, n).
 __device__ __forceinline__ int xcd_swizzle(int b, int n)

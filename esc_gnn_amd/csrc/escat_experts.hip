@@ -11,6 +11,10 @@ __attribute__((visibility("hidden"))) int escat_experts_plan_by_expert(const EPl
 __attribute__((visibility("hidden"))) int escat_experts_grad(int type, const EDims &n, const EPlan &p, const int *at, bool w2, const void *a, const void *b, const float *weights, int M, int N,
                        int chunk, float *part, void *out, void *db, hipStream_t st);
 
+__attribute__((visibility("hidden"))) bool escat_experts_few(int type, const EDims &n);
+__attribute__((visibility("hidden"))) int escat_experts_few_fwd(int type, const EDims &n, const int *experts, const void *x, const float *weights, const void *w1, const void *b1,
+                          const void *w2, const void *b2, float *h, void *y, hipStream_t st);
+
 static int check_dims(const char *who, const escat_experts_dims *n)
 {
     if (!n) return fail(ESCAT_EINVAL, "%s: dims is null", who);
@@ -52,20 +56,29 @@ static size_t chunk_bytes(const escat_experts_dims *n, int M, int N)
 extern "C" size_t escat_experts_workspace_bytes(const escat_experts_dims *n, int backward)
 {
     if (check_dims("escat_experts_workspace_bytes", n)) return 0;
+    if (!backward && escat_experts_few(n->type, dims_of(n))) return up((size_t)n->rows * n->k * n->h * 4) + 256;
     if (!backward) return hidden_bytes(n) + part_bytes(n, n->o) + 256;
     const size_t c1 = chunk_bytes(n, n->d, n->h), c2 = chunk_bytes(n, n->h, n->o);
     return 2 * hidden_bytes(n) + part_bytes(n, n->d) + by_expert_bytes(n) + up((size_t)((n->h + XN - 1) / XN) * n->rows * n->k * 4) + up((size_t)n->rows * n->k * 4) + (c1 > c2 ? c1 : c2) + 256;
 }
 
-extern "C" int escat_experts_fwd(const escat_experts_dims *n, const void *x, const float *weights, const void *w1, const void *b1, const void *w2,
-                                 const void *b2, const void *plan, void *y, void *workspace, size_t workspace_bytes, void *stream)
+extern "C" int escat_experts_fwd_needs_plan(const escat_experts_dims *n)
+{
+    if (check_dims("escat_experts_fwd_needs_plan", n)) return 1;
+    return escat_experts_few(n->type, dims_of(n)) ? 0 : 1;
+}
+
+extern "C" int escat_experts_fwd(const escat_experts_dims *n, const void *x, const float *weights, const int32_t *experts_of_rows, const void *w1, const void *b1,
+                                 const void *w2, const void *b2, const void *plan, void *y, void *workspace, size_t workspace_bytes, void *stream)
 {
     int rc = check_dims("escat_experts_fwd", n); if (rc) return rc;
     if (n->rows == 0) return ESCAT_OK;
-    if (!x || !weights || !w1 || !w2 || !plan || !y) return fail(ESCAT_EINVAL, "escat_experts_fwd: null pointer");
+    const bool few = escat_experts_few(n->type, dims_of(n));
+    if (!x || !weights || !w1 || !w2 || !y || (few ? !experts_of_rows : !plan)) return fail(ESCAT_EINVAL, "escat_experts_fwd: null pointer");
     if (!workspace || workspace_bytes < escat_experts_workspace_bytes(n, 0) || ((uintptr_t)workspace & 15))
         return fail(ESCAT_EWORKSPACE, "escat_experts_fwd: workspace of %zu bytes (16-byte aligned), needs %zu", workspace_bytes, escat_experts_workspace_bytes(n, 0));
     char *ws = (char *)workspace;
+    if (few) return escat_experts_few_fwd(n->type, dims_of(n), experts_of_rows, x, weights, w1, b1, w2, b2, (float *)ws, y, (hipStream_t)stream);
     const EPlan p = plan_of(const_cast<void *>(plan), n->rows, n->k, n->experts);
     return escat_experts_rows_fwd(n->type, dims_of(n), p, x, weights, w1, b1, w2, b2, ws, (float *)(ws + hidden_bytes(n)), y, (hipStream_t)stream);
 }

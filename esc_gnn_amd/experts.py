@@ -32,6 +32,10 @@ def _need_gpu(t: torch.Tensor, name: str):
         raise RuntimeError(f"escat: {name} must live on a GPU; the MI355X path has no CPU fallback")
 
 
+def _wants_grad(ts) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+
+
 class _Route(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, bias, k, score, groups, keep, group_top, renorm, scale):
@@ -126,30 +130,35 @@ def expert_counts(experts: torch.Tensor, n_experts: int) -> torch.Tensor:
     return counts
 
 
+def _mlp_forward(x, weights, experts, w1, b1, w2, b2):
+    """y, and the plan where the forward made one (few rows do without)"""
+    lib = _lib.load()
+    (rows, d), k, (E, h, _), o = x.shape, experts.shape[1], w1.shape, w2.shape[1]
+    dims = _lib.EscatExpertsDims(rows, DTYPE_CODES[x.dtype], d, h, o, E, k)
+    at = ctypes.addressof(dims)
+    y = torch.empty((rows, o), dtype=x.dtype, device=x.device)
+    size = lib.escat_experts_workspace_bytes(at, 0)
+    with _on(x.device) as stream:
+        plan = _plan(experts, rows, k, E, None, stream) if lib.escat_experts_fwd_needs_plan(at) else None
+        ws = torch.empty(size, dtype=torch.uint8, device=x.device)
+        rc = lib.escat_experts_fwd(at, x.data_ptr(), weights.data_ptr(), experts.data_ptr(), w1.data_ptr(), _ptr(b1), w2.data_ptr(), _ptr(b2),
+                                   _ptr(plan), y.data_ptr(), ws.data_ptr(), size, stream)
+    _lib.check(rc, "escat_experts_fwd")
+    return y, plan, dims
+
+
 class _ExpertMLP(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weights, experts, w1, b1, w2, b2):
-        lib = _lib.load()
-        (rows, d), k, (E, h, _), o = x.shape, experts.shape[1], w1.shape, w2.shape[1]
-        dims = _lib.EscatExpertsDims(rows, DTYPE_CODES[x.dtype], d, h, o, E, k)
-        at = ctypes.addressof(dims)
-        y = torch.empty(rows, o, dtype=x.dtype, device=x.device)
-        size = lib.escat_experts_workspace_bytes(at, 0)
-        with _on(x.device) as stream:
-            plan = _plan(experts, rows, k, E, None, stream)
-            ws = torch.empty(size, dtype=torch.uint8, device=x.device)
-            rc = lib.escat_experts_fwd(at, x.data_ptr(), weights.data_ptr(), w1.data_ptr(), _ptr(b1), w2.data_ptr(), _ptr(b2), plan.data_ptr(),
-                                       y.data_ptr(), ws.data_ptr(), size, stream)
-        _lib.check(rc, "escat_experts_fwd")
-        ctx.save_for_backward(x, weights, w1, b1, w2, b2)
-        ctx.plan, ctx.dims = plan, dims
+        y, ctx.plan, ctx.dims = _mlp_forward(x, weights, experts, w1, b1, w2, b2)
+        ctx.save_for_backward(x, weights, experts, w1, b1, w2, b2)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         lib = _lib.load()
-        x, weights, w1, b1, w2, b2 = ctx.saved_tensors
+        x, weights, experts, w1, b1, w2, b2 = ctx.saved_tensors
         dims = ctx.dims
         at = ctypes.addressof(dims)
         dy = dy.contiguous()
@@ -160,8 +169,9 @@ class _ExpertMLP(torch.autograd.Function):
         dw1, dw2 = new(w1, need[3] or need[4]), new(w2, need[5] or need[6])
         size = lib.escat_experts_workspace_bytes(at, 1)
         with _on(x.device) as stream:
+            plan = ctx.plan if ctx.plan is not None else _plan(experts, dims.rows, dims.k, dims.experts, None, stream)
             ws = torch.empty(size, dtype=torch.uint8, device=x.device)
-            rc = lib.escat_experts_bwd(at, x.data_ptr(), weights.data_ptr(), w1.data_ptr(), _ptr(b1), w2.data_ptr(), _ptr(b2), ctx.plan.data_ptr(),
+            rc = lib.escat_experts_bwd(at, x.data_ptr(), weights.data_ptr(), w1.data_ptr(), _ptr(b1), w2.data_ptr(), _ptr(b2), plan.data_ptr(),
                                        dy.data_ptr(), _ptr(dx), _ptr(dweights), _ptr(dw1), _ptr(db1), _ptr(dw2), _ptr(db2), ws.data_ptr(), size,
                                        stream)
         _lib.check(rc, "escat_experts_bwd")
@@ -177,7 +187,8 @@ def expert_mlp(x: torch.Tensor, weights: torch.Tensor, experts: torch.Tensor, w1
     they are cast to its type); weights (rows, k) fp32, experts (rows, k) int32 as route_experts gives them.  A pair whose
     expert lies outside [0, E) counts for nothing and gets no gradient; the same expert may come twice in a row.  Sums are
     fp32; with 16-bit types the weighted hidden rows and their gradients are rounded to the type in between.  The backward
-    computes the hidden rows again: the forward keeps nothing but its arguments and the sorted pairs.  Weights must be
+    computes the hidden rows again: the forward keeps nothing but its arguments and the sorted pairs.  For a few rows the forward
+    is a pair of matrix-vector kernels that read the weights in use once a pair, without sorting.  Weights must be
     contiguous; d, h, o are free (any alignment), k <= 64, E <= 1024, rows * k < 2^30.
     """
     if torch.is_autocast_enabled("cuda") and x.is_cuda:
@@ -207,5 +218,6 @@ def expert_mlp(x: torch.Tensor, weights: torch.Tensor, experts: torch.Tensor, w1
         x = pad(x, (0, more(d)))
         w1, w2 = pad(w1, (0, more(d), 0, more(h))), pad(w2, (0, more(h), 0, more(o)))
         b1, b2 = None if b1 is None else pad(b1, (0, more(h))), None if b2 is None else pad(b2, (0, more(o)))
-    y = _ExpertMLP.apply(x.contiguous(), weights.contiguous(), experts.contiguous(), w1, b1, w2, b2)
+    args = (x.contiguous(), weights.contiguous(), experts.contiguous(), w1, b1, w2, b2)
+    y = _ExpertMLP.apply(*args) if _wants_grad(args) else _mlp_forward(*args)[0]
     return y if o >= least else y[:, :o].contiguous()

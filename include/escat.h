@@ -583,7 +583,8 @@ int escat_route_bwd(const void *logits, int type, int64_t rows, int E, int k, in
  *   weights (rows, k) fp32.
  * Rows have at least 16 bytes: d, h and o >= 4 (fp32) or 8 (pad narrower ones with zeros).
  * escat_experts_plan sorts experts_of_rows (rows, k) by expert into `plan` (escat_experts_plan_bytes), on the GPU, nothing read
- * back; counts (experts) int32, optional, for k = 1: entries of each expert.  escat_experts_fwd / _bwd read a plan of the same experts array.
+ * back; counts (experts) int32, optional, for k = 1: entries of each expert.  escat_experts_fwd / _bwd read a plan of the same experts array;
+ * where escat_experts_fwd_needs_plan is 0 (few rows) the forward reads the array itself and plan may be NULL.
  * escat_experts_bwd: gradients for dy (rows, o); dx, dweights, dw1 + db1, dw2 + db2 may each be NULL (a bias's gradient only
  * together with its weight's); the others are written whole (experts without a row: zeros).  Workspaces: 16-byte aligned, contents
  * only used within the call.  No atomics: the same inputs give the same bits. */
@@ -592,8 +593,10 @@ size_t escat_experts_plan_bytes(int64_t rows, int k, int experts);
 int escat_experts_plan(const int32_t *experts_of_rows, int64_t rows, int k, int experts, void *plan, size_t plan_bytes, int32_t *counts,
                        void *stream);
 size_t escat_experts_workspace_bytes(const escat_experts_dims *dims, int backward);
-int escat_experts_fwd(const escat_experts_dims *dims, const void *x, const float *weights, const void *w1, const void *b1,
-                      const void *w2, const void *b2, const void *plan, void *y, void *workspace, size_t workspace_bytes, void *stream);
+int escat_experts_fwd_needs_plan(const escat_experts_dims *dims);
+int escat_experts_fwd(const escat_experts_dims *dims, const void *x, const float *weights, const int32_t *experts_of_rows, const void *w1,
+                      const void *b1, const void *w2, const void *b2, const void *plan, void *y, void *workspace, size_t workspace_bytes,
+                      void *stream);
 int escat_experts_bwd(const escat_experts_dims *dims, const void *x, const float *weights, const void *w1, const void *b1,
                       const void *w2, const void *b2, const void *plan, const void *dy, void *dx, float *dweights, void *dw1, void *db1,
                       void *dw2, void *db2, void *workspace, size_t workspace_bytes, void *stream);

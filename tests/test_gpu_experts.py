@@ -105,6 +105,10 @@ SHAPES = [  # rows, d, h, o, E, k
     (700, 1024, 40, 24, 6, 2),
     (5000, 40, 72, 48, 3, 2),
     (64, 8, 520, 16, 300, 6),
+    # more pairs than the form for few rows takes, by pair and with k = 1
+    (3000, 33, 65, 31, 64, 2),
+    (5000, 130, 129, 70, 40, 3),
+    (6000, 50, 40, 60, 5, 1),
     # enough rows for tiles by combination of experts (escat_experts.h): k = 2, 3; ragged sizes
     (2000, 40, 72, 136, 2, 2),
     (9000, 33, 47, 70, 3, 3),
