@@ -10,6 +10,7 @@
 
 #define FT 256
 #define FW (FT / 64)
+#define OW 8                                      // waves that share a row's results
 #define FEAT 4                                    // rows of weights (results) that a wave walks at once
 
 struct FewArgs {
@@ -83,36 +84,51 @@ __global__ void __launch_bounds__(FT) k_few_hidden(const FewArgs a)
 }
 
 template <typename T>
-__global__ void __launch_bounds__(FT) k_few_out(const FewArgs a)
+__global__ void __launch_bounds__(64 * OW) k_few_out(const FewArgs a)
 {
     constexpr int PER = Elem<T>::PER, CH = 64 * PER;
-    __shared__ float part[FW][FEAT];
+    __shared__ float part[OW][FEAT];
     const int H = a.n.h, O = a.n.o, k = a.n.k, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int t = blockIdx.y, f0 = blockIdx.x * FEAT;
-    const int chunks = (H + CH - 1) / CH;
+    const int chunks = (H + CH - 1) / CH, all = k * chunks;
     float s[FEAT];
 #pragma unroll
     for (int i = 0; i < FEAT; ++i) s[i] = 0.f;
-    for (int q = wave; q < k * chunks; q += FW) {
-        const int j = q / chunks, c = (q - j * chunks) * CH + lane * PER;
-        const int64_t p = (int64_t)t * k + j;
-        const int e = a.experts[p];
-        if (e < 0 || e >= a.n.E) continue;
-        const T *W = (const T *)a.w2 + (int64_t)e * O * H;
-        u4 v[FEAT];
+    for (int q0 = wave; q0 < all; q0 += 2 * OW) {            // two pieces of the (expert, hidden) axis in flight
+        u4 v[2][FEAT], hv[2][PER / 4];
+        bool live[2];
 #pragma unroll
-        for (int i = 0; i < FEAT; ++i) v[i] = piece_of(W + (int64_t)(f0 + i < O ? f0 + i : O - 1) * H, c, H);
-        float h[PER];
-        const float *hp = a.h + p * H;
+        for (int u = 0; u < 2; ++u) {
+            const int q = q0 + u * OW < all ? q0 + u * OW : q0, j = q / chunks, c = (q - j * chunks) * CH + lane * PER;
+            const int64_t p = (int64_t)t * k + j;
+            const int e = a.experts[p];
+            live[u] = q0 + u * OW < all && e >= 0 && e < a.n.E;
+            if (!live[u]) continue;
+            const T *W = (const T *)a.w2 + (int64_t)e * O * H;
+            const int at = c < H - PER ? c : H - PER;
 #pragma unroll
-        for (int z = 0; z < PER; ++z) h[z] = c + z < H ? hp[c + z] : 0.f;
-        const int over = c > H - PER ? c - (H - PER) : 0;
+            for (int i = 0; i < FEAT; ++i) v[u][i] = load16(W + (int64_t)(f0 + i < O ? f0 + i : O - 1) * H + at);
 #pragma unroll
-        for (int i = 0; i < FEAT; ++i) {
-            float fw[PER];
-            to_floats<T>(moved<T>(v[i], over), fw);
+            for (int i = 0; i < PER / 4; ++i) hv[u][i] = load16(a.h + p * H + at + 4 * i);
+        }
 #pragma unroll
-            for (int z = 0; z < PER; ++z) s[i] = fmaf(h[z], fw[z], s[i]);
+        for (int u = 0; u < 2; ++u) {
+            if (!live[u]) continue;
+            const int q = q0 + u * OW, c = (q % chunks) * CH + lane * PER, over = c > H - PER ? c - (H - PER) : 0;
+            // weights and h were read from the same place: where that lies before c (the end of a row), the elements before c are left out
+            float h[PER], fw[PER];
+#pragma unroll
+            for (int i = 0; i < PER / 4; ++i) {
+                const f4 f = __builtin_bit_cast(f4, hv[u][i]);
+#pragma unroll
+                for (int z = 0; z < 4; ++z) h[4 * i + z] = 4 * i + z >= over ? f[z] : 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < FEAT; ++i) {
+                to_floats<T>(v[u][i], fw);
+#pragma unroll
+                for (int z = 0; z < PER; ++z) s[i] = fmaf(h[z], z >= over ? fw[z] : 0.f, s[i]);
+            }
         }
     }
 #pragma unroll
@@ -122,7 +138,7 @@ __global__ void __launch_bounds__(FT) k_few_out(const FewArgs a)
         const int i = threadIdx.x;
         float y = 0.f;
 #pragma unroll
-        for (int w = 0; w < FW; ++w) y += part[w][i];
+        for (int w = 0; w < OW; ++w) y += part[w][i];
         if (a.b2)
             for (int j = 0; j < k; ++j) {
                 const int e = a.experts[(int64_t)t * k + j];
@@ -137,7 +153,7 @@ template <typename T> static int go(const FewArgs &a, hipStream_t st)
     const EDims &n = a.n;
     k_few_hidden<T><<<dim3((n.h + FW * FEAT - 1) / (FW * FEAT), (unsigned)(n.rows * n.k)), FT, 0, st>>>(a);
     CHECK_LAUNCH("experts: few rows, hidden");
-    k_few_out<T><<<dim3((n.o + FEAT - 1) / FEAT, (unsigned)n.rows), FT, 0, st>>>(a);
+    k_few_out<T><<<dim3((n.o + FEAT - 1) / FEAT, (unsigned)n.rows), 64 * OW, 0, st>>>(a);
     CHECK_LAUNCH("experts: few rows, out");
     return ESCAT_OK;
 }
