@@ -10,6 +10,7 @@ All three run on the current stream, read nothing back to the host, and give the
 floating-point atomics); they can be captured into a graph.  There is no CPU path.
 """
 import ctypes
+import functools
 import math
 from typing import Optional, Tuple
 import torch
@@ -48,6 +49,7 @@ class _Route(torch.autograd.Function):
                                          group_top, renorm, scale, weights.data_ptr(), experts.data_ptr(), stream)
         _lib.check(rc, "escat_route")
         ctx.mark_non_differentiable(experts)
+        ctx.set_materialize_grads(False)                  # (no zeros in the place of the experts' gradient)
         ctx.save_for_backward(logits, weights, experts)
         ctx.meta = (k, score, renorm, scale)
         return weights, experts
@@ -55,6 +57,8 @@ class _Route(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dweights, _):
+        if dweights is None:
+            return (None,) * 9
         logits, weights, experts = ctx.saved_tensors
         k, score, renorm, scale = ctx.meta
         rows, E = logits.shape
@@ -130,16 +134,23 @@ def expert_counts(experts: torch.Tensor, n_experts: int) -> torch.Tensor:
     return counts
 
 
+@functools.lru_cache(maxsize=256)
+def _sizes(*dims):
+    """what the library says of a call's sizes: the dims structure, whether the forward sorts, the forward's workspace"""
+    lib = _lib.load()
+    d = _lib.EscatExpertsDims(*dims)
+    at = ctypes.addressof(d)
+    return d, at, bool(lib.escat_experts_fwd_needs_plan(at)), lib.escat_experts_workspace_bytes(at, 0)
+
+
 def _mlp_forward(x, weights, experts, w1, b1, w2, b2):
     """y, and the plan where the forward made one (few rows do without)"""
     lib = _lib.load()
     (rows, d), k, (E, h, _), o = x.shape, experts.shape[1], w1.shape, w2.shape[1]
-    dims = _lib.EscatExpertsDims(rows, DTYPE_CODES[x.dtype], d, h, o, E, k)
-    at = ctypes.addressof(dims)
-    y = torch.empty((rows, o), dtype=x.dtype, device=x.device)
-    size = lib.escat_experts_workspace_bytes(at, 0)
+    dims, at, sorts, size = _sizes(rows, DTYPE_CODES[x.dtype], d, h, o, E, k)
+    y = x.new_empty((rows, o))
     with _on(x.device) as stream:
-        plan = _plan(experts, rows, k, E, None, stream) if lib.escat_experts_fwd_needs_plan(at) else None
+        plan = _plan(experts, rows, k, E, None, stream) if sorts else None
         ws = torch.empty(size, dtype=torch.uint8, device=x.device)
         rc = lib.escat_experts_fwd(at, x.data_ptr(), weights.data_ptr(), experts.data_ptr(), w1.data_ptr(), _ptr(b1), w2.data_ptr(), _ptr(b2),
                                    _ptr(plan), y.data_ptr(), ws.data_ptr(), size, stream)
@@ -203,14 +214,18 @@ def expert_mlp(x: torch.Tensor, weights: torch.Tensor, experts: torch.Tensor, w1
     if weights.dim() != 2 or weights.shape[0] != rows or experts.shape != weights.shape or not 1 <= weights.shape[1] <= 64 or weights.dtype is not torch.float32:
         raise ValueError(f"escat: weights and experts must be ({rows}, k), k <= 64, weights fp32: {tuple(weights.shape)} {weights.dtype}, {tuple(experts.shape)}")
     _check_experts(experts, E)
-    for name, t, shape in (("w1", w1, w1.shape), ("w2", w2, w2.shape), ("b1", b1, (E, h)), ("b2", b2, (E, o))):
-        if t is not None and (t.shape != shape or t.dtype is not x.dtype):
-            raise ValueError(f"escat: {name} must be {tuple(shape)} {x.dtype}: {tuple(t.shape)} {t.dtype}")
-        if t is not None and not t.is_contiguous():
+    dtype, at = x.dtype, x.get_device()
+    for name, t, shape in (("w1", w1, None), ("w2", w2, None), ("b1", b1, (E, h)), ("b2", b2, (E, o))):
+        if t is None:
+            continue
+        if (shape is not None and t.shape != shape) or t.dtype is not dtype:
+            raise ValueError(f"escat: {name} must be {shape or tuple(t.shape)} {dtype}: {tuple(t.shape)} {t.dtype}")
+        if not t.is_contiguous():
             raise ValueError(f"escat: {name} must be contiguous (strides {t.stride()})")
-    for name, t in (("weights", weights), ("experts", experts), ("w1", w1), ("w2", w2), ("b1", b1), ("b2", b2)):
-        if t is not None and t.device != x.device:
+        if t.get_device() != at:
             raise RuntimeError(f"escat: {name} lives on {t.device}, x on {x.device}")
+    if weights.get_device() != at or experts.get_device() != at:
+        raise RuntimeError(f"escat: weights and experts live on {weights.device} and {experts.device}, x on {x.device}")
     _need_gpu(x, "x")
     least = 4 if x.dtype is torch.float32 else 8            # the kernels move 16 bytes of a row at once: narrower ones get zeros
     if min(d, h, o) < least:

@@ -15,6 +15,8 @@ their gradients keep identical parameters.  An element whose state is not finite
 """
 import array
 import ctypes
+from itertools import chain
+from operator import attrgetter
 from typing import Optional, Sequence
 import torch
 
@@ -24,6 +26,10 @@ from .pyg_utilities import _ptr
 STATE_BLOCK = 256
 MAX_GROUPS = 16                                            # ESCAT_ADAMW_MAX_GROUPS
 DTYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+_DTYPE, _LAYOUT, _SHAPE = map(attrgetter, ("dtype", "layout", "shape"))
+_NUMEL, _DEVICE, _CONTIGUOUS, _PTR = torch.Tensor.numel, torch.Tensor.get_device, torch.Tensor.is_contiguous, torch.Tensor.data_ptr
 
 
 class _Group(ctypes.Structure):
@@ -39,12 +45,12 @@ class _on:
         self.index = device.index
 
     def __enter__(self):
-        self.before = torch.cuda._exchange_device(self.index)
+        self.before = torch._C._cuda_exchangeDevice(self.index)
         return torch._C._cuda_getCurrentRawStream(self.index)
 
     def __exit__(self, *_):
         if self.before != self.index:
-            torch.cuda._maybe_exchange_device(self.before)
+            torch._C._cuda_maybeExchangeDevice(self.before)
 
 
 def new_state8(n: int, device) -> tuple:
@@ -54,13 +60,13 @@ def new_state8(n: int, device) -> tuple:
 
 
 def dequantize_state(codes: torch.Tensor, scales: torch.Tensor, signed: bool) -> torch.Tensor:
-    """the fp32 values of an 8-bit state; signed: a first moment (exp_avg), else a second moment (exp_avg_sq)"""
+    """the fp32 values of an 8-bit state, in the shape of the codes; signed: a first moment (exp_avg), else a second moment (exp_avg_sq)"""
     if codes.dtype != torch.uint8 or scales.dtype != torch.float32 or not codes.is_contiguous() or not scales.is_contiguous() \
             or scales.numel() != -(-codes.numel() // STATE_BLOCK):
         raise ValueError("escat: an 8-bit state is contiguous uint8 codes with one fp32 scale per 256 elements")
     if not codes.is_cuda or scales.device != codes.device:
         raise RuntimeError("escat: the state must live on one GPU; the MI355X path has no CPU fallback")
-    out = torch.empty(codes.numel(), dtype=torch.float32, device=codes.device)
+    out = torch.empty_like(codes, dtype=torch.float32)
     with _on(codes.device) as stream:
         rc = _lib.load().escat_state8_values(codes.data_ptr(), scales.data_ptr(), codes.numel(), int(bool(signed)), out.data_ptr(), stream)
     _lib.check(rc, "escat_state8_values")
@@ -118,6 +124,38 @@ class _Tables:
                 t = self.by_type[key] = array.array("Q")
             t.extend(row)
 
+    def add_all(self, ps, gs, ms, vs, dev):
+        """add() for whole lists that are all alike (one parameter type, one gradient type, contiguous, no empty tensor), checked
+        a property at a time: a third of the time per tensor.  False: they are not, nothing was added."""
+        n = len(ps)
+        if n == 0 or len(set(map(_DTYPE, ps))) != 1 or len(set(map(_DTYPE, gs))) != 1:
+            return False
+        pt, gt = ps[0].dtype, gs[0].dtype
+        if pt not in DTYPE_CODES or (gt is not pt and gt is not torch.float32):
+            return False
+        bits = 8 if type(ms[0]) is tuple else 32
+        if bits == 8:
+            if set(map(type, ms)) != {tuple} or set(map(type, vs)) != {tuple} or set(map(len, ms)) != {2} or set(map(len, vs)) != {2}:
+                return False
+            (ms, mz), (vs, vz) = zip(*ms), zip(*vs)
+            scales = mz + vz
+        elif tuple in map(type, ms) or tuple in map(type, vs):
+            return False
+        else:
+            scales = ()
+        states = [*ms, *vs]
+        ns = list(map(_NUMEL, ps))
+        if set(map(_LAYOUT, gs)) != {torch.strided} or set(map(_DEVICE, [*ps, *gs, *states, *scales])) != {dev.index} \
+                or set(map(_DTYPE, states)) != {torch.uint8 if bits == 8 else torch.float32} or (scales and set(map(_DTYPE, scales)) != {torch.float32}) \
+                or not all(map(_CONTIGUOUS, [*ps, *gs, *states, *scales])) or 0 in ns or list(map(_SHAPE, ps)) != list(map(_SHAPE, gs)) \
+                or list(map(_NUMEL, states)) != ns * 2 or (scales and list(map(_NUMEL, scales)) != [-(-k // STATE_BLOCK) for k in ns] * 2):
+            return False
+        z = list(map(_PTR, scales)) or [0] * (2 * n)
+        q = list(map(_PTR, states))
+        rows = zip(map(_PTR, ps), map(_PTR, gs), q, q[n:], z, z[n:], ns, range(n))
+        self.by_type[(DTYPE_CODES[pt], DTYPE_CODES[gt], bits)] = array.array("Q", chain.from_iterable(rows))
+        return True
+
     def written(self):
         """addresses of what the step writes, to refuse a tensor that is listed twice"""
         for t in self.by_type.values():
@@ -167,8 +205,9 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
         raise ValueError("escat: step is an int32 tensor of one element")
     dev = step.device
     table = _Tables()
-    for i in range(n):
-        table.add(params[i], grads[i], exp_avgs[i], exp_avg_sqs[i], i, dev)
+    if dev.type != "cuda" or not table.add_all(params, grads, exp_avgs, exp_avg_sqs, dev):
+        for i in range(n):
+            table.add(params[i], grads[i], exp_avgs[i], exp_avg_sqs[i], i, dev)
     written = list(table.written())
     if len(set(written)) != len(written):
         raise ValueError("escat: a parameter or state is listed twice")
@@ -263,9 +302,11 @@ class AdamW(torch.optim.Optimizer):
         tables, groups, steps = {}, {}, {}
         for (key, gi), items in calls.items():
             t = tables[(key, gi)] = _Tables()
-            for p, st, at in items:
-                m, v = self._moments(st)
-                t.add(p, p.grad, m, v, at, dev)
+            moments = [self._moments(st) for _, st, _ in items]
+            if [at for _, _, at in items] != list(range(len(items))) or not t.add_all(
+                    [p for p, _, _ in items], [p.grad for p, _, _ in items], [m for m, _ in moments], [v for _, v in moments], dev):
+                for (p, st, at), (m, v) in zip(items, moments):
+                    t.add(p, p.grad, m, v, at, dev)
             g = self.param_groups[gi]
             groups.setdefault(key, []).append((gi, _Group(g["lr"], g["betas"][0], g["betas"][1], g["eps"], g["weight_decay"])))
             steps[key] = moved[key]
