@@ -36,6 +36,19 @@ template <int CTRL> __device__ __forceinline__ double dpp(double v)
     const int lo = __builtin_amdgcn_mov_dpp(__double2loint(v), CTRL, 0xf, 0xf, true), hi = __builtin_amdgcn_mov_dpp(__double2hiint(v), CTRL, 0xf, 0xf, true);
     return __hiloint2double(hi, lo);
 }
+// all lanes of a pair of 16-lane rows (of both halves of the wave) get the first (SIDE 0) or the second (SIDE 1) one's value
+template <int SIDE> __device__ __forceinline__ unsigned swap_row_u(unsigned v) { return __builtin_amdgcn_permlane16_swap(v, v, false, false)[SIDE]; }
+template <int SIDE> __device__ __forceinline__ unsigned swap_half_u(unsigned v) { return __builtin_amdgcn_permlane32_swap(v, v, false, false)[SIDE]; }
+template <int SIDE> __device__ __forceinline__ float swap_row(float v) { return __uint_as_float(swap_row_u<SIDE>(__float_as_uint(v))); }
+template <int SIDE> __device__ __forceinline__ float swap_half(float v) { return __uint_as_float(swap_half_u<SIDE>(__float_as_uint(v))); }
+template <int SIDE> __device__ __forceinline__ double swap_row(double v)
+{
+    return __hiloint2double((int)swap_row_u<SIDE>((unsigned)__double2hiint(v)), (int)swap_row_u<SIDE>((unsigned)__double2loint(v)));
+}
+template <int SIDE> __device__ __forceinline__ double swap_half(double v)
+{
+    return __hiloint2double((int)swap_half_u<SIDE>((unsigned)__double2hiint(v)), (int)swap_half_u<SIDE>((unsigned)__double2loint(v)));
+}
 struct OpMax { template <typename K> __device__ static K f(K a, K b) { return a > b ? a : b; } };
 struct OpSum { template <typename K> __device__ static K f(K a, K b) { return a + b; } };
 template <int LPR, typename OP, typename K> __device__ __forceinline__ K row_reduce(K v)
@@ -44,16 +57,18 @@ template <int LPR, typename OP, typename K> __device__ __forceinline__ K row_red
     if (LPR > 2) v = OP::f(v, dpp<0x4E>(v));                // quad_perm 2,3,0,1
     if (LPR > 4) v = OP::f(v, dpp<0x141>(v));               // row_half_mirror: the other four of eight
     if (LPR > 8) v = OP::f(v, dpp<0x140>(v));               // row_mirror: the other eight of sixteen
-    if (LPR > 16) v = OP::f(v, (K)__shfl_xor(v, 16, 64));
-    if (LPR > 32) v = OP::f(v, (K)__shfl_xor(v, 32, 64));
+    if (LPR > 16) v = OP::f(swap_row<0>(v), swap_row<1>(v));
+    if (LPR > 32) v = OP::f(swap_half<0>(v), swap_half<1>(v));
     return v;
 }
-// first of the row's lanes for which `has` holds (one does); l0 = the row's first lane
+// first of the row's lanes for which `has` holds (one does), counted in the row
 template <int LPR> __device__ __forceinline__ int first_lane(bool has, int l0)
 {
-    if (LPR == 1) return l0;
-    const uint64_t b = __ballot(has) >> l0;
-    return l0 + __builtin_ctzll(b);                          // lanes of later rows lie above the one that is found
+    if (LPR == 1) return 0;
+    const uint64_t b = __ballot(has);
+    if (LPR == 64) return __builtin_ctzll(b);
+    const uint32_t half = l0 & 32 ? (uint32_t)(b >> 32) : (uint32_t)b;       // (lanes of later rows lie above the one that is found)
+    return __builtin_ctz(LPR == 32 ? half : half >> (l0 & 31));
 }
 
 // lanes of one wave hand values over through LDS: order the accesses, no barrier between waves
@@ -69,37 +84,62 @@ __device__ bool pick(const RouteArgs &a, K (&key)[EPL], const K (&gkey)[EPL], bo
     const int e0 = lane_in_row * EPL;
     bool close = false;
     if (a.groups > 1) {
-        const int gs = a.E / a.groups;
+        const int gs = a.E / a.groups, lpg = gs / EPL;
+        if (lpg * EPL == gs && (lpg & (lpg - 1)) == 0) {      // a group is a power of two of whole lanes: all in registers
+            K b1 = gkey[0], b2 = -inf;                         // the lane's two largest, then the group's
 #pragma unroll
-        for (int i = 0; i < EPL; ++i) if (e0 + i < a.E) buf[e0 + i] = gkey[i];
-        wave_lds_sync();
-        K score = -inf;
-        if (lane_in_row < a.groups) {                        // one group a lane (LPR >= groups)
-            K b1 = -inf, b2 = -inf;
-            int at = lane_in_row % gs;                       // start at another place in each lane: other LDS banks
-            for (int i = 0; i < gs; ++i) {
-                const K v = buf[lane_in_row * gs + at];
-                at = at + 1 == gs ? 0 : at + 1;
-                if (v > b1) { b2 = b1; b1 = v; } else if (v > b2) b2 = v;
+            for (int i = 1; i < EPL; ++i) { const K v = gkey[i], lo = v < b1 ? v : b1; b1 = v > b1 ? v : b1; b2 = lo > b2 ? lo : b2; }
+            for (int m = 1; m < lpg; m <<= 1) {
+                const K o1 = __shfl_xor(b1, m, 64), o2 = __shfl_xor(b2, m, 64), lo = o1 < b1 ? o1 : b1;
+                b1 = o1 > b1 ? o1 : b1;
+                b2 = o2 > b2 ? o2 : b2; b2 = lo > b2 ? lo : b2;
             }
-            score = b1 == -inf ? -inf : b1 + (a.group_top == 2 && b2 > -inf ? b2 : (K)0);
-        }
-        wave_lds_sync();
-        uint64_t kept = 0;
-        K last = inf;
-        for (int r = 0; r <= a.keep; ++r) {
-            const K m = row_reduce<LPR, OpMax>(score);
-            if (CHECK && r > 0 && m > -inf) close |= !(last - m > (K)R_GAP * fmaxf(1.f, fabsf((float)last)));
-            if (r == a.keep || m == -inf) break;
-            const int at = first_lane<LPR>(score == m, l0);
-            kept |= 1ull << (at - l0);
-            if ((int)(threadIdx.x & 63) == at) score = -inf;
-            last = m;
-        }
+            K score = e0 >= a.E || b1 == -inf ? -inf : b1 + (a.group_top == 2 && b2 > -inf ? b2 : (K)0);
+            bool kept = false;
+            K last = inf;
+            for (int r = 0; r <= a.keep; ++r) {
+                const K m = row_reduce<LPR, OpMax>(score);
+                if (CHECK && r > 0 && m > -inf) close |= !(last - m > (K)R_GAP * fmaxf(1.f, fabsf((float)last)));
+                if (r == a.keep || m == -inf) break;
+                const int at = first_lane<LPR>(score == m, l0);
+                if ((at ^ lane_in_row) < lpg) { kept = true; score = -inf; }          // the same group: only bits below lpg differ
+                last = m;
+            }
 #pragma unroll
-        for (int i = 0; i < EPL; ++i) {
-            const int e = e0 + i;
-            if (e >= a.E || !((kept >> (e / gs)) & 1)) key[i] = -inf;
+            for (int i = 0; i < EPL; ++i) if (!kept) key[i] = -inf;
+        } else {
+#pragma unroll
+            for (int i = 0; i < EPL; ++i) if (e0 + i < a.E) buf[e0 + i] = gkey[i];
+            wave_lds_sync();
+            K score = -inf;
+            if (lane_in_row < a.groups) {                    // one group a lane (LPR >= groups)
+                K b1 = -inf, b2 = -inf;
+                int at = lane_in_row % gs;                   // start at another place in each lane: other LDS banks
+                for (int i = 0; i < gs; ++i) {
+                    const K v = buf[lane_in_row * gs + at];
+                    at = at + 1 == gs ? 0 : at + 1;
+                    if (v > b1) { b2 = b1; b1 = v; } else if (v > b2) b2 = v;
+                }
+                score = b1 == -inf ? -inf : b1 + (a.group_top == 2 && b2 > -inf ? b2 : (K)0);
+            }
+            wave_lds_sync();
+            uint64_t kept = 0;
+            K last = inf;
+            for (int r = 0; r <= a.keep; ++r) {
+                const K m = row_reduce<LPR, OpMax>(score);
+                if (CHECK && r > 0 && m > -inf) close |= !(last - m > (K)R_GAP * fmaxf(1.f, fabsf((float)last)));
+                if (r == a.keep || m == -inf) break;
+                const int at = first_lane<LPR>(score == m, l0);
+                kept |= 1ull << at;
+                if (lane_in_row == at) score = -inf;
+                last = m;
+            }
+            int g = e0 / gs, in_g = e0 - g * gs;
+#pragma unroll
+            for (int i = 0; i < EPL; ++i) {
+                if (e0 + i >= a.E || !((kept >> g) & 1)) key[i] = -inf;
+                if (++in_g == gs) { in_g = 0; ++g; }
+            }
         }
     }
     K last = inf;
@@ -115,7 +155,7 @@ __device__ bool pick(const RouteArgs &a, K (&key)[EPL], const K (&gkey)[EPL], bo
             break;
         }
         const int at = first_lane<LPR>(best == m, l0);
-        if ((int)(threadIdx.x & 63) == at) {
+        if (lane_in_row == at) {
             int w = EPL - 1;
 #pragma unroll
             for (int i = EPL - 2; i >= 0; --i) if (key[i] == m) w = i;
@@ -139,11 +179,14 @@ __global__ void __launch_bounds__(RT) k_route(const RouteArgs a)
 {
     extern __shared__ __align__(8) unsigned char lds[];
     constexpr int RPB = RT / LPR;
-    const int lane = threadIdx.x & 63, lane_in_row = threadIdx.x % LPR, l0 = lane - lane % LPR, r_in_b = threadIdx.x / LPR;
+    const int lane = threadIdx.x & 63; const int lane_in_row = threadIdx.x % LPR, l0 = lane - lane % LPR, r_in_b = threadIdx.x / LPR;
     const int e0 = lane_in_row * EPL;
     int *sel = (int *)lds + r_in_b * a.k;
     double *buf = (double *)(lds + ((size_t)RPB * a.k * 4 + 7) / 8 * 8) + (size_t)r_in_b * a.E;      // groups only
     const bool fp64_keys = a.bias != nullptr || a.groups > 1;
+    float bias[EPL];
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) bias[i] = a.bias && e0 + i < a.E ? a.bias[e0 + i] : 0.f;
     // all lanes of a wave go through the same number of rows: rows behind the last are worked on as rows without an expert
     for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.rows; r0 += (int64_t)gridDim.x * RPB) {
         const int64_t row = r0 + r_in_b;
@@ -179,8 +222,8 @@ __global__ void __launch_bounds__(RT) k_route(const RouteArgs a)
             const float inv = 1.f / sum;
 #pragma unroll
             for (int i = 0; i < EPL; ++i) {
-                const float s = a.score == 0 ? __expf(x[i] - top) * inv : 1.f / (1.f + __expf(-x[i]));
-                const float b = a.bias && e0 + i < a.E ? a.bias[e0 + i] : 0.f;
+                const float s = a.score == 0 ? __expf(x[i] - top) * inv : __builtin_amdgcn_rcpf(1.f + __expf(-x[i]));
+                const float b = bias[i];
                 const float v = s + b;
                 gkey[i] = x[i] == -R_INF ? -R_INF : v == v ? v : spoiled(x[i], 3.4e38f);
                 key[i] = a.bias ? gkey[i] : x[i] == x[i] ? x[i] : R_INF;
@@ -201,38 +244,41 @@ __global__ void __launch_bounds__(RT) k_route(const RouteArgs a)
 #pragma unroll
             for (int i = 0; i < EPL; ++i) {
                 const double s = a.score == 0 ? exp((double)x[i] - top2) / sum2 : 1.0 / (1.0 + exp(-(double)x[i]));
-                const double v = s + (a.bias && e0 + i < a.E ? (double)a.bias[e0 + i] : 0.0);
+                const double v = s + (double)bias[i];
                 gkey2[i] = x[i] == -R_INF ? -(double)R_INF : v == v ? v : (double)spoiled(x[i], 3.4e38f);
                 key2[i] = a.bias ? gkey2[i] : x[i] == x[i] ? (double)x[i] : (double)R_INF;
             }
             pick<LPR, EPL, double, false>(a, key2, gkey2, true, lane_in_row, l0, buf, sel);
         }
         wave_lds_sync();
-        // weights: the chosen logits once more (they are in the cache), k of them over the row's lanes
+        // weights: the chosen logits once more (they are in the cache), JN of the k to a lane
+        constexpr int JN = (ESCAT_ROUTE_MAX_K + LPR - 1) / LPR;
         const float base = top;
-        float m = -R_INF, z = 0.f;
-        if (a.score == 0 && a.renorm) {
-            for (int j = lane_in_row; j < a.k; j += LPR) { const int e = sel[j]; if (in && e >= 0) { const float v = to_f32(lg[e]); m = v > m ? v : m; } }
-            m = row_reduce<LPR, OpMax>(m);
+        float v[JN], m = -R_INF, z = 0.f;
+        int ex[JN];
+#pragma unroll
+        for (int i = 0; i < JN; ++i) {
+            const int j = lane_in_row + i * LPR;
+            ex[i] = in && j < a.k ? sel[j] : -1;
+            v[i] = ex[i] >= 0 ? to_f32(lg[ex[i]]) : -R_INF;
         }
+        if (a.score == 0 && a.renorm) {
+#pragma unroll
+            for (int i = 0; i < JN; ++i) m = v[i] > m ? v[i] : m;
+            m = row_reduce<LPR, OpMax>(m);
+        } else m = base;
+#pragma unroll
+        for (int i = 0; i < JN; ++i) { v[i] = ex[i] < 0 ? 0.f : a.score == 0 ? expf(v[i] - m) : sigmoid_f(v[i]); z += v[i]; }
         if (a.renorm) {
-            for (int j = lane_in_row; j < a.k; j += LPR) {
-                const int e = sel[j];
-                if (in && e >= 0) { const float v = to_f32(lg[e]); z += a.score == 0 ? expf(v - m) : sigmoid_f(v); }
-            }
             z = row_reduce<LPR, OpSum>(z);
             z = a.score == 0 ? z : z + 1e-20f;
         } else z = a.score == 0 ? sum : 1.f;
-        for (int j = lane_in_row; j < a.k; j += LPR) {
-            const int e = sel[j];
-            if (!in) continue;
-            float w = 0.f;
-            if (e >= 0) {
-                const float v = to_f32(lg[e]);
-                w = a.scale * ((a.score == 0 ? expf(v - (a.renorm ? m : base)) : sigmoid_f(v)) / z);
-            }
-            a.weights[row * a.k + j] = w;
-            a.experts[row * a.k + j] = e;
+#pragma unroll
+        for (int i = 0; i < JN; ++i) {
+            const int j = lane_in_row + i * LPR;
+            if (!in || j >= a.k) continue;
+            a.weights[row * a.k + j] = ex[i] < 0 ? 0.f : a.scale * (v[i] / z);
+            a.experts[row * a.k + j] = ex[i];
         }
         wave_lds_sync();
     }
@@ -378,7 +424,7 @@ extern "C" int escat_route(const void *logits, int type, int64_t rows, int E, in
     const size_t lds = ((size_t)rpb * k * 4 + 7) / 8 * 8 + (groups > 1 ? (size_t)rpb * E * 8 : 0);
     const int64_t want = (rows + rpb - 1) / rpb;
     const RouteArgs a = {logits, bias, weights, experts, rows, E, k, groups, keep_groups, group_top, score, renorm ? 1 : 0, scale};
-    return route_dispatch<LaunchFwd>(type, lpr, epl, a, (unsigned)(want < 65536 ? want : 65536), lds, (hipStream_t)stream);
+    return route_dispatch<LaunchFwd>(type, lpr, epl, a, (unsigned)(want < 2048 ? want : 2048), lds, (hipStream_t)stream);
 }
 
 extern "C" int escat_route_bwd(const void *logits, int type, int64_t rows, int E, int k, int score, int renorm, float scale, const float *weights,
