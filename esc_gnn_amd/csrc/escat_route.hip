@@ -49,7 +49,23 @@ template <int SIDE> __device__ __forceinline__ double swap_half(double v)
 {
     return __hiloint2double((int)swap_half_u<SIDE>((unsigned)__double2hiint(v)), (int)swap_half_u<SIDE>((unsigned)__double2loint(v)));
 }
-struct OpMax { template <typename K> __device__ static K f(K a, K b) { return a > b ? a : b; } };
+template <int SIDE> __device__ __forceinline__ int swap_row(int v) { return (int)swap_row_u<SIDE>((unsigned)v); }
+template <int SIDE> __device__ __forceinline__ int swap_half(int v) { return (int)swap_half_u<SIDE>((unsigned)v); }
+template <int CTRL> __device__ __forceinline__ int dpp(int v) { return __builtin_amdgcn_mov_dpp(v, CTRL, 0xf, 0xf, true); }
+
+// 32-bit keys are compared as whole numbers in the same order (one instruction a maximum, which DPP moves fold into)
+__device__ __forceinline__ int sortable(float f) { const int b = __float_as_int(f); return b ^ ((b >> 31) & 0x7fffffff); }
+__device__ __forceinline__ float value_of(int k) { return __int_as_float(k ^ ((k >> 31) & 0x7fffffff)); }
+__device__ __forceinline__ double value_of(double k) { return k; }
+template <typename K> struct Least;
+template <> struct Least<int> { static constexpr int v = (int)0x807fffff; };                 // sortable(-inf)
+template <> struct Least<double> { static constexpr double v = -__builtin_inf(); };
+__device__ __forceinline__ void to_key(float f, int &k) { k = sortable(f); }
+__device__ __forceinline__ void to_key(double f, double &k) { k = f; }
+struct OpMax {
+    template <typename K> __device__ static K f(K a, K b) { return a > b ? a : b; }
+    __device__ static float f(float a, float b) { return fmaxf(a, b); }
+};
 struct OpSum { template <typename K> __device__ static K f(K a, K b) { return a + b; } };
 template <int LPR, typename OP, typename K> __device__ __forceinline__ K row_reduce(K v)
 {
@@ -75,95 +91,117 @@ template <int LPR> __device__ __forceinline__ int first_lane(bool has, int l0)
 __device__ __forceinline__ void wave_lds_sync() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup"); __builtin_amdgcn_wave_barrier(); }
 
 // ------------------------------------------------------------------ the selection
-// key / gkey: the lane's EPL keys for experts and for group scores (-inf: cannot be chosen).  sel (LDS, of the row): k results.
-// Returns whether two keys that decided something were closer than their error (CHECK only).
-template <int LPR, int EPL, typename K, bool CHECK>
-__device__ bool pick(const RouteArgs &a, K (&key)[EPL], const K (&gkey)[EPL], bool key_exact, int lane_in_row, int l0, K *buf, int *sel)
+// key / gkey: the lane's EPL keys for experts and for group scores (Least: cannot be chosen), K = int (sortable) or double, V the
+// type of their values.  sel (LDS, of the row): k results.  Returns whether two keys that decided something were closer than
+// their error (CHECK only).
+template <typename V> __device__ __forceinline__ bool too_close(V last, V now) { return !(last - now > (V)R_GAP * fmaxf(1.f, fabsf((float)last))); }
+
+template <int LPR, typename K> __device__ __forceinline__ K other_lane(K v, int m)       // lane ^ m, m < LPR, inside a group of whole lanes
 {
-    const K inf = (K)R_INF;
+    if (m == 1) return dpp<0xB1>(v);
+    if (m == 2) return dpp<0x4E>(v);
+    return (K)__shfl_xor(v, m, 64);
+}
+
+template <int LPR, int EPL, typename K, typename V, bool CHECK>
+__device__ bool pick(const RouteArgs &a, K (&key)[EPL], const K (&gkey)[EPL], bool key_exact, int lane_in_row, int l0, V *buf, int *sel)
+{
+    constexpr K least = Least<K>::v;
+    const V inf = (V)R_INF;
     const int e0 = lane_in_row * EPL;
     bool close = false;
     if (a.groups > 1) {
         const int gs = a.E / a.groups, lpg = gs / EPL;
         if (lpg * EPL == gs && (lpg & (lpg - 1)) == 0) {      // a group is a power of two of whole lanes: all in registers
-            K b1 = gkey[0], b2 = -inf;                         // the lane's two largest, then the group's
+            K b1 = gkey[0], b2 = least;                        // the lane's two largest, then the group's
 #pragma unroll
             for (int i = 1; i < EPL; ++i) { const K v = gkey[i], lo = v < b1 ? v : b1; b1 = v > b1 ? v : b1; b2 = lo > b2 ? lo : b2; }
             for (int m = 1; m < lpg; m <<= 1) {
-                const K o1 = __shfl_xor(b1, m, 64), o2 = __shfl_xor(b2, m, 64), lo = o1 < b1 ? o1 : b1;
+                const K o1 = other_lane<LPR>(b1, m), o2 = other_lane<LPR>(b2, m), lo = o1 < b1 ? o1 : b1;
                 b1 = o1 > b1 ? o1 : b1;
                 b2 = o2 > b2 ? o2 : b2; b2 = lo > b2 ? lo : b2;
             }
-            K score = e0 >= a.E || b1 == -inf ? -inf : b1 + (a.group_top == 2 && b2 > -inf ? b2 : (K)0);
+            V sum = -inf;
+            if (e0 < a.E && b1 > least) sum = (V)value_of(b1) + (a.group_top == 2 && b2 > least ? (V)value_of(b2) : (V)0);
+            K score; to_key(sum, score);
             bool kept = false;
-            K last = inf;
+            V last = inf;
             for (int r = 0; r <= a.keep; ++r) {
                 const K m = row_reduce<LPR, OpMax>(score);
-                if (CHECK && r > 0 && m > -inf) close |= !(last - m > (K)R_GAP * fmaxf(1.f, fabsf((float)last)));
-                if (r == a.keep || m == -inf) break;
+                const V mv = (V)value_of(m);
+                if (CHECK && r > 0 && m > least) close |= too_close(last, mv);
+                if (r == a.keep || m == least) break;
                 const int at = first_lane<LPR>(score == m, l0);
-                if ((at ^ lane_in_row) < lpg) { kept = true; score = -inf; }          // the same group: only bits below lpg differ
-                last = m;
+                if ((at ^ lane_in_row) < lpg) { kept = true; score = least; }         // the same group: only bits below lpg differ
+                last = mv;
             }
 #pragma unroll
-            for (int i = 0; i < EPL; ++i) if (!kept) key[i] = -inf;
+            for (int i = 0; i < EPL; ++i) if (!kept) key[i] = least;
         } else {
 #pragma unroll
-            for (int i = 0; i < EPL; ++i) if (e0 + i < a.E) buf[e0 + i] = gkey[i];
+            for (int i = 0; i < EPL; ++i) if (e0 + i < a.E) buf[e0 + i] = (V)value_of(gkey[i]);
             wave_lds_sync();
-            K score = -inf;
+            V sum = -inf;
             if (lane_in_row < a.groups) {                    // one group a lane (LPR >= groups)
-                K b1 = -inf, b2 = -inf;
+                V b1 = -inf, b2 = -inf;
                 int at = lane_in_row % gs;                   // start at another place in each lane: other LDS banks
                 for (int i = 0; i < gs; ++i) {
-                    const K v = buf[lane_in_row * gs + at];
+                    const V v = buf[lane_in_row * gs + at];
                     at = at + 1 == gs ? 0 : at + 1;
                     if (v > b1) { b2 = b1; b1 = v; } else if (v > b2) b2 = v;
                 }
-                score = b1 == -inf ? -inf : b1 + (a.group_top == 2 && b2 > -inf ? b2 : (K)0);
+                sum = b1 == -inf ? -inf : b1 + (a.group_top == 2 && b2 > -inf ? b2 : (V)0);
             }
             wave_lds_sync();
+            K score; to_key(sum, score);
             uint64_t kept = 0;
-            K last = inf;
+            V last = inf;
             for (int r = 0; r <= a.keep; ++r) {
                 const K m = row_reduce<LPR, OpMax>(score);
-                if (CHECK && r > 0 && m > -inf) close |= !(last - m > (K)R_GAP * fmaxf(1.f, fabsf((float)last)));
-                if (r == a.keep || m == -inf) break;
+                const V mv = (V)value_of(m);
+                if (CHECK && r > 0 && m > least) close |= too_close(last, mv);
+                if (r == a.keep || m == least) break;
                 const int at = first_lane<LPR>(score == m, l0);
                 kept |= 1ull << at;
-                if (lane_in_row == at) score = -inf;
-                last = m;
+                if (lane_in_row == at) score = least;
+                last = mv;
             }
             int g = e0 / gs, in_g = e0 - g * gs;
 #pragma unroll
             for (int i = 0; i < EPL; ++i) {
-                if (e0 + i >= a.E || !((kept >> g) & 1)) key[i] = -inf;
+                if (e0 + i >= a.E || !((kept >> g) & 1)) key[i] = least;
                 if (++in_g == gs) { in_g = 0; ++g; }
             }
         }
     }
-    K last = inf;
-    for (int j = 0; j <= a.k; ++j) {
+    const bool check = CHECK && !key_exact;
+    V last = inf;
+    for (int j = 0; j < a.k + (check ? 1 : 0); ++j) {
         K best = key[0];
 #pragma unroll
         for (int i = 1; i < EPL; ++i) best = key[i] > best ? key[i] : best;
         const K m = row_reduce<LPR, OpMax>(best);
-        if (CHECK && !key_exact && j > 0 && m > -inf) close |= !(last - m > (K)R_GAP * fmaxf(1.f, fabsf((float)last)));
-        if (j == a.k) break;
-        if (m == -inf) {
+        if (check) {
+            const V mv = (V)value_of(m);
+            if (j > 0 && m > least) close |= too_close(last, mv);
+            last = mv;
+            if (j == a.k) break;
+        }
+        if (m == least) {
             if (lane_in_row == 0) for (int q = j; q < a.k; ++q) sel[q] = -1;
             break;
         }
         const int at = first_lane<LPR>(best == m, l0);
         if (lane_in_row == at) {
-            int w = EPL - 1;
+            int w = -1;
 #pragma unroll
-            for (int i = EPL - 2; i >= 0; --i) if (key[i] == m) w = i;
-#pragma unroll
-            for (int i = 0; i < EPL; ++i) if (i == w) key[i] = -inf;
+            for (int i = 0; i < EPL; ++i) {
+                const bool it = key[i] == m && w < 0;
+                w = it ? i : w;
+                key[i] = it ? least : key[i];
+            }
             sel[j] = e0 + w;
         }
-        last = m;
     }
     return close;
 }
@@ -182,7 +220,7 @@ __global__ void __launch_bounds__(RT) k_route(const RouteArgs a)
     const int lane = threadIdx.x & 63; const int lane_in_row = threadIdx.x % LPR, l0 = lane - lane % LPR, r_in_b = threadIdx.x / LPR;
     const int e0 = lane_in_row * EPL;
     int *sel = (int *)lds + r_in_b * a.k;
-    double *buf = (double *)(lds + ((size_t)RPB * a.k * 4 + 7) / 8 * 8) + (size_t)r_in_b * a.E;      // groups only
+    double *buf = (double *)(lds + (size_t)RPB * a.k * 8) + (size_t)r_in_b * a.E;      // groups only
     const bool fp64_keys = a.bias != nullptr || a.groups > 1;
     float bias[EPL];
 #pragma unroll
@@ -192,7 +230,8 @@ __global__ void __launch_bounds__(RT) k_route(const RouteArgs a)
         const int64_t row = r0 + r_in_b;
         const bool in = row < a.rows;
         const T *lg = (const T *)a.logits + (in ? row : 0) * a.E;
-        float x[EPL], key[EPL];
+        float x[EPL];
+        int key[EPL];
         if (in && e0 + EPL <= a.E) {
             const Pack<T, EPL> q = *(const Pack<T, EPL> *)(lg + e0);
 #pragma unroll
@@ -215,20 +254,20 @@ __global__ void __launch_bounds__(RT) k_route(const RouteArgs a)
         bool again = false;
         if (!fp64_keys) {
 #pragma unroll
-            for (int i = 0; i < EPL; ++i) key[i] = x[i] == x[i] ? x[i] : R_INF;
-            pick<LPR, EPL, float, false>(a, key, key, true, lane_in_row, l0, (float *)buf, sel);
+            for (int i = 0; i < EPL; ++i) key[i] = sortable(x[i] == x[i] ? x[i] : R_INF);
+            pick<LPR, EPL, int, float, false>(a, key, key, true, lane_in_row, l0, (float *)buf, sel);
         } else {
-            float gkey[EPL];
+            int gkey[EPL];
             const float inv = 1.f / sum;
 #pragma unroll
             for (int i = 0; i < EPL; ++i) {
                 const float s = a.score == 0 ? __expf(x[i] - top) * inv : __builtin_amdgcn_rcpf(1.f + __expf(-x[i]));
                 const float b = bias[i];
                 const float v = s + b;
-                gkey[i] = x[i] == -R_INF ? -R_INF : v == v ? v : spoiled(x[i], 3.4e38f);
-                key[i] = a.bias ? gkey[i] : x[i] == x[i] ? x[i] : R_INF;
+                gkey[i] = sortable(x[i] == -R_INF ? -R_INF : v == v ? v : spoiled(x[i], 3.4e38f));
+                key[i] = a.bias ? gkey[i] : sortable(x[i] == x[i] ? x[i] : R_INF);
             }
-            again = pick<LPR, EPL, float, true>(a, key, gkey, !a.bias, lane_in_row, l0, (float *)buf, sel);
+            again = pick<LPR, EPL, int, float, true>(a, key, gkey, !a.bias, lane_in_row, l0, (float *)buf, sel);
         }
         if (__any(again)) {
             double key2[EPL], gkey2[EPL];
@@ -248,38 +287,33 @@ __global__ void __launch_bounds__(RT) k_route(const RouteArgs a)
                 gkey2[i] = x[i] == -R_INF ? -(double)R_INF : v == v ? v : (double)spoiled(x[i], 3.4e38f);
                 key2[i] = a.bias ? gkey2[i] : x[i] == x[i] ? (double)x[i] : (double)R_INF;
             }
-            pick<LPR, EPL, double, false>(a, key2, gkey2, true, lane_in_row, l0, buf, sel);
+            pick<LPR, EPL, double, double, false>(a, key2, gkey2, true, lane_in_row, l0, buf, sel);
         }
         wave_lds_sync();
-        // weights: the chosen logits once more (they are in the cache), JN of the k to a lane
-        constexpr int JN = (ESCAT_ROUTE_MAX_K + LPR - 1) / LPR;
-        const float base = top;
-        float v[JN], m = -R_INF, z = 0.f;
-        int ex[JN];
-#pragma unroll
-        for (int i = 0; i < JN; ++i) {
-            const int j = lane_in_row + i * LPR;
-            ex[i] = in && j < a.k ? sel[j] : -1;
-            v[i] = ex[i] >= 0 ? to_f32(lg[ex[i]]) : -R_INF;
-        }
+        // weights: the chosen logits once more (they are in the cache), spread over the row's lanes; s_j waits in LDS next to sel
+        float m = -R_INF, z = 0.f;
         if (a.score == 0 && a.renorm) {
-#pragma unroll
-            for (int i = 0; i < JN; ++i) m = v[i] > m ? v[i] : m;
+            for (int j = lane_in_row; j < a.k; j += LPR) { const int e = sel[j]; if (in && e >= 0) { const float v = to_f32(lg[e]); m = v > m ? v : m; } }
             m = row_reduce<LPR, OpMax>(m);
-        } else m = base;
-#pragma unroll
-        for (int i = 0; i < JN; ++i) { v[i] = ex[i] < 0 ? 0.f : a.score == 0 ? expf(v[i] - m) : sigmoid_f(v[i]); z += v[i]; }
+        } else m = top;
+        float *sj = (float *)(sel + RPB * a.k);
+        for (int j = lane_in_row; j < a.k; j += LPR) {
+            const int e = sel[j];
+            const float v = in && e >= 0 ? to_f32(lg[e]) : 0.f;
+            const float q = e < 0 ? 0.f : a.score == 0 ? expf(v - m) : sigmoid_f(v);
+            sj[j] = q;
+            z += q;
+        }
         if (a.renorm) {
             z = row_reduce<LPR, OpSum>(z);
             z = a.score == 0 ? z : z + 1e-20f;
         } else z = a.score == 0 ? sum : 1.f;
-#pragma unroll
-        for (int i = 0; i < JN; ++i) {
-            const int j = lane_in_row + i * LPR;
-            if (!in || j >= a.k) continue;
-            a.weights[row * a.k + j] = ex[i] < 0 ? 0.f : a.scale * (v[i] / z);
-            a.experts[row * a.k + j] = ex[i];
-        }
+        if (in)
+            for (int j = lane_in_row; j < a.k; j += LPR) {
+                const int e = sel[j];
+                a.weights[row * a.k + j] = e < 0 ? 0.f : a.scale * (sj[j] / z);
+                a.experts[row * a.k + j] = e;
+            }
         wave_lds_sync();
     }
 }
@@ -296,7 +330,9 @@ template <typename T, int LPR, int EPL>
 __global__ void __launch_bounds__(RT) k_route_bwd(const RouteBwdArgs a)
 {
     constexpr int RPB = RT / LPR;
+    __shared__ __align__(16) float at_expert[RPB * LPR * EPL];             // the chosen experts' gradients find their places here
     const int lane_in_row = threadIdx.x % LPR, r_in_b = threadIdx.x / LPR, e0 = lane_in_row * EPL;
+    float *mine = at_expert + (size_t)threadIdx.x * EPL, *row_of = at_expert + (size_t)r_in_b * LPR * EPL;
     for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.rows; r0 += (int64_t)gridDim.x * RPB) {
         const int64_t row = r0 + r_in_b;
         const bool in = row < a.rows;
@@ -304,9 +340,9 @@ __global__ void __launch_bounds__(RT) k_route_bwd(const RouteBwdArgs a)
         const T *lg = (const T *)a.logits + rr * a.E;
         const float *dw = a.dw + rr * a.k, *w = a.weights + rr * a.k;
         const int *ex = a.experts + rr * a.k;
-        float d[EPL], s[EPL];
-        float z = 1.f, dot = 0.f;
-        if (a.score == 0 && !a.renorm) {
+        float s[EPL], z = 1.f, dot = 0.f;
+        const bool all = a.score == 0 && !a.renorm;           // every expert's logit has a gradient
+        if (all) {
             float top = -R_INF, sum = 0.f;
 #pragma unroll
             for (int i = 0; i < EPL; ++i) { s[i] = in && e0 + i < a.E ? to_f32(lg[e0 + i]) : -R_INF; top = fmaxf(top, s[i]); }
@@ -320,45 +356,43 @@ __global__ void __launch_bounds__(RT) k_route_bwd(const RouteBwdArgs a)
             for (int i = 0; i < EPL; ++i) s[i] /= sum;
             for (int j = lane_in_row; j < a.k; j += LPR) if (in && ex[j] >= 0) dot += w[j] * dw[j];
             dot = row_reduce<LPR, OpSum>(dot);                   // = scale sum_j s_j dw_j
-#pragma unroll
-            for (int i = 0; i < EPL; ++i) d[i] = -s[i] * dot;
-        } else {
-#pragma unroll
-            for (int i = 0; i < EPL; ++i) d[i] = 0.f;
-            if (a.renorm) {
-                float zz = 0.f;
-                for (int j = lane_in_row; j < a.k; j += LPR)
-                    if (in && ex[j] >= 0) {
-                        const float p = a.score == 0 ? w[j] : sigmoid_f(to_f32(lg[ex[j]]));
-                        dot += p * dw[j];
-                        zz += p;
-                    }
-                dot = row_reduce<LPR, OpSum>(dot);
-                if (a.score == 1) { z = row_reduce<LPR, OpSum>(zz) + 1e-20f; dot /= z; } else dot /= a.scale;
-            }
+        } else if (a.renorm) {
+            float zz = 0.f;
+            for (int j = lane_in_row; j < a.k; j += LPR)
+                if (in && ex[j] >= 0) {
+                    const float p = a.score == 0 ? w[j] : sigmoid_f(to_f32(lg[ex[j]]));
+                    dot += p * dw[j];
+                    zz += p;
+                }
+            dot = row_reduce<LPR, OpSum>(dot);
+            if (a.score == 1) { z = row_reduce<LPR, OpSum>(zz) + 1e-20f; dot /= z; } else dot /= a.scale;
         }
-        for (int j = 0; j < a.k; ++j) {                           // every lane looks at all k: k is small and they sit in the cache
+#pragma unroll
+        for (int i = 0; i < EPL; ++i) mine[i] = all ? -s[i] * dot : 0.f;
+        wave_lds_sync();
+        for (int j = lane_in_row; j < a.k; j += LPR) {            // no expert is chosen twice
             const int e = in ? ex[j] : -1;
-            if (e < e0 || e >= e0 + EPL) continue;                // (another lane's, or -1)
+            if (e < 0) continue;
             float v;
             if (a.score == 0) v = a.renorm ? w[j] * (dw[j] - dot) : w[j] * dw[j];
             else {
                 const float q = sigmoid_f(to_f32(lg[e]));
                 v = a.scale * q * (1.f - q) * (a.renorm ? (dw[j] - dot) / z : dw[j]);
             }
-#pragma unroll
-            for (int i = 0; i < EPL; ++i) if (i == e - e0) d[i] += v;
+            row_of[e] += v;
         }
+        wave_lds_sync();
         T *out = (T *)a.dl + rr * a.E;
         if (in && e0 + EPL <= a.E) {
             Pack<T, EPL> q;
 #pragma unroll
-            for (int i = 0; i < EPL; ++i) q.v[i] = from_f32<T>(d[i]);
+            for (int i = 0; i < EPL; ++i) q.v[i] = from_f32<T>(mine[i]);
             *(Pack<T, EPL> *)(out + e0) = q;
         } else if (in) {
 #pragma unroll
-            for (int i = 0; i < EPL; ++i) if (e0 + i < a.E) out[e0 + i] = from_f32<T>(d[i]);
+            for (int i = 0; i < EPL; ++i) if (e0 + i < a.E) out[e0 + i] = from_f32<T>(mine[i]);
         }
+        wave_lds_sync();
     }
 }
 
@@ -421,7 +455,7 @@ extern "C" int escat_route(const void *logits, int type, int64_t rows, int E, in
     if (!logits || !weights || !experts) return fail(ESCAT_EINVAL, "escat_route: null pointer");
     if (keep_groups == groups) groups = keep_groups = 1;             // every group stays: no groups
     const int epl = E > 512 ? 16 : 8, lpr = lanes_per_row(E, epl, groups), rpb = RT / lpr;
-    const size_t lds = ((size_t)rpb * k * 4 + 7) / 8 * 8 + (groups > 1 ? (size_t)rpb * E * 8 : 0);
+    const size_t lds = (size_t)rpb * k * 8 + (groups > 1 ? (size_t)rpb * E * 8 : 0);
     const int64_t want = (rows + rpb - 1) / rpb;
     const RouteArgs a = {logits, bias, weights, experts, rows, E, k, groups, keep_groups, group_top, score, renorm ? 1 : 0, scale};
     return route_dispatch<LaunchFwd>(type, lpr, epl, a, (unsigned)(want < 2048 ? want : 2048), lds, (hipStream_t)stream);
