@@ -193,13 +193,11 @@ __device__ bool pick(const RouteArgs &a, K (&key)[EPL], const K (&gkey)[EPL], bo
         }
         const int at = first_lane<LPR>(best == m, l0);
         if (lane_in_row == at) {
-            int w = -1;
+            int w = EPL - 1;
 #pragma unroll
-            for (int i = 0; i < EPL; ++i) {
-                const bool it = key[i] == m && w < 0;
-                w = it ? i : w;
-                key[i] = it ? least : key[i];
-            }
+            for (int i = EPL - 2; i >= 0; --i) w = key[i] == m ? i : w;
+#pragma unroll
+            for (int i = 0; i < EPL; ++i) key[i] = i == w ? least : key[i];
             sel[j] = e0 + w;
         }
     }
@@ -247,7 +245,7 @@ __global__ void __launch_bounds__(RT) k_route(const RouteArgs a)
             top = row_reduce<LPR, OpMax>(top);
             const float base = top == -R_INF ? 0.f : top;
 #pragma unroll
-            for (int i = 0; i < EPL; ++i) sum += a.renorm ? __expf(x[i] - base) : expf(x[i] - base);
+            for (int i = 0; i < EPL; ++i) sum += expf(x[i] - base);
             sum = row_reduce<LPR, OpSum>(sum);
             top = base;
         }
@@ -258,32 +256,50 @@ __global__ void __launch_bounds__(RT) k_route(const RouteArgs a)
             pick<LPR, EPL, int, float, false>(a, key, key, true, lane_in_row, l0, (float *)buf, sel);
         } else {
             int gkey[EPL];
-            const float inv = 1.f / sum;
+            float sc[EPL];
+            // (the form of the scores is asked for outside the loops over a lane's experts: inside it is a branch for each)
+            if (a.score == 0) {
+                const float inv = 1.f / sum;
+#pragma unroll
+                for (int i = 0; i < EPL; ++i) sc[i] = __expf(x[i] - top) * inv;
+            } else {
+#pragma unroll
+                for (int i = 0; i < EPL; ++i) sc[i] = __builtin_amdgcn_rcpf(1.f + __expf(-x[i]));
+            }
 #pragma unroll
             for (int i = 0; i < EPL; ++i) {
-                const float s = a.score == 0 ? __expf(x[i] - top) * inv : __builtin_amdgcn_rcpf(1.f + __expf(-x[i]));
-                const float b = bias[i];
-                const float v = s + b;
-                gkey[i] = sortable(x[i] == -R_INF ? -R_INF : v == v ? v : spoiled(x[i], 3.4e38f));
-                key[i] = a.bias ? gkey[i] : sortable(x[i] == x[i] ? x[i] : R_INF);
+                const float v = sc[i] + bias[i], t = v == v ? v : spoiled(x[i], 3.4e38f);
+                gkey[i] = sortable(x[i] == -R_INF ? -R_INF : t);
+            }
+            if (a.bias) {
+#pragma unroll
+                for (int i = 0; i < EPL; ++i) key[i] = gkey[i];
+            } else {
+#pragma unroll
+                for (int i = 0; i < EPL; ++i) key[i] = sortable(x[i] == x[i] ? x[i] : R_INF);
             }
             again = pick<LPR, EPL, int, float, true>(a, key, gkey, !a.bias, lane_in_row, l0, (float *)buf, sel);
         }
         if (__any(again)) {
             double key2[EPL], gkey2[EPL];
-            double top2 = -(double)R_INF, sum2 = 0.0;
             if (a.score == 0) {
+                double top2 = -(double)R_INF, sum2 = 0.0;
 #pragma unroll
                 for (int i = 0; i < EPL; ++i) top2 = fmax(top2, (double)x[i]);
                 top2 = row_reduce<LPR, OpMax>(top2);
                 top2 = top2 == -(double)R_INF ? 0.0 : top2;
-                for (int i = 0; i < EPL; ++i) sum2 += exp((double)x[i] - top2);
+#pragma unroll
+                for (int i = 0; i < EPL; ++i) { gkey2[i] = exp((double)x[i] - top2); sum2 += gkey2[i]; }
                 sum2 = row_reduce<LPR, OpSum>(sum2);
+#pragma unroll
+                for (int i = 0; i < EPL; ++i) gkey2[i] /= sum2;
+            } else {
+#pragma unroll
+                for (int i = 0; i < EPL; ++i) gkey2[i] = 1.0 / (1.0 + exp(-(double)x[i]));
             }
 #pragma unroll
             for (int i = 0; i < EPL; ++i) {
-                const double s = a.score == 0 ? exp((double)x[i] - top2) / sum2 : 1.0 / (1.0 + exp(-(double)x[i]));
-                const double v = s + (double)bias[i];
+                const double v = gkey2[i] + (double)bias[i];
                 gkey2[i] = x[i] == -R_INF ? -(double)R_INF : v == v ? v : (double)spoiled(x[i], 3.4e38f);
                 key2[i] = a.bias ? gkey2[i] : x[i] == x[i] ? (double)x[i] : (double)R_INF;
             }
