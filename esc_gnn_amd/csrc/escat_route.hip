@@ -129,10 +129,12 @@ __device__ bool pick(const RouteArgs &a, K (&key)[EPL], const K (&gkey)[EPL], bo
             for (int r = 0; r <= a.keep; ++r) {
                 const K m = row_reduce<LPR, OpMax>(score);
                 const V mv = (V)value_of(m);
-                if (CHECK && r > 0 && m > least) close |= too_close(last, mv);
-                if (r == a.keep || m == least) break;
+                if (CHECK && r > 0) close |= m > least && too_close(last, mv);
+                if (r == a.keep) break;
                 const int at = first_lane<LPR>(score == m, l0);
-                if ((at ^ lane_in_row) < lpg) { kept = true; score = least; }         // the same group: only bits below lpg differ
+                const bool it = (at ^ lane_in_row) < lpg && m > least;                // the same group: only bits below lpg differ
+                kept |= it;
+                score = it ? least : score;
                 last = mv;
             }
 #pragma unroll
@@ -174,32 +176,31 @@ __device__ bool pick(const RouteArgs &a, K (&key)[EPL], const K (&gkey)[EPL], bo
             }
         }
     }
+    // k rounds (one more to see how far behind the next one is); no round ends early: rows of a wave would part ways
     const bool check = CHECK && !key_exact;
     V last = inf;
-    for (int j = 0; j < a.k + (check ? 1 : 0); ++j) {
+    for (int j = 0; ; ++j) {
         K best = key[0];
 #pragma unroll
         for (int i = 1; i < EPL; ++i) best = key[i] > best ? key[i] : best;
         const K m = row_reduce<LPR, OpMax>(best);
+        const bool some = m > least;
         if (check) {
             const V mv = (V)value_of(m);
-            if (j > 0 && m > least) close |= too_close(last, mv);
+            close |= j > 0 && some && too_close(last, mv);
             last = mv;
-            if (j == a.k) break;
         }
-        if (m == least) {
-            if (lane_in_row == 0) for (int q = j; q < a.k; ++q) sel[q] = -1;
-            break;
-        }
+        if (j == a.k) break;
         const int at = first_lane<LPR>(best == m, l0);
-        if (lane_in_row == at) {
-            int w = EPL - 1;
+        const bool mine = lane_in_row == at;
+        int w = EPL - 1;
 #pragma unroll
-            for (int i = EPL - 2; i >= 0; --i) w = key[i] == m ? i : w;
+        for (int i = EPL - 2; i >= 0; --i) w = key[i] == m ? i : w;
+        if (mine) sel[j] = some ? e0 + w : -1;
+        w = mine ? w : -1;
 #pragma unroll
-            for (int i = 0; i < EPL; ++i) key[i] = i == w ? least : key[i];
-            sel[j] = e0 + w;
-        }
+        for (int i = 0; i < EPL; ++i) key[i] = i == w ? least : key[i];
+        if (!check && j + 1 == a.k) break;
     }
     return close;
 }
