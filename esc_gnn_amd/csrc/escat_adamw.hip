@@ -27,7 +27,7 @@
 #define AU 4                                     // blocks of a wave: all their loads are in flight before the first is used
 #define ACHUNK (AQ * AU * (AT / 64))             // elements of a workgroup
 #define ATENSORS 56                              // tensors of a launch: 56 x 64 B of kernel arguments
-#define NORM_WGS 1024
+#define NORM_WGS 2048                            // partial sums of a launch, at most
 #define TOP_M 245760.0f                          // 15 * 2^14
 #define TOP_V 15032385536.0f                     // 14 * 2^30
 #define HDR_FLOATS 64                            // workspace header: clip, then {step size, 1/sqrt(1 - b2^t)} per group
@@ -51,8 +51,10 @@ __global__ void __launch_bounds__(AT) k_grad_squares(const ATable tab, double *_
     __shared__ double red[AT / 64];
     const int tid = threadIdx.x;
     double acc = 0.0;
+    int at = find_tensor(tab, blockIdx.x);
     for (uint32_t c = blockIdx.x; c < tab.chunks; c += gridDim.x) {
-        const ATensor &t = tab.t[find_tensor(tab, c)];
+        while (at + 1 < tab.n && tab.t[at + 1].chunk0 <= c) ++at;
+        const ATensor &t = tab.t[at];
         const int64_t i0 = (int64_t)(c - t.chunk0) * ACHUNK;
         const G *g = (const G *)t.g;
         if (i0 + ACHUNK <= t.n) {
@@ -173,8 +175,10 @@ __device__ __forceinline__ AVals adamw_one(float p, float g, float m, float v, c
     g = g * clip;
     m = m * s.b1 + g * s.omb1;
     v = v * s.b2 + (g * g) * s.omb2;
-    const float num = m * size, den = sqrtf(v) * isb + s.eps;
-    return {p * s.decay - num / den, m, v};
+    // (hardware root and reciprocal, 1 unit in the last place of the update each: an exact root and quotient are 25 instructions more, which
+    // the 8-bit form has no room for; the moments do not pass here)
+    const float num = m * size, den = __builtin_amdgcn_sqrtf(v) * isb + s.eps;
+    return {p * s.decay - num * __builtin_amdgcn_rcpf(den), m, v};
 }
 
 template <typename P, typename G, int BITS>
@@ -294,17 +298,22 @@ __global__ void __launch_bounds__(AT) k_adamw(const ATable tab, const AScalars s
 template <bool SIGNED>
 __global__ void __launch_bounds__(AT) k_state8_values(const uint8_t *__restrict__ code, const float *__restrict__ scale, int64_t n, float *__restrict__ out)
 {
-    const int64_t i = ((int64_t)blockIdx.x * AT + threadIdx.x) * 4;
-    if (i >= n) return;
-    const float s = scale[i / AQ];
-    if (i + 4 <= n) {
-        const Pack<uint8_t, 4> c = *(const Pack<uint8_t, 4> *)(code + i);
-        Pack<float, 4> o;
+    const int64_t i0 = ((int64_t)blockIdx.x * AU * AT + threadIdx.x) * 4;
+    if (i0 + (AU - 1) * AT * 4 + 4 <= n) {
+        Pack<uint8_t, 4> c[AU];
+        float z[AU];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) o.v[k] = decode8<SIGNED>(c.v[k], s);
-        *(Pack<float, 4> *)(out + i) = o;
+        for (int u = 0; u < AU; ++u) { c[u] = *(const Pack<uint8_t, 4> *)(code + i0 + u * AT * 4); z[u] = scale[(i0 + u * AT * 4) / AQ]; }
+#pragma unroll
+        for (int u = 0; u < AU; ++u) {
+            Pack<float, 4> o;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o.v[k] = decode8<SIGNED>(c[u].v[k], z[u]);
+            *(Pack<float, 4> *)(out + i0 + u * AT * 4) = o;
+        }
     } else {
-        for (int64_t j = i; j < n; ++j) out[j] = decode8<SIGNED>(code[j], s);
+        for (int u = 0; u < AU; ++u)
+            for (int64_t j = i0 + u * AT * 4; j < i0 + u * AT * 4 + 4 && j < n; ++j) out[j] = decode8<SIGNED>(code[j], scale[j / AQ]);
     }
 }
 
@@ -361,17 +370,18 @@ extern "C" int escat_adamw_begin(const escat_adamw_tensor *tensors, int n_tensor
     if (finish && clip && !norm_out) return fail(ESCAT_EINVAL, "escat_adamw_begin: clipping needs norm_out");
     hipStream_t st = (hipStream_t)stream;
     double *partial = (double *)((char *)workspace + HDR_FLOATS * 4);
-    const int64_t room = (int64_t)((workspace_bytes - HDR_FLOATS * 4) / (NORM_WGS * 8));
+    const int64_t room = (int64_t)((workspace_bytes - HDR_FLOATS * 4) / 8);
     int slot = partial_slot;
     if (clip) {
         rc = for_tables(tensors, n_tensors, [&](const ATable &tab, int) {
-            if (slot >= room) return fail(ESCAT_EWORKSPACE, "escat_adamw_begin: workspace of %zu bytes holds %lld launches' sums", workspace_bytes, (long long)room);
-            double *out = partial + (size_t)slot++ * NORM_WGS;
-            // a full set of sums is always written: those of the workgroups without a chunk are 0
+            const unsigned wgs = tab.chunks < NORM_WGS ? tab.chunks : NORM_WGS;
+            if (slot + (int64_t)wgs > room) return fail(ESCAT_EWORKSPACE, "escat_adamw_begin: workspace of %zu bytes holds %lld partial sums", workspace_bytes, (long long)room);
+            double *out = partial + slot;
+            slot += (int)wgs;
             switch (grad_type) {
-            case ESCAT_F32: k_grad_squares<float><<<NORM_WGS, AT, 0, st>>>(tab, out); break;
-            case ESCAT_BF16: k_grad_squares<bf16_t><<<NORM_WGS, AT, 0, st>>>(tab, out); break;
-            default: k_grad_squares<f16_t><<<NORM_WGS, AT, 0, st>>>(tab, out); break;
+            case ESCAT_F32: k_grad_squares<float><<<wgs, AT, 0, st>>>(tab, out); break;
+            case ESCAT_BF16: k_grad_squares<bf16_t><<<wgs, AT, 0, st>>>(tab, out); break;
+            default: k_grad_squares<f16_t><<<wgs, AT, 0, st>>>(tab, out); break;
             }
             CHECK_LAUNCH("escat_adamw_begin: squares");
             return ESCAT_OK;
@@ -382,7 +392,7 @@ extern "C" int escat_adamw_begin(const escat_adamw_tensor *tensors, int n_tensor
     AGroups gr;
     gr.n = n_groups;
     for (int i = 0; i < n_groups; ++i) { gr.lr[i] = groups[i].lr; gr.b1[i] = groups[i].beta1; gr.b2[i] = groups[i].beta2; }
-    k_adamw_begin<<<1, AT, 0, st>>>(partial, clip ? slot * NORM_WGS : 0, clip ? 1 : 0, max_norm, gr, step, (float *)workspace, norm_out);
+    k_adamw_begin<<<1, AT, 0, st>>>(partial, clip ? slot : 0, clip ? 1 : 0, max_norm, gr, step, (float *)workspace, norm_out);
     CHECK_LAUNCH("escat_adamw_begin");
     return slot;
 }
@@ -425,7 +435,7 @@ extern "C" int escat_state8_values(const uint8_t *codes, const float *scales, in
 {
     if (n < 0 || (n > 0 && (!codes || !scales || !out))) return fail(ESCAT_EINVAL, "escat_state8_values: n = %lld or a null pointer", (long long)n);
     if (n == 0) return ESCAT_OK;
-    const int64_t wgs = (n + AT * 4 - 1) / (AT * 4);
+    const int64_t wgs = (n + AU * AT * 4 - 1) / (AU * AT * 4);
     if (wgs > 0xffffff) return fail(ESCAT_ERANGE, "escat_state8_values: n = %lld", (long long)n);
     hipStream_t st = (hipStream_t)stream;
     if (is_signed) k_state8_values<true><<<(unsigned)wgs, AT, 0, st>>>(codes, scales, n, out);

@@ -545,7 +545,7 @@ int escat_recover_factored(const int32_t *rowptr, const int32_t *col, const floa
  *   ordinal  number of the tensor among all that share `seed` (the rounding bits of 8-bit states depend on it)
  * A step is escat_adamw_begin (sums of squares when max_norm > 0, the step count, the scalars), then one
  * escat_adamw_update per group and pair of types, on one stream, with one workspace:
- *   escat_adamw_begin  returns the number of partial-sum slots filled so far (>= 0) or an error (< 0).  Gradients of several
+ *   escat_adamw_begin  returns the number of partial sums so far (>= 0) or an error (< 0).  Gradients of several
  *      types: one call per type with finish = 0, each given the previous call's return as partial_slot, the last with finish = 1.
  *      finish = 1 joins the sums, adds 1 to *step (device) and, if max_norm > 0, leaves the norm in *norm_out (device).
  *   escat_adamw_update reads the scalars of groups[group_index] as escat_adamw_begin left them.
