@@ -43,6 +43,18 @@ def max_over_ranks(seconds: float, device=None) -> float:
     return float(t.item())
 
 
+def allreduce_sum_(t: torch.Tensor) -> torch.Tensor:
+    """sum of a small tensor over the ranks, in place; identity when not distributed (gloo: by way of the host)"""
+    if dist.is_available() and dist.is_initialized() and dist.get_world_size() > 1:
+        if t.is_cuda and dist.get_backend() == "gloo":
+            h = t.cpu()
+            dist.all_reduce(h, op=dist.ReduceOp.SUM)
+            t.copy_(h)
+        else:
+            dist.all_reduce(t, op=dist.ReduceOp.SUM)
+    return t
+
+
 class FlatGradBucket:
     """
     One flat fp32 buffer aliasing the .grad of every parameter: backward writes

@@ -109,3 +109,15 @@ def test_experts_library_checks_its_arguments():
     assert lib.escat_experts_plan(16, 5, 1, 4, 16, 8, 0, 0) == -3
     assert lib.escat_experts_plan(16, 1 << 31, 1, 4, 16, 8, 0, 0) == -2
     assert lib.escat_experts_plan(16, 5, 2, 4, 16, 1 << 20, 16, 0) == -1                          # counts of k = 2
+
+
+def test_head_options_refuse():
+    from esc_gnn_amd.train_dp import DPTrainer, NodeExperts, ScatteringHead
+    kw = dict(diffusion_kwargs=dict(scales_type="dyadic", J=2, include_lowpass=True))
+    with pytest.raises(ValueError):
+        DPTrainer(C=3, optimizer="sgd", **kw)
+    with pytest.raises(ValueError):
+        NodeExperts(8, 2, 3)
+    head = ScatteringHead(4, 4, experts=4)
+    with pytest.raises(RuntimeError):                                             # CPU tensors
+        head(torch.zeros(6, 4), torch.zeros(6, 4), torch.zeros(6, dtype=torch.int64), 1)

@@ -1,0 +1,87 @@
+"""GPU tests of the training step with experts in the head and the multi-tensor AdamW (train_dp.DPTrainer's options)."""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def batch(B=48, n=64):
+    from esc_gnn_amd import synthetic
+    from esc_gnn_amd.process_pyg_data import build_PQ_batch
+    clouds = synthetic.ellipsoid_clouds(B, n, seed=3)
+    pos = torch.from_numpy(clouds.reshape(-1, 3)).to(DEV)
+    gp = torch.arange(B + 1, dtype=torch.int32, device=DEV) * n
+    b = build_PQ_batch(pos, gp, 5, {"kernel": "gaussian", "gaussian_eps": 0.05})
+    gid = torch.arange(B, device=DEV).repeat_interleave(n)
+    target = torch.from_numpy((clouds.max(1) - clouds.min(1)).max(1).astype(np.float32)).to(DEV)
+    pc = b["P"].csr(); rp = pc.rowptr.long()
+    rows = torch.repeat_interleave(torch.arange(pc.n, device=DEV), rp[1:] - rp[:-1]); cols = pc.col.long()
+    edge_index = torch.stack([cols[rows != cols], rows[rows != cols]])
+    return pos, pos, b["P"], b["Q"], gid, B, target, edge_index
+
+
+@pytest.mark.parametrize("amp", [False, True])
+@pytest.mark.parametrize("optimizer,clip", [("torch", 1.0), ("escat", None), ("escat", 1.0), ("escat8", 1.0)])
+def test_step_runs_with_experts(optimizer, clip, amp):
+    from esc_gnn_amd.train_dp import DPTrainer, NodeExperts
+    data = batch()
+    torch.manual_seed(0)
+    tr = DPTrainer(C=3, diffusion_kwargs=dict(scales_type="dyadic", J=3, include_lowpass=True), device=DEV, amp_bf16=amp, experts=6,
+                   optimizer=optimizer, max_grad_norm=clip)
+    before = [p.detach().clone() for p in tr.model.parameters()]
+    losses = [float(tr.step(*data).detach()) for _ in range(4)]
+    assert all(np.isfinite(losses))
+    m = [m for m in tr.model.mlp if isinstance(m, NodeExperts)][0]
+    assert int(m.load.sum()) == 0 and float(m.balance.abs().max()) <= 4 * m.rate + 1e-9
+    for (name, p), q in zip(tr.model.named_parameters(), before):
+        assert bool(torch.isfinite(p).all()) and not torch.equal(p, q), name
+    assert all(p.grad.data_ptr() >= tr.bucket.flat.data_ptr() for p in tr.model.parameters())
+    if optimizer != "torch":
+        assert (tr.opt.grad_norm is None) == (clip is None)
+
+
+def test_gradients_of_the_layer_against_64_bits():
+    """NodeExperts against the same formula in 64 bits on the experts that it chose; sums of <= 700 x 32 products, relative to the
+    largest entry 2000 u (u = 2^-24) holds with room"""
+    from esc_gnn_amd import route_experts
+    from esc_gnn_amd.train_dp import NodeExperts
+    torch.manual_seed(2)
+    layer = NodeExperts(32, 5, 2).to(DEV)
+    layer.balance.copy_(torch.tensor([0.02, -0.02, 0.0, 0.01, -0.01]))
+    x = torch.randn(700, 32, device=DEV).requires_grad_()
+    up = torch.randn(700, 32, device=DEV)
+    y = layer(x)
+    ps = dict(layer.named_parameters())
+    got = dict(zip(["x", *ps], torch.autograd.grad(y, [x, *ps.values()], up)))
+    w, e = route_experts(torch.nn.functional.linear(x, layer.router.weight).detach(), 2, bias=layer.balance)
+    assert int(layer.load.sum()) == 1400
+    q = {"x": x.detach().double().requires_grad_(), **{n: p.detach().double().requires_grad_() for n, p in ps.items()}}
+    w64 = torch.softmax((q["x"] @ q["router.weight"].t()).gather(1, e.long()), 1)
+    z = torch.stack([torch.nn.functional.silu(q["x"] @ q["w1"][i].t() + q["b1"][i]) @ q["w2"][i].t() + q["b2"][i] for i in range(5)], 1)
+    y64 = q["x"] + (w64[..., None] * z.gather(1, e.long()[..., None].expand(-1, -1, 32))).sum(1)
+    want = dict(zip(q, torch.autograd.grad(y64, list(q.values()), up.double())))
+    for n in want:
+        assert float((got[n].double() - want[n]).abs().max()) <= 2000 * 2.0 ** -24 * float(want[n].abs().max()), n
+
+
+def test_balance_bias_pulls_the_loads_together():
+    from esc_gnn_amd.train_dp import NodeExperts
+    torch.manual_seed(1)
+    layer = NodeExperts(16, 8, 2, rate=0.02).to(DEV)
+    x = torch.randn(4000, 16, device=DEV) + 0.5
+    spread = []
+    with torch.no_grad():
+        for _ in range(60):
+            layer(x)
+            spread.append(float(layer.load.float().std()))
+            layer.update_balance()
+    assert spread[-1] < 0.5 * spread[0]
+
+
+def test_default_head_is_as_before():
+    from esc_gnn_amd.train_dp import ScatteringHead
+    torch.manual_seed(0)
+    h = ScatteringHead(7, 9)
+    assert [tuple(p.shape) for p in h.parameters()] == [(16,), (16,), (256, 16), (256,), (256, 256), (256,), (1, 256), (1,)]
