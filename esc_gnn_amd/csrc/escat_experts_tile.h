@@ -44,12 +44,18 @@ template <typename T> __device__ __forceinline__ u4 load16(const T *p)
     u4 r; __builtin_memcpy(&r, &q, 16);
     return r;
 }
+// (by 32-bit selects: a 64-bit shift whose amount lies in the last VGPR of a kernel's allocation shifts by something else on this card)
 template <typename T> __device__ __forceinline__ u4 moved(u4 v, int s)
 {
-    unsigned __int128 x; __builtin_memcpy(&x, &v, 16);
-    x = s >= Elem<T>::PER ? 0 : x >> (s * 8 * (int)sizeof(T));
-    __builtin_memcpy(&v, &x, 16);
-    return v;
+    if (sizeof(T) == 2) {
+        const bool odd = s & 1;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { const unsigned next = i < 3 ? v[i + 1] : 0u; v[i] = odd ? __builtin_amdgcn_alignbit(next, v[i], 16) : v[i]; }
+        s >>= 1;
+    }
+    const bool one = s & 1, two = s & 2, all = s >= 4;
+    const u4 a = {one ? v[1] : v[0], one ? v[2] : v[1], one ? v[3] : v[2], one ? 0u : v[3]};
+    return u4{all ? 0u : two ? a[2] : a[0], all ? 0u : two ? a[3] : a[1], all || two ? 0u : a[2], all || two ? 0u : a[3]};
 }
 template <typename T> __device__ __forceinline__ void to_floats(u4 r, float (&f)[Elem<T>::PER])
 {

@@ -297,3 +297,16 @@ def test_a_run_of_them_together():
     opt = AdamW(ps.values(), lr=1e-2, state_bits=8, max_grad_norm=1.0)
     opt.step()
     assert all(bool(torch.isfinite(p).all()) and not torch.equal(p, before[n]) for n, p in ps.items())
+
+
+@pytest.mark.parametrize("shape", [(11403, 106, 57, 200, 34, 1), (9000, 112, 34, 48, 20, 4), (9000, 40, 185, 144, 12, 2)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_that_end_inside_a_piece_of_16_bytes(shape, dtype):
+    """two or three elements behind the last whole piece of a hidden row, more rows than the form for few takes"""
+    check(make(*shape, dtype, False, seed=11), dtype)
+
+
+@pytest.mark.parametrize("width", range(57, 66))
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_every_remainder_of_a_row(width, dtype):
+    check(make(2600, width, width + 3, width + 6, 6, 2, dtype, True, seed=width), dtype)
