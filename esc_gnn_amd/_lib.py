@@ -94,10 +94,11 @@ SIGNATURES = {
     "escat_route_bwd": (ci, [vp, ci, i64, ci, ci, ci, ci, ctypes.c_float, vp, vp, vp, vp, vp]),
     "escat_experts_plan_bytes": (sz, [i64, ci, ci]),
     "escat_experts_plan": (ci, [vp, i64, ci, ci, vp, sz, vp, vp]),
-    "escat_experts_workspace_bytes": (sz, [vp, ci]),
+    "escat_experts_hidden_bytes": (sz, [vp]),
+    "escat_experts_workspace_bytes": (sz, [vp, ci, ci]),
     "escat_experts_fwd_needs_plan": (ci, [vp]),
-    "escat_experts_fwd": (ci, [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]),
-    "escat_experts_bwd": (ci, [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]),
+    "escat_experts_fwd": (ci, [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]),
+    "escat_experts_bwd": (ci, [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]),
     "escat_lookup3": (ctypes.c_uint32, [ctypes.c_char_p, sz, ctypes.c_uint32]),
     "escat_build_workspace_bytes": (sz, [i64, ci, ci]),
     "escat_build_knn_P": (ci, [vp, vp, ci, i64, ci, ci, vp, vp, vp, i64, vp, vp, sz, vp]),

@@ -33,7 +33,7 @@ static int check_dims(const char *who, const escat_experts_dims *n)
 static EDims dims_of(const escat_experts_dims *n) { return {n->rows, n->d, n->h, n->o, n->experts, n->k}; }
 static size_t up(size_t b) { return (b + 255) & ~(size_t)255; }
 
-// workspace of the forward: h | by pair: results of the pairs;  of the backward: h | du | by pair: results of the pairs, by combination:
+// workspace of the forward: h (unless the caller keeps it) | by pair: results of the pairs;  of the backward: h (unless kept) | du | by pair: results of the pairs, by combination:
 // positions sorted by expert | parts of dw | weights by position | chunks of the
 // weight gradients (one after the other in the same place)
 static size_t part_bytes(const escat_experts_dims *n, int M) { return combo_keys(n->rows, n->experts, n->k) ? 0 : up((size_t)n->rows * n->k * M * 4); }
@@ -53,13 +53,16 @@ static size_t chunk_bytes(const escat_experts_dims *n, int M, int N)
     return c ? up((size_t)escat_experts_grad_chunks(P, n->experts, c) * ((size_t)M * N + N) * 4) : 0;
 }
 
-extern "C" size_t escat_experts_workspace_bytes(const escat_experts_dims *n, int backward)
+extern "C" size_t escat_experts_hidden_bytes(const escat_experts_dims *n) { return check_dims("escat_experts_hidden_bytes", n) ? 0 : hidden_bytes(n) + 256; }
+
+extern "C" size_t escat_experts_workspace_bytes(const escat_experts_dims *n, int backward, int hidden)
 {
     if (check_dims("escat_experts_workspace_bytes", n)) return 0;
+    const size_t own = hidden ? 0 : hidden_bytes(n);
     if (!backward && escat_experts_few(n->type, dims_of(n))) return up((size_t)n->rows * n->k * n->h * 4) + 256;
-    if (!backward) return hidden_bytes(n) + part_bytes(n, n->o) + 256;
+    if (!backward) return own + part_bytes(n, n->o) + 256;
     const size_t c1 = chunk_bytes(n, n->d, n->h), c2 = chunk_bytes(n, n->h, n->o);
-    return 2 * hidden_bytes(n) + part_bytes(n, n->d) + by_expert_bytes(n) + up((size_t)((n->h + XN - 1) / XN) * n->rows * n->k * 4) + up((size_t)n->rows * n->k * 4) + (c1 > c2 ? c1 : c2) + 256;
+    return own + hidden_bytes(n) + part_bytes(n, n->d) + by_expert_bytes(n) + up((size_t)((n->h + XN - 1) / XN) * n->rows * n->k * 4) + up((size_t)n->rows * n->k * 4) + (c1 > c2 ? c1 : c2) + 256;
 }
 
 extern "C" int escat_experts_fwd_needs_plan(const escat_experts_dims *n)
@@ -69,22 +72,25 @@ extern "C" int escat_experts_fwd_needs_plan(const escat_experts_dims *n)
 }
 
 extern "C" int escat_experts_fwd(const escat_experts_dims *n, const void *x, const float *weights, const int32_t *experts_of_rows, const void *w1, const void *b1,
-                                 const void *w2, const void *b2, const void *plan, void *y, void *workspace, size_t workspace_bytes, void *stream)
+                                 const void *w2, const void *b2, const void *plan, void *y, void *hidden, void *workspace, size_t workspace_bytes, void *stream)
 {
     int rc = check_dims("escat_experts_fwd", n); if (rc) return rc;
     if (n->rows == 0) return ESCAT_OK;
     const bool few = escat_experts_few(n->type, dims_of(n));
     if (!x || !weights || !w1 || !w2 || !y || (few ? !experts_of_rows : !plan)) return fail(ESCAT_EINVAL, "escat_experts_fwd: null pointer");
-    if (!workspace || workspace_bytes < escat_experts_workspace_bytes(n, 0) || ((uintptr_t)workspace & 15))
-        return fail(ESCAT_EWORKSPACE, "escat_experts_fwd: workspace of %zu bytes (16-byte aligned), needs %zu", workspace_bytes, escat_experts_workspace_bytes(n, 0));
+    if (hidden && ((uintptr_t)hidden & 15)) return fail(ESCAT_EINVAL, "escat_experts: hidden is not aligned to 16 bytes");
+    if (!workspace || workspace_bytes < escat_experts_workspace_bytes(n, 0, hidden != nullptr) || ((uintptr_t)workspace & 15))
+        return fail(ESCAT_EWORKSPACE, "escat_experts_fwd: workspace of %zu bytes (16-byte aligned), needs %zu", workspace_bytes, escat_experts_workspace_bytes(n, 0, hidden != nullptr));
     char *ws = (char *)workspace;
     if (few) return escat_experts_few_fwd(n->type, dims_of(n), experts_of_rows, x, weights, w1, b1, w2, b2, (float *)ws, y, (hipStream_t)stream);
     const EPlan p = plan_of(const_cast<void *>(plan), n->rows, n->k, n->experts);
-    return escat_experts_rows_fwd(n->type, dims_of(n), p, x, weights, w1, b1, w2, b2, ws, (float *)(ws + hidden_bytes(n)), y, (hipStream_t)stream);
+    void *h = hidden;
+    if (!h) { h = ws; ws += hidden_bytes(n); }
+    return escat_experts_rows_fwd(n->type, dims_of(n), p, x, weights, w1, b1, w2, b2, h, (float *)ws, y, (hipStream_t)stream);
 }
 
 extern "C" int escat_experts_bwd(const escat_experts_dims *n, const void *x, const float *weights, const void *w1, const void *b1, const void *w2,
-                                 const void *b2, const void *plan, const void *dy, void *dx, float *dweights, void *dw1, void *db1, void *dw2, void *db2,
+                                 const void *b2, const void *plan, const void *hidden, const void *dy, void *dx, float *dweights, void *dw1, void *db1, void *dw2, void *db2,
                                  void *workspace, size_t workspace_bytes, void *stream)
 {
     int rc = check_dims("escat_experts_bwd", n); if (rc) return rc;
@@ -92,11 +98,13 @@ extern "C" int escat_experts_bwd(const escat_experts_dims *n, const void *x, con
     if (!w1 || !w2 || !plan) return fail(ESCAT_EINVAL, "escat_experts_bwd: null pointer");
     if (n->rows > 0 && (!x || !weights || !dy)) return fail(ESCAT_EINVAL, "escat_experts_bwd: null pointer");
     if ((db1 && !dw1) || (db2 && !dw2)) return fail(ESCAT_EINVAL, "escat_experts_bwd: a bias's gradient comes with its weight's");
-    if (!workspace || workspace_bytes < escat_experts_workspace_bytes(n, 1) || ((uintptr_t)workspace & 15))
-        return fail(ESCAT_EWORKSPACE, "escat_experts_bwd: workspace of %zu bytes (16-byte aligned), needs %zu", workspace_bytes, escat_experts_workspace_bytes(n, 1));
+    if (hidden && ((uintptr_t)hidden & 15)) return fail(ESCAT_EINVAL, "escat_experts: hidden is not aligned to 16 bytes");
+    if (!workspace || workspace_bytes < escat_experts_workspace_bytes(n, 1, hidden != nullptr) || ((uintptr_t)workspace & 15))
+        return fail(ESCAT_EWORKSPACE, "escat_experts_bwd: workspace of %zu bytes (16-byte aligned), needs %zu", workspace_bytes, escat_experts_workspace_bytes(n, 1, hidden != nullptr));
     const int64_t P = n->rows * n->k;
     char *ws = (char *)workspace;
-    void *h = ws; ws += hidden_bytes(n);
+    void *h = const_cast<void *>(hidden);
+    if (!h) { h = ws; ws += hidden_bytes(n); }
     void *du = ws; ws += hidden_bytes(n);
     float *part = (float *)ws; ws += part_bytes(n, n->d);
     void *by_mem = ws; ws += by_expert_bytes(n);
@@ -105,7 +113,7 @@ extern "C" int escat_experts_bwd(const escat_experts_dims *n, const void *x, con
     float *chunks = (float *)ws;
     const EDims d = dims_of(n);
     const EPlan p = plan_of(const_cast<void *>(plan), n->rows, n->k, n->experts);
-    if (n->rows > 0) { rc = escat_experts_rows_bwd(n->type, d, p, x, weights, w1, b1, w2, b2, dy, h, du, part, dwp, sw, dx, dweights, st); if (rc) return rc; }
+    if (n->rows > 0) { rc = escat_experts_rows_bwd(n->type, d, p, x, weights, w1, b1, w2, b2, dy, hidden ? nullptr : h, du, part, dwp, sw, dx, dweights, st); if (rc) return rc; }
     // the weights' gradients (without rows: zeros) sum by expert
     EPlan by = p;
     const int *at = nullptr;

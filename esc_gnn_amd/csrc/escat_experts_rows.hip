@@ -4,8 +4,8 @@
 //   G = W2_e^T dy_t    dw_tj = h.G + b2.dy_t    du = w G silu'(u)    dx_t = sum_j W1_e^T du
 //
 // Rows are taken in the plan's order (sorted by expert), 128 to a tile.  The weight w goes into the hidden row before it is
-// rounded to the operands' type (w h): it then serves W2's product and W2's gradient without another pass.  Nothing of the
-// forward is kept for the backward: u is computed again next to G, in fp32, so that dw and silu' see no rounding of u, and the
+// rounded to the operands' type (w h): it then serves W2's product and W2's gradient without another pass.  The forward's (w h)
+// may be kept for the weights' gradient; u is computed again next to G, in fp32, so that dw and silu' see no rounding of u, and the
 // forward writes no u.  Results of the pairs are joined in fp32 by a pass of their own, in the order of the slots: no atomics.
 #include <type_traits>
 #include "escat_experts_tile.h"
@@ -238,14 +238,16 @@ __global__ void __launch_bounds__(XT, ((ahead_of<T, MODE>()) == 0 ? 3 : 2)) k_ex
     }
     const int *row = a.p.row;
     auto by_pos = [&](int r) { return (int64_t)(r0 + r) * per + dig; };
-    if (ONE) Spill<OUT>::all(lds, acc, am, bn, (OUT *)a.h + m0, M, rows, cols, by_pos);
+    if (MODE == BWD1 && DIRECT) { }                                 // the hidden rows are there already
+    else if (ONE) Spill<OUT>::all(lds, acc, am, bn, (OUT *)a.h + m0, M, rows, cols, by_pos);
     else if (DIRECT) Spill<OUT>::all(lds, acc, am, bn, (OUT *)a.out + m0, M, rows, cols, [&](int r) { return row[(int64_t)(r0 + r) * per]; });
     else Spill<OUT>::all(lds, acc, am, bn, (OUT *)a.part + m0, M, rows, cols, [&](int r) { return r0 + r; });
     if (MODE == BWD1) {
         const int r = threadIdx.x;
         const int64_t P = a.n.rows * a.n.k;
+        if (DIRECT) __syncthreads();
         if (r < rows) a.dwp[(int64_t)(m0 / XN) * P + by_pos(r)] = red[r] + red[128 + r] + (m0 == 0 && a.b2 ? red[256 + r] : 0.f);
-        __syncthreads();
+        if (!DIRECT) __syncthreads();
         Spill<OUT>::all(lds, acc2, am, bn, (OUT *)a.du + m0, M, rows, cols, by_pos);
     }
 }
@@ -330,7 +332,7 @@ template <typename T> static int fwd(RowArgs &a, void *y, hipStream_t st)
 }
 template <typename T> static int bwd(RowArgs &a, void *dx, float *dw, hipStream_t st)
 {
-    int rc = rows_launch<T, BWD1, false>(a, a.n.h, st); if (rc) return rc;
+    int rc = a.h ? rows_launch<T, BWD1, false>(a, a.n.h, st) : rows_launch<T, BWD1, true>(a, a.n.h, st); if (rc) return rc;
     const int64_t P = a.n.rows * a.n.k;
     if (dw) { k_join_dw<<<grid_for(P), XT, 0, st>>>(a.dwp, a.p.pos, P, (a.n.h + XN - 1) / XN, dw); CHECK_LAUNCH("experts: dw"); }
     return dx ? second<T, BWD2>(a, a.n.d, dx, st) : ESCAT_OK;

@@ -381,7 +381,7 @@ template <typename OUT> struct Spill {
                 struct alignas(16) { OUT v[PER]; } q;
                 __builtin_memcpy(&q, __builtin_assume_aligned(lds + r * STRIDE + c * (int)sizeof(OUT), 16), 16);
                 OUT *o = out + (int64_t)at(r + half * 64) * ld + c;
-                if (c + PER <= cols) { Pack<OUT, PER> p; __builtin_memcpy(&p, &q, 16); *(Pack<OUT, PER> *)o = p; }
+                if (c + PER <= cols) { typedef unsigned ua __attribute__((ext_vector_type(4), aligned(2))); ua p; __builtin_memcpy(&p, &q, 16); __builtin_nontemporal_store(p, (ua *)o); }
                 else {
 #pragma unroll
                     for (int z = 0; z < PER; ++z) if (c + z < cols) o[z] = q.v[z];

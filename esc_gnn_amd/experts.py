@@ -140,36 +140,40 @@ def _sizes(*dims):
     lib = _lib.load()
     d = _lib.EscatExpertsDims(*dims)
     at = ctypes.addressof(d)
-    return d, at, bool(lib.escat_experts_fwd_needs_plan(at)), lib.escat_experts_workspace_bytes(at, 0)
+    return d, at, bool(lib.escat_experts_fwd_needs_plan(at)), lib.escat_experts_workspace_bytes(at, 0, 0)
 
 
-def _mlp_forward(x, weights, experts, w1, b1, w2, b2):
-    """y, and the plan where the forward made one (few rows do without)"""
+def _mlp_forward(x, weights, experts, w1, b1, w2, b2, keep=False):
+    """y; the plan and (keep) the hidden rows where the forward made them (few rows do without)"""
     lib = _lib.load()
     (rows, d), k, (E, h, _), o = x.shape, experts.shape[1], w1.shape, w2.shape[1]
     dims, at, sorts, size = _sizes(rows, DTYPE_CODES[x.dtype], d, h, o, E, k)
-    y = x.new_empty((rows, o))
+    y, hidden = x.new_empty((rows, o)), None
     with _on(x.device) as stream:
         plan = _plan(experts, rows, k, E, None, stream) if sorts else None
+        if keep and sorts:
+            hidden = torch.empty(lib.escat_experts_hidden_bytes(at), dtype=torch.uint8, device=x.device)
+            size = lib.escat_experts_workspace_bytes(at, 0, 1)
         ws = torch.empty(size, dtype=torch.uint8, device=x.device)
         rc = lib.escat_experts_fwd(at, x.data_ptr(), weights.data_ptr(), experts.data_ptr(), w1.data_ptr(), _ptr(b1), w2.data_ptr(), _ptr(b2),
-                                   _ptr(plan), y.data_ptr(), ws.data_ptr(), size, stream)
+                                   _ptr(plan), y.data_ptr(), _ptr(hidden), ws.data_ptr(), size, stream)
     _lib.check(rc, "escat_experts_fwd")
-    return y, plan, dims
+    return y, plan, hidden, dims
 
 
 class _ExpertMLP(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weights, experts, w1, b1, w2, b2):
-        y, ctx.plan, ctx.dims = _mlp_forward(x, weights, experts, w1, b1, w2, b2)
-        ctx.save_for_backward(x, weights, experts, w1, b1, w2, b2)
+        wanted = ctx.needs_input_grad[5] or ctx.needs_input_grad[6]            # (the hidden rows serve w2's gradient)
+        y, plan, hidden, ctx.dims = _mlp_forward(x, weights, experts, w1, b1, w2, b2, keep=wanted)
+        ctx.save_for_backward(x, weights, experts, w1, b1, w2, b2, plan, hidden)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         lib = _lib.load()
-        x, weights, experts, w1, b1, w2, b2 = ctx.saved_tensors
+        x, weights, experts, w1, b1, w2, b2, plan, hidden = ctx.saved_tensors
         dims = ctx.dims
         at = ctypes.addressof(dims)
         dy = dy.contiguous()
@@ -178,12 +182,13 @@ class _ExpertMLP(torch.autograd.Function):
         dx, dweights = new(x, need[0]), new(weights, need[1])
         db1, db2 = new(b1, need[4]), new(b2, need[6])
         dw1, dw2 = new(w1, need[3] or need[4]), new(w2, need[5] or need[6])
-        size = lib.escat_experts_workspace_bytes(at, 1)
+        size = lib.escat_experts_workspace_bytes(at, 1, int(hidden is not None))
         with _on(x.device) as stream:
-            plan = ctx.plan if ctx.plan is not None else _plan(experts, dims.rows, dims.k, dims.experts, None, stream)
+            if plan is None:
+                plan = _plan(experts, dims.rows, dims.k, dims.experts, None, stream)
             ws = torch.empty(size, dtype=torch.uint8, device=x.device)
             rc = lib.escat_experts_bwd(at, x.data_ptr(), weights.data_ptr(), w1.data_ptr(), _ptr(b1), w2.data_ptr(), _ptr(b2), plan.data_ptr(),
-                                       dy.data_ptr(), _ptr(dx), _ptr(dweights), _ptr(dw1), _ptr(db1), _ptr(dw2), _ptr(db2), ws.data_ptr(), size,
+                                       _ptr(hidden), dy.data_ptr(), _ptr(dx), _ptr(dweights), _ptr(dw1), _ptr(db1), _ptr(dw2), _ptr(db2), ws.data_ptr(), size,
                                        stream)
         _lib.check(rc, "escat_experts_bwd")
         return dx, dweights, None, dw1 if need[3] else None, db1, dw2 if need[5] else None, db2
@@ -198,7 +203,8 @@ def expert_mlp(x: torch.Tensor, weights: torch.Tensor, experts: torch.Tensor, w1
     they are cast to its type); weights (rows, k) fp32, experts (rows, k) int32 as route_experts gives them.  A pair whose
     expert lies outside [0, E) counts for nothing and gets no gradient; the same expert may come twice in a row.  Sums are
     fp32; with 16-bit types the weighted hidden rows and their gradients are rounded to the type in between.  The backward
-    computes the hidden rows again: the forward keeps nothing but its arguments and the sorted pairs.  For a few rows the forward
+    computes the hidden rows again in fp32; with a gradient for w2 the forward keeps them in the operands' type (rows * k * h elements) next to its
+    arguments and the sorted pairs.  For a few rows the forward
     is a pair of matrix-vector kernels that read the weights in use once a pair, without sorting.  Weights must be
     contiguous; d, h, o are free (any alignment), k <= 64, E <= 1024, rows * k < 2^30.
     """

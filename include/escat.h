@@ -587,18 +587,21 @@ int escat_route_bwd(const void *logits, int type, int64_t rows, int E, int k, in
  * where escat_experts_fwd_needs_plan is 0 (few rows) the forward reads the array itself and plan may be NULL.
  * escat_experts_bwd: gradients for dy (rows, o); dx, dweights, dw1 + db1, dw2 + db2 may each be NULL (a bias's gradient only
  * together with its weight's); the others are written whole (experts without a row: zeros).  Workspaces: 16-byte aligned, contents
- * only used within the call.  No atomics: the same inputs give the same bits. */
+ * only used within the call.  hidden (escat_experts_hidden_bytes, 16-byte aligned): where a sorting forward leaves w silu(W1 x + b1) by position;
+ * the backward of the same inputs and plan that is given it does not write those rows again.  NULL for either: kept in the workspace, which is then
+ * larger (escat_experts_workspace_bytes with hidden = 0).  No atomics: the same inputs give the same bits. */
 typedef struct { int64_t rows; int32_t type, d, h, o, experts, k; } escat_experts_dims;
 size_t escat_experts_plan_bytes(int64_t rows, int k, int experts);
 int escat_experts_plan(const int32_t *experts_of_rows, int64_t rows, int k, int experts, void *plan, size_t plan_bytes, int32_t *counts,
                        void *stream);
-size_t escat_experts_workspace_bytes(const escat_experts_dims *dims, int backward);
+size_t escat_experts_hidden_bytes(const escat_experts_dims *dims);
+size_t escat_experts_workspace_bytes(const escat_experts_dims *dims, int backward, int hidden);
 int escat_experts_fwd_needs_plan(const escat_experts_dims *dims);
 int escat_experts_fwd(const escat_experts_dims *dims, const void *x, const float *weights, const int32_t *experts_of_rows, const void *w1,
-                      const void *b1, const void *w2, const void *b2, const void *plan, void *y, void *workspace, size_t workspace_bytes,
-                      void *stream);
+                      const void *b1, const void *w2, const void *b2, const void *plan, void *y, void *hidden, void *workspace,
+                      size_t workspace_bytes, void *stream);
 int escat_experts_bwd(const escat_experts_dims *dims, const void *x, const float *weights, const void *w1, const void *b1,
-                      const void *w2, const void *b2, const void *plan, const void *dy, void *dx, float *dweights, void *dw1, void *db1,
+                      const void *w2, const void *b2, const void *plan, const void *hidden, const void *dy, void *dx, float *dweights, void *dw1, void *db1,
                       void *dw2, void *db2, void *workspace, size_t workspace_bytes, void *stream);
 
 /* host utility (no GPU): Jenkins lookup3 "hashlittle", the checksum of HDF5 version-2 object headers

@@ -93,18 +93,18 @@ def test_experts_library_checks_its_arguments():
     dims = lambda *a: ctypes.addressof(keep.append(_lib.EscatExpertsDims(*a)) or keep[-1])       # noqa: E731
     keep = []
     good = (4, 0, 8, 8, 8, 2, 1)
-    assert lib.escat_experts_workspace_bytes(dims(*good), 1) > lib.escat_experts_workspace_bytes(dims(*good), 0) > 0
+    assert lib.escat_experts_workspace_bytes(dims(*good), 1, 0) > lib.escat_experts_workspace_bytes(dims(*good), 0, 0) > 0
     for at, value in ((0, -1), (1, 3), (2, 0), (3, 0), (4, 0), (5, 0), (6, 0)):
         bad = list(good); bad[at] = value
-        assert lib.escat_experts_workspace_bytes(dims(*bad), 0) == 0
-        assert lib.escat_experts_fwd(dims(*bad), *[0] * 10, 0, 0) == -1
-    assert lib.escat_experts_fwd(dims(1 << 30, 0, 8, 8, 8, 2, 1), *[0] * 10, 0, 0) == -2
-    assert lib.escat_experts_fwd(dims(4, 0, 8, 8, 8, 2000, 1), *[0] * 10, 0, 0) == -2
-    assert lib.escat_experts_fwd(dims(4, 1, 8, 4, 8, 2, 1), *[0] * 10, 0, 0) == -2                # bf16 rows of 8 bytes
-    assert lib.escat_experts_fwd(dims(*good), *[0] * 10, 0, 0) == -1                              # null pointers
-    assert lib.escat_experts_fwd(dims(*good), *[16] * 9, 16, 64, 0) == -3                        # small workspace
-    assert lib.escat_experts_fwd(dims(0, 0, 8, 8, 8, 2, 1), *[0] * 10, 0, 0) == 0                 # no rows
-    assert lib.escat_experts_bwd(dims(*good), *[16] * 8, 0, 0, 0, 16, 0, 0, 16, 1 << 20, 0) == -1          # db1 without dw1
+        assert lib.escat_experts_workspace_bytes(dims(*bad), 0, 0) == 0
+        assert lib.escat_experts_fwd(dims(*bad), *[0] * 11, 0, 0) == -1
+    assert lib.escat_experts_fwd(dims(1 << 30, 0, 8, 8, 8, 2, 1), *[0] * 11, 0, 0) == -2
+    assert lib.escat_experts_fwd(dims(4, 0, 8, 8, 8, 2000, 1), *[0] * 11, 0, 0) == -2
+    assert lib.escat_experts_fwd(dims(4, 1, 8, 4, 8, 2, 1), *[0] * 11, 0, 0) == -2                # bf16 rows of 8 bytes
+    assert lib.escat_experts_fwd(dims(*good), *[0] * 11, 0, 0) == -1                              # null pointers
+    assert lib.escat_experts_fwd(dims(*good), *[16] * 9, 0, 16, 64, 0) == -3                        # small workspace
+    assert lib.escat_experts_fwd(dims(0, 0, 8, 8, 8, 2, 1), *[0] * 11, 0, 0) == 0                 # no rows
+    assert lib.escat_experts_bwd(dims(*good), *[16] * 7, 0, 16, 0, 0, 0, 16, 0, 0, 16, 1 << 20, 0) == -1          # db1 without dw1
     assert lib.escat_experts_plan(0, 5, 1, 4, 16, 1 << 20, 0, 0) == -1
     assert lib.escat_experts_plan(16, 5, 1, 4, 16, 8, 0, 0) == -3
     assert lib.escat_experts_plan(16, 1 << 31, 1, 4, 16, 8, 0, 0) == -2
