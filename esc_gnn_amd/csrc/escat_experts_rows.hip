@@ -28,12 +28,13 @@ enum { FWD1, FWD2, BWD1, BWD2 };
 // 349 instead of 391 us for 137 GFLOP at K = 256, the same at K = 1024).  fp32 products are matrix-bound: two steps ahead.  BWD1 holds two
 // sets of accumulators: one step ahead, two workgroups.
 template <typename T, int MODE> constexpr int ahead_of() { return MODE == BWD1 ? 1 : sizeof(T) == 4 ? 2 : 0; }
+template <typename T, int MODE> constexpr int waves_of() { return ahead_of<T, MODE>() ? 2 : MODE == BWD2 ? 3 : 4; }
 
 // the hardware's exponential errs by |u| 2^-24: below what 16-bit operands leave, not below what fp32 ones do
 template <typename T> __device__ __forceinline__ float sigmoid_of(float u) { return __builtin_amdgcn_rcpf(1.f + (sizeof(T) == 4 ? expf(-u) : __expf(-u))); }
 
 template <typename T, int MODE, bool DIRECT>
-__global__ void __launch_bounds__(XT, ((ahead_of<T, MODE>()) == 0 ? 3 : 2)) k_expert_rows(const RowArgs a)
+__global__ void __launch_bounds__(XT, (waves_of<T, MODE>())) k_expert_rows(const RowArgs a)
 {
     constexpr int PER = Elem<T>::PER, KB = Elem<T>::KB;
     constexpr int AHEAD = ahead_of<T, MODE>();
@@ -86,16 +87,16 @@ __global__ void __launch_bounds__(XT, ((ahead_of<T, MODE>()) == 0 ? 3 : 2)) k_ex
         const int steps_d = (D + KB - 1) / KB;
         pipe.start(steps_d, A, B);
         fetch_rest();
-        pipe.run(steps_d, lds, am, bn, acc, A, B);
-        if constexpr (MODE == BWD1) {
-            // ---- W2^T dy into the second set, and b2 . dy on the way
+        if constexpr (MODE != BWD1) pipe.run(steps_d, lds, am, bn, acc, A, B);
+        else {
+            // ---- W2^T dy into the second set, and b2 . dy on the way (the first tile of features, for all)
             auto w2 = [&](int) { return (const char *)a.w2 + (int64_t)e * O * H * (int64_t)sizeof(T); };
-            OperandKM<T, decltype(w2)> A2(O, m0, M, w2);
             struct WithDot : OperandKCRows<T> {
                 const T *b2;
+                bool on;
                 float (&dot)[4];
                 u4 piece;
-                __device__ __forceinline__ WithDot(int K, const T *b2, float (&dot)[4]) : OperandKCRows<T>(K), b2(b2), dot(dot) {}
+                __device__ __forceinline__ WithDot(int K, const T *b2, bool on, float (&dot)[4]) : OperandKCRows<T>(K), b2(b2), on(on), dot(dot) {}
                 __device__ __forceinline__ void load(u4 (&r)[4], int set)
                 {
                     const int k0 = this->k0 + this->c, K = this->K;
@@ -104,12 +105,16 @@ __global__ void __launch_bounds__(XT, ((ahead_of<T, MODE>()) == 0 ? 3 : 2)) k_ex
                 }
                 __device__ __forceinline__ void fix(u4 (&r)[4], int set)
                 {
-                    u4 b[4] = {piece, piece, piece, piece};
-                    int k0 = this->fk0;
-                    fix_kc<T>(b, this->K, this->c, k0);
+                    if (on) {
+                        u4 b[4] = {piece, piece, piece, piece};
+                        int k0 = this->fk0;
+                        fix_kc<T>(b, this->K, this->c, k0);
+                        piece = b[0];
+                    }
                     OperandKCRows<T>::fix(r, set);
+                    if (!on) return;
                     float f[PER], g[PER];
-                    to_floats<T>(b[0], f);
+                    to_floats<T>(piece, f);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         to_floats<T>(r[i], g);
@@ -118,22 +123,16 @@ __global__ void __launch_bounds__(XT, ((ahead_of<T, MODE>()) == 0 ? 3 : 2)) k_ex
                     }
                 }
             };
-            clear(acc2);
+            OperandKM<T, decltype(w2)> A2(O, m0, M, w2);
+            const bool on = m0 == 0 && a.b2;
+            WithDot B2(O, on ? (const T *)a.b2 + (int64_t)e * O : dy[0], on, dot);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) B2.p[i] = dy[i];
             const int steps = (O + KB - 1) / KB;
             Pipe<AHEAD, T, true, false> pipe2;
-            if (m0 == 0 && a.b2) {
-                WithDot B2(O, (const T *)a.b2 + (int64_t)e * O, dot);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) B2.p[i] = dy[i];
-                pipe2.start(steps, A2, B2);
-                pipe2.run(steps, lds, am, bn, acc2, A2, B2);
-            } else {
-                OperandKCRows<T> B2(O);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) B2.p[i] = dy[i];
-                pipe2.start(steps, A2, B2);
-                pipe2.run(steps, lds, am, bn, acc2, A2, B2);
-            }
+            pipe.run(steps_d, lds, am, bn, acc, A, B, [&]() { pipe2.start(steps, A2, B2); });
+            clear(acc2);
+            pipe2.run(steps, lds, am, bn, acc2, A2, B2);
         }
     } else {
         // ---- W2 (w h) or W1^T du of the tile's experts, one after the other into the same accumulators
