@@ -11,9 +11,12 @@
 //   by combination  items = rows, key = the sorted k experts of a row as digits to the base E + 1 (E: routed nowhere), per = k: the k products
 //                   of a tile's rows end in the same accumulators, and results are written once, in their own type.
 //
-// By combination moves less memory (524288 rows x 256, k = 2: no 2.1 GB of fp32 results written and read again, 0.5 ms of 3.5) but
-// cuts the rows into E^k / k! groups and pads each to whole tiles: taken with 512 rows or more to a group (4 tiles: 12 % padding; at 128
-// the padding costs what it saves) and at most 1024 keys; k = 1 is always its case, the two are the same there.
+// By combination moves less memory (no fp32 results of pairs written and read again) but cuts the rows into C(E + k - 1, k) groups, pads each
+// to whole tiles, and a tile walks k experts one after the other: taken with 2048 rows or more to a group and at most 1024 keys.  Forward and
+// backward by combination / by pair, us, 256 wide, at 512, 1024, 2048, 4096 rows to a group:
+//   bf16, 8 experts, k = 2   197/180  257/279  377/443  617/774       fp32   565/522  896/837  1425/1453  2642/2725
+//   bf16, 4 experts, k = 3   199/144  244/225  335/380  530/645       fp32   440/353  709/632  1236/1203  2269/2291
+// k = 1 is always its case, the two are the same there.
 struct EDims { int64_t rows; int d, h, o, E, k; };
 static inline int combo_keys(int64_t rows, int E, int k)        // number of keys by combination, 0 = by pair
 {
@@ -22,7 +25,7 @@ static inline int combo_keys(int64_t rows, int E, int k)        // number of key
     if (k == 1) return (int)keys;
     if (keys > 1024) return 0;
     for (int j = 0; j < k; ++j) groups = groups * (E + j) / (j + 1);         // multisets of k experts
-    return rows >= 512 * groups ? (int)keys : 0;
+    return rows >= 2048 * groups ? (int)keys : 0;
 }
 
 // A position is item * per + digit; of the plan (device memory, int32):
@@ -71,11 +74,6 @@ __device__ __forceinline__ int key_digit(const EPlan &p, int key, int j)
     for (int i = p.per - 1; i > j; --i) key /= p.base;
     return key % p.base;
 }
-
-// bytes of weights that the pairs of a call may read, each for itself, in the form for few rows (escat_experts_few.hip)
-#ifndef ESCAT_FEW_BYTES
-#define ESCAT_FEW_BYTES (512ll << 20)
-#endif
 
 // workgroups of a launch go round the eight XCDs one by one, each with its own L2: give each XCD a run of neighbouring work items
 // (neighbours share the expert's weights and the rows).  A permutation of [0, n).

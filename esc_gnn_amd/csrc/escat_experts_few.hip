@@ -158,11 +158,18 @@ template <typename T> static int go(const FewArgs &a, hipStream_t st)
     return ESCAT_OK;
 }
 
-// when the bytes that every pair reads for itself are fewer than what sorting and 128-row tiles cost; at most 65535 pairs (grid.y)
+// Taken where its estimate is below that of sorting and tiles, both in us: here every pair reads its expert's weights for itself (mostly from the
+// caches, 10 TB/s) and sums its features; there the weights in use come from memory once, after a floor that the steps along a tile set.
+// Forward, this form / tiles, us, k = 2, at 32, 128, 512, 2048 pairs:
+//   bf16  64 wide, 8 experts 8/22  11/23  26/29  86/31      256, 8 11/27  26/28  83/33  306/37      1024, 16 28/51  83/53  308/59      2048, 64 98/151  333/272
+//   fp32  64 wide, 8 experts 7/31  10/33  21/38  66/41      256, 8 10/58  21/58  65/64  245/67      1024, 16 37/162  104/163  400/170  2048, 64 176/529  587/1028
 bool escat_experts_few(int type, const EDims &n)
 {
-    const int64_t P = n.rows * n.k, each = (int64_t)n.h * (n.d + n.o) * escat_type_bytes(type);
-    return P <= 4096 && P * each <= ESCAT_FEW_BYTES;
+    const double P = (double)n.rows * n.k, each = (double)n.h * (n.d + n.o) * escat_type_bytes(type);
+    if (P > 4096) return false;
+    const double here = 6 + P * (each * 1e-7 + (n.h + n.o) * 1.7e-4);
+    const double tiles = 17 + (n.d + n.h) * (type == ESCAT_F32 ? 0.07 : 0.014) + (P < n.E ? P : n.E) * each * 2.2e-7;
+    return here < tiles;
 }
 
 int escat_experts_few_fwd(int type, const EDims &n, const int *experts, const void *x, const float *weights, const void *w1, const void *b1, const void *w2,

@@ -203,13 +203,14 @@ __global__ void __launch_bounds__(XT) k_grad_join(const GradArgs g)
     }
 }
 
-// rows of a chunk: none cut where an expert's tiles alone fill the chip four times over, else about 1024 workgroups in all, none of
-// fewer than 512 rows
+// rows of a chunk: none cut where the experts' tiles alone are 1024 workgroups or more; else about 720 in all, which with a last chunk for each
+// expert are one round of three a CU (8 experts, 1048576 pairs, 256 x 256 in bf16: 274 and 257 us for the two gradients, 1024: 294 and 284,
+// 1440: 272 and 261 but 8 us more to join), none of fewer than 512 rows
 int escat_experts_grad_chunk(int64_t P, int E, int M, int N)
 {
     const int64_t tiles = (int64_t)((M + XN - 1) / XN) * ((N + XN - 1) / XN);
     if (tiles * E >= 1024 || P <= 512) return 0;
-    const int64_t want = (1024 + tiles - 1) / tiles;
+    const int64_t want = (720 + tiles - 1) / tiles;
     int64_t r = (P + want - 1) / want;
     r = (r + 63) / 64 * 64;
     return (int)(r < 512 ? 512 : r);

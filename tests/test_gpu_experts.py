@@ -105,14 +105,19 @@ SHAPES = [  # rows, d, h, o, E, k
     (700, 1024, 40, 24, 6, 2),
     (5000, 40, 72, 48, 3, 2),
     (64, 8, 520, 16, 300, 6),
+    # few rows: the form without sorting
+    (60, 242, 256, 250, 8, 2),
+    (20, 1024, 40, 24, 6, 2),
+    (33, 17, 300, 40, 64, 4),
+    (100, 130, 66, 258, 2, 2),
     # more pairs than the form for few rows takes, by pair and with k = 1
     (3000, 33, 65, 31, 64, 2),
     (5000, 130, 129, 70, 40, 3),
     (6000, 50, 40, 60, 5, 1),
     # enough rows for tiles by combination of experts (escat_experts.h): k = 2, 3; ragged sizes
-    (2000, 40, 72, 136, 2, 2),
-    (9000, 33, 47, 70, 3, 3),
-    (6000, 242, 66, 130, 4, 2),
+    (7000, 40, 72, 136, 2, 2),
+    (21000, 33, 47, 70, 3, 3),
+    (21000, 242, 66, 130, 4, 2),
 ]
 
 
@@ -210,7 +215,7 @@ def test_counts_and_the_same_bits_again():
         e = torch.randint(-1, E + 1, (P,), generator=torch.Generator().manual_seed(P), dtype=torch.int32).to(DEV)
         want = torch.bincount(e[(e >= 0) & (e < E)].long(), minlength=E)
         assert torch.equal(expert_counts(e, E).long(), want)
-    t = make(20000, 64, 64, 64, 5, 2, torch.bfloat16, True, seed=6)
+    t = make(32000, 64, 64, 64, 5, 2, torch.bfloat16, True, seed=6)
     outs = []
     st = torch.cuda.Stream()
     for i in range(3):
