@@ -5,7 +5,7 @@ __attribute__((visibility("hidden"))) int escat_experts_rows_fwd(int type, const
                            const void *w2, const void *b2, void *h, float *part, void *y, hipStream_t st);
 __attribute__((visibility("hidden"))) int escat_experts_rows_bwd(int type, const EDims &n, const EPlan &p, const void *x, const float *weights, const void *w1, const void *b1,
                            const void *w2, const void *b2, const void *dy, void *h, void *du, float *part, float *dwp, float *ws, void *dx, float *dw, hipStream_t st);
-__attribute__((visibility("hidden"))) int escat_experts_grad_chunk(int64_t P, int E, int M, int N);
+__attribute__((visibility("hidden"))) int escat_experts_grad_chunk(int type, int64_t P, int E, int M, int N);
 __attribute__((visibility("hidden"))) int64_t escat_experts_grad_chunks(int64_t P, int E, int chunk);
 __attribute__((visibility("hidden"))) int escat_experts_plan_by_expert(const EPlan &p, int64_t P, int E, const EPlan &by, hipStream_t st);
 __attribute__((visibility("hidden"))) int escat_experts_grad(int type, const EDims &n, const EPlan &p, const int *at, bool w2, const void *a, const void *b, const float *weights, int M, int N,
@@ -49,7 +49,7 @@ static size_t hidden_bytes(const escat_experts_dims *n) { return up((size_t)n->r
 static size_t chunk_bytes(const escat_experts_dims *n, int M, int N)
 {
     const int64_t P = n->rows * n->k;
-    const int c = escat_experts_grad_chunk(P, n->experts, M, N);
+    const int c = escat_experts_grad_chunk(n->type, P, n->experts, M, N);
     return c ? up((size_t)escat_experts_grad_chunks(P, n->experts, c) * ((size_t)M * N + N) * 4) : 0;
 }
 
@@ -123,7 +123,7 @@ extern "C" int escat_experts_bwd(const escat_experts_dims *n, const void *x, con
         rc = escat_experts_plan_by_expert(p, P, n->experts, by, st); if (rc) return rc;
         at = by.pair;
     }
-    if (dw2) { rc = escat_experts_grad(n->type, d, by, at, true, h, dy, sw, n->h, n->o, escat_experts_grad_chunk(P, n->experts, n->h, n->o), chunks, dw2, db2, st); if (rc) return rc; }
-    if (dw1) { rc = escat_experts_grad(n->type, d, by, at, false, x, du, sw, n->d, n->h, escat_experts_grad_chunk(P, n->experts, n->d, n->h), chunks, dw1, db1, st); if (rc) return rc; }
+    if (dw2) { rc = escat_experts_grad(n->type, d, by, at, true, h, dy, sw, n->h, n->o, escat_experts_grad_chunk(n->type, P, n->experts, n->h, n->o), chunks, dw2, db2, st); if (rc) return rc; }
+    if (dw1) { rc = escat_experts_grad(n->type, d, by, at, false, x, du, sw, n->d, n->h, escat_experts_grad_chunk(n->type, P, n->experts, n->d, n->h), chunks, dw1, db1, st); if (rc) return rc; }
     return ESCAT_OK;
 }

@@ -8,8 +8,6 @@
 // gradients ride along: a tile's B pieces pass through registers anyway.
 #include "escat_experts_tile.h"
 
-#define GRAD_AHEAD(T) (sizeof(T) == 4 ? 2 : 0)
-
 struct GradArgs {
     EDims n;
     EPlan p;                   // by pair: items in the order of the sums
@@ -51,7 +49,7 @@ __device__ __forceinline__ int find_chunk(const int *count, int E, int chunk, in
 
 // W2: A by sorted position, B gathered by row and weighted for db; else A gathered by row, B by sorted position
 template <typename T, bool W2>
-__global__ void __launch_bounds__(XT, GRAD_AHEAD(T) == 0 ? 3 : 2) k_expert_grad(const GradArgs g)
+__global__ void __launch_bounds__(XT, 3) k_expert_grad(const GradArgs g)
 {
     constexpr int PER = Elem<T>::PER, KB = Elem<T>::KB;
     extern __shared__ __align__(16) char lds[];
@@ -90,7 +88,7 @@ __global__ void __launch_bounds__(XT, GRAD_AHEAD(T) == 0 ? 3 : 2) k_expert_grad(
     } it{g, ra, rb, 0};
     struct OpA {
         Items &it; const GradArgs &g; ColsKM<T> cols; int K, fk0;
-        __device__ __forceinline__ void load(u4 (&r)[4], int)
+        __device__ __forceinline__ void load(u4 (&r)[4])
         {
 #pragma unroll
             for (int i = 0; i < 4; ++i) { it.row[i] = it.row_next[i]; it.pos[i] = it.pos_next[i]; }
@@ -98,20 +96,20 @@ __global__ void __launch_bounds__(XT, GRAD_AHEAD(T) == 0 ? 3 : 2) k_expert_grad(
 #pragma unroll
             for (int i = 0; i < 4; ++i) r[i] = load16((const T *)g.a + (int64_t)(W2 ? it.pos[i] : it.row[i]) * g.M + cols.at);
         }
-        __device__ __forceinline__ void fix(u4 (&r)[4], int) { cols.fix(r, K - fk0, fk0 + KB <= K); fk0 += KB; }
+        __device__ __forceinline__ void fix(u4 (&r)[4]) { cols.fix(r, K - fk0, fk0 + KB <= K); fk0 += KB; }
     } A{it, g, ColsKM<T>(m0, M), K, 0};
     struct OpB {
         Items &it; const GradArgs &g; ColsKM<T> cols; int K, fk0; bool sums;
-        float w[2][4], db[PER];
-        __device__ __forceinline__ void load(u4 (&r)[4], int set)
+        float w[4], db[PER];
+        __device__ __forceinline__ void load(u4 (&r)[4])
         {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 r[i] = load16((const T *)g.b + (int64_t)(W2 ? it.row[i] : it.pos[i]) * g.N + cols.at);
-                if (W2) w[set][i] = g.weights[it.pos[i]];
+                if (W2) w[i] = g.weights[it.pos[i]];
             }
         }
-        __device__ __forceinline__ void fix(u4 (&r)[4], int set)
+        __device__ __forceinline__ void fix(u4 (&r)[4])
         {
             cols.fix(r, K - fk0, fk0 + KB <= K);
             fk0 += KB;
@@ -121,7 +119,7 @@ __global__ void __launch_bounds__(XT, GRAD_AHEAD(T) == 0 ? 3 : 2) k_expert_grad(
             for (int i = 0; i < 4; ++i) {
                 to_floats<T>(r[i], f);
 #pragma unroll
-                for (int z = 0; z < PER; ++z) db[z] = W2 ? fmaf(w[set][i], f[z], db[z]) : db[z] + f[z];
+                for (int z = 0; z < PER; ++z) db[z] = W2 ? fmaf(w[i], f[z], db[z]) : db[z] + f[z];
             }
         }
     } B{it, g, ColsKM<T>(n0, N), K, 0, sums};
@@ -131,7 +129,7 @@ __global__ void __launch_bounds__(XT, GRAD_AHEAD(T) == 0 ? 3 : 2) k_expert_grad(
     clear(acc);
     if (K > 0) it.fetch();
     const int steps = (K + KB - 1) / KB;
-    Pipe<GRAD_AHEAD(T), T, true, true> pipe;
+    Pipe<T, true, true> pipe;
     pipe.start(steps, A, B);
     pipe.run(steps, lds, am, bn, acc, A, B);
 
@@ -203,17 +201,18 @@ __global__ void __launch_bounds__(XT) k_grad_join(const GradArgs g)
     }
 }
 
-// rows of a chunk: none cut where the experts' tiles alone are 1024 workgroups or more; else about 720 in all, which with a last chunk for each
-// expert are one round of three a CU (8 experts, 1048576 pairs, 256 x 256 in bf16: 274 and 257 us for the two gradients, 1024: 294 and 284,
-// 1440: 272 and 261 but 8 us more to join), none of fewer than 512 rows
-int escat_experts_grad_chunk(int64_t P, int E, int M, int N)
+// rows of a chunk: none cut where the experts' tiles alone are 1024 workgroups or more; else, with a last chunk for each expert, about one round: 720 in
+// all, three a CU (8 experts, 1048576 pairs, 256 x 256 in bf16: 274 and 257 us for the two gradients, 1024: 294 and 284,
+// 1440: 272 and 261 but 8 us more to join); in fp32, which the matrix units bound, two a CU (32768 pairs, 256 x 242 and 256 x 256: 55 and 54 us, 720:
+// 65 and 65).  No chunk has fewer than 256 rows.
+int escat_experts_grad_chunk(int type, int64_t P, int E, int M, int N)
 {
     const int64_t tiles = (int64_t)((M + XN - 1) / XN) * ((N + XN - 1) / XN);
-    if (tiles * E >= 1024 || P <= 512) return 0;
-    const int64_t want = (720 + tiles - 1) / tiles;
+    if (tiles * E >= 1024 || P <= 256) return 0;
+    const int64_t want = ((type == ESCAT_F32 ? 480 : 720) + tiles - 1) / tiles;
     int64_t r = (P + want - 1) / want;
     r = (r + 63) / 64 * 64;
-    return (int)(r < 512 ? 512 : r);
+    return (int)(r < 256 ? 256 : r);
 }
 int64_t escat_experts_grad_chunks(int64_t P, int E, int chunk) { return chunk ? P / chunk + (E < P ? E : P) : E; }
 
@@ -223,7 +222,7 @@ template <typename T, bool W2> static int launch(const GradArgs &g, hipStream_t 
     const int64_t mt = (g.M + XN - 1) / XN, stripes = (tiles / mt * g.n.E + 7) / 8 * 8;
     const int64_t wgs = g.chunk ? tiles * escat_experts_grad_chunks(g.n.rows * g.n.k, g.n.E, g.chunk) : stripes * mt;
     if (wgs > 0xffffff) return fail(ESCAT_ERANGE, "experts: %lld tiles", (long long)wgs);
-    constexpr size_t lds = LDS_BYTES(GRAD_AHEAD(T));
+    constexpr size_t lds = LDS_BYTES;
     int rc = set_lds(k_expert_grad<T, W2>, lds); if (rc) return rc;
     k_expert_grad<T, W2><<<(unsigned)wgs, XT, lds, st>>>(g);
     CHECK_LAUNCH("experts: weight gradient");

@@ -24,11 +24,9 @@ struct RowArgs {
 };
 
 enum { FWD1, FWD2, BWD1, BWD2 };
-// 16-bit products: one LDS buffer and three workgroups a CU, which hide each other's waits (measured against two steps ahead in two workgroups:
-// 349 instead of 391 us for 137 GFLOP at K = 256, the same at K = 1024).  fp32 products are matrix-bound: two steps ahead.  BWD1 holds two
-// sets of accumulators: one step ahead, two workgroups.
-template <typename T, int MODE> constexpr int ahead_of() { return MODE == BWD1 ? 1 : sizeof(T) == 4 ? 2 : 0; }
-template <typename T, int MODE> constexpr int waves_of() { return ahead_of<T, MODE>() ? 2 : MODE == BWD2 ? 3 : 4; }
+// waves on a SIMD (workgroups of a CU) that the registers leave room for: BWD1 holds two sets of accumulators.  Four instead of three for the forward's
+// 16-bit products, with 16 bytes a lane spilled: 283 instead of 305 us and 223 instead of 244 (524288 rows, k = 2, 256 x 256)
+template <typename T, int MODE> constexpr int waves_of() { return MODE == BWD1 ? 2 : MODE == BWD2 || sizeof(T) == 4 ? 3 : 4; }
 
 // the hardware's exponential errs by |u| 2^-24: below what 16-bit operands leave, not below what fp32 ones do
 template <typename T> __device__ __forceinline__ float sigmoid_of(float u) { return __builtin_amdgcn_rcpf(1.f + (sizeof(T) == 4 ? expf(-u) : __expf(-u))); }
@@ -37,7 +35,6 @@ template <typename T, int MODE, bool DIRECT>
 __global__ void __launch_bounds__(XT, (waves_of<T, MODE>())) k_expert_rows(const RowArgs a)
 {
     constexpr int PER = Elem<T>::PER, KB = Elem<T>::KB;
-    constexpr int AHEAD = ahead_of<T, MODE>();
     extern __shared__ __align__(16) char lds[];
     const int D = a.n.d, H = a.n.h, O = a.n.o;
     const int M = MODE == FWD2 ? O : MODE == BWD2 ? D : H;          // features of the result
@@ -83,7 +80,7 @@ __global__ void __launch_bounds__(XT, (waves_of<T, MODE>())) k_expert_rows(const
             B.p[i] = (const T *)a.x + row * D;
             if (MODE == BWD1) dy[i] = (const T *)a.dy + row * O;
         }
-        Pipe<AHEAD, T, false, false> pipe;
+        Pipe<T, false, false> pipe;
         const int steps_d = (D + KB - 1) / KB;
         pipe.start(steps_d, A, B);
         fetch_rest();
@@ -97,13 +94,13 @@ __global__ void __launch_bounds__(XT, (waves_of<T, MODE>())) k_expert_rows(const
                 float (&dot)[4];
                 u4 piece;
                 __device__ __forceinline__ WithDot(int K, const T *b2, bool on, float (&dot)[4]) : OperandKCRows<T>(K), b2(b2), on(on), dot(dot) {}
-                __device__ __forceinline__ void load(u4 (&r)[4], int set)
+                __device__ __forceinline__ void load(u4 (&r)[4])
                 {
                     const int k0 = this->k0 + this->c, K = this->K;
                     piece = load16(b2 + (k0 < K - PER ? k0 : K - PER));
-                    OperandKCRows<T>::load(r, set);
+                    OperandKCRows<T>::load(r);
                 }
-                __device__ __forceinline__ void fix(u4 (&r)[4], int set)
+                __device__ __forceinline__ void fix(u4 (&r)[4])
                 {
                     if (on) {
                         u4 b[4] = {piece, piece, piece, piece};
@@ -111,7 +108,7 @@ __global__ void __launch_bounds__(XT, (waves_of<T, MODE>())) k_expert_rows(const
                         fix_kc<T>(b, this->K, this->c, k0);
                         piece = b[0];
                     }
-                    OperandKCRows<T>::fix(r, set);
+                    OperandKCRows<T>::fix(r);
                     if (!on) return;
                     float f[PER], g[PER];
                     to_floats<T>(piece, f);
@@ -129,7 +126,7 @@ __global__ void __launch_bounds__(XT, (waves_of<T, MODE>())) k_expert_rows(const
 #pragma unroll
             for (int i = 0; i < 4; ++i) B2.p[i] = dy[i];
             const int steps = (O + KB - 1) / KB;
-            Pipe<AHEAD, T, true, false> pipe2;
+            Pipe<T, true, false> pipe2;
             pipe.run(steps_d, lds, am, bn, acc, A, B, [&]() { pipe2.start(steps, A2, B2); });
             clear(acc2);
             pipe2.run(steps, lds, am, bn, acc2, A2, B2);
@@ -154,12 +151,12 @@ __global__ void __launch_bounds__(XT, (waves_of<T, MODE>())) k_expert_rows(const
             OperandKC<T, decltype(weights)> A(H, weights);
 #pragma unroll
             for (int i = 0; i < 4; ++i) A.off[i] = (uint32_t)(m0 + SC::row(i) < M ? m0 + SC::row(i) : M - 1) * (uint32_t)H * (uint32_t)sizeof(T);
-            Pipe<AHEAD, T, false, false> pipe;
+            Pipe<T, false, false> pipe;
             pipe.start(steps, A, B);
             pipe.run(steps, lds, am, bn, acc, A, B);
         } else {
             OperandKM<T, decltype(weights)> A(H, m0, M, weights);
-            Pipe<AHEAD, T, true, false> pipe;
+            Pipe<T, true, false> pipe;
             pipe.start(steps, A, B);
             pipe.run(steps, lds, am, bn, acc, A, B);
         }
@@ -304,7 +301,7 @@ template <typename T, int MODE, bool DIRECT> static int rows_launch(const RowArg
     const int64_t items = a.p.base ? a.n.rows : a.n.rows * a.n.k;
     const int64_t wgs = plan_max_tiles(items, a.p.keys) * ((M + XN - 1) / XN) * (ONE ? a.p.per : 1);
     if (wgs > 0xffffff) return fail(ESCAT_ERANGE, "experts: %lld tiles", (long long)wgs);
-    constexpr size_t lds = LDS_BYTES((ahead_of<T, MODE>()));
+    constexpr size_t lds = LDS_BYTES;
     int rc = set_lds(k_expert_rows<T, MODE, DIRECT>, lds); if (rc) return rc;
     k_expert_rows<T, MODE, DIRECT><<<(unsigned)wgs, XT, lds, st>>>(a);
     CHECK_LAUNCH("experts: rows");

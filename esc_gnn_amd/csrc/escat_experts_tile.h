@@ -2,8 +2,7 @@
 //
 // C[m][n] += sum_k A[m][k] B[n][k], m = features (A side), n = rows of activations or features (B side).  256 threads, four
 // waves of 64 x 64 each (2 x 2 MFMA blocks of 32 x 32, fp32 accumulators).  One step covers KB values of k: 64 of 16 bits or 32 of
-// 32 bits, 128 bytes of a row.  Operands come from memory through registers into one of two LDS buffers while the other is
-// multiplied: one barrier a step.
+// 32 bits, 128 bytes of a row.  Operands come from memory through registers into LDS.
 //
 // An operand lies in memory with k contiguous ("KC": rows of activations, W1 / W2 in the forward) or with m contiguous ("KM": the
 // weights in the backward, both operands of a weight gradient).  In LDS:
@@ -153,97 +152,41 @@ __device__ __forceinline__ void tile_step(const char *la, const char *lb, int am
     }
 }
 
-// ---- the loop over the steps.  a / b: operands with load(regs, set) -- the thread's pieces of the next step, AHEAD = 1 or 2 steps ahead of
-// their use (a step's products take less time than memory does; 1 where two sets of accumulators leave no registers for 2) -- and
-// fix(regs, set) -- the same pieces once they have arrived (a use inside load would wait for them there); both are called once a step, in
-// order; set = step & 1, or 0.  start() issues the first loads, so that a kernel can do other things until run(); run calls `next` before
-// the last products, when no load is left to issue.  lds: 4 tiles (A0 B0 A1 B1), free to be written on return.
+// ---- the loop over the steps.  a / b: operands with load(regs) -- the thread's pieces of the next step -- and fix(regs) -- the same pieces once
+// they have arrived (a use inside load would wait for them there); both are called once a step, in order.  One buffer in LDS and one set of
+// registers, two barriers a step: the two to four workgroups of a CU hide each other's waits.  (Measured against loads one or two steps ahead into
+// a second buffer, which leaves room for two workgroups: 349 us instead of 391 for 137 GFLOP in bf16 at K = 256, the same at K = 1024; fp32
+// 4 GFLOP at K = 256 62 us instead of 68.)  start() issues the first loads, so that a kernel can do other things until run(); run calls `next`
+// before the last products, when no load is left to issue.  lds is free to be written on return.
 struct Nothing { __device__ void operator()() const {} };
-// AHEAD = 0: one buffer (A0 B0) and one set of registers, two barriers a step; three workgroups share a CU and hide each other's waits
-template <int AHEAD, typename T, bool AKM, bool BKM> struct Pipe {
-    u4 a0[4], b0[4], a1[4], b1[4];
-#define LOAD(S) { a.load(a##S, S); b.load(b##S, S); }
-#define STORE_TO(S, D) { a.fix(a##S, S); b.fix(b##S, S); Stage<T, AKM>::store(buf##D, a##S); Stage<T, BKM>::store(buf##D + TILE_BYTES, b##S); __syncthreads(); }
-#define STORE(S) STORE_TO(S, S)
-#define MULTIPLY(S) tile_step<T, AKM, BKM>(buf##S, buf##S + TILE_BYTES, am, bn, acc);
+template <typename T, bool AKM, bool BKM> struct Pipe {
+    u4 ra[4], rb[4];
     template <typename A, typename B> __device__ __forceinline__ void start(int steps, A &a, B &b)
     {
-        if (steps > 0) LOAD(0)
-        if (AHEAD == 2 && steps > 1) LOAD(1)
+        if (steps > 0) { a.load(ra); b.load(rb); }
+    }
+    template <typename A, typename B> __device__ __forceinline__ void store(char *lds, A &a, B &b)
+    {
+        a.fix(ra); b.fix(rb);
+        Stage<T, AKM>::store(lds, ra); Stage<T, BKM>::store(lds + TILE_BYTES, rb);
+        __syncthreads();
     }
     // no load under a condition inside the loop: it would make the compiler wait for all of them at every turn
     template <typename A, typename B, typename N = Nothing>
     __device__ __forceinline__ void run(int steps, char *lds, int am, int bn, acc_t (&acc)[2][2], A &a, B &b, N next = N())
     {
         if (steps == 0) { next(); return; }
-        char *buf0 = lds, *buf1 = lds + 2 * TILE_BYTES;
-        if constexpr (AHEAD == 0) {
-            for (int s = 1; s < steps; ++s) {
-                STORE(0)
-                LOAD(0)
-                MULTIPLY(0)
-                __syncthreads();
-            }
-            STORE(0)
-            next();
-            MULTIPLY(0)
-        } else if constexpr (AHEAD == 1) {
-            STORE(0)
-            int s = 0;
-            for (; s + 2 < steps; s += 2) {
-                LOAD(0)
-                MULTIPLY(0)
-                STORE_TO(0, 1)
-                LOAD(0)
-                MULTIPLY(1)
-                STORE(0)
-            }
-            if (s + 2 == steps) {
-                LOAD(0)
-                MULTIPLY(0)
-                STORE_TO(0, 1)
-                next();
-                MULTIPLY(1)
-            } else {
-                next();
-                MULTIPLY(0)
-            }
-        } else if (steps == 1) {
-            STORE(0)
-            next();
-            MULTIPLY(0)
-        } else {
-            STORE(0)
-            int s = 0;
-            for (; s + 3 < steps; s += 2) {
-                LOAD(0)
-                MULTIPLY(0)
-                STORE(1)
-                LOAD(1)
-                MULTIPLY(1)
-                STORE(0)
-            }
-            if (s + 3 == steps) {
-                LOAD(0)
-                MULTIPLY(0)
-                STORE(1)
-                MULTIPLY(1)
-                STORE(0)
-                next();
-                MULTIPLY(0)
-            } else {
-                MULTIPLY(0)
-                STORE(1)
-                next();
-                MULTIPLY(1)
-            }
+        for (int s = 1; s < steps; ++s) {
+            store(lds, a, b);
+            a.load(ra); b.load(rb);
+            tile_step<T, AKM, BKM>(lds, lds + TILE_BYTES, am, bn, acc);
+            __syncthreads();
         }
+        store(lds, a, b);
+        next();
+        tile_step<T, AKM, BKM>(lds, lds + TILE_BYTES, am, bn, acc);
         __syncthreads();
     }
-#undef LOAD
-#undef STORE
-#undef STORE_TO
-#undef MULTIPLY
 };
 
 template <typename T> __device__ __forceinline__ void fix_kc(u4 (&r)[4], int K, int c, int &k0);
@@ -256,7 +199,7 @@ template <typename T, typename SEG> struct OperandKC {
     const char *base;
     uint32_t off[4];
     __device__ __forceinline__ OperandKC(int K, SEG seg) : seg(seg), K(K), c(Stage<T, false>::chunk() * Elem<T>::PER), k0(0), j(0), fk0(0), base(seg(0)) {}
-    __device__ __forceinline__ void load(u4 (&r)[4], int)
+    __device__ __forceinline__ void load(u4 (&r)[4])
     {
         constexpr int PER = Elem<T>::PER;
         const uint32_t at = (uint32_t)(k0 + c < K - PER ? k0 + c : K - PER) * (uint32_t)sizeof(T);
@@ -265,7 +208,7 @@ template <typename T, typename SEG> struct OperandKC {
         k0 += Elem<T>::KB;
         if (k0 >= K) { k0 = 0; base = seg(++j); }
     }
-    __device__ __forceinline__ void fix(u4 (&r)[4], int) { fix_kc<T>(r, K, c, fk0); }
+    __device__ __forceinline__ void fix(u4 (&r)[4]) { fix_kc<T>(r, K, c, fk0); }
 };
 template <typename T> __device__ __forceinline__ void fix_kc(u4 (&r)[4], int K, int c, int &k0)
 {
@@ -283,7 +226,7 @@ template <typename T> struct OperandKCRows {
     const T *p[4];
     int K, c, k0, fk0;
     __device__ __forceinline__ explicit OperandKCRows(int K) : K(K), c(Stage<T, false>::chunk() * Elem<T>::PER), k0(0), fk0(0) {}
-    __device__ __forceinline__ void load(u4 (&r)[4], int)
+    __device__ __forceinline__ void load(u4 (&r)[4])
     {
         constexpr int PER = Elem<T>::PER;
         const int at = k0 + c < K - PER ? k0 + c : K - PER;
@@ -291,7 +234,7 @@ template <typename T> struct OperandKCRows {
         for (int i = 0; i < 4; ++i) r[i] = load16(p[i] + at);
         k0 += Elem<T>::KB;
     }
-    __device__ __forceinline__ void fix(u4 (&r)[4], int) { fix_kc<T>(r, K, c, fk0); }
+    __device__ __forceinline__ void fix(u4 (&r)[4]) { fix_kc<T>(r, K, c, fk0); }
 };
 // where the thread's pieces of a row of M features begin (KM), and how far they are to be moved
 template <typename T> struct ColsKM {
@@ -330,7 +273,7 @@ template <typename T, typename SEG> struct OperandKM {
         off = (uint32_t)Stage<T, true>::row(0) * row + (uint32_t)cols.at * (uint32_t)sizeof(T);
         last = (uint32_t)(K - 1) * row + (uint32_t)cols.at * (uint32_t)sizeof(T);
     }
-    __device__ __forceinline__ void load(u4 (&r)[4], int)
+    __device__ __forceinline__ void load(u4 (&r)[4])
     {
         const uint32_t o = off + (uint32_t)k0 * row;
 #pragma unroll
@@ -341,7 +284,7 @@ template <typename T, typename SEG> struct OperandKM {
         k0 += Elem<T>::KB;
         if (k0 >= K) { k0 = 0; base = seg(++j); }
     }
-    __device__ __forceinline__ void fix(u4 (&r)[4], int)
+    __device__ __forceinline__ void fix(u4 (&r)[4])
     {
         cols.fix(r, K - fk0, fk0 + Elem<T>::KB <= K);
         fk0 += Elem<T>::KB;
@@ -351,7 +294,9 @@ template <typename T, typename SEG> struct OperandKM {
 
 // ---- results through LDS, so that memory is written in whole rows of the tile: rows [0, rows), features [0, cols) to out + at(row) * ld.
 // A row of 128 OUT is STRIDE bytes from the next: 16 more than its size, so that the runs of 32 rows fall on different banks.  32-bit
-// results go in two halves of 64 rows: 34 KB hold either.  lds is free before (the caller's barrier) and in use on return.
+// results go in two halves of 64 rows: 34 KB hold either.  lds is free before (the caller's barrier) and in use on return.  The stores do not
+// stay in the caches: another kernel reads what is written here, and 512 MB of it push out the weights and the rows that workgroups share
+// (524288 rows, k = 2, 256 x 256 in bf16: W1 x 297 instead of 344 us, with the gradient of u 786 instead of 890).
 template <typename OUT> struct Spill {
     static constexpr int STRIDE = 128 * (int)sizeof(OUT) + 16, ROWS = sizeof(OUT) == 4 ? 64 : 128, BYTES = ROWS * STRIDE;
     template <typename AT>
@@ -390,9 +335,8 @@ template <typename OUT> struct Spill {
         }
     }
 };
-// LDS of a kernel whose Pipe is AHEAD steps ahead
-#define LDS_BYTES(AHEAD) ((AHEAD) == 0 ? 34816 : 4 * TILE_BYTES)
-static_assert(Spill<float>::BYTES <= 34816 && Spill<bf16_t>::BYTES <= 34816 && 2 * TILE_BYTES <= 34816, "LDS_BYTES");
+#define LDS_BYTES 34816                           // of a kernel: two tiles, or results on their way out
+static_assert(Spill<float>::BYTES <= LDS_BYTES && Spill<bf16_t>::BYTES <= LDS_BYTES && 2 * TILE_BYTES <= LDS_BYTES, "LDS_BYTES");
 
 __device__ __forceinline__ void clear(acc_t (&acc)[2][2])
 {
