@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(XT, (waves_of<T, MODE>())) k_expert_rows(const
             B.p[i] = (const T *)a.x + row * D;
             if (MODE == BWD1) dy[i] = (const T *)a.dy + row * O;
         }
-        Pipe<T, false, false> pipe;
+        Pipe<T, false, false, MODE == BWD1> pipe;
         const int steps_d = (D + KB - 1) / KB;
         pipe.start(steps_d, A, B);
         fetch_rest();
@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(XT, (waves_of<T, MODE>())) k_expert_rows(const
 #pragma unroll
             for (int i = 0; i < 4; ++i) B2.p[i] = dy[i];
             const int steps = (O + KB - 1) / KB;
-            Pipe<T, true, false> pipe2;
+            Pipe<T, true, false, true> pipe2;
             pipe.run(steps_d, lds, am, bn, acc, A, B, [&]() { pipe2.start(steps, A2, B2); });
             clear(acc2);
             pipe2.run(steps, lds, am, bn, acc2, A2, B2);
