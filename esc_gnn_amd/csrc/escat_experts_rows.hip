@@ -7,6 +7,12 @@
 // rounded to the operands' type (w h): it then serves W2's product and W2's gradient without another pass.  The forward's (w h)
 // may be kept for the weights' gradient; u is computed again next to G, in fp32, so that dw and silu' see no rounding of u, and the
 // forward writes no u.  Results of the pairs are joined in fp32 by a pass of their own, in the order of the slots: no atomics.
+//
+// 524288 rows, k = 2 of 8 experts, 256 x 256 x 256 in bf16: 137 GFLOP a product, W1 x 273 us (0.8 GB), W2 h 230 us (0.8 GB), u, G and du 592 us
+// (two products, 1.1 GB), W1^T du 220 us (0.8 GB): neither the matrix units (a quarter of the cycles) nor memory bound; a workgroup's chain of
+// tile, row, pieces and epilogue is, four steps of 64 long.  64 experts of 256 rows, 1024 x 2048 x 1024: 69 GFLOP a product (86 with the tiles' last
+// rows) in 125 to 131 us, 38 % of the matrix cycles at 1.75 GHz.  Tiles of 256 x 128 in eight waves, tiles in an order that shares weights, and
+// s_setprio around the products each left these times as they are.
 #include <type_traits>
 #include "escat_experts_tile.h"
 
@@ -24,8 +30,8 @@ struct RowArgs {
 };
 
 enum { FWD1, FWD2, BWD1, BWD2 };
-// waves on a SIMD (workgroups of a CU) that the registers leave room for: BWD1 holds two sets of accumulators.  Four instead of three for the forward's
-// 16-bit products, with 16 bytes a lane spilled: 283 instead of 305 us and 223 instead of 244 (524288 rows, k = 2, 256 x 256)
+// Waves on a SIMD (workgroups of a CU) that the registers leave room for: BWD1 holds two sets of accumulators.  Four instead of three for the
+// forward's 16-bit products: 273 instead of 305 us and 230 instead of 244 (524288 rows, k = 2, 256 x 256).
 template <typename T, int MODE> constexpr int waves_of() { return MODE == BWD1 ? 2 : MODE == BWD2 || sizeof(T) == 4 ? 3 : 4; }
 
 // the hardware's exponential errs by |u| 2^-24: below what 16-bit operands leave, not below what fp32 ones do
@@ -50,18 +56,7 @@ __global__ void __launch_bounds__(XT, (waves_of<T, MODE>())) k_expert_rows(const
 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, am = (wave & 1) * 64, bn = (wave >> 1) * 64;
     typedef Stage<T, false> SC;
-    // rows behind the last of the tile repeat it: their results are not written
-    const int rl[2] = {bn + (lane & 31) < rows ? bn + (lane & 31) : 0, bn + 32 + (lane & 31) < rows ? bn + 32 + (lane & 31) : 0};
-    float wr[2];                                                    // weights of the two rows whose results the lane holds
-    __shared__ __align__(16) float bias[XN];
-    float bias_m = 0.f;
-    // what the epilogue needs, asked for once the first pieces of the operands are on their way
-    auto fetch_rest = [&]() {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) wr[j] = ONE ? a.weights[a.p.pair[(int64_t)(r0 + rl[j]) * per + dig]] : 0.f;
-        const int m = m0 + (int)(threadIdx.x % XN);
-        if (ONE && a.b1) bias_m = to_f32(((const T *)a.b1)[(int64_t)e * M + (m < M ? m : M - 1)]);
-    };
+    __shared__ __align__(16) float bias[XN], weight[XN];           // of the tile's features; of its rows
     acc_t acc[2][2], acc2[2][2];
     clear(acc);
     float dot[4] = {0.f, 0.f, 0.f, 0.f};                            // BWD1: the thread's share of b2 . dy of its rows
@@ -80,10 +75,14 @@ __global__ void __launch_bounds__(XT, (waves_of<T, MODE>())) k_expert_rows(const
             B.p[i] = (const T *)a.x + row * D;
             if (MODE == BWD1) dy[i] = (const T *)a.dy + row * O;
         }
+        const int me = threadIdx.x % XN;
+        const int pair = a.p.pair[(int64_t)(r0 + (me < rows ? me : 0)) * per + dig];
         Pipe<T, false, false, MODE == BWD1> pipe;
         const int steps_d = (D + KB - 1) / KB;
         pipe.start(steps_d, A, B);
-        fetch_rest();
+        // what the epilogue needs waits in LDS
+        const float w_me = a.weights[pair], b_me = a.b1 ? to_f32(((const T *)a.b1)[(int64_t)e * M + (m0 + me < M ? m0 + me : M - 1)]) : 0.f;
+        if (threadIdx.x < XN) { weight[me] = w_me; bias[me] = b_me; }
         if constexpr (MODE != BWD1) pipe.run(steps_d, lds, am, bn, acc, A, B);
         else {
             // ---- W2^T dy into the second set, and b2 . dy on the way (the first tile of features, for all)
@@ -171,7 +170,8 @@ __global__ void __launch_bounds__(XT, (waves_of<T, MODE>())) k_expert_rows(const
             __syncthreads();
 #pragma unroll
             for (int jj = 0; jj < 2; ++jj) {
-                const float w = a.weights[a.p.pair[(int64_t)(r0 + rl[jj]) * per + j]];
+                const int r = bn + 32 * jj + (lane & 31);
+                const float w = a.weights[a.p.pair[(int64_t)(r0 + (r < rows ? r : 0)) * per + j]];
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -186,10 +186,6 @@ __global__ void __launch_bounds__(XT, (waves_of<T, MODE>())) k_expert_rows(const
     // ---- epilogue.  The lane holds, for each of two rows, runs of four features; they leave through LDS
     typedef typename std::conditional<ONE || DIRECT, T, float>::type OUT;
     const int cols = M - m0 < XN ? M - m0 : XN;
-    if (ONE) {
-        if (threadIdx.x < XN) bias[threadIdx.x] = bias_m;
-        __syncthreads();
-    }
     __shared__ float red[3 * 128];                                  // BWD1: sums over the features of a half, b2 . dy
     if (MODE == BWD1) {
 #pragma unroll
@@ -202,7 +198,7 @@ __global__ void __launch_bounds__(XT, (waves_of<T, MODE>())) k_expert_rows(const
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         const int r = bn + 32 * j + (lane & 31);
-        const float w = wr[j];
+        const float w = ONE ? weight[r] : 0.f;
         float sum = 0.f;
 #pragma unroll
         for (int i = 0; i < 2; ++i)
