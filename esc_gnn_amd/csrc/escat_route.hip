@@ -13,6 +13,9 @@
 // exponential.  64-bit exponentials for every logit cost more than the memory traffic (E = 256: ~26 us of issue against 14 us), so
 // keys are computed in 32 bits with a bound on their error, and a wave in which two keys that decide something lie within that
 // bound repeats the selection with 64-bit keys (about one wave in 500 at E = 256, k = 8).
+//
+// 65537 rows of 256 bf16 logits, k = 8, bias and 4 of 8 groups: 74 us forward (34 MB read: 7 us; what bounds it is the instructions of the
+// selection, 1200 for the two rows of a wave), 17 us backward.  524288 rows of 8 fp32 logits, k = 2: 12 us forward (25 MB, 2.1 TB/s), 9 us backward.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include "escat_dev.h"
@@ -21,7 +24,8 @@
 #define RT 256
 #define R_INF __builtin_inff()
 // two 32-bit keys further apart than this (times max(1, size)) are in the order of their exact values: exp and the sum of up to
-// 1024 of them err by at most 1e-6 of s <= 1, a pair of them (group score) by 2e-6, the sum with the bias by 2^-24 of its size
+// 1024 of them err by at most 1e-6 of s <= 1, a pair of them (group score) by 2e-6, the sum with the bias by 2^-24 of its size; a place
+// in a lane takes the last 3 bits of a key (E > 512: 4), 1e-6 (1.9e-6) of its size
 #define R_GAP 7.62939453125e-6f
 
 struct RouteArgs {
@@ -103,6 +107,52 @@ template <int LPR, typename K> __device__ __forceinline__ K other_lane(K v, int 
     return (K)__shfl_xor(v, m, 64);
 }
 
+// largest first (a merge-exchange network: 19 exchanges of 8)
+template <int N> __device__ __forceinline__ void sort_down(int (&k)[N])
+{
+#pragma unroll
+    for (int p = 1; p < N; p *= 2)
+#pragma unroll
+        for (int q = p; q >= 1; q /= 2)
+#pragma unroll
+            for (int j = q % p; j + q < N; j += 2 * q)
+#pragma unroll
+                for (int i = 0; i < q; ++i)
+                    if (i + j + q < N && (i + j) / (2 * p) == (i + j + q) / (2 * p)) {
+                        const int a = k[i + j], b = k[i + j + q];
+                        k[i + j] = a > b ? a : b;
+                        k[i + j + q] = a > b ? b : a;
+                    }
+}
+
+// The rounds where close keys are decided again anyway and a row has 16 lanes or more: the place in the lane goes into the key's last bits (2^-20
+// of it: R_GAP leaves room), the lane's keys are sorted once, and a round looks at their heads alone.  Lane j keeps the j-th result.
+template <int LPR, int EPL>
+__device__ __forceinline__ bool pick_sorted(const RouteArgs &a, int (&key)[EPL], int lane_in_row, int l0, int *sel)
+{
+    constexpr int least = Least<int>::v;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) key[i] = key[i] > least ? (key[i] & -EPL) | (EPL - 1 - i) : least;
+    sort_down(key);
+    int my_key = least, my = -1, m = least;
+    for (int j = 0; j < a.k; ++j) {
+        m = row_reduce<LPR, OpMax>(key[0]);
+        const int at = first_lane<LPR>(key[0] == m, l0);
+        const int e = m > least ? at * EPL + (~m & (EPL - 1)) : -1;
+        if (lane_in_row == j) { my_key = m; my = e; }
+        const bool mine = lane_in_row == at;
+#pragma unroll
+        for (int i = 0; i < EPL; ++i) key[i] = mine ? (i + 1 < EPL ? key[i + 1] : least) : key[i];
+    }
+    if (lane_in_row < a.k) sel[lane_in_row] = my;
+    // each result against the one before it, and the first that was left against the last
+    const int before = __shfl_up(my_key, 1, 64), left = row_reduce<LPR, OpMax>(key[0]);
+    const bool pair = lane_in_row > 0 && lane_in_row < a.k && my_key > least;
+    bool close = pair && too_close(value_of(before), value_of(my_key));
+    close |= left > least && too_close(value_of(m), value_of(left));
+    return close;
+}
+
 template <int LPR, int EPL, typename K, typename V, bool CHECK>
 __device__ bool pick(const RouteArgs &a, K (&key)[EPL], const K (&gkey)[EPL], bool key_exact, int lane_in_row, int l0, V *buf, int *sel)
 {
@@ -176,6 +226,7 @@ __device__ bool pick(const RouteArgs &a, K (&key)[EPL], const K (&gkey)[EPL], bo
             }
         }
     }
+    if constexpr (CHECK && LPR >= 16) { if (!key_exact) return pick_sorted<LPR, EPL>(a, key, lane_in_row, l0, sel) || close; }
     // k rounds (one more to see how far behind the next one is); no round ends early: rows of a wave would part ways
     const bool check = CHECK && !key_exact;
     V last = inf;
