@@ -113,7 +113,7 @@ extern "C" int escat_experts_bwd(const escat_experts_dims *n, const void *x, con
     float *chunks = (float *)ws;
     const EDims d = dims_of(n);
     const EPlan p = plan_of(const_cast<void *>(plan), n->rows, n->k, n->experts);
-    if (n->rows > 0) { rc = escat_experts_rows_bwd(n->type, d, p, x, weights, w1, b1, w2, b2, dy, hidden ? nullptr : h, du, part, dwp, sw, dx, dweights, st); if (rc) return rc; }
+    if (n->rows > 0) { rc = escat_experts_rows_bwd(n->type, d, p, x, weights, w1, b1, w2, b2, dy, hidden || !dw2 ? nullptr : h, du, part, dwp, sw, dx, dweights, st); if (rc) return rc; }
     // the weights' gradients (without rows: zeros) sum by expert
     EPlan by = p;
     const int *at = nullptr;

@@ -21,7 +21,7 @@ struct RowArgs {
     EPlan p;
     const void *x, *w1, *b1, *w2, *b2, *dy;
     const float *weights;
-    void *h;                   // (P, H) by position: w silu(u)
+    void *h;                   // (P, H) by position: w silu(u); BWD1: NULL = kept by the forward, or not needed
     void *du;                  // (P, H) by position
     float *part;               // by pair: (P, O) or (P, D) fp32, what the joining pass reads
     void *out;                 // by combination: y or dx

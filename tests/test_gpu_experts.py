@@ -315,3 +315,70 @@ def test_rows_that_end_inside_a_piece_of_16_bytes(shape, dtype):
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
 def test_every_remainder_of_a_row(width, dtype):
     check(make(2600, width, width + 3, width + 6, 6, 2, dtype, True, seed=width), dtype)
+
+
+@pytest.mark.parametrize("shape", [(3000, 33, 65, 31, 64, 2), (5000, 40, 72, 48, 3, 1), (7000, 40, 72, 136, 2, 2)])
+def test_only_what_is_asked_for_of_many_rows(shape):
+    """each gradient alone, with and without the forward's hidden rows, equals the one among all"""
+    from esc_gnn_amd import expert_mlp
+    t = make(*shape, torch.bfloat16, True, seed=12)
+    a = {n: t[n].detach().requires_grad_() for n in NAMES}
+    full = dict(zip(NAMES, torch.autograd.grad(expert_mlp(a["x"], a["weights"], t["experts"], a["w1"], a["b1"], a["w2"], a["b2"]), [a[n] for n in NAMES], t["up"])))
+    for n in NAMES:
+        q = {m: t[m].detach().requires_grad_(m == n) for m in NAMES}
+        g, = torch.autograd.grad(expert_mlp(q["x"], q["weights"], t["experts"], q["w1"], q["b1"], q["w2"], q["b2"]), q[n], t["up"])
+        assert torch.equal(g, full[n]), n
+
+
+class Guarded:
+    """device memory of so many bytes between two runs of a pattern"""
+    def __init__(self, nbytes):
+        self.n = nbytes
+        self.all = torch.full((nbytes + 8192,), 0x5A, dtype=torch.uint8, device=DEV)
+
+    def ptr(self):
+        return self.all.data_ptr() + 4096
+
+    def view(self, dtype, shape):
+        return self.all[4096:4096 + self.n].view(dtype).view(shape)
+
+    def intact(self):
+        return bool((self.all[:4096] == 0x5A).all()) and bool((self.all[4096 + self.n:] == 0x5A).all())
+
+
+@pytest.mark.parametrize("shape", [(3, 17, 33, 9, 2, 2), (300, 242, 256, 250, 8, 2), (3000, 33, 65, 31, 64, 2), (5000, 41, 70, 45, 3, 1), (7000, 40, 77, 137, 2, 2),
+                                   (700, 1030, 43, 24, 6, 2)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("keep", [False, True])
+def test_nothing_is_written_outside(shape, dtype, keep):
+    """every buffer that the library writes lies between two patterns; a workspace is exactly as large as it says, full of NaN before"""
+    import ctypes
+    from esc_gnn_amd import _lib
+    lib = _lib.load()
+    rows, d, h, o, E, k = shape
+    t = make(*shape, dtype, True, seed=13)
+    size = t["x"].element_size()
+    dims = _lib.EscatExpertsDims(rows, 0 if dtype is torch.float32 else 1, d, h, o, E, k)
+    at = ctypes.addressof(dims)
+    p = {n: t[n].contiguous().data_ptr() for n in NAMES + ("up", "experts")}
+    plan = Guarded(lib.escat_experts_plan_bytes(rows, k, E))
+    _lib.check(lib.escat_experts_plan(p["experts"], rows, k, E, plan.ptr(), plan.n, 0, 0), "plan")
+    sorts = bool(lib.escat_experts_fwd_needs_plan(at))
+    hid = Guarded(lib.escat_experts_hidden_bytes(at)) if keep and sorts else None
+    hp = hid.ptr() if hid else 0
+    ws = [Guarded(lib.escat_experts_workspace_bytes(at, b, int(hid is not None))) for b in (0, 1)]
+    for w in ws + ([hid] if hid else []):
+        w.all[4096:4096 + w.n] = 0xFF
+    y = Guarded(rows * o * size)
+    _lib.check(lib.escat_experts_fwd(at, p["x"], p["weights"], p["experts"], p["w1"], p["b1"], p["w2"], p["b2"], plan.ptr(), y.ptr(), hp, ws[0].ptr(), ws[0].n, 0), "fwd")
+    g = {n: Guarded(t[n].numel() * t[n].element_size()) for n in NAMES}
+    _lib.check(lib.escat_experts_bwd(at, p["x"], p["weights"], p["w1"], p["b1"], p["w2"], p["b2"], plan.ptr(), hp, p["up"], g["x"].ptr(), g["weights"].ptr(), g["w1"].ptr(),
+                                     g["b1"].ptr(), g["w2"].ptr(), g["b2"].ptr(), ws[1].ptr(), ws[1].n, 0), "bwd")
+    torch.cuda.synchronize()
+    for n, b in dict(g, plan=plan, y=y, fwd=ws[0], bwd=ws[1], **({"hidden": hid} if hid else {})).items():
+        assert b.intact(), n
+    want = formula(t)
+    for n in NAMES + ("y",):
+        got = (y if n == "y" else g[n]).view(torch.float32 if n == "weights" else dtype, want[n].shape)
+        # (how near is the other tests' matter: here a wrong buffer would be nowhere near)
+        assert float((got.double() - want[n]).norm()) <= 0.02 * float(want[n].norm()) + 1e-30, n

@@ -1,4 +1,11 @@
-"""GPU tests of the training step with experts in the head and the multi-tensor AdamW (train_dp.DPTrainer's options)."""
+"""
+GPU tests of the training step with experts in the head and the multi-tensor AdamW (train_dp.DPTrainer's options).
+"""
+import os
+import socket
+import subprocess
+import sys
+import time
 import numpy as np
 import pytest
 import torch
@@ -7,10 +14,10 @@ pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
 
 
-def batch(B=48, n=64):
+def batch(B=48, n=64, seed=3):
     from esc_gnn_amd import synthetic
     from esc_gnn_amd.process_pyg_data import build_PQ_batch
-    clouds = synthetic.ellipsoid_clouds(B, n, seed=3)
+    clouds = synthetic.ellipsoid_clouds(B, n, seed=seed)
     pos = torch.from_numpy(clouds.reshape(-1, 3)).to(DEV)
     gp = torch.arange(B + 1, dtype=torch.int32, device=DEV) * n
     b = build_PQ_batch(pos, gp, 5, {"kernel": "gaussian", "gaussian_eps": 0.05})
@@ -85,3 +92,33 @@ def test_default_head_is_as_before():
     torch.manual_seed(0)
     h = ScatteringHead(7, 9)
     assert [tuple(p.shape) for p in h.parameters()] == [(16,), (16,), (256, 16), (256,), (256, 256), (256,), (1, 256), (1,)]
+
+
+@pytest.mark.parametrize("optimizer", ["escat", "escat8"])
+def test_two_ranks_keep_the_same_parameters(tmp_path, optimizer):
+    """two processes share the GPU over gloo, each with clouds of its own: parameters and the balance bias stay equal bit for bit"""
+    with socket.socket() as sk:
+        sk.bind(("127.0.0.1", 0))
+        port = sk.getsockname()[1]
+    here = os.path.dirname(os.path.abspath(__file__))
+    outs = [str(tmp_path / f"r{r}.pt") for r in range(2)]
+    logs = [open(str(tmp_path / f"r{r}.log"), "w+") for r in range(2)]
+    procs = [subprocess.Popen([sys.executable, os.path.join(here, "dp_experts_worker.py"), outs[r], optimizer], stdout=logs[r], stderr=subprocess.STDOUT,
+                              env=dict(os.environ, RANK=str(r), LOCAL_RANK=str(r), WORLD_SIZE="2", MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))) for r in range(2)]
+    try:
+        end = time.monotonic() + 90
+        while any(p.poll() is None for p in procs) and time.monotonic() < end and not any(p.poll() not in (None, 0) for p in procs):
+            time.sleep(0.1)
+    finally:
+        for p in procs:
+            if p.poll() is None:
+                p.kill()
+            p.wait(timeout=30)
+    for p, f in zip(procs, logs):
+        f.seek(0)
+        assert p.returncode == 0, f.read()[-3000:]
+    a, b = (torch.load(o, weights_only=True) for o in outs)
+    assert list(a) == list(b) and any("balance" in n for n in a)
+    for n in a:
+        if "running_" not in n:                                   # (BatchNorm's statistics are each rank's own, with experts or without)
+            assert torch.equal(a[n], b[n]), n
