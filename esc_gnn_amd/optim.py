@@ -220,6 +220,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
         ws = torch.empty(lib.escat_adamw_workspace_bytes(n), dtype=torch.uint8, device=dev)
         _begin(lib, [table], float(max_grad_norm or 0.0), [group], step, ws, norm, stream)
         _update(lib, table, group, 0, int(seed) & 0xFFFFFFFF, step, ws, stream)
+    torch._C._increment_version(params)                    # a backward that saved one of them shall say so, as after torch's own step
     return norm
 
 
@@ -324,6 +325,7 @@ class AdamW(torch.optim.Optimizer):
                     _begin(lib, list(tables.values()), max_norm, [g for _, g in part], step, ws, norm, stream)
                     for i, (gi, g) in enumerate(part):
                         _update(lib, tables[(key, gi)], g, i, seed, step, ws, stream)
+        torch._C._increment_version([p for items in calls.values() for p, _, _ in items])
         self.grad_norm = norm
         return loss
 

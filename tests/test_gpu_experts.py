@@ -114,6 +114,11 @@ SHAPES = [  # rows, d, h, o, E, k
     (3000, 33, 65, 31, 64, 2),
     (5000, 130, 129, 70, 40, 3),
     (6000, 50, 40, 60, 5, 1),
+    # many experts, many slots
+    (6000, 24, 16, 24, 1024, 2),
+    (6000, 24, 16, 24, 1024, 1),
+    (40, 24, 40, 16, 100, 40),
+    (900, 24, 40, 16, 7, 64),
     # enough rows for tiles by combination of experts (escat_experts.h): k = 2, 3; ragged sizes
     (7000, 40, 72, 136, 2, 2),
     (21000, 33, 47, 70, 3, 3),

@@ -122,3 +122,59 @@ def test_two_ranks_keep_the_same_parameters(tmp_path, optimizer):
     for n in a:
         if "running_" not in n:                                   # (BatchNorm's statistics are each rank's own, with experts or without)
             assert torch.equal(a[n], b[n]), n
+
+
+def test_a_captured_training_step_of_the_layer():
+    """routing, experts, gradients and the optimizer's step in one graph: replays on new rows, with eager work between, equal the eager steps"""
+    from esc_gnn_amd import adamw_step, expert_mlp, new_state8, route_experts
+    from esc_gnn_amd.train_dp import NodeExperts
+    torch.manual_seed(5)
+    layer = NodeExperts(40, 6, 2).to(DEV)
+    names = [n for n, _ in layer.named_parameters()]
+    rows = [torch.randn(900, 40, device=DEV) for _ in range(4)]
+    ups = [torch.randn(900, 40, device=DEV) for _ in range(4)]
+
+    def fresh():
+        ps = {n: p.detach().clone().requires_grad_() for n, p in layer.named_parameters()}
+        sizes = [p.numel() for p in ps.values()]
+        return ps, [new_state8(k, p.device) for k, p in zip(sizes, ps.values())], [new_state8(k, p.device) for k, p in zip(sizes, ps.values())], torch.zeros(1, dtype=torch.int32, device=DEV)
+
+    def step(state, x, up):
+        ps, m, v, count = state
+        w, e = route_experts(torch.nn.functional.linear(x, ps["router.weight"]), 2, bias=layer.balance)
+        y = x + expert_mlp(x, w, e, ps["w1"], ps["b1"], ps["w2"], ps["b2"])
+        grads = torch.autograd.grad(y, [ps[n] for n in names], up)
+        adamw_step([ps[n].detach() for n in names], list(grads), m, v, count, lr=1e-2, max_grad_norm=1.0)
+        return y.detach()
+    eager, caught, warm = fresh(), fresh(), fresh()
+    x, up = rows[0].clone(), ups[0].clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step(warm, x, up)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = step(caught, x, up)
+    for i in range(4):
+        x.copy_(rows[i]); up.copy_(ups[i])
+        graph.replay()
+        want = step(eager, rows[i], ups[i])                         # (eager work between the replays)
+        torch.cuda.synchronize()
+        assert torch.equal(y, want), i
+        for n in names:
+            assert torch.equal(caught[0][n], eager[0][n]), (i, n)
+    assert int(caught[3]) == 4
+
+
+def test_a_backward_behind_the_optimizers_step_is_refused():
+    """what a graph saved and the step has changed since: an error, as with torch's optimizers"""
+    from esc_gnn_amd import AdamW
+    p = torch.nn.Parameter(torch.randn(64, device=DEV))
+    opt = AdamW([p], lr=0.1)
+    (p * 2).sum().backward()
+    y = (p * p).sum()
+    opt.step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
