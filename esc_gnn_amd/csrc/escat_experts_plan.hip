@@ -88,56 +88,37 @@ __device__ __forceinline__ int wave_scan_incl(int v)
     return v;
 }
 
-// one workgroup of 1024: hist becomes each chunk's first position within its expert; counts, first positions, tiles
-__global__ void __launch_bounds__(1024) k_plan_scan(int E, int blocks, EPlan p)
+// counts of the keys -> first positions and tiles, by one workgroup
+struct KeyScan { int cnt[1025], first[1026], tfirst[1026]; };
+__device__ __forceinline__ void scan_keys(int E, KeyScan &k, const EPlan &p)
 {
-    __shared__ int cnt[1025], first[1026], tfirst[1026];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int e = wave; e < E; e += 16) {
-        int *h = p.hist + (int64_t)e * blocks;
-        int run = 0;
-        for (int b0 = 0; b0 < blocks; b0 += 64) {
-            const int v = b0 + lane < blocks ? h[b0 + lane] : 0;
-            const int inc = wave_scan_incl(v);
-            if (b0 + lane < blocks) h[b0 + lane] = run + inc - v;
-            run += __shfl(inc, 63, 64);
-        }
-        if (lane == 0) cnt[e] = run;
-    }
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
     __syncthreads();
     if (wave == 0) {
         int run = 0, trun = 0;
         for (int e0 = 0; e0 < E; e0 += 64) {
-            const int v = e0 + lane < E ? cnt[e0 + lane] : 0, t = (v + XM - 1) / XM;
+            const int v = e0 + lane < E ? k.cnt[e0 + lane] : 0, t = (v + XM - 1) / XM;
             const int inc = wave_scan_incl(v), tinc = wave_scan_incl(t);
-            if (e0 + lane < E) { first[e0 + lane] = run + inc - v; tfirst[e0 + lane] = trun + tinc - t; }
+            if (e0 + lane < E) { k.first[e0 + lane] = run + inc - v; k.tfirst[e0 + lane] = trun + tinc - t; }
             run += __shfl(inc, 63, 64); trun += __shfl(tinc, 63, 64);
         }
-        if (lane == 0) { first[E] = run; tfirst[E] = trun; *p.n_tiles = trun; }
+        if (lane == 0) { k.first[E] = run; k.tfirst[E] = trun; *p.n_tiles = trun; }
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < E; e += 1024) { p.count[e] = cnt[e]; p.first[e] = first[e]; }
-    if (threadIdx.x == 0) p.first[E] = first[E];
-    for (int e = wave; e < E; e += 16)
-        for (int t = tfirst[e] + lane; t < tfirst[e + 1]; t += 64) {
-            const int at = (t - tfirst[e]) * XM;
-            *(int4 *)(p.tile + 4 * t) = make_int4(e, first[e] + at, cnt[e] - at < XM ? cnt[e] - at : XM, 0);
+    for (int e = threadIdx.x; e < E; e += blockDim.x) { p.count[e] = k.cnt[e]; p.first[e] = k.first[e]; }
+    if (threadIdx.x == 0) p.first[E] = k.first[E];
+    for (int e = wave; e < E; e += waves)
+        for (int t = k.tfirst[e] + lane; t < k.tfirst[e + 1]; t += 64) {
+            const int at = (t - k.tfirst[e]) * XM;
+            *(int4 *)(p.tile + 4 * t) = make_int4(e, k.first[e] + at, k.cnt[e] - at < XM ? k.cnt[e] - at : XM, 0);
         }
 }
 
-__global__ void __launch_bounds__(PT) k_plan_place(const Items it, int bits, EPlan p)
+// the chunk's items to their places; cnt[wave][key]: the next position of each wave
+__device__ __forceinline__ void place_items(const Items &it, int64_t c0, int bits, int *cnt, const EPlan &p)
 {
     const int E = it.keys;
-    extern __shared__ int cnt[];
-    const int64_t c0 = (int64_t)blockIdx.x * PLAN_CHUNK;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    wave_counts(it, c0, bits, cnt);
-    for (int e = threadIdx.x; e < E; e += PT) {               // counts -> the next position of each wave
-        int s = p.first[e] + p.hist[(int64_t)e * gridDim.x + blockIdx.x];
-#pragma unroll
-        for (int w = 0; w < PW; ++w) { const int c = cnt[w * E + e]; cnt[w * E + e] = s; s += c; }
-    }
-    __syncthreads();
     for (int s = 0; s < PLAN_CHUNK / PT; ++s) {
         const int64_t i = c0 + wave * (PLAN_CHUNK / PW) + s * 64 + lane;
         const int e = key_of(it, i);
@@ -163,6 +144,63 @@ __global__ void __launch_bounds__(PT) k_plan_place(const Items it, int bits, EPl
     }
 }
 
+// one workgroup of 1024: hist becomes each chunk's first position within its expert; counts, first positions, tiles
+__global__ void __launch_bounds__(1024) k_plan_scan(int E, int blocks, EPlan p)
+{
+    __shared__ KeyScan k;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int e = wave; e < E; e += 16) {
+        int *h = p.hist + (int64_t)e * blocks;
+        int run = 0;
+        for (int b0 = 0; b0 < blocks; b0 += 64) {
+            const int v = b0 + lane < blocks ? h[b0 + lane] : 0;
+            const int inc = wave_scan_incl(v);
+            if (b0 + lane < blocks) h[b0 + lane] = run + inc - v;
+            run += __shfl(inc, 63, 64);
+        }
+        if (lane == 0) k.cnt[e] = run;
+    }
+    scan_keys(E, k, p);
+}
+
+__global__ void __launch_bounds__(PT) k_plan_place(const Items it, int bits, EPlan p)
+{
+    const int E = it.keys;
+    extern __shared__ int cnt[];
+    const int64_t c0 = (int64_t)blockIdx.x * PLAN_CHUNK;
+    wave_counts(it, c0, bits, cnt);
+    for (int e = threadIdx.x; e < E; e += PT) {               // counts -> the next position of each wave
+        int s = p.first[e] + p.hist[(int64_t)e * gridDim.x + blockIdx.x];
+#pragma unroll
+        for (int w = 0; w < PW; ++w) { const int c = cnt[w * E + e]; cnt[w * E + e] = s; s += c; }
+    }
+    __syncthreads();
+    place_items(it, c0, bits, cnt, p);
+}
+
+// all of it in one workgroup, for at most one chunk of items: one launch instead of three
+__global__ void __launch_bounds__(PT) k_plan_small(const Items it, int bits, EPlan p)
+{
+    const int E = it.keys;
+    extern __shared__ int cnt[];
+    __shared__ KeyScan k;
+    wave_counts(it, 0, bits, cnt);
+    for (int e = threadIdx.x; e < E; e += PT) {
+        int s = 0;
+#pragma unroll
+        for (int w = 0; w < PW; ++w) s += cnt[w * E + e];
+        k.cnt[e] = s;
+    }
+    scan_keys(E, k, p);
+    for (int e = threadIdx.x; e < E; e += PT) {
+        int s = k.first[e];
+#pragma unroll
+        for (int w = 0; w < PW; ++w) { const int c = cnt[w * E + e]; cnt[w * E + e] = s; s += c; }
+    }
+    __syncthreads();
+    place_items(it, 0, bits, cnt, p);
+}
+
 __global__ void __launch_bounds__(PT) k_copy_counts(const int *__restrict__ count, int E, int *__restrict__ out)
 {
     for (int e = threadIdx.x; e < E; e += PT) out[e] = count[e];
@@ -174,10 +212,13 @@ static int run_plan(const Items &it, const EPlan &p, hipStream_t st)
     const int blocks = (int)plan_blocks(it.n);
     int bits = 0; while ((1 << bits) < it.keys) ++bits;
     const size_t lds = (size_t)PW * it.keys * 4;
-    if (blocks) { k_plan_hist<<<blocks, PT, lds, st>>>(it, bits, p.hist); CHECK_LAUNCH("escat_experts_plan: histogram"); }
+    if (blocks <= 1) { k_plan_small<<<1, PT, lds, st>>>(it, bits, p); CHECK_LAUNCH("escat_experts_plan"); return ESCAT_OK; }
+    k_plan_hist<<<blocks, PT, lds, st>>>(it, bits, p.hist);
+    CHECK_LAUNCH("escat_experts_plan: histogram");
     k_plan_scan<<<1, 1024, 0, st>>>(it.keys, blocks, p);
     CHECK_LAUNCH("escat_experts_plan: scan");
-    if (blocks) { k_plan_place<<<blocks, PT, lds, st>>>(it, bits, p); CHECK_LAUNCH("escat_experts_plan: place"); }
+    k_plan_place<<<blocks, PT, lds, st>>>(it, bits, p);
+    CHECK_LAUNCH("escat_experts_plan: place");
     return ESCAT_OK;
 }
 
