@@ -161,14 +161,14 @@ template <typename T> static int go(const FewArgs &a, hipStream_t st)
 // Taken where its estimate is below that of sorting and tiles, both in us: here every pair reads its expert's weights for itself (mostly from the
 // caches, 10 TB/s) and sums its features; there the weights in use come from memory once, after a floor that the steps along a tile set.
 // Forward, this form / tiles, us, k = 2, at 32, 128, 512, 2048 pairs:
-//   bf16  64 wide, 8 experts 8/22  11/23  26/29  86/31      256, 8 11/27  26/28  83/33  306/37      1024, 16 28/51  83/53  308/59      2048, 64 98/151  333/272
-//   fp32  64 wide, 8 experts 7/31  10/33  21/38  66/41      256, 8 10/58  21/58  65/64  245/67      1024, 16 37/162  104/163  400/170  2048, 64 176/529  587/1028
+//   bf16  64 wide, 8 experts 7/18  10/19  26/23  86/25      256, 8 10/22  25/23  83/28  306/30      1024, 16 28/46  83/48  318/53      2048, 64 99/145  330/268
+//   fp32  64 wide, 8 experts 7/26  10/28  21/32  66/35      256, 8  9/53  21/54  65/58  245/61      1024, 16 37/158  104/160  399/165  2048, 64 177/524  586/1029
 bool escat_experts_few(int type, const EDims &n)
 {
     const double P = (double)n.rows * n.k, each = (double)n.h * (n.d + n.o) * escat_type_bytes(type);
     if (P > 4096) return false;
     const double here = 6 + P * (each * 1e-7 + (n.h + n.o) * 1.7e-4);
-    const double tiles = 17 + (n.d + n.h) * (type == ESCAT_F32 ? 0.07 : 0.014) + (P < n.E ? P : n.E) * each * 2.2e-7;
+    const double tiles = 11 + (n.d + n.h) * (type == ESCAT_F32 ? 0.07 : 0.014) + (P < n.E ? P : n.E) * each * 2.2e-7;
     return here < tiles;
 }
 
