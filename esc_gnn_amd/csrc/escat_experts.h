@@ -14,8 +14,8 @@
 // By combination moves less memory (no fp32 results of pairs written and read again) but cuts the rows into C(E + k - 1, k) groups, pads each
 // to whole tiles, and a tile walks k experts one after the other: taken with 2048 rows or more to a group and at most 1024 keys.  Forward and
 // backward by combination / by pair, us, 256 wide, at 512, 1024, 2048, 4096 rows to a group:
-//   bf16, 8 experts, k = 2   197/180  257/279  377/443  617/774       fp32   565/522  896/837  1425/1453  2642/2725
-//   bf16, 4 experts, k = 3   199/144  244/225  335/380  530/645       fp32   440/353  709/632  1236/1203  2269/2291
+//   bf16, 8 experts, k = 2   205/184  255/277  379/444  610/769       fp32   512/457  781/764  1415/1405  2573/2638
+//   bf16, 4 experts, k = 3   203/150  251/236  336/377  527/644       fp32   439/347  701/629  1177/1154  2208/2204
 // k = 1 is always its case, the two are the same there.
 struct EDims { int64_t rows; int d, h, o, E, k; };
 static inline int combo_keys(int64_t rows, int E, int k)        // number of keys by combination, 0 = by pair
