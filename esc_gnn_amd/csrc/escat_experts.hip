@@ -2,9 +2,9 @@
 #include "escat_experts.h"
 
 __attribute__((visibility("hidden"))) int escat_experts_rows_fwd(int type, const EDims &n, const EPlan &p, const void *x, const float *weights, const void *w1, const void *b1,
-                           const void *w2, const void *b2, void *h, float *part, void *y, hipStream_t st);
+                           const void *w2, const void *b2, void *h, float *u, float *part, void *y, hipStream_t st);
 __attribute__((visibility("hidden"))) int escat_experts_rows_bwd(int type, const EDims &n, const EPlan &p, const void *x, const float *weights, const void *w1, const void *b1,
-                           const void *w2, const void *b2, const void *dy, void *h, void *du, float *part, float *dwp, float *ws, void *dx, float *dw, hipStream_t st);
+                           const void *w2, const void *b2, const void *dy, void *h, void *du, float *u, float *part, float *dwp, float *ws, void *dx, float *dw, hipStream_t st);
 __attribute__((visibility("hidden"))) int escat_experts_grad_chunk(int type, int64_t P, int E, int M, int N);
 __attribute__((visibility("hidden"))) int64_t escat_experts_grad_chunks(int64_t P, int E, int chunk);
 __attribute__((visibility("hidden"))) int escat_experts_plan_by_expert(const EPlan &p, int64_t P, int E, const EPlan &by, hipStream_t st);
@@ -53,7 +53,7 @@ static size_t chunk_bytes(const escat_experts_dims *n, int M, int N)
     return c ? up((size_t)escat_experts_grad_chunks(P, n->experts, c) * ((size_t)M * N + N) * 4) : 0;
 }
 
-extern "C" size_t escat_experts_hidden_bytes(const escat_experts_dims *n) { return check_dims("escat_experts_hidden_bytes", n) ? 0 : hidden_bytes(n) + 256; }
+extern "C" size_t escat_experts_hidden_bytes(const escat_experts_dims *n) { return check_dims("escat_experts_hidden_bytes", n) ? 0 : hidden_bytes(n) * (keeps_u(n->type, n->d) ? 2 : 1) + 256; }
 
 extern "C" size_t escat_experts_workspace_bytes(const escat_experts_dims *n, int backward, int hidden)
 {
@@ -86,7 +86,7 @@ extern "C" int escat_experts_fwd(const escat_experts_dims *n, const void *x, con
     const EPlan p = plan_of(const_cast<void *>(plan), n->rows, n->k, n->experts);
     void *h = hidden;
     if (!h) { h = ws; ws += hidden_bytes(n); }
-    return escat_experts_rows_fwd(n->type, dims_of(n), p, x, weights, w1, b1, w2, b2, h, (float *)ws, y, (hipStream_t)stream);
+    return escat_experts_rows_fwd(n->type, dims_of(n), p, x, weights, w1, b1, w2, b2, h, hidden && keeps_u(n->type, n->d) ? (float *)((char *)hidden + hidden_bytes(n)) : nullptr, (float *)ws, y, (hipStream_t)stream);
 }
 
 extern "C" int escat_experts_bwd(const escat_experts_dims *n, const void *x, const float *weights, const void *w1, const void *b1, const void *w2,
@@ -113,7 +113,8 @@ extern "C" int escat_experts_bwd(const escat_experts_dims *n, const void *x, con
     float *chunks = (float *)ws;
     const EDims d = dims_of(n);
     const EPlan p = plan_of(const_cast<void *>(plan), n->rows, n->k, n->experts);
-    if (n->rows > 0) { rc = escat_experts_rows_bwd(n->type, d, p, x, weights, w1, b1, w2, b2, dy, hidden || !dw2 ? nullptr : h, du, part, dwp, sw, dx, dweights, st); if (rc) return rc; }
+    if (n->rows > 0) { rc = escat_experts_rows_bwd(n->type, d, p, x, weights, w1, b1, w2, b2, dy, hidden || !dw2 ? nullptr : h, du,
+                                                      hidden && keeps_u(n->type, n->d) ? (float *)((char *)const_cast<void *>(hidden) + hidden_bytes(n)) : nullptr, part, dwp, sw, dx, dweights, st); if (rc) return rc; }
     // the weights' gradients (without rows: zeros) sum by expert
     EPlan by = p;
     const int *at = nullptr;

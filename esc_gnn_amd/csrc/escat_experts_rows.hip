@@ -5,8 +5,8 @@
 //
 // Rows are taken in the plan's order (sorted by expert), 128 to a tile.  The weight w goes into the hidden row before it is
 // rounded to the operands' type (w h): it then serves W2's product and W2's gradient without another pass.  The forward's (w h)
-// may be kept for the weights' gradient; u is computed again next to G, in fp32, so that dw and silu' see no rounding of u, and the
-// forward writes no u.  Results of the pairs are joined in fp32 by a pass of their own, in the order of the slots: no atomics.
+// may be kept for the weights' gradient.  dw and silu' see no rounding of u: with 16-bit operands u is computed again next to G, with fp32 ones, whose
+// products cost more than reading it, the forward leaves it (keeps_u).  Results of the pairs are joined in fp32 by a pass of their own, in the order of the slots: no atomics.
 //
 // 524288 rows, k = 2 of 8 experts, 256 x 256 x 256 in bf16: 137 GFLOP a product, W1 x 273 us (0.8 GB), W2 h 230 us (0.8 GB), u, G and du 592 us
 // (two products, 1.1 GB), W1^T du 220 us (0.8 GB): neither the matrix units (a quarter of the cycles) nor memory bound; a workgroup's chain of
@@ -23,16 +23,19 @@ struct RowArgs {
     const float *weights;
     void *h;                   // (P, H) by position: w silu(u); BWD1: NULL = kept by the forward, or not needed
     void *du;                  // (P, H) by position
+    float *u;                  // (P, H) by position, fp32: FWD1 leaves it, BWD1U reads it
     float *part;               // by pair: (P, O) or (P, D) fp32, what the joining pass reads
     void *out;                 // by combination: y or dx
     float *dwp;                // (feature tiles of H, P) by position: parts of dw
     float *ws;                 // (P) by position: w (BWD1 leaves them for the weights' gradients)
 };
 
-enum { FWD1, FWD2, BWD1, BWD2 };
-// Waves on a SIMD (workgroups of a CU) that the registers leave room for: BWD1 holds two sets of accumulators.  Four instead of three for the
+enum { FWD1, FWD2, BWD1, BWD2, BWD1U };                            // BWD1U: BWD1 with u from memory
+// Waves on a SIMD (workgroups of a CU) that the registers leave room for: BWD1 holds two sets of accumulators, BWD1U
+// what it reads of u (with three it spills: 91 instead of 81 us).  Four instead of three for the
 // forward's 16-bit products: 273 instead of 305 us and 230 instead of 244 (524288 rows, k = 2, 256 x 256).
-template <typename T, int MODE> constexpr int waves_of() { return MODE == BWD1 ? 2 : MODE == BWD2 || sizeof(T) == 4 ? 3 : 4; }
+template <typename T, int MODE> constexpr int waves_of() { return MODE == BWD1 || MODE == BWD1U ? 2 : MODE == BWD2 || sizeof(T) == 4 ? 3 : 4; }
+// DIRECT: FWD2, BWD2: results by row; FWD1: leaves u; BWD1: writes no hidden rows
 
 // the hardware's exponential errs by |u| 2^-24: below what 16-bit operands leave, not below what fp32 ones do
 template <typename T> __device__ __forceinline__ float sigmoid_of(float u) { return __builtin_amdgcn_rcpf(1.f + (sizeof(T) == 4 ? expf(-u) : __expf(-u))); }
@@ -44,7 +47,8 @@ __global__ void __launch_bounds__(XT, (waves_of<T, MODE>())) k_expert_rows(const
     extern __shared__ __align__(16) char lds[];
     const int D = a.n.d, H = a.n.h, O = a.n.o;
     const int M = MODE == FWD2 ? O : MODE == BWD2 ? D : H;          // features of the result
-    constexpr bool ONE = MODE == FWD1 || MODE == BWD1;             // a tile's product with one of its experts, or with all
+    constexpr bool B1 = MODE == BWD1 || MODE == BWD1U;
+    constexpr bool ONE = MODE == FWD1 || B1;                       // a tile's product with one of its experts, or with all
     const int mt = (M + XN - 1) / XN, per = a.p.per, of = ONE ? per * mt : mt;
     const int live = *a.p.n_tiles * of;                              // (the grid covers the most tiles there can be)
     if ((int)blockIdx.x >= live) return;
@@ -73,17 +77,17 @@ __global__ void __launch_bounds__(XT, (waves_of<T, MODE>())) k_expert_rows(const
             const int64_t row = a.p.row[(int64_t)(r0 + r) * per + dig];
             A.off[i] = (uint32_t)m * (uint32_t)D * (uint32_t)sizeof(T);
             B.p[i] = (const T *)a.x + row * D;
-            if (MODE == BWD1) dy[i] = (const T *)a.dy + row * O;
+            if (B1) dy[i] = (const T *)a.dy + row * O;
         }
         const int me = threadIdx.x % XN;
         const int pair = a.p.pair[(int64_t)(r0 + (me < rows ? me : 0)) * per + dig];
         Pipe<T, false, false, MODE == BWD1> pipe;
         const int steps_d = (D + KB - 1) / KB;
-        pipe.start(steps_d, A, B);
+        if (MODE != BWD1U) pipe.start(steps_d, A, B);
         // what the epilogue needs waits in LDS
         const float w_me = a.weights[pair], b_me = a.b1 ? to_f32(((const T *)a.b1)[(int64_t)e * M + (m0 + me < M ? m0 + me : M - 1)]) : 0.f;
         if (threadIdx.x < XN) { weight[me] = w_me; bias[me] = b_me; }
-        if constexpr (MODE != BWD1) pipe.run(steps_d, lds, am, bn, acc, A, B);
+        if constexpr (!B1) pipe.run(steps_d, lds, am, bn, acc, A, B);
         else {
             // ---- W2^T dy into the second set, and b2 . dy on the way (the first tile of features, for all)
             auto w2 = [&](int) { return (const char *)a.w2 + (int64_t)e * O * H * (int64_t)sizeof(T); };
@@ -126,7 +130,8 @@ __global__ void __launch_bounds__(XT, (waves_of<T, MODE>())) k_expert_rows(const
             for (int i = 0; i < 4; ++i) B2.p[i] = dy[i];
             const int steps = (O + KB - 1) / KB;
             Pipe<T, true, false, true> pipe2;
-            pipe.run(steps_d, lds, am, bn, acc, A, B, [&]() { pipe2.start(steps, A2, B2); });
+            if constexpr (MODE == BWD1U) pipe2.start(steps, A2, B2);
+            else pipe.run(steps_d, lds, am, bn, acc, A, B, [&]() { pipe2.start(steps, A2, B2); });
             clear(acc2);
             pipe2.run(steps, lds, am, bn, acc2, A2, B2);
         }
@@ -187,7 +192,7 @@ __global__ void __launch_bounds__(XT, (waves_of<T, MODE>())) k_expert_rows(const
     typedef typename std::conditional<ONE || DIRECT, T, float>::type OUT;
     const int cols = M - m0 < XN ? M - m0 : XN;
     __shared__ float red[3 * 128];                                  // BWD1: sums over the features of a half, b2 . dy
-    if (MODE == BWD1) {
+    if (B1) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
 #pragma unroll
@@ -195,24 +200,48 @@ __global__ void __launch_bounds__(XT, (waves_of<T, MODE>())) k_expert_rows(const
             if (SC::chunk() == 0) red[256 + SC::row(i)] = dot[i];
         }
     }
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const int r = bn + 32 * j + (lane & 31);
-        const float w = ONE ? weight[r] : 0.f;
-        float sum = 0.f;
+    const int *row = a.p.row;
+    auto by_pos = [&](int r) { return (int64_t)(r0 + r) * per + dig; };
+    constexpr bool LEAVES_U = MODE == FWD1 && DIRECT;
+    if constexpr (LEAVES_U) {
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
+                const f4 bv = *(const f4 *)(bias + am + 32 * i + 8 * q + 4 * (lane >> 5));
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int z = 0; z < 4; ++z) acc[i][j][4 * q + z] += bv[z];
+            }
+        Spill<float>::all(lds, acc, am, bn, a.u + m0, M, rows, cols, by_pos);
+        __syncthreads();
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int r = bn + 32 * j + (lane & 31);
+        const float w = ONE ? weight[r] : 0.f;
+        const float *ur = MODE == BWD1U ? a.u + by_pos(r < rows ? r : rows - 1) * M + m0 : nullptr;
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
                 const int mt_ = am + 32 * i + 8 * q + 4 * (lane >> 5);
                 f4 bv = {0.f, 0.f, 0.f, 0.f};
-                if (ONE) bv = *(const f4 *)(bias + mt_);
+                if (ONE && MODE != BWD1U && !LEAVES_U) bv = *(const f4 *)(bias + mt_);
+                if constexpr (MODE == BWD1U) {
+                    if (mt_ + 4 <= cols) bv = __builtin_bit_cast(f4, load16(ur + mt_));
+                    else {
+#pragma unroll
+                        for (int z = 0; z < 4; ++z) if (mt_ + z < cols) bv[z] = ur[mt_ + z];
+                    }
+                }
 #pragma unroll
                 for (int z = 0; z < 4; ++z) {
-                    float v = acc[i][j][4 * q + z];
-                    if (ONE) v += bv[z];
+                    float v = MODE == BWD1U ? bv[z] : acc[i][j][4 * q + z] + bv[z];
                     if (MODE == FWD1) v = w * (v * sigmoid_of<T>(v));
-                    if (MODE == BWD1) {
+                    if (B1) {
                         const float g = acc2[i][j][4 * q + z];
                         const float sg = sigmoid_of<T>(v), hh = v * sg;
                         sum = fmaf(hh, g, sum);                     // (features behind the last: g = 0)
@@ -222,19 +251,18 @@ __global__ void __launch_bounds__(XT, (waves_of<T, MODE>())) k_expert_rows(const
                     acc[i][j][4 * q + z] = v;
                 }
             }
-        if (MODE == BWD1 && m0 == 0 && am == 0 && lane < 32 && r < rows) a.ws[(int64_t)(r0 + r) * per + dig] = w;
-        if (MODE == BWD1) {
+        }
+        if (B1 && m0 == 0 && am == 0 && lane < 32 && r < rows) a.ws[(int64_t)(r0 + r) * per + dig] = w;
+        if (B1) {
             sum += __shfl_xor(sum, 32, 64);
             if (lane < 32) red[(wave & 1) * 128 + r] = sum;
         }
     }
-    const int *row = a.p.row;
-    auto by_pos = [&](int r) { return (int64_t)(r0 + r) * per + dig; };
-    if (MODE == BWD1 && DIRECT) { }                                 // the hidden rows are there already
+    if (B1 && DIRECT) { }                                 // the hidden rows are there already
     else if (ONE) Spill<OUT>::all(lds, acc, am, bn, (OUT *)a.h + m0, M, rows, cols, by_pos);
     else if (DIRECT) Spill<OUT>::all(lds, acc, am, bn, (OUT *)a.out + m0, M, rows, cols, [&](int r) { return row[(int64_t)(r0 + r) * per]; });
     else Spill<OUT>::all(lds, acc, am, bn, (OUT *)a.part + m0, M, rows, cols, [&](int r) { return r0 + r; });
-    if (MODE == BWD1) {
+    if (B1) {
         const int r = threadIdx.x;
         const int64_t P = a.n.rows * a.n.k;
         if (DIRECT) __syncthreads();
@@ -293,7 +321,7 @@ __global__ void __launch_bounds__(XT) k_join_dw(const float *__restrict__ dwp, c
 // ------------------------------------------------------------------ launches (called by escat_experts.hip)
 template <typename T, int MODE, bool DIRECT> static int rows_launch(const RowArgs &a, int M, hipStream_t st)
 {
-    constexpr bool ONE = MODE == FWD1 || MODE == BWD1;
+    constexpr bool ONE = MODE == FWD1 || MODE == BWD1 || MODE == BWD1U;
     const int64_t items = a.p.base ? a.n.rows : a.n.rows * a.n.k;
     const int64_t wgs = plan_max_tiles(items, a.p.keys) * ((M + XN - 1) / XN) * (ONE ? a.p.per : 1);
     if (wgs > 0xffffff) return fail(ESCAT_ERANGE, "experts: %lld tiles", (long long)wgs);
@@ -319,26 +347,33 @@ template <typename T, int MODE> static int second(RowArgs &a, int M, void *out, 
 
 template <typename T> static int fwd(RowArgs &a, void *y, hipStream_t st)
 {
-    int rc = rows_launch<T, FWD1, false>(a, a.n.h, st); if (rc) return rc;
+    int rc;
+    if constexpr (sizeof(T) == 4) rc = a.u ? rows_launch<T, FWD1, true>(a, a.n.h, st) : rows_launch<T, FWD1, false>(a, a.n.h, st);
+    else rc = rows_launch<T, FWD1, false>(a, a.n.h, st);
+    if (rc) return rc;
     return second<T, FWD2>(a, a.n.o, y, st);
 }
 template <typename T> static int bwd(RowArgs &a, void *dx, float *dw, hipStream_t st)
 {
-    int rc = a.h ? rows_launch<T, BWD1, false>(a, a.n.h, st) : rows_launch<T, BWD1, true>(a, a.n.h, st); if (rc) return rc;
+    int rc = ESCAT_OK;
+    bool done = false;
+    if constexpr (sizeof(T) == 4) if (a.u) { rc = rows_launch<T, BWD1U, true>(a, a.n.h, st); done = true; }
+    if (!done) rc = a.h ? rows_launch<T, BWD1, false>(a, a.n.h, st) : rows_launch<T, BWD1, true>(a, a.n.h, st);
+    if (rc) return rc;
     const int64_t P = a.n.rows * a.n.k;
     if (dw) { k_join_dw<<<grid_for(P), XT, 0, st>>>(a.dwp, a.p.pos, P, (a.n.h + XN - 1) / XN, dw); CHECK_LAUNCH("experts: dw"); }
     return dx ? second<T, BWD2>(a, a.n.d, dx, st) : ESCAT_OK;
 }
 
 int escat_experts_rows_fwd(int type, const EDims &n, const EPlan &p, const void *x, const float *weights, const void *w1, const void *b1, const void *w2,
-                           const void *b2, void *h, float *part, void *y, hipStream_t st)
+                           const void *b2, void *h, float *u, float *part, void *y, hipStream_t st)
 {
-    RowArgs a = {n, p, x, w1, b1, w2, b2, nullptr, weights, h, nullptr, part, nullptr, nullptr, nullptr};
+    RowArgs a = {n, p, x, w1, b1, w2, b2, nullptr, weights, h, nullptr, u, part, nullptr, nullptr, nullptr};
     return type == ESCAT_F32 ? fwd<float>(a, y, st) : type == ESCAT_BF16 ? fwd<bf16_t>(a, y, st) : fwd<f16_t>(a, y, st);
 }
 int escat_experts_rows_bwd(int type, const EDims &n, const EPlan &p, const void *x, const float *weights, const void *w1, const void *b1, const void *w2,
-                           const void *b2, const void *dy, void *h, void *du, float *part, float *dwp, float *ws, void *dx, float *dw, hipStream_t st)
+                           const void *b2, const void *dy, void *h, void *du, float *u, float *part, float *dwp, float *ws, void *dx, float *dw, hipStream_t st)
 {
-    RowArgs a = {n, p, x, w1, b1, w2, b2, dy, weights, h, du, part, nullptr, dwp, ws};
+    RowArgs a = {n, p, x, w1, b1, w2, b2, dy, weights, h, du, u, part, nullptr, dwp, ws};
     return type == ESCAT_F32 ? bwd<float>(a, dx, dw, st) : type == ESCAT_BF16 ? bwd<bf16_t>(a, dx, dw, st) : bwd<f16_t>(a, dx, dw, st);
 }

@@ -164,8 +164,7 @@ def _mlp_forward(x, weights, experts, w1, b1, w2, b2, keep=False):
 class _ExpertMLP(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weights, experts, w1, b1, w2, b2):
-        wanted = ctx.needs_input_grad[5] or ctx.needs_input_grad[6]            # (the hidden rows serve w2's gradient)
-        y, plan, hidden, ctx.dims = _mlp_forward(x, weights, experts, w1, b1, w2, b2, keep=wanted)
+        y, plan, hidden, ctx.dims = _mlp_forward(x, weights, experts, w1, b1, w2, b2, keep=True)
         ctx.save_for_backward(x, weights, experts, w1, b1, w2, b2, plan, hidden)
         return y
 
@@ -203,8 +202,8 @@ def expert_mlp(x: torch.Tensor, weights: torch.Tensor, experts: torch.Tensor, w1
     they are cast to its type); weights (rows, k) fp32, experts (rows, k) int32 as route_experts gives them.  A pair whose
     expert lies outside [0, E) counts for nothing and gets no gradient; the same expert may come twice in a row.  Sums are
     fp32; with 16-bit types the weighted hidden rows and their gradients are rounded to the type in between.  The backward
-    computes the hidden rows again in fp32; with a gradient for w2 the forward keeps them in the operands' type (rows * k * h elements) next to its
-    arguments and the sorted pairs.  For a few rows the forward
+    sees the hidden rows unrounded: it computes them again with 16-bit types.  A forward that gradients are wanted of keeps rows * k * h elements of its
+    type (fp32 with d > 64: twice that) next to its arguments and the sorted pairs.  For a few rows the forward
     is a pair of matrix-vector kernels that read the weights in use once a pair, without sorting.  Weights must be
     contiguous; d, h, o are free (any alignment), k <= 64, E <= 1024, rows * k < 2^30.
     """
