@@ -68,9 +68,10 @@ static inline EPlan plan_of(void *mem, int64_t rows, int k, int E) { return plan
 static inline int64_t plan_ints(int64_t rows, int k, int E) { int64_t n; plan_view(nullptr, rows, k, E, combo_keys(rows, E, k), &n); return n; }
 
 // Whether a training forward leaves u in fp32 next to the hidden rows: 8 bytes an element written and read (2 ps at 4.8 TB/s), or 2 d operations once more
-// (0.033 d ps at the 60 TFLOP/s that fp32 tiles reach; 0.004 d with 16-bit operands).  Forward and backward in fp32, kept / computed again, us, 32768 rows, k = 2 of 8
-// experts, d -> 256 -> 256: d = 32 518/507, 64 528/528, 128 555/577, 256 669/734; 8192 rows, 16 of 1024 -> 1024 -> 1024 1988/2296
-static inline bool keeps_u(int type, int d) { return type == ESCAT_F32 && d > 64; }
+// (0.033 d ps at the 60 TFLOP/s that fp32 tiles reach; 0.003 d with 16-bit operands).  Forward and backward, kept / computed again, us:
+//   fp32  32768 rows, k = 2 of 8 experts, d -> 256 -> 256: d = 32 518/507  64 528/528  128 555/577  256 669/734;  8192 rows, 16 of 1024 -> 1024 -> 1024 1988/2296
+//   bf16  d -> 256 -> 256: 262144 rows of 256 1061/1001  131072 of 512 742/727  65536 of 768 660/685  of 1024 800/837;  8192 rows, 64 of 1024 -> 2048 -> 1024 897/945
+static inline bool keeps_u(int type, int d) { return d > (type == ESCAT_F32 ? 64 : 640); }
 
 // expert of digit j of a key; E (base - 1): none
 __device__ __forceinline__ int key_digit(const EPlan &p, int key, int j)

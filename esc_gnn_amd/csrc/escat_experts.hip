@@ -53,7 +53,7 @@ static size_t chunk_bytes(const escat_experts_dims *n, int M, int N)
     return c ? up((size_t)escat_experts_grad_chunks(P, n->experts, c) * ((size_t)M * N + N) * 4) : 0;
 }
 
-extern "C" size_t escat_experts_hidden_bytes(const escat_experts_dims *n) { return check_dims("escat_experts_hidden_bytes", n) ? 0 : hidden_bytes(n) * (keeps_u(n->type, n->d) ? 2 : 1) + 256; }
+extern "C" size_t escat_experts_hidden_bytes(const escat_experts_dims *n) { return check_dims("escat_experts_hidden_bytes", n) ? 0 : hidden_bytes(n) + (keeps_u(n->type, n->d) ? up((size_t)n->rows * n->k * n->h * 4) : 0) + 256; }
 
 extern "C" size_t escat_experts_workspace_bytes(const escat_experts_dims *n, int backward, int hidden)
 {

@@ -5,8 +5,8 @@
 //
 // Rows are taken in the plan's order (sorted by expert), 128 to a tile.  The weight w goes into the hidden row before it is
 // rounded to the operands' type (w h): it then serves W2's product and W2's gradient without another pass.  The forward's (w h)
-// may be kept for the weights' gradient.  dw and silu' see no rounding of u: with 16-bit operands u is computed again next to G, with fp32 ones, whose
-// products cost more than reading it, the forward leaves it (keeps_u).  Results of the pairs are joined in fp32 by a pass of their own, in the order of the slots: no atomics.
+// may be kept for the weights' gradient.  dw and silu' see no rounding of u: it is computed again next to G in fp32, or, where
+// that costs more than reading it, left in fp32 by the forward (keeps_u).  Results of the pairs are joined in fp32 by a pass of their own, in the order of the slots: no atomics.
 //
 // 524288 rows, k = 2 of 8 experts, 256 x 256 x 256 in bf16: 137 GFLOP a product, W1 x 273 us (0.8 GB), W2 h 230 us (0.8 GB), u, G and du 592 us
 // (two products, 1.1 GB), W1^T du 220 us (0.8 GB): neither the matrix units (a quarter of the cycles) nor memory bound; a workgroup's chain of
@@ -32,7 +32,7 @@ struct RowArgs {
 
 enum { FWD1, FWD2, BWD1, BWD2, BWD1U };                            // BWD1U: BWD1 with u from memory
 // Waves on a SIMD (workgroups of a CU) that the registers leave room for: BWD1 holds two sets of accumulators, BWD1U
-// what it reads of u (with three it spills: 91 instead of 81 us).  Four instead of three for the
+// what it reads of u (with three it spills: 91 instead of 81 us in fp32, 209 instead of 177 in bf16).  Four instead of three for the
 // forward's 16-bit products: 273 instead of 305 us and 230 instead of 244 (524288 rows, k = 2, 256 x 256).
 template <typename T, int MODE> constexpr int waves_of() { return MODE == BWD1 || MODE == BWD1U ? 2 : MODE == BWD2 || sizeof(T) == 4 ? 3 : 4; }
 // DIRECT: FWD2, BWD2: results by row; FWD1: leaves u; BWD1: writes no hidden rows
@@ -347,18 +347,12 @@ template <typename T, int MODE> static int second(RowArgs &a, int M, void *out, 
 
 template <typename T> static int fwd(RowArgs &a, void *y, hipStream_t st)
 {
-    int rc;
-    if constexpr (sizeof(T) == 4) rc = a.u ? rows_launch<T, FWD1, true>(a, a.n.h, st) : rows_launch<T, FWD1, false>(a, a.n.h, st);
-    else rc = rows_launch<T, FWD1, false>(a, a.n.h, st);
-    if (rc) return rc;
+    int rc = a.u ? rows_launch<T, FWD1, true>(a, a.n.h, st) : rows_launch<T, FWD1, false>(a, a.n.h, st); if (rc) return rc;
     return second<T, FWD2>(a, a.n.o, y, st);
 }
 template <typename T> static int bwd(RowArgs &a, void *dx, float *dw, hipStream_t st)
 {
-    int rc = ESCAT_OK;
-    bool done = false;
-    if constexpr (sizeof(T) == 4) if (a.u) { rc = rows_launch<T, BWD1U, true>(a, a.n.h, st); done = true; }
-    if (!done) rc = a.h ? rows_launch<T, BWD1, false>(a, a.n.h, st) : rows_launch<T, BWD1, true>(a, a.n.h, st);
+    int rc = a.u ? rows_launch<T, BWD1U, true>(a, a.n.h, st) : a.h ? rows_launch<T, BWD1, false>(a, a.n.h, st) : rows_launch<T, BWD1, true>(a, a.n.h, st);
     if (rc) return rc;
     const int64_t P = a.n.rows * a.n.k;
     if (dw) { k_join_dw<<<grid_for(P), XT, 0, st>>>(a.dwp, a.p.pos, P, (a.n.h + XN - 1) / XN, dw); CHECK_LAUNCH("experts: dw"); }

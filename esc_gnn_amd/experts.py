@@ -202,8 +202,8 @@ def expert_mlp(x: torch.Tensor, weights: torch.Tensor, experts: torch.Tensor, w1
     they are cast to its type); weights (rows, k) fp32, experts (rows, k) int32 as route_experts gives them.  A pair whose
     expert lies outside [0, E) counts for nothing and gets no gradient; the same expert may come twice in a row.  Sums are
     fp32; with 16-bit types the weighted hidden rows and their gradients are rounded to the type in between.  The backward
-    sees the hidden rows unrounded: it computes them again with 16-bit types.  A forward that gradients are wanted of keeps rows * k * h elements of its
-    type (fp32 with d > 64: twice that) next to its arguments and the sorted pairs.  For a few rows the forward
+    sees the hidden rows unrounded.  A forward that gradients are wanted of keeps rows * k * h elements of its type, and with d > 64 (16-bit types: d > 640)
+    as many in fp32, next to its arguments and the sorted pairs.  For a few rows the forward
     is a pair of matrix-vector kernels that read the weights in use once a pair, without sorting.  Weights must be
     contiguous; d, h, o are free (any alignment), k <= 64, E <= 1024, rows * k < 2^30.
     """

@@ -587,7 +587,7 @@ int escat_route_bwd(const void *logits, int type, int64_t rows, int E, int k, in
  * where escat_experts_fwd_needs_plan is 0 (few rows) the forward reads the array itself and plan may be NULL.
  * escat_experts_bwd: gradients for dy (rows, o); dx, dweights, dw1 + db1, dw2 + db2 may each be NULL (a bias's gradient only
  * together with its weight's); the others are written whole (experts without a row: zeros).  Workspaces: 16-byte aligned, contents
- * only used within the call.  hidden (escat_experts_hidden_bytes, 16-byte aligned): where a sorting forward leaves w silu(W1 x + b1) by position (fp32 with d > 64: W1 x + b1, too);
+ * only used within the call.  hidden (escat_experts_hidden_bytes, 16-byte aligned): where a sorting forward leaves w silu(W1 x + b1) by position (d > 64, with 16-bit types > 640: W1 x + b1 in fp32, too);
  * the backward of the same inputs and plan that is given it does not write those rows again.  NULL for either: kept in the workspace, which is then
  * larger (escat_experts_workspace_bytes with hidden = 0).  No atomics: the same inputs give the same bits. */
 typedef struct { int64_t rows; int32_t type, d, h, o, experts, k; } escat_experts_dims;

@@ -114,6 +114,9 @@ SHAPES = [  # rows, d, h, o, E, k
     (3000, 33, 65, 31, 64, 2),
     (5000, 130, 129, 70, 40, 3),
     (6000, 50, 40, 60, 5, 1),
+    # u kept by the forward with 16-bit types, by pair and by combination, ragged
+    (700, 700, 140, 130, 6, 2),
+    (7000, 650, 70, 40, 2, 2),
     # many experts, many slots
     (6000, 24, 16, 24, 1024, 2),
     (6000, 24, 16, 24, 1024, 1),
@@ -352,7 +355,7 @@ class Guarded:
 
 
 @pytest.mark.parametrize("shape", [(3, 17, 33, 9, 2, 2), (300, 242, 256, 250, 8, 2), (3000, 33, 65, 31, 64, 2), (5000, 41, 70, 45, 3, 1), (7000, 40, 77, 137, 2, 2),
-                                   (700, 1030, 43, 24, 6, 2)])
+                                   (700, 1030, 43, 24, 6, 2), (2500, 1030, 143, 24, 6, 2)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("keep", [False, True])
 def test_nothing_is_written_outside(shape, dtype, keep):
