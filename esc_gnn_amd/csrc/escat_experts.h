@@ -38,7 +38,6 @@ struct EPlan {
     int *tile;        // 4 x max_tiles: key, first item, items, 0
     int *pair;        // P         position -> pair
     int *row;         // P         position -> row of the activations
-    int *expert;      // P         position -> expert, -1 = none
     int *pos;         // P         pair -> position, -1 = not routed
     int *hist;        // keys x blocks: scratch of the sort
 };
@@ -58,7 +57,7 @@ static inline EPlan plan_view(void *mem, int64_t rows, int k, int E, int combo, 
     p.count = q; q += p.keys; p.first = q; q += p.keys + 1; p.n_tiles = q; q += 1;
     q += (4 - (q - (int *)mem) % 4) % 4;
     p.tile = q; q += 4 * plan_max_tiles(items, p.keys);
-    p.pair = q; q += P; p.row = q; q += P; p.expert = q; q += P; p.pos = q; q += P;
+    p.pair = q; q += P; p.row = q; q += P; p.pos = q; q += P;
     p.hist = q; q += p.keys * plan_blocks(items);
     if (ints) *ints = q - (int *)mem;
     return p;

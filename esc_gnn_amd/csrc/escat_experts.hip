@@ -7,7 +7,7 @@ __attribute__((visibility("hidden"))) int escat_experts_rows_bwd(int type, const
                            const void *w2, const void *b2, const void *dy, void *h, void *du, float *u, float *part, float *dwp, float *ws, void *dx, float *dw, hipStream_t st);
 __attribute__((visibility("hidden"))) int escat_experts_grad_chunk(int type, int64_t P, int E, int M, int N);
 __attribute__((visibility("hidden"))) int64_t escat_experts_grad_chunks(int64_t P, int E, int chunk);
-__attribute__((visibility("hidden"))) int escat_experts_plan_by_expert(const EPlan &p, int64_t P, int E, const EPlan &by, hipStream_t st);
+__attribute__((visibility("hidden"))) int escat_experts_plan_by_expert(const EPlan &p, int64_t rows, int E, const EPlan &by, hipStream_t st);
 __attribute__((visibility("hidden"))) int escat_experts_grad(int type, const EDims &n, const EPlan &p, const int *at, bool w2, const void *a, const void *b, const float *weights, int M, int N,
                        int chunk, float *part, void *out, void *db, hipStream_t st);
 
@@ -43,7 +43,7 @@ static size_t by_expert_bytes(const escat_experts_dims *n)
     if (!combo_keys(n->rows, n->experts, n->k) || n->k == 1) return 0;
     int64_t ints;
     plan_view(nullptr, n->rows * n->k, 1, n->experts, 0, &ints);
-    return up((size_t)ints * 4);
+    return up((size_t)(ints + (int64_t)combo_keys(n->rows, n->experts, n->k) * n->k) * 4);             // and where each key's runs begin
 }
 static size_t hidden_bytes(const escat_experts_dims *n) { return up((size_t)n->rows * n->k * n->h * escat_type_bytes(n->type)); }
 static size_t chunk_bytes(const escat_experts_dims *n, int M, int N)
@@ -119,9 +119,10 @@ extern "C" int escat_experts_bwd(const escat_experts_dims *n, const void *x, con
     EPlan by = p;
     const int *at = nullptr;
     if (p.base && n->k > 1 && (dw1 || dw2)) {
-        by = plan_view(by_mem, P, 1, n->experts, 0, nullptr);
-        by.pos = by.expert = nullptr;
-        rc = escat_experts_plan_by_expert(p, P, n->experts, by, st); if (rc) return rc;
+        int64_t ints;
+        by = plan_view(by_mem, P, 1, n->experts, 0, &ints);
+        by.hist = (int *)by_mem + ints;
+        rc = escat_experts_plan_by_expert(p, n->rows, n->experts, by, st); if (rc) return rc;
         at = by.pair;
     }
     if (dw2) { rc = escat_experts_grad(n->type, d, by, at, true, h, dy, sw, n->h, n->o, escat_experts_grad_chunk(n->type, P, n->experts, n->h, n->o), chunks, dw2, db2, st); if (rc) return rc; }

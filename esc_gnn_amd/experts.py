@@ -205,7 +205,8 @@ def expert_mlp(x: torch.Tensor, weights: torch.Tensor, experts: torch.Tensor, w1
     sees the hidden rows unrounded.  A forward that gradients are wanted of keeps rows * k * h elements of its type, and with d > 64 (16-bit types: d > 640)
     as many in fp32, next to its arguments and the sorted pairs.  For a few rows the forward
     is a pair of matrix-vector kernels that read the weights in use once a pair, without sorting.  Weights must be
-    contiguous; d, h, o are free (any alignment), k <= 64, E <= 1024, rows * k < 2^30.
+    contiguous; d, h, o are free (any alignment), k <= 64, E <= 1024, rows * k < 2^30, and a product has fewer than 2^24 tiles of 128 x 128
+    (EscatError otherwise).
     """
     if torch.is_autocast_enabled("cuda") and x.is_cuda:
         t = torch.get_autocast_dtype("cuda")

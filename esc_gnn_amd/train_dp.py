@@ -1,5 +1,5 @@
 """
-Minimal data-parallel ESc-GNN training step (BASELINE cfg4).
+Minimal data-parallel ESc-GNN training step.
 
 What a step does, per rank (one process per GPU, graphs sharded, RCCL only for the gradients):
   1. orders-0/1/2 scattering of both tracks on the rank's batch -- esc_gnn_amd.scatter (the hot path; like the
@@ -14,7 +14,7 @@ Optional (off by default): `experts` = E widens the head at the cost per node of
 expert_mlp, kept in balance by a selection bias); `optimizer` = "escat" / "escat8" takes the multi-tensor AdamW of
 esc_gnn_amd.optim with states in 32 / 8 bits; `max_grad_norm` clips as the reference does (training/train.py:411-415).
 The reference gets 3 from Accelerate/DDP (training/train.py:408, :483-492); the heads themselves are plain PyTorch
-and out of the hot-path scope.
+but for the optional operators.
 """
 from typing import Dict
 import torch
