@@ -117,6 +117,9 @@ SHAPES = [  # rows, d, h, o, E, k
     # u kept by the forward with 16-bit types, by pair and by combination, ragged
     (700, 700, 140, 130, 6, 2),
     (7000, 650, 70, 40, 2, 2),
+    # combinations of six, and of one expert with itself
+    (15000, 20, 24, 16, 2, 6),
+    (5000, 20, 24, 16, 1, 2),
     # many experts, many slots
     (6000, 24, 16, 24, 1024, 2),
     (6000, 24, 16, 24, 1024, 1),
