@@ -14,7 +14,7 @@
 // keys are computed in 32 bits with a bound on their error, and a wave in which two keys that decide something lie within that
 // bound repeats the selection with 64-bit keys (about one wave in 500 at E = 256, k = 8).
 //
-// 65537 rows of 256 bf16 logits, k = 8, bias and 4 of 8 groups: 74 us forward (34 MB read: 7 us; what bounds it is the instructions of the
+// 65537 rows of 256 bf16 logits, k = 8, bias and 4 of 8 groups: 72 us forward (34 MB read: 7 us; what bounds it is the instructions of the
 // selection, 1200 for the two rows of a wave), 17 us backward.  524288 rows of 8 fp32 logits, k = 2: 12 us forward (25 MB, 2.1 TB/s), 9 us backward.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -174,18 +174,16 @@ __device__ bool pick(const RouteArgs &a, K (&key)[EPL], const K (&gkey)[EPL], bo
             V sum = -inf;
             if (e0 < a.E && b1 > least) sum = (V)value_of(b1) + (a.group_top == 2 && b2 > least ? (V)value_of(b2) : (V)0);
             K score; to_key(sum, score);
-            bool kept = false;
-            V last = inf;
-            for (int r = 0; r <= a.keep; ++r) {
-                const K m = row_reduce<LPR, OpMax>(score);
-                const V mv = (V)value_of(m);
-                if (CHECK && r > 0) close |= m > least && too_close(last, mv);
-                if (r == a.keep) break;
-                const int at = first_lane<LPR>(score == m, l0);
-                const bool it = (at ^ lane_in_row) < lpg && m > least;                // the same group: only bits below lpg differ
-                kept |= it;
-                score = it ? least : score;
-                last = mv;
+            int ahead = 0;                                   // groups that come before the lane's
+            const int mine = lane_in_row / lpg;
+            for (int g = 0; g < a.groups; ++g) {
+                const K o = __shfl(score, l0 + g * lpg, 64);
+                ahead += o > score || (o == score && g < mine);
+            }
+            const bool kept = ahead < a.keep && score > least;
+            if constexpr (CHECK) {                           // the least that stays against the largest that goes (~ turns the order round)
+                const int stays = ~row_reduce<LPR, OpMax>(kept ? ~score : least), goes = row_reduce<LPR, OpMax>(kept ? least : score);
+                close |= goes > least && too_close(value_of(stays), value_of(goes));
             }
 #pragma unroll
             for (int i = 0; i < EPL; ++i) if (!kept) key[i] = least;
