@@ -293,6 +293,10 @@ class AdamW(torch.optim.Optimizer):
         # a step count is shared by the parameters that took every step together; where some stay behind, the others get their own
         moved = {}
         for key, (behind, ps) in seen.items():
+            if ps:
+                count = self.state[ps[0]]["step"]
+                if count.dtype is not torch.int32 or count.numel() != 1 or count.device != dev:
+                    raise ValueError(f"escat: step must be an int32 tensor of one element on {dev}: {count.dtype}, {tuple(count.shape)} on {count.device}")
             if behind and ps:
                 own = self.state[ps[0]]["step"].clone()
                 for p in ps:
@@ -330,15 +334,41 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def load_state_dict(self, state_dict):
-        saved = state_dict["state"]
-        for st in saved.values():
-            if st and (8 if "exp_avg_codes" in st else 32) != self.state_bits:
-                raise ValueError(f"escat: the loaded states do not have {self.state_bits} bits")
+        """A state dict of this class, or of torch.optim.AdamW: the count becomes int32, moments that torch held in a 16-bit type fp32,
+        both with the values they had.  States of another step (amsgrad, maximize, decay inside the gradient) are refused."""
+        saved, groups = state_dict["state"], state_dict["param_groups"]
+        for g in groups:
+            if g.get("amsgrad") or g.get("maximize") or (g.get("weight_decay") and not g.get("decoupled_weight_decay", True)):
+                raise ValueError("escat: the loaded states are of another step: amsgrad, maximize and coupled weight decay are not served")
+        names = {"step"} | ({n + e for n in ("exp_avg", "exp_avg_sq") for e in ("_codes", "_scales")} if self.state_bits == 8 else {"exp_avg", "exp_avg_sq"})
+        ids = [i for g in groups for i in g["params"]]
+        counts = {}
+        for i, p in zip(ids, [p for g in self.param_groups for p in g["params"]]):
+            st = saved.get(i)
+            if not st:
+                continue
+            if set(st) != names:
+                raise ValueError(f"escat: a state with {self.state_bits} bits holds {sorted(names)}, the loaded one {sorted(st)}")
+            step = torch.as_tensor(st["step"])
+            t = float(step) if step.numel() == 1 else -1.0
+            if not (0 <= t < 2 ** 31 and t == int(t)):
+                raise ValueError(f"escat: step must be a whole number of steps: {st['step']}")
+            counts[i] = int(t)
+            for name in names - {"step"}:
+                n = -(-p.numel() // STATE_BLOCK) if name.endswith("_scales") else p.numel()
+                if st[name].numel() != n or not (st[name].dtype is torch.uint8 if name.endswith("_codes") else st[name].is_floating_point()):
+                    raise ValueError(f"escat: {name} of a parameter of shape {tuple(p.shape)} has {st[name].numel()} elements of {st[name].dtype}")
         super().load_state_dict(state_dict)
         # the base class casts states to the parameter's type: take them as they were saved instead
-        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         shared = {}
         for i, p in zip(ids, [p for g in self.param_groups for p in g["params"]]):
-            if saved.get(i):
-                st = self.state[p] = {name: t.detach().to(device=p.device, copy=True) for name, t in saved[i].items()}
-                st["step"] = shared.setdefault(int(st["step"]), st["step"])
+            if i in counts:
+                st = self.state[p] = {}
+                for name in saved[i]:
+                    if name == "step":
+                        if counts[i] not in shared:
+                            shared[counts[i]] = torch.full((1,), counts[i], dtype=torch.int32, device=p.device)
+                        st[name] = shared[counts[i]]
+                    else:
+                        dtype = torch.uint8 if name.endswith("_codes") else torch.float32
+                        st[name] = saved[i][name].detach().to(device=p.device, dtype=dtype, copy=True).contiguous()

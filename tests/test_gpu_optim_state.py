@@ -1,0 +1,53 @@
+"""
+GPU tests of the optimizer's states over their life: taken from torch's AdamW in mid-run, copied, captured.
+u = 2^-24, half a step of fp32.
+"""
+import copy
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+DEV = "cuda:0"
+
+
+def _grads(ps, it):
+    for i, p in enumerate(ps):
+        p.grad = torch.randn(p.shape, device=DEV, generator=torch.Generator(device=DEV).manual_seed(100 * it + i)).to(p.dtype)
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(fused=True), dict(capturable=True), dict(foreach=False)])
+def test_goes_on_where_torchs_left_off(kw):
+    """8 steps by torch, 5 more by both.  A step errs by some 30 u of its update (|update| <= 5 lr = 0.025) and 4 u of the parameter, and
+    what the moments are off by (8 u a step) passes on to the next: 5 steps stay under 1000 u of max(|p|, 1).  A count that is not
+    taken over would show as a third or more of an update, 1e-3"""
+    from esc_gnn_amd import AdamW
+    torch.manual_seed(0)
+    a = [torch.nn.Parameter(torch.randn(s, device=DEV)) for s in ((33, 7), (300,), (1,), (64, 65))]
+    groups = lambda ps: [{"params": ps[:2]}, {"params": ps[2:], "lr": 5e-3, "betas": (0.8, 0.95)}]               # noqa: E731
+    ref = torch.optim.AdamW(groups(a), lr=1e-3, **kw)
+    for it in range(8):
+        _grads(a, it); ref.step()
+    b = [torch.nn.Parameter(p.detach().clone()) for p in a]
+    opt = AdamW(groups(b), lr=0.5)                                                  # (the loaded groups' settings count)
+    opt.load_state_dict(ref.state_dict())
+    for it in range(8, 13):
+        _grads(a, it); ref.step()
+        _grads(b, it); opt.step()
+        for x, y in zip(a, b):
+            assert float((x - y).detach().abs().max()) <= 1000 * U * max(1.0, float(x.detach().abs().max())), it
+    assert all(int(opt.state[p]["step"]) == 13 for p in b)
+
+
+def test_a_count_of_another_type_is_refused_at_the_step():
+    from esc_gnn_amd import AdamW
+    p = torch.nn.Parameter(torch.ones(5, device=DEV))
+    opt = AdamW([p])
+    p.grad = torch.ones_like(p)
+    opt.step()
+    before = p.detach().clone()
+    for bad in (torch.ones(1, device=DEV), torch.ones(2, dtype=torch.int32, device=DEV), torch.ones(1, dtype=torch.int32)):
+        opt.state[p]["step"] = bad
+        with pytest.raises(ValueError, match="step"):
+            opt.step()
+        assert torch.equal(p, before)

@@ -1,0 +1,75 @@
+"""State dicts that the optimizer takes and refuses: host work, no GPU."""
+import copy
+import pytest
+import torch
+
+
+def _torch_dict(kind=torch.optim.AdamW, steps=100, dtype=torch.float32, **kw):
+    ps = [torch.nn.Parameter(torch.ones(n, dtype=dtype)) for n in (3, 300)]
+    opt = kind(ps, lr=2e-3, **kw)
+    for _ in range(steps):
+        for p in ps:
+            p.grad = torch.ones_like(p)
+        opt.step()
+    return ps, opt.state_dict()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_torchs_state_dict_is_taken_as_what_it_means(dtype):
+    """torch counts steps in fp32 and holds the moments in the parameter's type: here int32 and fp32, the values the same"""
+    from esc_gnn_amd import AdamW
+    ps, saved = _torch_dict(dtype=dtype)
+    opt = AdamW([torch.nn.Parameter(p.detach().clone()) for p in ps])
+    opt.load_state_dict(copy.deepcopy(saved))
+    assert opt.param_groups[0]["lr"] == 2e-3
+    for i, p in enumerate(opt.param_groups[0]["params"]):
+        st = opt.state[p]
+        assert set(st) == {"step", "exp_avg", "exp_avg_sq"}
+        assert st["step"].dtype is torch.int32 and st["step"].shape == (1,) and int(st["step"]) == 100
+        for name in ("exp_avg", "exp_avg_sq"):
+            assert st[name].dtype is torch.float32 and torch.equal(st[name], saved["state"][i][name].float())
+    assert opt.state[opt.param_groups[0]["params"][0]]["step"] is opt.state[opt.param_groups[0]["params"][1]]["step"]
+
+
+def test_a_count_may_be_a_number_and_must_be_a_whole_one():
+    from esc_gnn_amd import AdamW
+    ps, saved = _torch_dict(steps=3)
+    saved["state"][0]["step"] = 3
+    opt = AdamW(ps)
+    opt.load_state_dict(saved)
+    assert int(opt.state[ps[0]]["step"]) == 3
+    for bad in (2.5, -1, float("nan"), 2 ** 31, torch.zeros(2)):
+        saved["state"][0]["step"] = bad
+        with pytest.raises(ValueError, match="step"):
+            opt.load_state_dict(saved)
+        assert int(opt.state[ps[0]]["step"]) == 3                                  # a refused load changes nothing
+
+
+@pytest.mark.parametrize("kind,kw", [(torch.optim.AdamW, dict(amsgrad=True)), (torch.optim.AdamW, dict(maximize=True)),
+                                     (torch.optim.Adam, dict(weight_decay=0.1)), (torch.optim.SGD, dict(momentum=0.9)), (torch.optim.RAdam, dict(weight_decay=0.1))])
+def test_states_of_another_step_are_refused(kind, kw):
+    from esc_gnn_amd import AdamW
+    ps, saved = _torch_dict(kind, 2, **kw)
+    opt = AdamW(ps, lr=7e-3)
+    with pytest.raises(ValueError):
+        opt.load_state_dict(saved)
+    assert opt.param_groups[0]["lr"] == 7e-3 and not opt.state
+
+
+def test_plain_adam_without_decay_is_the_same_step():
+    from esc_gnn_amd import AdamW
+    ps, saved = _torch_dict(torch.optim.Adam, 2)
+    opt = AdamW(ps)
+    opt.load_state_dict(saved)
+    assert opt.param_groups[0]["weight_decay"] == 0 and int(opt.state[ps[0]]["step"]) == 2
+
+
+def test_missing_or_wrong_entries_are_refused():
+    from esc_gnn_amd import AdamW
+    ps, saved = _torch_dict(steps=2)
+    opt = AdamW(ps)
+    for change in (lambda st: st.pop("exp_avg_sq"), lambda st: st.update(exp_avg=torch.zeros(4)), lambda st: st.pop("step")):
+        other = copy.deepcopy(saved)
+        change(other["state"][0])
+        with pytest.raises(ValueError):
+            opt.load_state_dict(other)
