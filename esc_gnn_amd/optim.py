@@ -333,6 +333,13 @@ class AdamW(torch.optim.Optimizer):
         self.grad_norm = norm
         return loss
 
+    def state_dict(self):
+        """As torch's: the moments themselves.  Each parameter has a count of its own here (in the optimizer those that took every step together
+        share one), so that an optimizer that counts by parameter, torch's among them, does not count a shared one several times."""
+        out = super().state_dict()
+        out["state"] = {i: {n: t.clone() if n == "step" else t for n, t in st.items()} for i, st in out["state"].items()}
+        return out
+
     def load_state_dict(self, state_dict):
         """A state dict of this class, or of torch.optim.AdamW: the count becomes int32, moments that torch held in a 16-bit type fp32,
         both with the values they had.  States of another step (amsgrad, maximize, decay inside the gradient) are refused."""

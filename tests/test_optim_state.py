@@ -73,3 +73,23 @@ def test_missing_or_wrong_entries_are_refused():
         change(other["state"][0])
         with pytest.raises(ValueError):
             opt.load_state_dict(other)
+
+
+def test_torch_takes_this_optimizers_state_dict():
+    """the other way: the names and values are what torch's AdamW reads"""
+    from esc_gnn_amd import AdamW
+    ps, saved = _torch_dict(steps=4)
+    mine = AdamW(ps, lr=2e-3)
+    mine.load_state_dict(copy.deepcopy(saved))
+    outs = []
+    for source in (saved, mine.state_dict()):
+        qs = [torch.nn.Parameter(p.detach().clone()) for p in ps]
+        opt = torch.optim.AdamW(qs, lr=2e-3)
+        opt.load_state_dict(copy.deepcopy(source))
+        for q in qs:
+            q.grad = torch.full_like(q, 0.3)
+        opt.step()
+        assert all(float(opt.state[q]["step"]) == 5 for q in qs)
+        outs.append(qs)
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
