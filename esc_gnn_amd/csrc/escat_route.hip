@@ -257,8 +257,8 @@ __device__ bool pick(const RouteArgs &a, K (&key)[EPL], const K (&gkey)[EPL], bo
 __device__ __forceinline__ float sigmoid_f(float x) { return 1.f / (1.f + expf(-x)); }
 
 // key of a score that is NaN: largest where the logit itself is the cause (NaN, or +inf under a softmax), next to it in the
-// rest of such a row
-__device__ __forceinline__ float spoiled(float x, float next) { return x == x && x < R_INF ? next : R_INF; }
+// rest of such a row; a bias of -inf masks here too (its sum with a NaN does not)
+__device__ __forceinline__ float spoiled(float x, float bias, float next) { return bias == -R_INF ? -R_INF : x == x && x < R_INF ? next : R_INF; }
 
 template <typename T, int LPR, int EPL>
 __global__ void __launch_bounds__(RT) k_route(const RouteArgs a)
@@ -318,7 +318,7 @@ __global__ void __launch_bounds__(RT) k_route(const RouteArgs a)
             }
 #pragma unroll
             for (int i = 0; i < EPL; ++i) {
-                const float v = sc[i] + bias[i], t = v == v ? v : spoiled(x[i], 3.4e38f);
+                const float v = sc[i] + bias[i], t = v == v ? v : spoiled(x[i], bias[i], 3.4e38f);
                 gkey[i] = sortable(x[i] == -R_INF ? -R_INF : t);
             }
             if (a.bias) {
@@ -350,7 +350,7 @@ __global__ void __launch_bounds__(RT) k_route(const RouteArgs a)
 #pragma unroll
             for (int i = 0; i < EPL; ++i) {
                 const double v = gkey2[i] + (double)bias[i];
-                gkey2[i] = x[i] == -R_INF ? -(double)R_INF : v == v ? v : (double)spoiled(x[i], 3.4e38f);
+                gkey2[i] = x[i] == -R_INF ? -(double)R_INF : v == v ? v : (double)spoiled(x[i], bias[i], 3.4e38f);
                 key2[i] = a.bias ? gkey2[i] : x[i] == x[i] ? (double)x[i] : (double)R_INF;
             }
             pick<LPR, EPL, double, double, false>(a, key2, gkey2, true, lane_in_row, l0, buf, sel);
