@@ -24,8 +24,9 @@
 #define RT 256
 #define R_INF __builtin_inff()
 // two 32-bit keys further apart than this (times max(1, size)) are in the order of their exact values: exp and the sum of up to
-// 1024 of them err by at most 1e-6 of s <= 1, a pair of them (group score) by 2e-6, the sum with the bias by 2^-24 of its size; a place
-// in a lane takes the last 3 bits of a key (E > 512: 4), 1e-6 (1.9e-6) of its size
+// 1024 of them err by at most 1e-6 of s <= 1, the sum with the bias by 2^-24 of its size; a place in a lane takes the last 3 bits of a key
+// (E > 512: 4), 1e-6 (1.9e-6) of its size.  A group score adds two keys, whose biases may cancel: its size is that of its terms, at most
+// B = max(1, the largest |bias|): 4 2^-24 (1 + B) + 2e-6 off, two of them 9e-7 + 4e-6 B at most
 #define R_GAP 7.62939453125e-6f
 
 struct RouteArgs {
@@ -97,8 +98,8 @@ __device__ __forceinline__ void wave_lds_sync() { __builtin_amdgcn_fence(__ATOMI
 // ------------------------------------------------------------------ the selection
 // key / gkey: the lane's EPL keys for experts and for group scores (Least: cannot be chosen), K = int (sortable) or double, V the
 // type of their values.  sel (LDS, of the row): k results.  Returns whether two keys that decided something were closer than
-// their error (CHECK only).
-template <typename V> __device__ __forceinline__ bool too_close(V last, V now) { return !(last - now > (V)R_GAP * fmaxf(1.f, fabsf((float)last))); }
+// their error (CHECK only; terms: the size of what a group score adds, at least 1).
+template <typename V> __device__ __forceinline__ bool too_close(V last, V now, float size = 1.f) { return !(last - now > (V)R_GAP * fmaxf(size, fabsf((float)last))); }
 
 template <int LPR, typename K> __device__ __forceinline__ K other_lane(K v, int m)       // lane ^ m, m < LPR, inside a group of whole lanes
 {
@@ -154,7 +155,7 @@ __device__ __forceinline__ bool pick_sorted(const RouteArgs &a, int (&key)[EPL],
 }
 
 template <int LPR, int EPL, typename K, typename V, bool CHECK>
-__device__ bool pick(const RouteArgs &a, K (&key)[EPL], const K (&gkey)[EPL], bool key_exact, int lane_in_row, int l0, V *buf, int *sel)
+__device__ bool pick(const RouteArgs &a, K (&key)[EPL], const K (&gkey)[EPL], bool key_exact, float terms, int lane_in_row, int l0, V *buf, int *sel)
 {
     constexpr K least = Least<K>::v;
     const V inf = (V)R_INF;
@@ -183,7 +184,7 @@ __device__ bool pick(const RouteArgs &a, K (&key)[EPL], const K (&gkey)[EPL], bo
             const bool kept = ahead < a.keep && score > least;
             if constexpr (CHECK) {                           // the least that stays against the largest that goes (~ turns the order round)
                 const int stays = ~row_reduce<LPR, OpMax>(kept ? ~score : least), goes = row_reduce<LPR, OpMax>(kept ? least : score);
-                close |= goes > least && too_close(value_of(stays), value_of(goes));
+                close |= goes > least && too_close(value_of(stays), value_of(goes), terms);
             }
 #pragma unroll
             for (int i = 0; i < EPL; ++i) if (!kept) key[i] = least;
@@ -209,7 +210,7 @@ __device__ bool pick(const RouteArgs &a, K (&key)[EPL], const K (&gkey)[EPL], bo
             for (int r = 0; r <= a.keep; ++r) {
                 const K m = row_reduce<LPR, OpMax>(score);
                 const V mv = (V)value_of(m);
-                if (CHECK && r > 0 && m > least) close |= too_close(last, mv);
+                if (CHECK && r > 0 && m > least) close |= too_close(last, mv, terms);
                 if (r == a.keep || m == least) break;
                 const int at = first_lane<LPR>(score == m, l0);
                 kept |= 1ull << at;
@@ -273,6 +274,12 @@ __global__ void __launch_bounds__(RT) k_route(const RouteArgs a)
     float bias[EPL];
 #pragma unroll
     for (int i = 0; i < EPL; ++i) bias[i] = a.bias && e0 + i < a.E ? a.bias[e0 + i] : 0.f;
+    float terms = 1.f;
+    if (a.bias && a.groups > 1) {
+#pragma unroll
+        for (int i = 0; i < EPL; ++i) terms = fabsf(bias[i]) < R_INF ? fmaxf(terms, fabsf(bias[i])) : terms;
+        terms = row_reduce<LPR, OpMax>(terms);
+    }
     // all lanes of a wave go through the same number of rows: rows behind the last are worked on as rows without an expert
     for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.rows; r0 += (int64_t)gridDim.x * RPB) {
         const int64_t row = r0 + r_in_b;
@@ -303,10 +310,11 @@ __global__ void __launch_bounds__(RT) k_route(const RouteArgs a)
         if (!fp64_keys) {
 #pragma unroll
             for (int i = 0; i < EPL; ++i) key[i] = sortable(x[i] == x[i] ? x[i] : R_INF);
-            pick<LPR, EPL, int, float, false>(a, key, key, true, lane_in_row, l0, (float *)buf, sel);
+            pick<LPR, EPL, int, float, false>(a, key, key, true, 1.f, lane_in_row, l0, (float *)buf, sel);
         } else {
             int gkey[EPL];
             float sc[EPL];
+            bool nan = false;
             // (the form of the scores is asked for outside the loops over a lane's experts: inside it is a branch for each)
             if (a.score == 0) {
                 const float inv = 1.f / sum;
@@ -318,8 +326,13 @@ __global__ void __launch_bounds__(RT) k_route(const RouteArgs a)
             }
 #pragma unroll
             for (int i = 0; i < EPL; ++i) {
-                const float v = sc[i] + bias[i], t = v == v ? v : spoiled(x[i], bias[i], 3.4e38f);
-                gkey[i] = sortable(x[i] == -R_INF ? -R_INF : t);
+                sc[i] += bias[i];
+                nan |= sc[i] != sc[i];
+                gkey[i] = sortable(x[i] == -R_INF ? -R_INF : sc[i]);
+            }
+            if (__any(nan)) {                                    // (rare: not a select for every logit)
+#pragma unroll
+                for (int i = 0; i < EPL; ++i) if (x[i] != -R_INF && sc[i] != sc[i]) gkey[i] = sortable(spoiled(x[i], bias[i], 3.4e38f));
             }
             if (a.bias) {
 #pragma unroll
@@ -328,7 +341,7 @@ __global__ void __launch_bounds__(RT) k_route(const RouteArgs a)
 #pragma unroll
                 for (int i = 0; i < EPL; ++i) key[i] = sortable(x[i] == x[i] ? x[i] : R_INF);
             }
-            again = pick<LPR, EPL, int, float, true>(a, key, gkey, !a.bias, lane_in_row, l0, (float *)buf, sel);
+            again = pick<LPR, EPL, int, float, true>(a, key, gkey, !a.bias, terms, lane_in_row, l0, (float *)buf, sel);
         }
         if (__any(again)) {
             double key2[EPL], gkey2[EPL];
@@ -353,7 +366,7 @@ __global__ void __launch_bounds__(RT) k_route(const RouteArgs a)
                 gkey2[i] = x[i] == -R_INF ? -(double)R_INF : v == v ? v : (double)spoiled(x[i], bias[i], 3.4e38f);
                 key2[i] = a.bias ? gkey2[i] : x[i] == x[i] ? (double)x[i] : (double)R_INF;
             }
-            pick<LPR, EPL, double, double, false>(a, key2, gkey2, true, lane_in_row, l0, buf, sel);
+            pick<LPR, EPL, double, double, false>(a, key2, gkey2, true, 1.f, lane_in_row, l0, buf, sel);
         }
         wave_lds_sync();
         // weights: the chosen logits once more (they are in the cache), spread over the row's lanes; s_j waits in LDS next to sel

@@ -76,3 +76,24 @@ def test_softmax(E, k, groups, keep, dtype):
             assert bool(cause[r, chosen[0]]), r
     assert bool(torch.isfinite(w[[0, 1, 2, 3]]).all())                               # the weights are a softmax over the chosen logits alone
     assert bool(torch.isfinite(w[12:]).all()) and not bool((masked[at[12:].clamp(min=0).long()] & (at[12:] >= 0)).any())
+
+
+@pytest.mark.parametrize("size", [30.0, 1e3, 1e4, 1e6])
+@pytest.mark.parametrize("E,groups,keep,dtype", [(8, 4, 2, torch.float32), (24, 4, 2, torch.float32), (64, 8, 3, torch.float32), (256, 16, 7, torch.bfloat16), (512, 64, 20, torch.float32)])
+def test_groups_whose_large_biases_cancel(E, groups, keep, dtype, size):
+    """two biases of opposite sign in each group: their sum, near that of the next group, has less than the rounding of its terms.  Which
+    groups stay is decided by the 64-bit sums"""
+    from esc_gnn_amd import route_experts
+    gen = torch.Generator().manual_seed(int(size) + E)
+    gs = E // groups
+    rows = 3000
+    x = torch.randn(rows, E, generator=gen).to(dtype)
+    bias = torch.full((E,), -4 * size)
+    a = size * (1 + torch.rand(groups, generator=gen))
+    for g in range(groups):
+        at = g * gs + torch.randperm(gs, generator=gen)[:2]
+        bias[at[0]], bias[at[1]] = a[g], -a[g]
+    k = min(2 * keep, 8)
+    _, at = route_experts(x.to(DEV), k, score="sigmoid", bias=bias.to(DEV), groups=groups, keep_groups=keep)
+    want, _ = plain(x.double().numpy(), k, "sigmoid", bias.double().numpy(), groups, keep, 2, True, 1.0)
+    assert np.array_equal(at.cpu().numpy(), want)
