@@ -7,13 +7,14 @@ router picks for it.
     load = expert_counts(experts, E)                                 # rows per expert, for a balance bias
 
 All three run on the current stream, read nothing back to the host, and give the same bits for the same inputs (no
-floating-point atomics); they can be captured into a graph.  There is no CPU path.
+floating-point atomics); they can be captured into a graph.  There is no CPU path, and no forward-mode differentiation (an error).
 """
 import ctypes
 import functools
 import math
 from typing import Optional, Tuple
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 from torch.nn.functional import pad
 
@@ -34,6 +35,9 @@ def _need_gpu(t: torch.Tensor, name: str):
 
 
 def _wants_grad(ts) -> bool:
+    """whether a call goes by its autograd function: for a gradient, or to be refused where a tensor has a forward-mode tangent"""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        return True
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
 
 
