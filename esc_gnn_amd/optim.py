@@ -242,6 +242,10 @@ class AdamW(torch.optim.Optimizer):
         self.state_bits, self.max_grad_norm, self.seed, self.grad_norm = state_bits, max_grad_norm, int(seed), None
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
 
+    def __getstate__(self):
+        """what a copy or a pickle takes along: the base class names its own attributes alone"""
+        return {**super().__getstate__(), **{n: getattr(self, n) for n in ("state_bits", "max_grad_norm", "seed", "grad_norm")}}
+
     def _state_of(self, p, fresh):
         """a parameter's state; `fresh`: the step count that the parameters which begin in this step share"""
         st = self.state[p]

@@ -51,3 +51,23 @@ def test_a_count_of_another_type_is_refused_at_the_step():
         with pytest.raises(ValueError, match="step"):
             opt.step()
         assert torch.equal(p, before)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_copy_goes_on_by_itself(bits):
+    """a deep copy (with its own parameters) makes the same steps, bit for bit, and neither counts for the other"""
+    from esc_gnn_amd import AdamW
+    ps = [torch.nn.Parameter(torch.randn(n, device=DEV)) for n in (700, 33)]
+    opt = AdamW(ps, state_bits=bits, max_grad_norm=0.3, seed=5)
+    for it in range(2):
+        _grads(ps, it); opt.step()
+    other = copy.deepcopy(opt)
+    assert torch.equal(other.grad_norm, opt.grad_norm)
+    qs = other.param_groups[0]["params"]
+    for it in range(2, 4):
+        _grads(ps, it); opt.step()
+    assert int(other.state[qs[0]]["step"]) == 2
+    for it in range(2, 4):
+        _grads(qs, it); other.step()
+    for p, q in zip(ps, qs):
+        assert p is not q and torch.equal(p, q) and all(torch.equal(opt.state[p][n], other.state[q][n]) for n in opt.state[p])

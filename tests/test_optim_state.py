@@ -93,3 +93,28 @@ def test_torch_takes_this_optimizers_state_dict():
         outs.append(qs)
     for a, b in zip(*outs):
         assert torch.equal(a, b)
+
+
+def _copies():
+    import io
+    import pickle
+
+    def by_torch(o):
+        f = io.BytesIO(); torch.save(o, f); f.seek(0)
+        return torch.load(f, weights_only=False)                                   # (written two lines above)
+    return [("deepcopy", copy.deepcopy), ("pickle", lambda o: pickle.loads(pickle.dumps(o))), ("torch.save", by_torch)]
+
+
+@pytest.mark.parametrize("how", _copies(), ids=lambda h: h[0])
+def test_a_copy_keeps_its_settings(how):
+    from esc_gnn_amd import AdamW
+    ps, saved = _torch_dict(steps=2)
+    opt = AdamW(ps, max_grad_norm=0.5, seed=11)
+    opt.load_state_dict(saved)
+    other = how[1](opt)
+    assert (other.state_bits, other.max_grad_norm, other.seed, other.grad_norm) == (32, 0.5, 11, None)
+    qs = other.param_groups[0]["params"]
+    assert other.state[qs[0]]["step"] is other.state[qs[1]]["step"] and int(other.state[qs[0]]["step"]) == 2
+    assert other.state[qs[0]]["step"] is not opt.state[ps[0]]["step"]
+    other.load_state_dict(opt.state_dict())                                        # (loading leaves the settings alone)
+    assert (other.state_bits, other.max_grad_norm, other.seed) == (32, 0.5, 11)
