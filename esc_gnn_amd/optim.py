@@ -229,7 +229,8 @@ class AdamW(torch.optim.Optimizer):
     torch.optim.AdamW's step on the kernels above.  state_bits: 32 or 8 (states); max_grad_norm: clip by the global norm of
     all gradients, `grad_norm` then holds the last step's (on the GPU); seed: of the 8-bit states' rounding.  Parameter
     groups may differ in lr, betas, eps and weight_decay.  A parameter without a gradient is left alone and does not count
-    the step; parameters live on one GPU.
+    the step; parameters live on one GPU.  A step that is captured finds its states there: take one with the same gradients
+    present before the capture (RuntimeError otherwise).
     """
 
     def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, *,
@@ -258,6 +259,12 @@ class AdamW(torch.optim.Optimizer):
                     st[name] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.contiguous_format)
         return st
 
+    @staticmethod
+    def _not_in_a_capture(dev):
+        with torch.cuda.device(dev):
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("escat: this step makes states or step counts, which a capture would make anew at every replay: take one such step before it")
+
     def _moments(self, st):
         if self.state_bits == 8:
             return ((st["exp_avg_codes"], st["exp_avg_scales"]), (st["exp_avg_sq_codes"], st["exp_avg_sq_scales"]))
@@ -273,6 +280,7 @@ class AdamW(torch.optim.Optimizer):
 
         def fresh():
             if not made:
+                self._not_in_a_capture(dev)
                 made.append(torch.zeros(1, dtype=torch.int32, device=dev))
             return made[0]
 
@@ -302,6 +310,7 @@ class AdamW(torch.optim.Optimizer):
                 if count.dtype is not torch.int32 or count.numel() != 1 or count.device != dev:
                     raise ValueError(f"escat: step must be an int32 tensor of one element on {dev}: {count.dtype}, {tuple(count.shape)} on {count.device}")
             if behind and ps:
+                self._not_in_a_capture(dev)
                 own = self.state[ps[0]]["step"].clone()
                 for p in ps:
                     self.state[p]["step"] = own

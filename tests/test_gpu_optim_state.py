@@ -71,3 +71,37 @@ def test_a_copy_goes_on_by_itself(bits):
         _grads(qs, it); other.step()
     for p, q in zip(ps, qs):
         assert p is not q and torch.equal(p, q) and all(torch.equal(opt.state[p][n], other.state[q][n]) for n in opt.state[p])
+
+
+def test_a_capture_that_would_make_states_is_refused():
+    """states and counts made inside a capture would be made anew by every replay: the step has to refuse, and to go on afterwards"""
+    from esc_gnn_amd import AdamW
+    ps = [torch.nn.Parameter(torch.randn(n, device=DEV)) for n in (700, 33)]
+    for p in ps:
+        p.grad = torch.ones_like(p)
+    before = [p.detach().clone() for p in ps]
+    opt = AdamW(ps)
+    with pytest.raises(RuntimeError, match="capture"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            opt.step()
+    assert all(torch.equal(p, q) for p, q in zip(ps, before))
+    opt.step()
+    # a parameter that stays behind makes the others' count their own
+    ps[1].grad = None
+    with pytest.raises(RuntimeError, match="capture"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            opt.step()
+    assert int(opt.state[ps[0]]["step"]) == int(opt.state[ps[1]]["step"]) == 1
+    opt.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    ref = copy.deepcopy(opt)
+    for k in range(3):
+        graph.replay()
+        for q, p in zip(ref.param_groups[0]["params"], ps):
+            q.grad = None if p.grad is None else p.grad.clone()
+        ref.step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(ps, ref.param_groups[0]["params"]))
+        assert int(opt.state[ps[0]]["step"]) == 3 + k and int(opt.state[ps[1]]["step"]) == 1
