@@ -50,14 +50,14 @@ class NodeExperts(nn.Module):
             logits = nn.functional.linear(x.float(), self.router.weight.float())
         weights, experts = route_experts(logits, self.per_node, bias=self.balance)
         if self.training:
-            self.load = self.load + expert_counts(experts, self.balance.numel())
+            self.load += expert_counts(experts, self.balance.numel())        # in place: a captured forward goes on counting here
         return x + expert_mlp(x, weights, experts, self.w1, self.b1, self.w2, self.b2)
 
     @torch.no_grad()
     def update_balance(self):
         load = allreduce_sum_(self.load).float()
         self.balance += self.rate * torch.sign(load.mean() - load)
-        self.load = torch.zeros_like(self.load)
+        self.load.zero_()
 
 
 class ScatteringHead(nn.Module):
