@@ -520,7 +520,7 @@ static int check_route(const char *who, int type, int64_t rows, int E, int k, in
     if (rows < 0 || E < 1 || k < 1 || k > E) return fail(ESCAT_EINVAL, "%s: rows = %lld, E = %d, k = %d", who, (long long)rows, E, k);
     if (E > ESCAT_ROUTE_MAX_EXPERTS || k > ESCAT_ROUTE_MAX_K) return fail(ESCAT_ERANGE, "%s: E = %d (at most %d), k = %d (at most %d)", who, E, ESCAT_ROUTE_MAX_EXPERTS, k, ESCAT_ROUTE_MAX_K);
     if (score != 0 && score != 1) return fail(ESCAT_EINVAL, "%s: score = %d (0 softmax, 1 sigmoid)", who, score);
-    if (!(scale > 0.f)) return fail(ESCAT_EINVAL, "%s: scale = %g", who, (double)scale);
+    if (!(scale > 0.f) || scale == R_INF) return fail(ESCAT_EINVAL, "%s: scale = %g", who, (double)scale);
     return ESCAT_OK;
 }
 

@@ -102,8 +102,8 @@ def route_experts(logits: torch.Tensor, k: int, *, score: str = "softmax", bias:
     keep = groups if keep_groups is None else keep_groups
     if not 1 <= keep <= groups or group_top not in (1, 2):
         raise ValueError(f"escat: keep_groups = {keep} (1..{groups}), group_top = {group_top} (1 or 2)")
-    if not (scale > 0.0 and math.isfinite(scale)):
-        raise ValueError(f"escat: scale must be positive: {scale}")
+    if not 0.0 < ctypes.c_float(float(scale)).value < math.inf:                  # (the kernels' type)
+        raise ValueError(f"escat: scale must be a positive fp32 number: {scale}")
     if bias is not None and (bias.shape != (E,) or bias.dtype is not torch.float32 or bias.device != logits.device):
         raise ValueError(f"escat: bias must be ({E},) fp32 on {logits.device}: {tuple(bias.shape)} {bias.dtype} {bias.device}")
     _need_gpu(logits, "logits")
