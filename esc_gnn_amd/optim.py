@@ -156,12 +156,15 @@ class _Tables:
         self.by_type[(DTYPE_CODES[pt], DTYPE_CODES[gt], bits)] = array.array("Q", chain.from_iterable(rows))
         return True
 
-    def written(self):
-        """addresses of what the step writes, to refuse a tensor that is listed twice"""
-        for t in self.by_type.values():
-            yield from t[0::8]
-            yield from t[2::8]
-            yield from t[3::8]
+    def clashes(self, count):
+        """whether the step would write a tensor twice (`count`: its address is the step count's) or one that it reads as a gradient"""
+        written, read = [count], set()
+        for (_, _, bits), t in self.by_type.items():
+            for at in (0, 2, 3, 4, 5) if bits == 8 else (0, 2, 3):
+                written += t[at::8]
+            read.update(t[1::8])
+        once = set(written)
+        return len(once) != len(written) or not read.isdisjoint(once)
 
 
 def _begin(lib, tables, max_norm, groups, step, ws, norm, stream):
@@ -208,9 +211,8 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     if dev.type != "cuda" or not table.add_all(params, grads, exp_avgs, exp_avg_sqs, dev):
         for i in range(n):
             table.add(params[i], grads[i], exp_avgs[i], exp_avg_sqs[i], i, dev)
-    written = list(table.written())
-    if len(set(written)) != len(written):
-        raise ValueError("escat: a parameter or state is listed twice")
+    if table.clashes(step.data_ptr()):
+        raise ValueError("escat: a parameter, state or count is listed twice, or as a gradient")
     if dev.type != "cuda":
         raise RuntimeError("escat: tensors must live on a GPU; the MI355X path has no CPU fallback")
     lib = _lib.load()

@@ -118,3 +118,20 @@ def test_a_copy_keeps_its_settings(how):
     assert other.state[qs[0]]["step"] is not opt.state[ps[0]]["step"]
     other.load_state_dict(opt.state_dict())                                        # (loading leaves the settings alone)
     assert (other.state_bits, other.max_grad_norm, other.seed) == (32, 0.5, 11)
+
+
+def test_adamw_refuses_scales_and_a_count_that_are_listed_twice():
+    """states of two tensors, or of both moments, that share their scales; a count that is one of the states"""
+    from esc_gnn_amd import adamw_step
+    z, c = lambda n=300: torch.zeros(n), lambda: torch.zeros(300, dtype=torch.uint8)     # noqa: E731
+    s, step = torch.zeros(2), torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(ValueError, match="twice"):
+        adamw_step([z()], [z()], [(c(), s)], [(c(), s)], step)
+    with pytest.raises(ValueError, match="twice"):
+        adamw_step([z(), z()], [z(), z()], [(c(), s), (c(), s)], [(c(), z(2)), (c(), z(2))], step)
+    one = torch.zeros(1)
+    with pytest.raises(ValueError, match="twice"):
+        adamw_step([one], [z(1)], [z(1)], [z(1)], one.view(torch.int32))
+    g = z()
+    with pytest.raises(ValueError, match="twice"):
+        adamw_step([z()], [g], [g], [z()], step)                                      # a gradient that the step would write
