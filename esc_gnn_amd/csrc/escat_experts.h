@@ -12,8 +12,9 @@
 //                   of a tile's rows end in the same accumulators, and results are written once, in their own type.
 //
 // By combination moves less memory (no fp32 results of pairs written and read again) but cuts the rows into C(E + k - 1, k) groups, pads each
-// to whole tiles, and a tile walks k experts one after the other: taken with 2048 rows or more to a group and at most 1024 keys.  Forward and
-// backward by combination / by pair, us, 256 wide, at 512, 1024, 2048, 4096 rows to a group:
+// to whole tiles, and a tile walks k experts one after the other: taken with 2048 rows or more to a group and at most 1024 keys.  One number for
+// all: with 8 experts bf16 crosses over near 1024 rows (8 % left there) and fp32 near 2048 (1 % either way).  Forward and backward by
+// combination / by pair, us, 256 wide, at 512, 1024, 2048, 4096 rows to a group:
 //   bf16, 8 experts, k = 2   205/184  255/277  379/444  610/769       fp32   512/457  781/764  1415/1405  2573/2638
 //   bf16, 4 experts, k = 3   203/150  251/236  336/377  527/644       fp32   439/347  701/629  1177/1154  2208/2204
 // k = 1 is always its case, the two are the same there.
@@ -48,7 +49,6 @@ struct EPlan {
 static inline int64_t plan_items(int64_t rows, int k, int combo) { return combo ? rows : rows * k; }
 static inline int64_t plan_blocks(int64_t items) { return (items + PLAN_CHUNK - 1) / PLAN_CHUNK; }
 static inline int64_t plan_max_tiles(int64_t items, int keys) { return items / XM + (keys < items ? keys : items) + 1; }
-static inline int plan_keys(int64_t rows, int k, int E) { const int c = combo_keys(rows, E, k); return c ? c : E; }
 static inline EPlan plan_view(void *mem, int64_t rows, int k, int E, int combo, int64_t *ints)
 {
     EPlan p; int *q = (int *)mem;

@@ -27,7 +27,7 @@ typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 
-template <typename T> struct Elem;                // PER: elements of 16 bytes; KB: k of a step; SUB: MFMA groups of a step
+template <typename T> struct Elem;                // PER: elements of 16 bytes; KB: k of a step
 template <> struct Elem<float> { static constexpr int PER = 4, KB = 32; };
 template <> struct Elem<bf16_t> { static constexpr int PER = 8, KB = 64; };
 template <> struct Elem<f16_t> { static constexpr int PER = 8, KB = 64; };
@@ -84,9 +84,6 @@ template <typename T, bool KM> struct Stage {
 };
 
 // ---- one step's products of a wave: acc[i][j] += A block i x B block j
-template <typename T, bool KM> struct Frag;
-template <typename T> struct Frag16 { s8 v; };
-
 template <typename T> __device__ __forceinline__ s8 frag_kc(const char *lds, int row, int sub)
 {
     const int l = threadIdx.x & 63, r = row + (l & 31), c = sub * 2 + (l >> 5);

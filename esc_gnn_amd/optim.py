@@ -5,9 +5,10 @@ AdamW over many tensors at once, states in 32 or in 8 bits, with the clip by the
     opt = AdamW(model.parameters(), lr=1e-3, state_bits=8, max_grad_norm=1.0)      # a torch.optim.Optimizer
     adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr=...)                 # the same on plain tensors
 
-A step is three launches with clipping and two without, however many tensors there are (csrc/escat_adamw.hip; 56 tensors
-to a launch).  The step count lives on the GPU: a captured step counts on when it is replayed (lr and the other
-hyperparameters are constants of the captured graph).  The same inputs give the same bits.
+A step of up to 56 tensors of one type is three launches with clipping and two without (csrc/escat_adamw.hip): the squares, the
+count with the scalars, the update.  Squares and update are one each per 56 tensors and type (the update: per group of settings
+too), and parameters that count their steps apart (some paused) make a call each.  The step count lives on the GPU: a captured step
+counts on when it is replayed (lr and the other hyperparameters are constants of the captured graph).  The same inputs give the same bits.
 
 8-bit states hold one byte per element and moment and one fp32 scale per 256 elements: 2.03 bytes a parameter instead of
 8.  They are rounded stochastically, by bits that depend on (seed, step, tensor, element) only, so ranks that average
@@ -229,7 +230,8 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
 class AdamW(torch.optim.Optimizer):
     """
     torch.optim.AdamW's step on the kernels above.  state_bits: 32 or 8 (states); max_grad_norm: clip by the global norm of
-    all gradients, `grad_norm` then holds the last step's (on the GPU); seed: of the 8-bit states' rounding.  Parameter
+    all gradients, `grad_norm` then holds the last step's (on the GPU); seed: of the 8-bit states' rounding.  These three are
+    the constructor's: a copy or pickle has them, a state dict (states and groups, as torch's) does not.  Parameter
     groups may differ in lr, betas, eps and weight_decay.  A parameter without a gradient is left alone and does not count
     the step; parameters live on one GPU.  A step that is captured finds its states there: take one with the same gradients
     present before the capture (RuntimeError otherwise).

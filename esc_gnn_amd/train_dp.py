@@ -11,7 +11,7 @@ What a step does, per rank (one process per GPU, graphs sharded, RCCL only for t
      MSE loss;
   3. backward into ONE flat fp32 gradient bucket, one all-reduce (sum) / world, AdamW step.
 Optional (off by default): `experts` = E widens the head at the cost per node of k of its E small MLPs (route_experts +
-expert_mlp, kept in balance by a selection bias); `optimizer` = "escat" / "escat8" takes the multi-tensor AdamW of
+expert_mlp, kept in balance by a selection bias that an all-reduce of E counts follows); `optimizer` = "escat" / "escat8" takes the multi-tensor AdamW of
 esc_gnn_amd.optim with states in 32 / 8 bits; `max_grad_norm` clips as the reference does (training/train.py:411-415).
 The reference gets 3 from Accelerate/DDP (training/train.py:408, :483-492); the heads themselves are plain PyTorch
 but for the optional operators.
@@ -111,7 +111,7 @@ class DPTrainer:
             pred = self.model(Ws, inv, graph_id, n_graphs)
         loss = torch.nn.functional.mse_loss(pred.float(), target)
         loss.backward()                       # grads land in the flat bucket (p.grad are views of it)
-        self.bucket.allreduce_mean()          # the step's only collective
+        self.bucket.allreduce_mean()          # the step's only collective but for the experts' loads below
         if self.max_grad_norm is not None and isinstance(self.opt, torch.optim.AdamW):
             torch.nn.utils.clip_grad_norm_(self.model.parameters(), self.max_grad_norm)
         self.opt.step()

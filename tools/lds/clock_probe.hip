@@ -1,6 +1,6 @@
 // clock_probe: the shader clock an LDS + packed-FMA loop actually runs at (all CUs busy), from the ratio of the
 // shader cycle counter (s_memtime) to the constant 100 MHz counter (s_memrealtime) inside the kernel.
-//   build: hipcc -O3 --offload-arch=gfx950 -o clock_probe clock_probe.hip
+//   build: hipcc -O3 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -o clock_probe clock_probe.hip
 #include <hip/hip_runtime.h>
 #include <cstdio>
 typedef float f4 __attribute__((ext_vector_type(4)));

@@ -1,6 +1,6 @@
 // LDS gather micro-benchmark: how many LDS cycles does one ds_read_b128 wave-instruction cost for a given
 // lane -> 16-byte-slot pattern?  Used to check the bank-conflict model the SELL slot planner is built on.
-//   build: hipcc -O3 --offload-arch=gfx950 -o lds_gather_bench lds_gather_bench.hip
+//   build: hipcc -O3 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -o lds_gather_bench lds_gather_bench.hip
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdlib>

@@ -4,7 +4,7 @@
 //   K1  K0 without the dependent x gather (x row taken from the lane index): what the rowptr -> col -> x chain costs
 //   K2  staged: a workgroup copies the contiguous block range of RPB rows into LDS with 16-byte loads issued together,
 //       gathers the x rows of those blocks into LDS, then LPR lanes per row compute out of LDS
-//   build: hipcc -O3 --offload-arch=gfx950 -o step_bench step_bench.hip
+//   build: hipcc -O3 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -o step_bench step_bench.hip
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdlib>

@@ -1,7 +1,7 @@
 // HBM streaming micro-benchmark in the shape of the chain kernel's operator load: one persistent workgroup per CU,
 // every wave pulls a contiguous run of "slots" (2304 B per slot and lane group: two 1-KiB dwordx4 pieces + one 256-B
 // dword piece) into registers in one burst, then "computes" for a while.  Which variant reaches the HBM rate?
-//   build: hipcc -O3 --offload-arch=gfx950 -o stream_bench stream_bench.hip
+//   build: hipcc -O3 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -o stream_bench stream_bench.hip
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdlib>
