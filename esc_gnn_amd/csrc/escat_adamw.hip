@@ -169,16 +169,17 @@ __device__ __forceinline__ float finite_size(float x) { const float a = fabsf(x)
 
 // ------------------------------------------------------------------ the update
 // The hardware's root takes a v below 2^-126 for 0, which an eps of 1e-8 hides and one of 0 does not (m / 0): such a v goes through it multiplied by
-// 2^64.  64 Mi fp32 parameters: 8-bit states 224 instead of 220 us, 32-bit ones 363 either way
-__device__ __forceinline__ float root_of(float v)
+// 2^64.  SMALL: whether that may show (root_shows)
+template <bool SMALL> __device__ __forceinline__ float root_of(float v)
 {
+    if (!SMALL) return __builtin_amdgcn_sqrtf(v);
     const bool low = v < 1.2621774483536189e-29f;                                      // 2^-96
     const float r = __builtin_amdgcn_sqrtf(low ? v * 18446744073709551616.0f : v);
     return low ? r * 2.3283064365386963e-10f : r;                                      // 2^-32
 }
 
 struct AVals { float p, m, v; };
-__device__ __forceinline__ AVals adamw_one(float p, float g, float m, float v, const AScalars &s, float clip, float size, float isb)
+template <bool SMALL> __device__ __forceinline__ AVals adamw_one(float p, float g, float m, float v, const AScalars &s, float clip, float size, float isb)
 {
 #pragma clang fp contract(off)
     g = g * clip;
@@ -186,11 +187,11 @@ __device__ __forceinline__ AVals adamw_one(float p, float g, float m, float v, c
     v = v * s.b2 + (g * g) * s.omb2;
     // (hardware root and reciprocal, 1 unit in the last place of the update each: an exact root and quotient are 25 instructions more, which
     // the 8-bit form has no room for; the moments do not pass here)
-    const float num = m * size, den = root_of(v) * isb + s.eps;
+    const float num = m * size, den = root_of<SMALL>(v) * isb + s.eps;
     return {p * s.decay - num * __builtin_amdgcn_rcpf(den), m, v};
 }
 
-template <typename P, typename G, int BITS>
+template <typename P, typename G, int BITS, bool SMALL>
 __global__ void __launch_bounds__(AT) k_adamw(const ATable tab, const AScalars s, const int *__restrict__ step, const float *__restrict__ hdr)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -250,7 +251,7 @@ __global__ void __launch_bounds__(AT) k_adamw(const ATable tab, const AScalars s
         float mx = 0.f, vx = 0.f;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const AVals r = adamw_one(p[u][k], g[u][k], m[u][k], v[u][k], s, clip, size, isb);
+            const AVals r = adamw_one<SMALL>(p[u][k], g[u][k], m[u][k], v[u][k], s, clip, size, isb);
             p[u][k] = r.p; m[u][k] = r.m; v[u][k] = r.v;
             if (BITS == 8 && (whole || i0 + u * AQ + k < n)) { mx = fmaxf(mx, finite_size(r.m)); vx = fmaxf(vx, finite_size(r.v)); }
         }
@@ -406,11 +407,17 @@ extern "C" int escat_adamw_begin(const escat_adamw_tensor *tensors, int n_tensor
     return slot;
 }
 
+// A root taken for 0 is short of at most 2^-63, times its scalar 1 / sqrt(1 - b2^t) <= 1 / sqrt(1 - b2): beyond 2^-23 of eps that shows in the
+// update (eps = 1e-8: not for b2 up to 1 - 8e-9).  The 8-bit form, which its instructions bound, looks after it only then: 64 Mi fp32 parameters
+// 220 us without, 224 with; the 32-bit form always, 363 us either way
+static bool root_shows(double eps, double b2) { return eps * sqrt(1.0 - b2) < 9.094947017729282e-13; }            // 2^-40
+
 template <typename P, typename G>
-static int launch_update(const ATable &tab, const AScalars &s, int bits, const int32_t *step, const float *hdr, hipStream_t st)
+static int launch_update(const ATable &tab, const AScalars &s, int bits, bool small, const int32_t *step, const float *hdr, hipStream_t st)
 {
-    if (bits == 32) k_adamw<P, G, 32><<<tab.chunks, AT, 0, st>>>(tab, s, step, hdr);
-    else k_adamw<P, G, 8><<<tab.chunks, AT, 0, st>>>(tab, s, step, hdr);
+    if (bits == 32) k_adamw<P, G, 32, true><<<tab.chunks, AT, 0, st>>>(tab, s, step, hdr);
+    else if (small) k_adamw<P, G, 8, true><<<tab.chunks, AT, 0, st>>>(tab, s, step, hdr);
+    else k_adamw<P, G, 8, false><<<tab.chunks, AT, 0, st>>>(tab, s, step, hdr);
     CHECK_LAUNCH("escat_adamw_update");
     return ESCAT_OK;
 }
@@ -432,11 +439,12 @@ extern "C" int escat_adamw_update(const escat_adamw_tensor *tensors, int n_tenso
                         (float)(1.0 - group->lr * group->weight_decay), seed, group_index};
     hipStream_t st = (hipStream_t)stream;
     const float *hdr = (const float *)workspace;
+    const bool small = root_shows(group->eps, group->beta2);
     return for_tables(tensors, n_tensors, [&](const ATable &tab, int) {
-        if (param_type == ESCAT_F32) return launch_update<float, float>(tab, s, state_bits, step, hdr, st);
+        if (param_type == ESCAT_F32) return launch_update<float, float>(tab, s, state_bits, small, step, hdr, st);
         if (param_type == ESCAT_BF16)
-            return grad_type == ESCAT_BF16 ? launch_update<bf16_t, bf16_t>(tab, s, state_bits, step, hdr, st) : launch_update<bf16_t, float>(tab, s, state_bits, step, hdr, st);
-        return grad_type == ESCAT_F16 ? launch_update<f16_t, f16_t>(tab, s, state_bits, step, hdr, st) : launch_update<f16_t, float>(tab, s, state_bits, step, hdr, st);
+            return grad_type == ESCAT_BF16 ? launch_update<bf16_t, bf16_t>(tab, s, state_bits, small, step, hdr, st) : launch_update<bf16_t, float>(tab, s, state_bits, small, step, hdr, st);
+        return grad_type == ESCAT_F16 ? launch_update<f16_t, f16_t>(tab, s, state_bits, small, step, hdr, st) : launch_update<f16_t, float>(tab, s, state_bits, small, step, hdr, st);
     });
 }
 
