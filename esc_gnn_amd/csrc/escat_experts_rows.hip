@@ -8,8 +8,8 @@
 // may be kept for the weights' gradient.  dw and silu' see no rounding of u: it is computed again next to G in fp32, or, where
 // that costs more than reading it, left in fp32 by the forward (keeps_u).  Results of the pairs are joined in fp32 by a pass of their own, in the order of the slots: no atomics.
 //
-// 524288 rows, k = 2 of 8 experts, 256 x 256 x 256 in bf16: 137 GFLOP a product, W1 x 273 us (0.8 GB), W2 h 230 us (0.8 GB), u, G and du 585 us
-// (two products, 1.1 GB), W1^T du 220 us (0.8 GB): neither the matrix units (a quarter of the cycles) nor memory bound; a workgroup's chain of
+// 524288 rows, k = 2 of 8 experts, 256 x 256 x 256 in bf16: 137 GFLOP a product, W1 x 276 us (0.86 GB), W2 h 230 us (0.91 GB), u, G and du 594 us
+// (two products, 1.15 GB), W1^T du 221 us (0.82 GB; bytes by FETCH_SIZE, doubled, and WRITE_SIZE): neither the matrix units (a quarter of the cycles) nor memory bound; a workgroup's chain of
 // tile, row, pieces and epilogue is, four steps of 64 long.  64 experts of 256 rows, 1024 x 2048 x 1024: 69 GFLOP a product (86 with the tiles' last
 // rows) in 125 to 131 us, 38 % of the matrix cycles at about 1.75 GHz (W1 x 146 where it leaves u, G and du 176 with u read).  Tiles of 256 x 128 in
 // eight waves, tiles in an order that shares weights, s_setprio around the products and leaving out the products of rows behind a tile's last each

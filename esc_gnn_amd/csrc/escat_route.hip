@@ -14,7 +14,7 @@
 // keys are computed in 32 bits with a bound on their error, and a wave in which two keys that decide something lie within that
 // bound repeats the selection with 64-bit keys (about one wave in 500 at E = 256, k = 8).
 //
-// 65537 rows of 256 bf16 logits, k = 8, bias and 4 of 8 groups: 72 us forward (34 MB read: 7 us; what bounds it is the instructions of the
+// 65537 rows of 256 bf16 logits, k = 8, bias and 4 of 8 groups: 71 us forward (34 MB read: 7 us; what bounds it is the instructions of the
 // selection, 1200 for the two rows of a wave), 17 us backward.  524288 rows of 8 fp32 logits, k = 2: 12 us forward (25 MB, 2.1 TB/s), 9 us backward.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
