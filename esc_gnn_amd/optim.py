@@ -351,10 +351,17 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def state_dict(self):
-        """As torch's: the moments themselves.  Each parameter has a count of its own here (in the optimizer those that took every step together
-        share one), so that an optimizer that counts by parameter, torch's among them, does not count a shared one several times."""
+        """As torch's: the moments themselves, and for each parameter a count of its own as torch keeps it, an fp32 number on the CPU (beyond
+        2^24 steps fp64).  In the optimizer those that took every step together share one, on the GPU: this call waits for it."""
         out = super().state_dict()
-        out["state"] = {i: {n: t.clone() if n == "step" else t for n, t in st.items()} for i, st in out["state"].items()}
+        seen = {}
+
+        def count(t):
+            if id(t) not in seen:
+                seen[id(t)] = int(t)
+            k = seen[id(t)]
+            return torch.tensor(float(k), dtype=torch.float32 if k <= 1 << 24 else torch.float64)
+        out["state"] = {i: {n: count(t) if n == "step" else t for n, t in st.items()} for i, st in out["state"].items()}
         return out
 
     def load_state_dict(self, state_dict):

@@ -105,3 +105,26 @@ def test_a_capture_that_would_make_states_is_refused():
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(ps, ref.param_groups[0]["params"]))
         assert int(opt.state[ps[0]]["step"]) == 3 + k and int(opt.state[ps[1]]["step"]) == 1
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(fused=True), dict(capturable=True), dict(foreach=False)])
+def test_torch_goes_on_where_this_one_left_off(kw):
+    """the other way: 8 steps here, then 5 by both; the bound is counted in the test above"""
+    from esc_gnn_amd import AdamW
+    torch.manual_seed(1)
+    a = [torch.nn.Parameter(torch.randn(s, device=DEV)) for s in ((33, 7), (300,), (1,), (64, 65))]
+    opt = AdamW(a, lr=1e-3)
+    for it in range(8):
+        _grads(a, it); opt.step()
+    b = [torch.nn.Parameter(p.detach().clone()) for p in a]
+    ref = torch.optim.AdamW(b, lr=0.5, **kw)
+    saved = copy.deepcopy(opt.state_dict())
+    for g, own in zip(saved["param_groups"], ref.param_groups):
+        g.update({n: v for n, v in own.items() if n not in g})                        # (how torch is to run it)
+    ref.load_state_dict(saved)
+    for it in range(8, 13):
+        _grads(a, it); opt.step()
+        _grads(b, it); ref.step()
+        for x, y in zip(a, b):
+            assert float((x - y).detach().abs().max()) <= 1000 * U * max(1.0, float(y.detach().abs().max())), it
+    assert all(int(ref.state[p]["step"]) == 13 for p in b)

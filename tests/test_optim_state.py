@@ -135,3 +135,20 @@ def test_adamw_refuses_scales_and_a_count_that_are_listed_twice():
     g = z()
     with pytest.raises(ValueError, match="twice"):
         adamw_step([z()], [g], [g], [z()], step)                                      # a gradient that the step would write
+
+
+def test_a_count_in_the_dict_is_as_torch_keeps_it():
+    from esc_gnn_amd import AdamW
+    ps, saved = _torch_dict(steps=4)
+    for n in (4, 2 ** 24, 2 ** 24 + 1, 2 ** 31 - 1):
+        saved["state"][0]["step"] = saved["state"][1]["step"] = n
+        opt = AdamW(ps)
+        opt.load_state_dict(saved)
+        out = opt.state_dict()["state"]
+        for st in out.values():
+            assert st["step"].shape == () and st["step"].device.type == "cpu" and st["step"].dtype is (torch.float32 if n <= 2 ** 24 else torch.float64)
+            assert int(st["step"]) == n
+        assert out[0]["step"] is not out[1]["step"] and out[0]["exp_avg"] is opt.state[ps[0]]["exp_avg"]
+        again = AdamW(ps)
+        again.load_state_dict(opt.state_dict())
+        assert int(again.state[ps[0]]["step"]) == n and again.state[ps[0]]["step"].dtype is torch.int32
